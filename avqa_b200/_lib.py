@@ -49,6 +49,13 @@ _SIGS = {
     "avq_device_fault": ([_P, _P], _I),
     "avq_quantize_noalloc": ([_I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P,
                               _P, _P, _P, _P, _P], _I),
+    "avq_rotary": ([_I, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _I, _P, _I, _P, _L, _I, _P, _P, _P, _P, _P],
+                   _I),
+    "avq_paged_append": ([_I, _P, _P, _I, _P, _P, _P, _P, _P, _P, _I, _I, _P, _P, _P, _P, _I, _I, _P, _L, _I, _P, _P, _I,
+                          _I, _I, _I, _P, _P, _I, _P, _I, _P, _P], _I),
+    "avq_paged_attention_workspace_size": ([_I, _I, _I, _I, _I, _I, _I], _Z),
+    "avq_paged_attention": ([_I, _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _P, _L, _I, _P, _P, _I, _I, _I, _I, _F, _I,
+                             _P, _P, _P, _Z, _P], _I),
     "avq_profile_begin": ([], _I),
     "avq_profile_end": ([ctypes.c_char_p, _I, _P, _P, _I], _I),
 }

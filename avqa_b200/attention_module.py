@@ -19,6 +19,10 @@ reference offers but no benchmark configuration uses -- BCAR codebook
 adaptation, the threshold router, the adaptive budget scheduler, learnable
 HVAQ parameters and the dense "reference" execution mode -- raise
 :class:`BackendError` instead of silently running elsewhere.
+
+Beyond the reference: with a ``rotary`` embedding the projected queries and
+keys are rotated by their positions before any of this, and the dense path
+attends over a :class:`~avqa_b200.cache.BlockKVCache` in place.
 """
 from __future__ import annotations
 
@@ -29,10 +33,11 @@ from torch import nn
 
 from avqa_b200 import ops
 from avqa_b200.backend import Backend, CUDABackend
-from avqa_b200.cache import KVCache, PagedKVCache
+from avqa_b200.cache import BlockKVCache, KVCache, PagedKVCache
 from avqa_b200.codebook import HierarchicalCodebook
 from avqa_b200.config import AVQConfig
-from avqa_b200.exceptions import BackendError, DeviceError, DtypeError, RoutingError, ShapeError
+from avqa_b200.exceptions import (BackendError, ConfigurationError, DeviceError, DtypeError, RoutingError,
+                                  ShapeError)
 
 SUPPORTED_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 
@@ -40,9 +45,14 @@ SUPPORTED_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 class AVQAttention(nn.Module):
     """AVQ attention (hierarchical VQ keys, parent attention, routed child correction)."""
 
-    def __init__(self, config: AVQConfig, *, in_proj: bool = True, out_proj: bool = True) -> None:
+    def __init__(self, config: AVQConfig, *, in_proj: bool = True, out_proj: bool = True, rotary=None) -> None:
         super().__init__()
         self.config = config
+        head_dim = config.attention.embed_dim // config.attention.num_heads
+        if rotary is not None and rotary.head_dim != head_dim:
+            raise ConfigurationError("the rotary embedding's head_dim differs from the module's",
+                                     {"head_dim": head_dim, "rotary": rotary.head_dim})
+        self.rotary = rotary  # a RotaryEmbedding, or None
         self.backend = Backend.create(config.backend.name)
         E = config.attention.embed_dim
         if in_proj:
@@ -131,15 +141,19 @@ class AVQAttention(nn.Module):
     # -- forward -----------------------------------------------------------------
 
     def forward(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, mask: torch.Tensor | None = None,
-                kv_cache: KVCache | None = None) -> torch.Tensor:
+                kv_cache: KVCache | None = None, positions: torch.Tensor | None = None) -> torch.Tensor:
+        """``positions`` (with ``rotary`` only): where the new tokens are, as
+        :class:`~avqa_b200.rotary.RotaryEmbedding` takes them; queries and keys
+        are then the same tokens.  Without it the keys follow the cached ones
+        and the last query is at the last key's position."""
         c = self.config
         if c.precision.autocast:
             with torch.autocast(device_type=query.device.type, dtype=getattr(torch, c.precision.dtype)):
-                return self.forward_impl(query, key, value, mask, kv_cache)
-        return self.forward_impl(query, key, value, mask, kv_cache)
+                return self.forward_impl(query, key, value, mask, kv_cache, positions)
+        return self.forward_impl(query, key, value, mask, kv_cache, positions)
 
-    def forward_impl(self, query, key, value, mask=None, kv_cache=None) -> torch.Tensor:
-        return cuda_run_pipeline(self, query, key, value, mask, kv_cache)
+    def forward_impl(self, query, key, value, mask=None, kv_cache=None, positions=None) -> torch.Tensor:
+        return cuda_run_pipeline(self, query, key, value, mask, kv_cache, positions=positions)
 
     def forward_chunked(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
                         chunk_size: int) -> torch.Tensor:
@@ -167,7 +181,8 @@ def hvaq_mode(config: AVQConfig) -> int:
 
 
 def cuda_run_pipeline(m, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
-                      mask: torch.Tensor | None = None, kv_cache=None, chunk_size: int = 0) -> torch.Tensor:
+                      mask: torch.Tensor | None = None, kv_cache=None, chunk_size: int = 0,
+                      positions: torch.Tensor | None = None) -> torch.Tensor:
     """The reference pipeline (pipeline.py:276-399) on the CUDA library.
 
     ``m`` is any module with the reference ``AVQAttention`` attributes
@@ -187,9 +202,16 @@ def cuda_run_pipeline(m, query: torch.Tensor, key: torch.Tensor, value: torch.Te
     q = AVQAttention.split_heads(qp, H)
     k = AVQAttention.split_heads(kp, H)
     v = AVQAttention.split_heads(vp, H)
+    dense = not c.refinement.enabled or c.execution.mode == "reference"
+    if isinstance(kv_cache, BlockKVCache):
+        if not dense:
+            raise BackendError("the quantized path does not attend over a BlockKVCache; use a PagedKVCache, or "
+                               "execution.mode = 'reference'")
+        return block_dense_path(m, q, k, v, mask, kv_cache, chunk_size, positions)
+    q, k = rotated(m, q, k, kv_cache, positions)
     m.sync_codebook_device(q)
     backend: CUDABackend = m.backend  # type: ignore[assignment]
-    if not c.refinement.enabled or c.execution.mode == "reference":
+    if dense:
         # pipeline.py:310-312: no scheduler, or the reference mode: dense
         # attention over the (cached) keys with the resolved mask
         return dense_path(m, q, k, v, mask, kv_cache, chunk_size)
@@ -222,6 +244,54 @@ def cuda_run_pipeline(m, query: torch.Tensor, key: torch.Tensor, value: torch.Te
                         present=present)
         ready = None  # later chunks are ordered after the first one's wait
     return m.dropout(m.out_proj(out))
+
+
+def rotated(m, q: torch.Tensor, k: torch.Tensor, kv_cache=None,
+            positions: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """``q [B, H, T, D]`` and ``k [B, H, S, D]`` rotated by the module's
+    ``rotary`` embedding, if it has one: the keys follow the cached ones, and
+    query t is at the last key's position minus T - 1 - t (the alignment of
+    the causal mask, attention_module.py:369-390)."""
+    rotary = getattr(m, "rotary", None)
+    if rotary is None:
+        if positions is not None:
+            raise BackendError("positions need a module with a rotary embedding")
+        return q, k
+    T, S = q.shape[2], k.shape[2]
+    if positions is not None:
+        if T != S:
+            raise ShapeError("positions need queries and keys of the same tokens", expected=S, actual=T)
+        return rotary(q, k, positions)
+    if kv_cache is not None and getattr(kv_cache, "max_size", 0) > 0:
+        raise BackendError("a cache that drops keys does not know the new tokens' positions; pass positions")
+    past = 0 if kv_cache is None else kv_cache.size
+    if T == S:
+        return rotary(q, k, offset=past)
+    return rotary(q, offset=past + S - T), rotary(k, offset=past)
+
+
+def block_dense_path(m, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: torch.Tensor | None, kv_cache,
+                     chunk_size: int = 0, positions: torch.Tensor | None = None) -> torch.Tensor:
+    """The dense path over a :class:`BlockKVCache`: the new tokens' keys and
+    values go into its pages and the queries attend to them there, without
+    the concatenated cache of :func:`dense_path`.  The scores stay fp32 here."""
+    B, H, T, D = q.shape
+    if mask is not None or chunk_size > 0:
+        raise BackendError("a user mask or query chunks over a BlockKVCache are not supported; "
+                           "causal attention over it is (config.causal)")
+    if k.shape[2] != T:
+        raise ShapeError("a BlockKVCache attends with the tokens that it appends", expected=k.shape[2], actual=T)
+    rotary = getattr(m, "rotary", None)
+    if positions is not None:
+        if rotary is None and kv_cache.rotary is None:
+            raise BackendError("positions need a rotary embedding")
+        if positions.dim() == 3 or (positions.dim() == 2 and (rotary or kv_cache.rotary).num_axes == 1):
+            positions = positions.expand(*positions.shape[:-2], B, T).flatten(-2)
+        else:
+            positions = positions.repeat(*[1] * (positions.dim() - 1), B)
+    qp, kp, vp = (x.transpose(1, 2).reshape(B * T, H, D) for x in (q, k, v))
+    out = kv_cache.attend(qp, kp, vp, [T] * B, positions, causal=m.config.causal, rotary=rotary)
+    return m.dropout(m.out_proj(out.view(B, T, H * D)))
 
 
 def dense_path(m, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: torch.Tensor | None, kv_cache,
@@ -377,5 +447,5 @@ def resolve_quantization(m, k: torch.Tensor, v: torch.Tensor, cb: ops.PreparedCo
     return st
 
 
-__all__ = ["AVQAttention", "codeword_mask", "cuda_run_pipeline", "global_min_valid", "hvaq_mode", "query_chunks",
-           "resolve_quantization"]
+__all__ = ["AVQAttention", "block_dense_path", "codeword_mask", "cuda_run_pipeline", "global_min_valid", "hvaq_mode",
+           "query_chunks", "resolve_quantization", "rotated"]

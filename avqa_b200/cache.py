@@ -14,6 +14,9 @@ appends are written into the current page by the append kernel.
 from __future__ import annotations
 
 from abc import ABC, abstractmethod
+from collections.abc import Sequence
+from contextlib import contextmanager
+from dataclasses import dataclass
 
 import torch
 
@@ -192,4 +195,191 @@ class PagedKVCache(KVCache):
         return len(self.key_pages)
 
 
-__all__ = ["InMemoryKVCache", "KVCache", "PagedKVCache"]
+@dataclass(frozen=True)
+class PagedBatch:
+    """One step's packed batch over a page pool: the lists that
+    :func:`avqa_b200.ops.paged_append` and :func:`~avqa_b200.ops.paged_attention` take."""
+
+    block_table: torch.Tensor  # [B, W] int32: the pages of each sequence
+    kv_len: torch.Tensor  # [B] int32: tokens of each sequence, with the new ones
+    q_start: torch.Tensor  # [B + 1] int32: where each sequence's new tokens begin
+    max_q_len: int  # the most new tokens of a sequence
+    tokens: int  # new tokens in all
+
+
+class BlockKVCache(KVCache):
+    """A pool of pages ``[num_pages, H, page_size, D]`` shared by sequences of
+    different lengths, each with its own list of pages.
+
+    Unlike :class:`PagedKVCache`, whose pages hold a whole batch of equal
+    lengths, sequences here grow by different numbers of tokens
+    (:meth:`reserve`), end one by one (:meth:`release` gives their pages back)
+    and may have fewer key heads than the queries.  Appends and attention run
+    on the pages in place (:meth:`attend`).  ``AVQAttention`` attends through
+    it on its dense path (``execution.mode = "reference"`` or refinement off).
+
+    ``rotary``: a :class:`~avqa_b200.rotary.RotaryEmbedding` that rotates keys
+    as they are appended and queries as they attend.
+    """
+
+    def __init__(self, num_pages: int, page_size: int = 16, num_heads: int = 1, head_dim: int = 64, rotary=None,
+                 device: str | torch.device = "cuda", dtype: torch.dtype = torch.float32) -> None:
+        super().__init__()
+        for name, n in (("num_pages", num_pages), ("page_size", page_size), ("num_heads", num_heads),
+                        ("head_dim", head_dim)):
+            if n <= 0:
+                raise ConfigurationError(f"{name} must be > 0, got {n}", {name: n})
+        if rotary is not None and rotary.head_dim != head_dim:
+            raise ConfigurationError("the rotary embedding's head_dim differs from the cache's",
+                                     {"head_dim": head_dim, "rotary": rotary.head_dim})
+        self.num_pages, self.page_size, self.num_heads, self.head_dim = num_pages, page_size, num_heads, head_dim
+        self.rotary, self.device, self.dtype = rotary, torch.device(device), dtype
+        self.key_pool = torch.zeros(num_pages, num_heads, page_size, head_dim, dtype=dtype, device=device)
+        self.value_pool = torch.zeros_like(self.key_pool)
+        self.lengths: list[int] = []  # tokens of each sequence
+        self.pages: list[list[int]] = []  # its pages, in order
+        self.free_pages = list(range(num_pages - 1, -1, -1))
+
+    # -- sequences ---------------------------------------------------------------
+
+    def reserve(self, new: Sequence[int]) -> PagedBatch:
+        """Make room for ``new[b]`` more tokens of each sequence b (a longer
+        list than before starts new sequences) and return the step's lists.
+        The cache is unchanged when the pool cannot hold them."""
+        new = [int(n) for n in new]
+        if len(new) < len(self.lengths) or any(n < 0 for n in new):
+            raise ShapeError("every sequence needs a number of new tokens, 0 or more", expected=len(self.lengths),
+                             actual=new)
+        grown = [(self.lengths[b] if b < len(self.lengths) else 0) + n for b, n in enumerate(new)]
+        need = [-(-length // self.page_size) for length in grown]
+        more = [n - (len(self.pages[b]) if b < len(self.pages) else 0) for b, n in enumerate(need)]
+        if sum(more) > len(self.free_pages):
+            raise NotInitializedError(f"paged KV cache is full ({self.num_pages} pages)",
+                                      {"needed": sum(more), "free": len(self.free_pages)})
+        self.pages.extend([] for _ in range(len(new) - len(self.pages)))
+        for b, n in enumerate(more):
+            self.pages[b].extend(self.free_pages.pop() for _ in range(n))
+        self.lengths = grown
+        B, W = len(new), max([1, *need])
+        starts = [0]
+        for n in new:
+            starts.append(starts[-1] + n)
+        rows = [p + [0] * (W - len(p)) for p in self.pages]
+        # one copy carries all lists
+        flat = torch.tensor([x for row in rows for x in row] + self.lengths + starts, dtype=torch.int32)
+        if self.device.type == "cuda":
+            flat = flat.pin_memory().to(self.device, non_blocking=True)
+        return PagedBatch(flat[:B * W].view(B, W), flat[B * W:B * W + B], flat[B * W + B:], max([0, *new]),
+                          starts[-1])
+
+    def release(self, sequence: int) -> None:
+        """End a sequence: its pages return to the pool, its place stays, empty."""
+        if not 0 <= sequence < len(self.lengths):
+            raise ShapeError("no such sequence", expected=f"[0, {len(self.lengths)})", actual=sequence)
+        self.free_pages.extend(reversed(self.pages[sequence]))
+        self.pages[sequence] = []
+        self.lengths[sequence] = 0
+
+    # -- packed steps --------------------------------------------------------------
+
+    def attend(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, new: Sequence[int],
+               positions: torch.Tensor | None = None, causal: bool = True, window: int = 0,
+               scale: float | None = None, rotary=None) -> torch.Tensor:
+        """Append the packed new tokens ``key``/``value`` ``[N, H, D]`` (``new[b]``
+        of sequence b) and attend with ``query [N, Hq, D]`` over each
+        sequence's pages; returns ``[N, Hq, D]``.  See
+        :func:`avqa_b200.ops.paged_append` and
+        :func:`~avqa_b200.ops.paged_attention`; ``rotary`` stands in for the
+        cache's own."""
+        from avqa_b200 import ops
+        if rotary is not None and self.rotary is not None:
+            raise ConfigurationError("the cache rotates by its own embedding already")
+        if sum(new) != key.shape[0]:
+            raise ShapeError("the new tokens do not add up to the packed ones", expected=sum(new),
+                             actual=key.shape[0])
+        self._check(key, value)
+        rotary = self.rotary if rotary is None else rotary
+        with self._step(new) as batch:
+            lists = (self.key_pool, self.value_pool, batch.block_table, batch.kv_len, batch.q_start)
+            rotated = ops.paged_append(key, value, *lists, q=query if rotary is not None else None, rotary=rotary,
+                                       positions=positions)
+            return ops.paged_attention(query if rotated is None else rotated, *lists, causal=causal, window=window,
+                                       scale=scale, max_q_len=batch.max_q_len)
+
+    @contextmanager
+    def _step(self, new: Sequence[int]):
+        """:meth:`reserve`, taken back when the step is refused."""
+        lengths, counts = list(self.lengths), [len(p) for p in self.pages]
+        try:
+            yield self.reserve(new)
+        except Exception:
+            for b in range(len(self.pages) - 1, -1, -1):
+                keep = counts[b] if b < len(counts) else 0
+                self.free_pages.extend(reversed(self.pages[b][keep:]))
+                del self.pages[b][keep:]
+            del self.pages[len(counts):]
+            self.lengths = lengths
+            raise
+
+    def _check(self, key: torch.Tensor, value: torch.Tensor) -> None:
+        want = (self.num_heads, self.head_dim)
+        if tuple(key.shape[-2:]) != want or key.shape != value.shape:
+            raise ShapeError(f"key/value shape mismatch: key={tuple(key.shape)}, value={tuple(value.shape)}",
+                             expected=want, actual=tuple(key.shape[-2:]))
+
+    # -- the KVCache interface -----------------------------------------------------------
+
+    def append(self, key: torch.Tensor, value: torch.Tensor) -> None:
+        """Append ``[B, H, T, D]``, T tokens to every sequence."""
+        from avqa_b200 import ops
+        B, _, T, D = key.shape
+        k, v = (x.to(device=self.device, dtype=self.dtype).transpose(1, 2).reshape(B * T, -1, D) for x in (key, value))
+        self._check(k, v)
+        with self._step([T] * B) as batch:
+            ops.paged_append(k, v, self.key_pool, self.value_pool, batch.block_table, batch.kv_len, batch.q_start,
+                             rotary=self.rotary)
+
+    def lookup(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """The keys (as stored: rotated) and values ``[B, H, S, D]``, when every sequence has S tokens."""
+        S = self.size
+        if any(n != S for n in self.lengths):
+            raise ShapeError("sequences of different lengths have no common tensor", expected=S, actual=self.lengths)
+        if S == 0:
+            empty = torch.zeros(max(1, len(self.lengths)), self.num_heads, 0, self.head_dim, dtype=self.dtype,
+                                device=self.device)
+            return empty, empty.clone()
+        pages = torch.tensor(self.pages, device=self.device)
+        return tuple(pool[pages].transpose(1, 2).reshape(len(self.lengths), self.num_heads, -1, self.head_dim)[:, :, :S]
+                     for pool in (self.key_pool, self.value_pool))
+
+    def reset(self) -> None:
+        self.lengths, self.pages = [], []
+        self.free_pages = list(range(self.num_pages - 1, -1, -1))
+        self.quant_states.clear()
+
+    def state_dict(self) -> dict[str, torch.Tensor]:
+        used = [p for pages in self.pages for p in pages]
+        return {"schema_version": torch.tensor(1, dtype=torch.int32),
+                "page_size": torch.tensor(self.page_size, dtype=torch.int32),
+                "num_heads": torch.tensor(self.num_heads, dtype=torch.int32),
+                "head_dim": torch.tensor(self.head_dim, dtype=torch.int32),
+                "lengths": torch.tensor(self.lengths, dtype=torch.int64),
+                "key_pages": self.key_pool[used].clone(), "value_pages": self.value_pool[used].clone()}
+
+    def load_state_dict(self, state: dict[str, torch.Tensor]) -> None:
+        for name in ("page_size", "num_heads", "head_dim"):
+            if name in state and int(state[name]) != getattr(self, name):
+                raise ShapeError(f"{name} mismatch", expected=getattr(self, name), actual=int(state[name]))
+        self.reset()
+        self.reserve(state["lengths"].tolist())
+        used = [p for pages in self.pages for p in pages]
+        self.key_pool[used] = state["key_pages"].to(device=self.device, dtype=self.dtype)
+        self.value_pool[used] = state["value_pages"].to(device=self.device, dtype=self.dtype)
+
+    @property
+    def size(self) -> int:
+        """Tokens of the longest sequence."""
+        return max(self.lengths, default=0)
+
+
+__all__ = ["BlockKVCache", "InMemoryKVCache", "KVCache", "PagedBatch", "PagedKVCache"]

@@ -1,6 +1,7 @@
 // extern "C" entry points (include/avqa_b200.h): argument checks, dtype
 // dispatch and error reporting around the kernel launchers.
 #include <climits>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -13,6 +14,7 @@
 
 #include "../../include/avqa_b200.h"
 #include "avq_kernels.cuh"
+#include "avq_paged.cuh"
 
 namespace {
 
@@ -399,9 +401,234 @@ int avq_reduce_min(const int* v, int n, int* out, void* stream) {
 
 int avq_device_fault(int* code, void* stream) {
   if (!code) return fail(AVQ_ERR_ARG, "avq_device_fault: null pointer");
-  if (avq::read_device_fault(code, (cudaStream_t)stream) != AVQ_OK)
+  cudaStream_t st = (cudaStream_t)stream;
+  int rotary = 0, paged = 0;
+  if (avq::read_device_fault(code, st) != AVQ_OK || avq::read_fault_rotary(&rotary, st) != AVQ_OK ||
+      avq::read_fault_paged(&paged, st) != AVQ_OK)
     return fail(AVQ_ERR_CUDA, "avq_device_fault: %s", cudaGetErrorString(cudaGetLastError()));
+  *code |= rotary | paged;
   return AVQ_OK;
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// Rotary positions, the paged append and paged attention.
+
+namespace {
+
+// The host's frequencies and axes as the kernels take them; AVQ_OK or an error.
+int rotary_spec(const char* what, int D, int rotary_dim, int interleaved, const double* frequencies, const int* axes,
+                int num_axes, int reversed, avq::RotarySpec* spec) {
+  if (D <= 0 || D > 2 * avq::kMaxPairs)
+    return fail(AVQ_ERR_UNSUPPORTED, "%s: head_dim must be in [1, %d], got %d", what, 2 * avq::kMaxPairs, D);
+  if (rotary_dim < 0 || rotary_dim > D || rotary_dim % 2)
+    return fail(AVQ_ERR_ARG, "%s: rotary_dim must be even and in [0, head_dim], got %d", what, rotary_dim);
+  if (num_axes < 1 || num_axes > 255) return fail(AVQ_ERR_ARG, "%s: bad number of axes %d", what, num_axes);
+  if (rotary_dim > 0 && !frequencies) return fail(AVQ_ERR_ARG, "%s: null frequencies", what);
+  std::memset(spec, 0, sizeof(*spec));
+  spec->pairs = rotary_dim / 2;
+  spec->interleaved = interleaved != 0;
+  spec->axes = num_axes;
+  spec->reversed = reversed != 0;
+  for (int i = 0; i < spec->pairs; ++i) {
+    spec->half_turns[i] = frequencies[i] / 3.14159265358979323846;
+    const int ax = axes ? axes[i] : 0;
+    if (ax < 0 || ax >= num_axes)
+      return fail(AVQ_ERR_ARG, "%s: axis %d of frequency %d is not in [0, %d)", what, ax, i, num_axes);
+    spec->axis[i] = (unsigned char)ax;
+  }
+  return AVQ_OK;
+}
+
+avq::Strides2 st2(const long long* s) { return avq::Strides2{s[0], s[1]}; }
+avq::PoolStrides pst(const long long* s) { return avq::PoolStrides{s[0], s[1], s[2]}; }
+
+// The sizes of a packed batch and its pool.
+int paged_sizes(const char* what, int B, int N, int Hkv, int num_pages, int page_size, int table_width) {
+  if (B < 0 || N < 0 || Hkv <= 0 || num_pages < 0 || page_size <= 0 || table_width < 0)
+    return fail(AVQ_ERR_ARG, "%s: bad sizes", what);
+  if ((long long)page_size * table_width > INT_MAX)
+    return fail(AVQ_ERR_ARG, "%s: page_size * table width %lld exceeds INT_MAX", what,
+                (long long)page_size * table_width);
+  return AVQ_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int avq_rotary(int dtype, const void* q, const long long* q_strides, int Hq, const void* k, const long long* k_strides,
+               int Hk, int B, int T, int D, int rotary_dim, int interleaved, const double* frequencies, const int* axes,
+               int num_axes, const void* positions, int position_bytes, const long long* position_strides,
+               long long position0, int reversed, void* q_out, const long long* q_out_strides, void* k_out,
+               const long long* k_out_strides, void* stream) {
+  if (bad_dtype(dtype)) return fail(AVQ_ERR_ARG, "avq_rotary: bad dtype %d", dtype);
+  if (B < 0 || T < 0 || Hq < 0 || Hk < 0) return fail(AVQ_ERR_ARG, "avq_rotary: bad sizes");
+  if ((long long)B * T > INT_MAX) return fail(AVQ_ERR_ARG, "avq_rotary: B*T exceeds INT_MAX");
+  if ((long long)Hq + Hk > 4096) return fail(AVQ_ERR_UNSUPPORTED, "avq_rotary: more than 4096 heads");
+  avq::RotarySpec spec;
+  int rc = rotary_spec("avq_rotary", D, rotary_dim, interleaved, frequencies, axes, num_axes, reversed, &spec);
+  if (rc != AVQ_OK) return rc;
+  if ((long long)B * T == 0 || Hq + Hk == 0) return AVQ_OK;
+  if ((Hq && (!q || !q_strides || !q_out || !q_out_strides)) || (Hk && (!k || !k_strides || !k_out || !k_out_strides)) ||
+      (positions && !position_strides))
+    return fail(AVQ_ERR_ARG, "avq_rotary: null pointer");
+  if (positions && position_bytes != 4 && position_bytes != 8)
+    return fail(AVQ_ERR_ARG, "avq_rotary: positions must have 4 or 8 bytes, got %d", position_bytes);
+  avq::RotaryArgs a{};
+  if (Hq)
+    a.q = avq::RotaryRows{q, q_out, q_strides[0], q_strides[1], q_strides[2], q_out_strides[0], q_out_strides[1],
+                          q_out_strides[2], Hq};
+  if (Hk)
+    a.k = avq::RotaryRows{k, k_out, k_strides[0], k_strides[1], k_strides[2], k_out_strides[0], k_out_strides[1],
+                          k_out_strides[2], Hk};
+  a.B = B;
+  a.T = T;
+  a.D = D;
+  a.positions = positions;
+  a.pos_bytes = position_bytes;
+  if (positions) {
+    a.pa = position_strides[0];
+    a.pb = position_strides[1];
+    a.pt = position_strides[2];
+  }
+  a.pos0 = position0;
+  cudaStream_t st = (cudaStream_t)stream;
+  switch (dtype) {
+    case 0: rc = avq::launch_rotary<avq::DT_F32>(spec, a, st); break;
+    case 1: rc = avq::launch_rotary<avq::DT_BF16>(spec, a, st); break;
+    default: rc = avq::launch_rotary<avq::DT_F16>(spec, a, st); break;
+  }
+  return finish(rc, "avq_rotary");
+}
+
+int avq_paged_append(int dtype, const void* q, const long long* q_strides, int Hq, void* q_out,
+                     const long long* q_out_strides, const void* k, const long long* k_strides, const void* v,
+                     const long long* v_strides, int Hkv, int D, void* key_pool, const long long* key_pool_strides,
+                     void* value_pool, const long long* value_pool_strides, int num_pages, int page_size,
+                     const int* block_table, long long table_stride, int table_width, const int* kv_len,
+                     const int* q_start, int B, int N, int rotary_dim, int interleaved, const double* frequencies,
+                     const int* axes, int num_axes, const void* positions, int position_bytes,
+                     const long long* position_strides, void* stream) {
+  if (bad_dtype(dtype)) return fail(AVQ_ERR_ARG, "avq_paged_append: bad dtype %d", dtype);
+  int rc = paged_sizes("avq_paged_append", B, N, Hkv, num_pages, page_size, table_width);
+  if (rc != AVQ_OK) return rc;
+  if (Hq < 0) return fail(AVQ_ERR_ARG, "avq_paged_append: bad sizes");
+  if ((long long)Hq + 2ll * Hkv > 4096) return fail(AVQ_ERR_UNSUPPORTED, "avq_paged_append: more than 4096 heads");
+  avq::RotarySpec spec;
+  rc = rotary_spec("avq_paged_append", D, rotary_dim, interleaved, frequencies, axes, num_axes, 0, &spec);
+  if (rc != AVQ_OK) return rc;
+  if (B == 0 || N == 0) return AVQ_OK;
+  if (!k || !k_strides || !v || !v_strides || !key_pool_strides || !value_pool_strides || !kv_len || !q_start ||
+      (num_pages && (!key_pool || !value_pool)) || (table_width && !block_table) ||
+      (Hq && (!q || !q_strides || !q_out || !q_out_strides)) || (positions && !position_strides))
+    return fail(AVQ_ERR_ARG, "avq_paged_append: null pointer");
+  if (positions && position_bytes != 4 && position_bytes != 8)
+    return fail(AVQ_ERR_ARG, "avq_paged_append: positions must have 4 or 8 bytes, got %d", position_bytes);
+  avq::PagedAppendArgs a{};
+  if (Hq)
+    a.q = avq::RotaryRows{q, q_out, 0, q_strides[1], q_strides[0], 0, q_out_strides[1], q_out_strides[0], Hq};
+  a.k = k;
+  a.ks = st2(k_strides);
+  a.v = v;
+  a.vs = st2(v_strides);
+  a.kpool = key_pool;
+  a.kps = pst(key_pool_strides);
+  a.vpool = value_pool;
+  a.vps = pst(value_pool_strides);
+  a.table = block_table;
+  a.table_stride = table_stride;
+  a.kv_len = kv_len;
+  a.q_start = q_start;
+  a.B = B;
+  a.N = N;
+  a.Hkv = Hkv;
+  a.D = D;
+  a.num_pages = num_pages;
+  a.page_size = page_size;
+  a.W = table_width;
+  a.positions = positions;
+  a.pos_bytes = position_bytes;
+  if (positions) {
+    a.pa = position_strides[0];
+    a.pt = position_strides[1];
+  }
+  cudaStream_t st = (cudaStream_t)stream;
+  switch (dtype) {
+    case 0: rc = avq::launch_paged_append<avq::DT_F32>(spec, a, st); break;
+    case 1: rc = avq::launch_paged_append<avq::DT_BF16>(spec, a, st); break;
+    default: rc = avq::launch_paged_append<avq::DT_F16>(spec, a, st); break;
+  }
+  return finish(rc, "avq_paged_append");
+}
+
+size_t avq_paged_attention_workspace_size(int dtype, int B, int N, int H, int Hkv, int D, int max_q_len) {
+  if (bad_dtype(dtype) || B < 0 || N < 0 || Hkv <= 0 || H < Hkv || H % Hkv || D <= 0 || D > 256 || max_q_len < 0)
+    return 0;
+  return avq::paged_attn_workspace_bytes(dtype, B, N, H, Hkv, D, max_q_len);
+}
+
+int avq_paged_attention(int dtype, const void* q, const long long* q_strides, int H, const void* key_pool,
+                        const long long* key_pool_strides, const void* value_pool,
+                        const long long* value_pool_strides, int Hkv, int D, int num_pages, int page_size,
+                        const int* block_table, long long table_stride, int table_width, const int* kv_len,
+                        const int* q_start, int B, int N, int causal, int window, float scale, int max_q_len, void* out,
+                        const long long* out_strides, void* workspace, size_t workspace_bytes, void* stream) {
+  if (bad_dtype(dtype)) return fail(AVQ_ERR_ARG, "avq_paged_attention: bad dtype %d", dtype);
+  int rc = paged_sizes("avq_paged_attention", B, N, Hkv, num_pages, page_size, table_width);
+  if (rc != AVQ_OK) return rc;
+  if (D <= 0 || D > 256)
+    return fail(AVQ_ERR_UNSUPPORTED, "avq_paged_attention: head_dim must be in [1, 256], got %d", D);
+  if (H < Hkv || H % Hkv)
+    return fail(AVQ_ERR_ARG, "avq_paged_attention: %d query heads are no multiple of %d key heads", H, Hkv);
+  if (window < 0 || (window > 0 && !causal))
+    return fail(AVQ_ERR_ARG, "avq_paged_attention: a window needs causal, and a size >= 0");
+  if (!std::isfinite(scale)) return fail(AVQ_ERR_ARG, "avq_paged_attention: scale must be finite");
+  if (max_q_len < 0) return fail(AVQ_ERR_ARG, "avq_paged_attention: bad max_q_len %d", max_q_len);
+  if (((long long)N * H + (long long)B * Hkv) > INT_MAX / 2 || (long long)N * H * D > (1ll << 40))
+    return fail(AVQ_ERR_ARG, "avq_paged_attention: N*H = %lld is too large", (long long)N * H);
+  if (B == 0 || N == 0) return AVQ_OK;
+  if (!q || !q_strides || !out || !out_strides || !key_pool_strides || !value_pool_strides || !kv_len || !q_start ||
+      (num_pages && (!key_pool || !value_pool)) || (table_width && !block_table))
+    return fail(AVQ_ERR_ARG, "avq_paged_attention: null pointer");
+  const size_t need = avq::paged_attn_workspace_bytes(dtype, B, N, H, Hkv, D, max_q_len);
+  if (workspace_bytes < need || !workspace)
+    return fail(AVQ_ERR_WORKSPACE, "avq_paged_attention: workspace %zu < %zu bytes", workspace_bytes, need);
+  avq::PagedAttnArgs a{};
+  a.q = q;
+  a.qs = st2(q_strides);
+  a.kpool = key_pool;
+  a.kps = pst(key_pool_strides);
+  a.vpool = value_pool;
+  a.vps = pst(value_pool_strides);
+  a.table = block_table;
+  a.table_stride = table_stride;
+  a.kv_len = kv_len;
+  a.q_start = q_start;
+  a.B = B;
+  a.N = N;
+  a.H = H;
+  a.Hkv = Hkv;
+  a.D = D;
+  a.num_pages = num_pages;
+  a.page_size = page_size;
+  a.W = table_width;
+  a.causal = causal != 0;
+  a.window = window;
+  a.scale_log2 = (float)((double)scale * 1.4426950408889634);
+  a.out = out;
+  a.os = st2(out_strides);
+  a.max_q = max_q_len;
+  a.workspace = workspace;
+  a.workspace_bytes = workspace_bytes;
+  cudaStream_t st = (cudaStream_t)stream;
+  switch (dtype) {
+    case 0: rc = avq::launch_paged_attention<avq::DT_F32>(a, st); break;
+    case 1: rc = avq::launch_paged_attention<avq::DT_BF16>(a, st); break;
+    default: rc = avq::launch_paged_attention<avq::DT_F16>(a, st); break;
+  }
+  return finish(rc, "avq_paged_attention");
 }
 
 }  // extern "C"

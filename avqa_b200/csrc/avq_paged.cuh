@@ -1,0 +1,138 @@
+// Shared declarations of the packed-batch operators: rotary positions
+// (avq_rotary.cu), the paged append (avq_rotary.cu) and attention over a page
+// pool (avq_paged_attn.cu, avq_paged_attn_tc.cu).
+//
+// A packed batch holds the new tokens of all sequences one behind the other:
+// tokens q_start[b] .. q_start[b+1]-1 belong to sequence b, which holds
+// kv_len[b] tokens with them.  New token i of sequence b has the position
+// kv_len[b] - (q_start[b+1] - i); position p lives in slot p % page_size of
+// pool page block_table[b][p / page_size].
+//
+// The lists are device data that the host never reads, so the kernels check
+// them: a sequence whose token range is not inside [0, N] counts as empty, a
+// length beyond the table's row is cut to it, a page outside the pool is
+// neither written nor read, and each of these raises kFaultTables in the
+// device fault word that avq_device_fault reports.
+#pragma once
+
+#include "avq_kernels.cuh"
+
+namespace avq {
+
+constexpr int kFaultTables = 2;  // bit 1 of the device fault record (bit 0: an abandoned wait)
+constexpr int kSms = 148;
+
+struct Strides2 {  // element strides of a packed [N, H, D] operand (token, head)
+  long long t, h;
+};
+struct PoolStrides {  // element strides of a [pages, H, page_size, D] pool (page, head, slot)
+  long long p, h, s;
+};
+
+// ---- rotary positions ---------------------------------------------------------------
+
+constexpr int kMaxPairs = 128;  // head_dim <= 256
+
+struct RotarySpec {
+  int pairs;        // R/2 rotated pairs; dimensions >= 2 * pairs pass through
+  int interleaved;  // pairs (2i, 2i+1) instead of (i, i + R/2)
+  int axes;
+  int reversed;     // rotate by the negative angle (the gradient)
+  double half_turns[kMaxPairs];  // angle per position, in units of pi
+  unsigned char axis[kMaxPairs];
+};
+
+struct RotaryRows {  // rows [b, h, t, 0..D) of one operand and where they go
+  const void* src;
+  void* dst;
+  long long sb, sh, st, db, dh, dt;
+  int heads;
+};
+
+struct RotaryArgs {
+  RotaryRows q, k;   // heads 0: absent
+  int B, T, D;
+  const void* positions;  // int32 / int64 [axes, B, T] by strides, or nullptr: pos0 + t
+  int pos_bytes;
+  long long pa, pb, pt;
+  long long pos0;
+};
+
+struct PagedAppendArgs {
+  RotaryRows q;      // optional (heads 0); sb, db unused
+  const void* k;
+  Strides2 ks;
+  const void* v;
+  Strides2 vs;
+  void* kpool;
+  PoolStrides kps;
+  void* vpool;
+  PoolStrides vps;
+  const int* table;
+  long long table_stride;
+  const int* kv_len;
+  const int* q_start;
+  int B, N, Hkv, D, num_pages, page_size, W;
+  int rotate;
+  const void* positions;  // [axes, N] by strides, or nullptr: the cache position
+  int pos_bytes;
+  long long pa, pt;
+};
+
+template <int DT>
+int launch_rotary(const RotarySpec& spec, const RotaryArgs& a, cudaStream_t st);
+template <int DT>
+int launch_paged_append(const RotarySpec& spec, const PagedAppendArgs& a, cudaStream_t st);
+int read_fault_rotary(int* code, cudaStream_t st);
+
+// ---- paged attention ------------------------------------------------------------------
+
+struct PagedAttnArgs {
+  const void* q;
+  Strides2 qs;
+  const void* kpool;
+  PoolStrides kps;
+  const void* vpool;
+  PoolStrides vps;
+  const int* table;
+  long long table_stride;
+  const int* kv_len;
+  const int* q_start;
+  int B, N, H, Hkv, D, num_pages, page_size, W;
+  int causal, window;
+  float scale_log2;  // softmax scale * log2(e): the kernels work with exp2
+  void* out;
+  Strides2 os;
+  int max_q;         // host bound of the new tokens per sequence, 0: unknown
+  void* workspace;
+  size_t workspace_bytes;
+};
+
+size_t paged_attn_workspace_bytes(int dtype, int B, int N, int H, int Hkv, int D, int max_q);
+template <int DT>
+int launch_paged_attention(const PagedAttnArgs& a, cudaStream_t st);
+int read_fault_paged(int* code, cudaStream_t st);
+
+// ---- device helpers -------------------------------------------------------------------
+
+struct SeqRange {
+  int q0, n;   // first packed token, new tokens
+  int len;     // tokens with the new ones, cut to the table's row
+  int pos0;    // position of the first new token (negative when len < n)
+};
+
+// Sequence b's range, checked; *bad is raised where the lists are not sound.
+__device__ __forceinline__ SeqRange load_seq(const int* q_start, const int* kv_len, int b, int N, long long room,
+                                             bool* bad) {
+  SeqRange s;
+  const int a = q_start[b], e = q_start[b + 1], len = kv_len[b];
+  const bool sound = a >= 0 && e >= a && e <= N;
+  s.q0 = sound ? a : 0;
+  s.n = sound ? e - a : 0;
+  s.len = len < 0 ? 0 : (len > room ? (int)room : len);
+  s.pos0 = len - s.n;
+  *bad = *bad || !sound || len < 0 || len > room;
+  return s;
+}
+
+}  // namespace avq

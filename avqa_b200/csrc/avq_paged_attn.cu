@@ -1,0 +1,571 @@
+// Attention of a packed batch of new tokens over a page pool:
+//
+//   out[i, h] = sum_j p_ij v_j,  p_i = softmax_j(scale * q[i, h] . k_j)
+//
+// over the keys j that token i sees: every key of its sequence, or with
+// `causal` those at its own position and before, or of these the last
+// `window`.  Query head h reads key head h / (H / Hkv).  A token that sees no
+// key gets zeros.
+//
+// paged_attn_mma_kernel: the kernel of few rows (single tokens, short drafts)
+// and of every type and head width.  Its rows are the (token, head of the
+// group) pairs of one sequence and key head, 16 to a CTA, so that one read of
+// a key serves the whole group; the sequence's keys are cut into spans, a CTA
+// each.  Memory bounds it: every key and value is read once, by cp.async into
+// a ring of each warp's own (16 keys a stage), so that no barrier joins the
+// warps until their sums meet at the end.  The span follows from the lengths,
+// which only the device knows: every CTA adds up the batch's work, takes the
+// span that cuts it into about kTargetCtas pieces, and finds its own piece.
+//
+// The scores, the running maximum and sum, and the output are fp32.  bf16 and
+// fp16 multiply on mma.sync with the probabilities rounded to the dtype
+// (their error is of the size of the output's own rounding); fp32 operands
+// are split in two tf32 parts, whose three products carry 22 bits.
+//
+// combine_kernel joins the pieces of a row by their maxima and sums, in the
+// order of the keys.
+#include <algorithm>
+#include <cmath>
+
+#include "avq_mma.cuh"
+#include "avq_paged.cuh"
+
+namespace avq {
+
+namespace {
+
+__device__ int g_fault_tables_paged;
+
+constexpr int kRows = 16, kWarps = 4, kStepKeys = 16;
+constexpr int kTargetCtas = 4 * kSms, kMinSpan = 128;
+
+struct Piece {  // what one CTA works on
+  int b, group, head, span_i;  // sequence, row group, key head, index of the span
+  int nspan;                   // spans of the sequence
+  SeqRange seq;
+  int lo, hi;                  // keys of the span
+  bool found;
+};
+
+// Rows of sequence b that this kernel owns, in groups of kRows.
+__device__ __forceinline__ int row_groups(const PagedAttnArgs& a, int G, int n, int row_max) {
+  const long long rows = (long long)n * G;
+  return rows > row_max ? 0 : (int)((rows + kRows - 1) / kRows);
+}
+
+// First key that any token of the sequence sees.
+__device__ __forceinline__ int first_key(const PagedAttnArgs& a, const SeqRange& s) {
+  if (a.window <= 0) return 0;
+  const int f = s.pos0 - a.window + 1;
+  return f > 0 ? min(f, s.len) : 0;
+}
+
+// Finds the piece of index `at`: a (sequence, key head, span, row group) when `spans`, else a
+// (sequence, key head, row group) with every span of it.  Each warp does the same work.
+__device__ Piece find_piece(const PagedAttnArgs& a, int row_max, long long at, bool spans, bool report,
+                            long long* first_slot) {
+  const int lane = threadIdx.x & 31, G = a.H / a.Hkv;
+  const long long room = (long long)a.W * a.page_size;
+  bool bad = false;
+  long long total = 0;
+  for (int b = lane; b < a.B; b += 32) {
+    const SeqRange s = load_seq(a.q_start, a.kv_len, b, a.N, room, &bad);
+    total += (long long)row_groups(a, G, s.n, row_max) * a.Hkv * (s.len - first_key(a, s));
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  if (report && bad) atomicOr(&g_fault_tables_paged, kFaultTables);
+  long long span = (total + kTargetCtas - 1) / kTargetCtas;
+  span = (max(span, (long long)kMinSpan) + kWarps * kStepKeys - 1) / (kWarps * kStepKeys) * (kWarps * kStepKeys);
+  Piece p;
+  p.found = false;
+  long long before = 0, slots = 0;  // pieces and partial slots of the sequences before
+  for (int b0 = 0; b0 < a.B; b0 += 32) {
+    const int b = b0 + lane;
+    SeqRange s{0, 0, 0, 0};
+    int groups = 0, ns = 0, f = 0;
+    bool ignore = false;
+    if (b < a.B) {
+      s = load_seq(a.q_start, a.kv_len, b, a.N, room, &ignore);
+      groups = row_groups(a, G, s.n, row_max);
+      f = first_key(a, s);
+      ns = max(1, (int)((s.len - f + span - 1) / span));
+    }
+    const long long mine = (long long)groups * a.Hkv * ns, count = spans ? mine : (long long)groups * a.Hkv;
+    long long pre = count, pre_slots = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long x = __shfl_up_sync(0xffffffffu, pre, o), y = __shfl_up_sync(0xffffffffu, pre_slots, o);
+      if (lane >= o) {
+        pre += x;
+        pre_slots += y;
+      }
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, before + pre > at);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      const long long rel = at - before - __shfl_sync(0xffffffffu, pre - count, src);
+      const long long base = slots + __shfl_sync(0xffffffffu, pre_slots - mine, src);
+      p.b = b0 + src;
+      p.seq.q0 = __shfl_sync(0xffffffffu, s.q0, src);
+      p.seq.n = __shfl_sync(0xffffffffu, s.n, src);
+      p.seq.len = __shfl_sync(0xffffffffu, s.len, src);
+      p.seq.pos0 = __shfl_sync(0xffffffffu, s.pos0, src);
+      p.nspan = __shfl_sync(0xffffffffu, ns, src);
+      groups = __shfl_sync(0xffffffffu, groups, src);
+      f = __shfl_sync(0xffffffffu, f, src);
+      // row groups of one span lie side by side: they read the same keys
+      p.group = (int)(rel % groups);
+      const int rest = (int)(rel / groups);
+      p.span_i = spans ? rest % p.nspan : 0;
+      p.head = spans ? rest / p.nspan : rest;
+      p.lo = (int)min((long long)p.seq.len, f + p.span_i * span);
+      p.hi = (int)min((long long)p.seq.len, f + (p.span_i + 1) * span);
+      p.found = true;
+      if (first_slot) *first_slot = base + ((long long)p.head * p.nspan) * groups + p.group;
+      // the slot of span i is first_slot + i * groups
+      if (first_slot && !spans) p.lo = groups;  // the stride, for the caller that walks the spans
+      return p;
+    }
+    before += __shfl_sync(0xffffffffu, pre, 31);
+    slots += __shfl_sync(0xffffffffu, pre_slots, 31);
+  }
+  return p;
+}
+
+// Keys visible to the token at position pos: [first, last).
+__device__ __forceinline__ int2 visible(const PagedAttnArgs& a, int pos, int len) {
+  int last = len, first = 0;
+  if (a.causal) last = pos < 0 ? 0 : min(len, pos + 1);
+  if (a.window > 0) first = max(0, pos - a.window + 1);
+  return make_int2(first, last);
+}
+
+// ---- operands -----------------------------------------------------------------------
+
+template <int DT> struct Operand {
+  using T = typename Storage<DT>::T;
+  static constexpr int kPad = 8;    // a row of D + 8 elements keeps ldmatrix free of bank conflicts
+};
+template <> struct Operand<DT_F32> {
+  using T = float;
+  static constexpr int kPad = 4;    // rows 4 words apart: the key and value fragments' lanes hit 32 banks
+};
+
+__device__ __forceinline__ void mma_tf32(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// x = hi + lo + (less than 2^-22 of x), both tf32.
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+  // an infinity or NaN is all in the high part
+  const float rest = isfinite(x) ? x - __uint_as_float(hi) : 0.f;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(rest));
+}
+__device__ __forceinline__ void mma_split(float* d, const uint32_t* ah, const uint32_t* al, float b0, float b1) {
+  uint32_t h0, l0, h1, l1;
+  split_tf32(b0, h0, l0);
+  split_tf32(b1, h1, l1);
+  mma_tf32(d, al, h0, h1);
+  mma_tf32(d, ah, l0, l1);
+  mma_tf32(d, ah, h0, h1);
+}
+
+template <int DT, int DP>
+constexpr int stage_elems() { return 2 * kStepKeys * (DP + Operand<DT>::kPad); }
+// Stages of a warp's ring: as many as leave room for two CTAs on an SM (one for the widest rows).
+template <int DT, int DP>
+constexpr int ring_stages() {
+  const int row = DP * (int)sizeof(typename Storage<DT>::T);
+  return row <= 128 ? 5 : (row <= 256 ? 3 : (row <= 512 ? 2 : 1));
+}
+template <int DT, int DP>
+constexpr size_t mma_smem() {
+  const size_t T = sizeof(typename Storage<DT>::T);
+  const size_t ring = (size_t)kWarps * ring_stages<DT, DP>() * stage_elems<DT, DP>() * T;
+  const size_t merge = (size_t)kWarps * kRows * (DP + 2) * sizeof(float);
+  return std::max(ring, merge) + (size_t)kRows * (DP + Operand<DT>::kPad) * T;
+}
+
+template <int DT, int DP, bool WIDE>
+__global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const PagedAttnArgs a, int row_max,
+                                                                     float* __restrict__ part) {
+  using T = typename Storage<DT>::T;
+  constexpr int LDS = DP + Operand<DT>::kPad, NT = DP / 8, STAGES = ring_stages<DT, DP>();
+  constexpr int EPC = 16 / (int)sizeof(T), CPR = DP / EPC;  // elements of a 16-byte chunk, chunks of a row
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.H / a.Hkv;
+  asm volatile("griddepcontrol.launch_dependents;");
+  long long slot = 0;
+  const Piece p = find_piece(a, row_max, blockIdx.x, true, blockIdx.x == 0 && warp == 0, &slot);
+  if (!p.found) return;
+  slot += (long long)p.span_i * row_groups(a, G, p.seq.n, row_max);
+  T* sq = reinterpret_cast<T*>(smem_raw);                                  // [kRows][LDS]
+  T* ring = sq + kRows * LDS + warp * STAGES * stage_elems<DT, DP>();       // this warp's stages
+  const int row0 = p.group * kRows, nrow = min(kRows, p.seq.n * G - row0);
+
+  for (int i = tid; i < kRows * DP; i += kWarps * 32) {
+    const int r = i / DP, d = i - r * DP;
+    T x = from_f<DT>(0.f);
+    if (r < nrow && d < a.D) {
+      const int tok = p.seq.q0 + (row0 + r) / G, h = p.head * G + (row0 + r) % G;
+      x = static_cast<const T*>(a.q)[(long long)tok * a.qs.t + (long long)h * a.qs.h + d];
+    }
+    sq[r * LDS + d] = x;
+  }
+
+  // the keys that any row of the group sees
+  const int ra = lane >> 2, rb = ra + 8;
+  const int2 va = visible(a, p.seq.pos0 + (row0 + min(ra, nrow - 1)) / G, p.seq.len);
+  const int2 vb = visible(a, p.seq.pos0 + (row0 + min(rb, nrow - 1)) / G, p.seq.len);
+  const int2 vf = visible(a, p.seq.pos0 + row0 / G, p.seq.len);
+  const int2 vl = visible(a, p.seq.pos0 + (row0 + nrow - 1) / G, p.seq.len);
+  const int lo = max(p.lo, vf.x), hi = min(p.hi, vl.y);
+  const int steps = hi > lo ? (hi - lo + kWarps * kStepKeys - 1) / (kWarps * kStepKeys) : 0;
+  const T* kbase = static_cast<const T*>(a.kpool) + (long long)p.head * a.kps.h;
+  const T* vbase = static_cast<const T*>(a.vpool) + (long long)p.head * a.vps.h;
+  const int* row_table = a.table + (long long)p.b * a.table_stride;
+  bool bad = false;
+
+  // One stage: 16 keys and their values.  Keys outside the span, and pages outside the pool, read as zeros.
+  auto load = [&](int step) {
+    const int k0 = lo + (step * kWarps + warp) * kStepKeys;
+    T* dst = ring + (step % STAGES) * stage_elems<DT, DP>();
+    // each lane looks up one key; the chunks' lanes take the address from it
+    const int key = k0 + (lane & 15);
+    long long ko = -1, vo = -1;
+    if (step < steps && key < hi) {
+      const int page = row_table[key / a.page_size], s = key % a.page_size;
+      if (page >= 0 && page < a.num_pages) {
+        ko = (long long)page * a.kps.p + (long long)s * a.kps.s;
+        vo = (long long)page * a.vps.p + (long long)s * a.vps.s;
+      } else {
+        bad = true;
+      }
+    }
+    if constexpr (WIDE) {
+#pragma unroll
+      for (int i = 0; i < kStepKeys * CPR / 32; ++i) {
+        const int x = i * 32 + lane, r = x / CPR, c = (x % CPR) * EPC;
+        const long long k_at = __shfl_sync(0xffffffffu, ko, r), v_at = __shfl_sync(0xffffffffu, vo, r);
+        const bool ok = k_at >= 0 && c < a.D;
+        cp_async16(dst + r * LDS + c, kbase + (ok ? k_at + c : 0), ok);
+        cp_async16(dst + (kStepKeys + r) * LDS + c, vbase + (ok ? v_at + c : 0), ok);
+      }
+    } else {
+      for (int r = 0; r < kStepKeys; ++r) {
+        const long long k_at = __shfl_sync(0xffffffffu, ko, r), v_at = __shfl_sync(0xffffffffu, vo, r);
+        for (int c = lane; c < DP; c += 32) {
+          const bool ok = k_at >= 0 && c < a.D;
+          dst[r * LDS + c] = ok ? kbase[k_at + c] : from_f<DT>(0.f);
+          dst[(kStepKeys + r) * LDS + c] = ok ? vbase[v_at + c] : from_f<DT>(0.f);
+        }
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) load(i);
+
+  __syncthreads();
+  uint32_t qf[DT == DT_F32 ? 1 : DP / 16][4];
+  if constexpr (DT != DT_F32) {
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk)
+      ldsm_x4(qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3], sq + (lane & 15) * LDS + kk * 16 + (lane >> 4) * 8);
+  }
+  float o[NT][4];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+  float ma = -INFINITY, mb = -INFINITY, la = 0.f, lb = 0.f;
+  const int ct = (lane & 3) * 2;
+
+  for (int step = 0; step < steps; ++step) {
+    load(step + STAGES - 1);
+    cp_async_wait<STAGES - 1>();
+    __syncwarp();
+    const T* sk = ring + (step % STAGES) * stage_elems<DT, DP>();
+    const T* sv = sk + kStepKeys * LDS;
+    float s[2][4];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+    if constexpr (DT != DT_F32) {
+#pragma unroll
+      for (int kk = 0; kk < DP / 16; ++kk) {
+        uint32_t b0, b1, b2, b3;
+        const int qd = lane >> 3;
+        ldsm_x4(b0, b1, b2, b3, sk + ((qd >> 1) * 8 + (lane & 7)) * LDS + kk * 16 + (qd & 1) * 8);
+        mma16816<DT>(s[0], qf[kk], b0, b1);
+        mma16816<DT>(s[1], qf[kk], b2, b3);
+      }
+    } else {
+#pragma unroll 4
+      for (int kk = 0; kk < DP / 8; ++kk) {
+        const int c = kk * 8 + (lane & 3), r = lane >> 2;
+        uint32_t ah[4], al[4];
+        split_tf32(to_f(sq[r * LDS + c]), ah[0], al[0]);
+        split_tf32(to_f(sq[(r + 8) * LDS + c]), ah[1], al[1]);
+        split_tf32(to_f(sq[r * LDS + c + 4]), ah[2], al[2]);
+        split_tf32(to_f(sq[(r + 8) * LDS + c + 4]), ah[3], al[3]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          mma_split(s[j], ah, al, to_f(sk[(j * 8 + r) * LDS + c]), to_f(sk[(j * 8 + r) * LDS + c + 4]));
+      }
+    }
+    const int k0 = lo + (step * kWarps + warp) * kStepKeys;
+    float ta = -INFINITY, tb = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = k0 + j * 8 + ct + (e & 1);
+        const int2 v = e >= 2 ? vb : va;
+        const bool seen = key >= v.x && key < min(v.y, hi);
+        s[j][e] = seen ? s[j][e] * a.scale_log2 : -INFINITY;
+        if (e >= 2) tb = fmaxf(tb, s[j][e]);
+        else ta = fmaxf(ta, s[j][e]);
+        // (fmaxf drops a NaN score; its probability is NaN and carries it into the sum)
+      }
+#pragma unroll
+    for (int of = 1; of <= 2; of <<= 1) {
+      ta = fmaxf(ta, __shfl_xor_sync(0xffffffffu, ta, of));
+      tb = fmaxf(tb, __shfl_xor_sync(0xffffffffu, tb, of));
+    }
+    const float na = fmaxf(ma, ta), nb = fmaxf(mb, tb);
+    if (__any_sync(0xffffffffu, na > ma || nb > mb)) {
+      const float ca = na > ma ? exp2f(ma - na) : 1.f, cb = nb > mb ? exp2f(mb - nb) : 1.f;
+      la *= ca;
+      lb *= cb;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        o[j][0] *= ca;
+        o[j][1] *= ca;
+        o[j][2] *= cb;
+        o[j][3] *= cb;
+      }
+      ma = na;
+      mb = nb;
+    }
+    // a row with no visible key so far keeps probabilities of zero
+    const float xa = ma == -INFINITY ? 0.f : ma, xb = mb == -INFINITY ? 0.f : mb;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      s[j][0] = exp2f(s[j][0] - xa);
+      s[j][1] = exp2f(s[j][1] - xa);
+      s[j][2] = exp2f(s[j][2] - xb);
+      s[j][3] = exp2f(s[j][3] - xb);
+      la += s[j][0] + s[j][1];
+      lb += s[j][2] + s[j][3];
+    }
+    if constexpr (DT != DT_F32) {
+      const uint32_t pf[4] = {pack2<DT>(s[0][0], s[0][1]), pack2<DT>(s[0][2], s[0][3]), pack2<DT>(s[1][0], s[1][1]),
+                              pack2<DT>(s[1][2], s[1][3])};
+#pragma unroll
+      for (int jj = 0; jj < NT / 2; ++jj) {
+        uint32_t b0, b1, b2, b3;
+        const int qd = lane >> 3;
+        ldsm_x4_t(b0, b1, b2, b3, sv + ((qd & 1) * 8 + (lane & 7)) * LDS + jj * 16 + (qd >> 1) * 8);
+        mma16816<DT>(o[2 * jj], pf, b0, b1);
+        mma16816<DT>(o[2 * jj + 1], pf, b2, b3);
+      }
+    } else {
+      // the k index t of the fragment stands for key 2t, t + 4 for key 2t + 1: the accumulators' own layout
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint32_t ph[4], pl[4];
+        split_tf32(s[j][0], ph[0], pl[0]);
+        split_tf32(s[j][2], ph[1], pl[1]);
+        split_tf32(s[j][1], ph[2], pl[2]);
+        split_tf32(s[j][3], ph[3], pl[3]);
+#pragma unroll
+        for (int jj = 0; jj < NT; ++jj) {
+          const T* v0 = sv + (j * 8 + ct) * LDS + jj * 8 + (lane >> 2);
+          mma_split(o[jj], ph, pl, to_f(v0[0]), to_f(v0[LDS]));
+        }
+      }
+    }
+    __syncwarp();
+  }
+  cp_async_wait<0>();
+#pragma unroll
+  for (int of = 1; of <= 2; of <<= 1) {
+    la += __shfl_xor_sync(0xffffffffu, la, of);
+    lb += __shfl_xor_sync(0xffffffffu, lb, of);
+  }
+  if (bad) atomicOr(&g_fault_tables_paged, kFaultTables);
+  __syncthreads();  // every warp is done with its ring
+
+  // the warps' sums meet: one row's maximum, then the scaled sums
+  float* sm = reinterpret_cast<float*>(sq + kRows * LDS);  // [kWarps][kRows] maxima, then sums, then outputs
+  float* sl = sm + kWarps * kRows;
+  float* so = sl + kWarps * kRows;  // [kWarps][kRows][DP]
+  if ((lane & 3) == 0) {
+    sm[warp * kRows + ra] = ma;
+    sm[warp * kRows + rb] = mb;
+  }
+  __syncthreads();
+  float Ma = sm[ra], Mb = sm[rb];
+#pragma unroll
+  for (int w = 1; w < kWarps; ++w) {
+    Ma = fmaxf(Ma, sm[w * kRows + ra]);
+    Mb = fmaxf(Mb, sm[w * kRows + rb]);
+  }
+  const float fa = ma == -INFINITY ? 0.f : exp2f(ma - Ma), fb = mb == -INFINITY ? 0.f : exp2f(mb - Mb);
+  // (a maximum of +inf gives NaN here and in the probabilities, as a softmax over +inf does)
+  if ((lane & 3) == 0) {
+    sl[warp * kRows + ra] = la * fa;
+    sl[warp * kRows + rb] = lb * fb;
+  }
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    float* w = so + (warp * kRows + ra) * DP + j * 8 + ct;
+    *reinterpret_cast<float2*>(w) = make_float2(o[j][0] * fa, o[j][1] * fa);
+    *reinterpret_cast<float2*>(w + 8 * DP) = make_float2(o[j][2] * fb, o[j][3] * fb);
+  }
+  __syncthreads();
+  for (int i = tid; i < nrow * DP; i += kWarps * 32) {
+    const int r = i / DP, d = i - r * DP;
+    if (d >= a.D) continue;
+    float x = 0.f, l = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      x += so[(w * kRows + r) * DP + d];
+      l += sl[w * kRows + r];
+    }
+    if (p.nspan == 1) {
+      const int tok = p.seq.q0 + (row0 + r) / G, h = p.head * G + (row0 + r) % G;
+      const int2 v = visible(a, p.seq.pos0 + (row0 + r) / G, p.seq.len);
+      // a row that sees no key is zero; one whose keys all score -inf is 0 / 0
+      static_cast<T*>(a.out)[(long long)tok * a.os.t + (long long)h * a.os.h + d] =
+          from_f<DT>(v.y > v.x ? x / l : 0.f);
+    } else {
+      float* w = part + slot * (kRows * (DP + 2));
+      w[r * DP + d] = x;
+      if (d == 0) {
+        float M = sm[r];
+        for (int k = 1; k < kWarps; ++k) M = fmaxf(M, sm[k * kRows + r]);
+        w[kRows * DP + r] = M;
+        w[kRows * DP + kRows + r] = l;
+      }
+    }
+  }
+}
+
+// Joins the spans of one (sequence, key head, row group).
+template <int DT, int DP>
+__global__ void __launch_bounds__(128) combine_kernel(const PagedAttnArgs a, int row_max, long long pieces,
+                                                      const float* __restrict__ part) {
+  using T = typename Storage<DT>::T;
+  const int G = a.H / a.Hkv;
+  long long slot = 0;
+  const Piece p = find_piece(a, row_max, blockIdx.x, false, false, &slot);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!p.found || p.nspan == 1) return;
+  const int stride = p.lo, row0 = p.group * kRows, nrow = min(kRows, p.seq.n * G - row0);
+  // token ranges that overlap could name more pieces than there are slots
+  if (slot + (long long)(p.nspan - 1) * stride >= pieces) return;
+  const long long step = (long long)stride * (kRows * (DP + 2));
+  const float* base = part + slot * (kRows * (DP + 2));
+  for (int i = threadIdx.x; i < nrow * DP; i += 128) {
+    const int r = i / DP, d = i - r * DP;
+    if (d >= a.D) continue;
+    float M = -INFINITY;
+    for (int s = 0; s < p.nspan; ++s) M = fmaxf(M, base[s * step + kRows * DP + r]);
+    float x = 0.f, l = 0.f;
+    for (int s = 0; s < p.nspan; ++s) {
+      const float* w = base + s * step;
+      const float m = w[kRows * DP + r], f = m == -INFINITY ? 0.f : exp2f(m - M);
+      // a span whose rows saw nothing (or only -inf) adds nothing
+      if (m == -INFINITY && w[kRows * DP + kRows + r] == 0.f) continue;
+      x = fmaf(w[r * DP + d], f, x);
+      l = fmaf(w[kRows * DP + kRows + r], f, l);
+    }
+    const int tok = p.seq.q0 + (row0 + r) / G, h = p.head * G + (row0 + r) % G;
+    const int2 v = visible(a, p.seq.pos0 + (row0 + r) / G, p.seq.len);
+    static_cast<T*>(a.out)[(long long)tok * a.os.t + (long long)h * a.os.h + d] = from_f<DT>(v.y > v.x ? x / l : 0.f);
+  }
+}
+
+// CTAs that hold every piece: the target, one partly filled span for each (row group, key head).
+long long most_items(int B, int N, int H, int Hkv) {
+  const long long G = H / Hkv;
+  return ((long long)N * G / kRows + B) * Hkv;
+}
+long long most_pieces(int B, int N, int H, int Hkv) { return most_items(B, N, H, Hkv) + kTargetCtas; }
+
+int padded_dim(int D) { return D <= 64 ? 64 : (D <= 128 ? 128 : 256); }
+
+bool wide_rows(const void* p, std::initializer_list<long long> strides, int elem) {
+  if (reinterpret_cast<uintptr_t>(p) % 16) return false;
+  for (long long s : strides)
+    if (s * elem % 16) return false;
+  return true;
+}
+
+template <int DT, int DP>
+int launch_mma(const PagedAttnArgs& a, int row_max, cudaStream_t st) {
+  using T = typename Storage<DT>::T;
+  const int E = (int)sizeof(T);
+  const bool wide = a.D * E % 16 == 0 && wide_rows(a.kpool, {a.kps.p, a.kps.h, a.kps.s}, E) &&
+                    wide_rows(a.vpool, {a.vps.p, a.vps.h, a.vps.s}, E);
+  const long long pieces = most_pieces(a.B, a.N, a.H, a.Hkv), items = most_items(a.B, a.N, a.H, a.Hkv);
+  float* part = static_cast<float*>(a.workspace);
+  const size_t smem = mma_smem<DT, DP>();
+  auto kfn = wide ? paged_attn_mma_kernel<DT, DP, true> : paged_attn_mma_kernel<DT, DP, false>;
+  if (cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return AVQ_ERR_CUDA;
+  {
+    AVQ_TIMED("paged_attn", st);
+    kfn<<<(unsigned)pieces, kWarps * 32, smem, st>>>(a, row_max, part);
+    if (cudaPeekAtLastError() != cudaSuccess) return AVQ_ERR_CUDA;
+  }
+  AVQ_TIMED("paged_combine", st);
+  // the launch overlaps the attention kernel's end; the kernel waits for its results itself
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)items);
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, combine_kernel<DT, DP>, a, row_max, pieces, (const float*)part) == cudaSuccess
+             ? AVQ_OK
+             : AVQ_ERR_CUDA;
+}
+
+}  // namespace
+
+size_t paged_attn_workspace_bytes(int dtype, int B, int N, int H, int Hkv, int D, int max_q) {
+  const int DP = padded_dim(D);
+  return align_up((size_t)most_pieces(B, N, H, Hkv) * kRows * (DP + 2) * sizeof(float));
+}
+
+template <int DT>
+int launch_paged_attention(const PagedAttnArgs& a, cudaStream_t st) {
+  if (a.B == 0 || a.N == 0) return AVQ_OK;
+  if (a.D <= 64) return launch_mma<DT, 64>(a, 1 << 30, st);
+  if (a.D <= 128) return launch_mma<DT, 128>(a, 1 << 30, st);
+  return launch_mma<DT, 256>(a, 1 << 30, st);
+}
+
+int read_fault_paged(int* code, cudaStream_t st) {
+  int zero = 0;
+  if (cudaMemcpyFromSymbolAsync(code, g_fault_tables_paged, sizeof(int), 0, cudaMemcpyDeviceToHost, st) !=
+          cudaSuccess ||
+      cudaMemcpyToSymbolAsync(g_fault_tables_paged, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st) !=
+          cudaSuccess ||
+      cudaStreamSynchronize(st) != cudaSuccess)
+    return AVQ_ERR_CUDA;
+  return AVQ_OK;
+}
+
+template int launch_paged_attention<DT_F32>(const PagedAttnArgs&, cudaStream_t);
+template int launch_paged_attention<DT_BF16>(const PagedAttnArgs&, cudaStream_t);
+template int launch_paged_attention<DT_F16>(const PagedAttnArgs&, cudaStream_t);
+
+}  // namespace avq

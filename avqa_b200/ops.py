@@ -11,12 +11,13 @@ from __future__ import annotations
 
 from dataclasses import dataclass
 
+import contextlib
 import ctypes
 
 import torch
 
 from avqa_b200 import _lib
-from avqa_b200.exceptions import BackendError, DeviceError
+from avqa_b200.exceptions import BackendError, DeviceError, DtypeError, ShapeError
 
 
 def _cuda(t: torch.Tensor, name: str) -> None:
@@ -319,5 +320,216 @@ def forward(q: torch.Tensor, cb: PreparedCodebook, st: QuantState, P: int, passe
     return out, diag
 
 
+# -- rotary positions, the paged append and paged attention ---------------------------
+
+_POSITION_BYTES = {torch.int32: 4, torch.int64: 8}
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on_device(dev: torch.device):
+    """A guard that makes ``dev`` current where it is not (a launch goes to the current device)."""
+    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _same(name: str, t: torch.Tensor, dev: torch.device, dtype: torch.dtype | None = None) -> None:
+    if t.device != dev:
+        raise DeviceError(f"{name} must be on the same device", expected=str(dev), actual=str(t.device))
+    if dtype is not None and t.dtype != dtype:
+        raise DtypeError(f"{name} has the wrong dtype", expected=str(dtype), actual=str(t.dtype))
+
+
+def _positions_operand(positions: torch.Tensor | None, axes: int, B: int, T: int, dev: torch.device):
+    """(pointer, bytes, ctypes strides {axis, b, t}) of positions ``[T]``, ``[B, T]`` with one
+    axis, or ``[axes, T]`` / ``[axes, B, T]``."""
+    if positions is None:
+        return None, 0, None
+    _same("positions", positions, dev)
+    nbytes = _POSITION_BYTES.get(positions.dtype)
+    if nbytes is None:
+        raise DtypeError("positions must be int32 or int64", expected="int32 | int64", actual=str(positions.dtype))
+    shape, st = tuple(positions.shape), positions.stride()
+    ok = 1 <= len(shape) <= 3 and shape[-1] == T
+    if len(shape) == 1:
+        strides = (0, 0, st[0])
+    elif len(shape) == 2 and axes == 1:
+        ok = ok and shape[0] in (1, B)
+        strides = (0, st[0] if shape[0] > 1 else 0, st[1])
+    elif len(shape) == 2:
+        ok = ok and shape[0] == axes
+        strides = (st[0], 0, st[1])
+    elif len(shape) == 3:
+        ok = ok and shape[0] == axes and shape[1] in (1, B)
+        strides = (st[0], st[1] if shape[1] > 1 else 0, st[2])
+    if not ok:
+        raise ShapeError("positions do not fit the tokens", expected=f"[{T}] or [{axes} axes, {B}, {T}]", actual=shape)
+    return positions.data_ptr(), nbytes, (ctypes.c_longlong * 3)(*strides)
+
+
+def rotary(embedding, q: torch.Tensor, k: torch.Tensor | None = None, positions: torch.Tensor | None = None,
+           offset: int = 0, reverse: bool = False) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Rotate ``q [B, H, T, D]`` and ``k [B, Hk, T, D]`` (or ``None``) by a
+    :class:`~avqa_b200.rotary.RotaryEmbedding` (by the negative angle with
+    ``reverse``) into new tensors; no gradient is recorded here."""
+    lib = _lib.load()
+    _cuda(q, "query")
+    dev = q.device
+    B, H, T, D = q.shape
+    q_out = torch.empty_like(q)
+    kp = ks = kop = kos = k_out = None
+    Hk = 0
+    if k is not None:
+        _same("key", k, dev, q.dtype)
+        k_out = torch.empty_like(k)
+        kp, ks, kop, kos, Hk = k.data_ptr(), _lib.strides3(k), k_out.data_ptr(), _lib.strides3(k_out), k.shape[1]
+    pos, pos_bytes, pos_strides = _positions_operand(positions, embedding.num_axes, B, T, dev)
+    with _on_device(dev):
+        rc = lib.avq_rotary(_lib.dtype_code(q.dtype), q.data_ptr(), _lib.strides3(q), H, kp, ks, Hk, B, T, D,
+                            embedding.rotary_dim, embedding.interleaved, embedding.c_frequencies, embedding.c_axes,
+                            embedding.num_axes, pos, pos_bytes, pos_strides, offset, reverse, q_out.data_ptr(),
+                            _lib.strides3(q_out), kop, kos, _lib.stream_of(dev))
+    _lib.check(rc, "avq_rotary")
+    return q_out, k_out
+
+
+def _packed(t: torch.Tensor, name: str, heads: int | None, tokens: int | None, dim: int | None):
+    """Element strides (token, head) of a packed ``[N, H, D]`` operand."""
+    shape = t.shape
+    if t.dim() != 3 or (heads is not None and shape[1] != heads) or (tokens is not None and shape[0] != tokens) or (
+            dim is not None and shape[2] != dim):
+        raise ShapeError(f"{name} must be packed [tokens, heads, head_dim]", expected=(tokens, heads, dim),
+                         actual=tuple(shape))
+    if shape[2] > 1 and t.stride(2) != 1:
+        raise BackendError(f"{name} must have a contiguous last dimension", {"stride": tuple(t.stride())})
+    return (ctypes.c_longlong * 2)(t.stride(0), t.stride(1))
+
+
+def _pool(key_pool: torch.Tensor, value_pool: torch.Tensor, block_table: torch.Tensor, kv_len: torch.Tensor,
+          q_start: torch.Tensor, dev: torch.device, dtype: torch.dtype, D: int) -> tuple[int, int, int, int]:
+    """Check a page pool and a batch's lists; (batch, heads, pages, page size)."""
+    if key_pool.dim() != 4 or key_pool.shape[3] != D or value_pool.shape != key_pool.shape:
+        raise ShapeError("pools must be [pages, heads, page_size, head_dim], the values' like the keys'",
+                         expected=("pages", "heads", "page_size", D),
+                         actual=(tuple(key_pool.shape), tuple(value_pool.shape)))
+    for name, t in (("key_pool", key_pool), ("value_pool", value_pool)):
+        _same(name, t, dev, dtype)
+    for name, t in (("block_table", block_table), ("kv_len", kv_len), ("q_start", q_start)):
+        _same(name, t, dev, torch.int32)
+    B = kv_len.shape[0] if kv_len.dim() == 1 else -1
+    if block_table.dim() != 2 or tuple(q_start.shape) != (B + 1,) or block_table.shape[0] != B:
+        raise ShapeError("the batch's lists disagree: block_table [B, W], kv_len [B], q_start [B + 1]",
+                         expected=("[B, W]", "[B]", "[B + 1]"),
+                         actual=(tuple(block_table.shape), tuple(kv_len.shape), tuple(q_start.shape)))
+    if (block_table.shape[1] > 1 and block_table.stride(1) != 1) or (B > 1 and kv_len.stride(0) != 1) or (
+            q_start.stride(0) != 1):
+        raise BackendError("the batch's lists must be contiguous along their last dimension")
+    pages, heads, page_size, _ = key_pool.shape
+    return B, heads, pages, page_size
+
+
+def paged_append(k: torch.Tensor, v: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor,
+                 block_table: torch.Tensor, kv_len: torch.Tensor, q_start: torch.Tensor,
+                 q: torch.Tensor | None = None, rotary=None, positions: torch.Tensor | None = None,
+                 q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Write a packed batch's new ``k``/``v`` ``[N, Hkv, D]`` to their pages,
+    the keys rotated on the way when ``rotary`` (a
+    :class:`~avqa_b200.rotary.RotaryEmbedding`) is given; ``q [N, H, D]`` is
+    rotated in the same launch and returned (in ``q_out`` if given, which may
+    be ``q``).
+
+    ``key_pool``/``value_pool`` ``[pages, Hkv, page_size, D]`` (any page, head
+    and slot strides); ``block_table [B, W]``, ``kv_len [B]`` (with the new
+    tokens) and ``q_start [B + 1]`` are int32 on the device.  New token i of n
+    is at position ``kv_len - n + i``, which ``positions`` (``[N]``, or
+    ``[axes, N]``) replaces for the rotation only.  Tokens behind
+    ``q_start[B]`` are left alone.  Serving only: no gradient is recorded."""
+    lib = _lib.load()
+    _cuda(k, "key")
+    dev, dt = k.device, k.dtype
+    ks = _packed(k, "key", None, None, None)
+    N, Hkv, D = k.shape
+    _same("value", v, dev, dt)
+    vs = _packed(v, "value", Hkv, N, D)
+    B, heads, pages, page_size = _pool(key_pool, value_pool, block_table, kv_len, q_start, dev, dt, D)
+    if heads != Hkv:
+        raise ShapeError("the pool's heads differ from the keys'", expected=heads, actual=Hkv)
+    H, qp, qs, qop, qos = 0, None, None, None, None
+    if q is not None:
+        _same("query", q, dev, dt)
+        qs = _packed(q, "query", None, N, D)
+        if q_out is None:
+            q_out = torch.empty_like(q)
+        _same("q_out", q_out, dev, dt)
+        qos = _packed(q_out, "q_out", q.shape[1], N, D)
+        H, qp, qop = q.shape[1], q.data_ptr(), q_out.data_ptr()
+    elif q_out is not None:
+        raise BackendError("q_out needs q")
+    R, inter, freq, axes, num_axes = 0, False, None, None, 1
+    if rotary is not None:
+        if rotary.head_dim != D:
+            raise ShapeError("the rotary embedding's head_dim differs from the keys'", expected=rotary.head_dim,
+                             actual=D)
+        R, inter, num_axes = rotary.rotary_dim, rotary.interleaved, rotary.num_axes
+        freq, axes = rotary.c_frequencies, rotary.c_axes
+    elif positions is not None:
+        raise BackendError("positions need a rotary embedding")
+    pos, pos_bytes, pos_st = _positions_operand(positions, num_axes, 1, N, dev)
+    if pos_st is not None:
+        pos_st = (ctypes.c_longlong * 2)(pos_st[0], pos_st[2])
+    with _on_device(dev):
+        rc = lib.avq_paged_append(_lib.dtype_code(dt), qp, qs, H, qop, qos, k.data_ptr(), ks, v.data_ptr(), vs, Hkv, D,
+                                  key_pool.data_ptr(), _lib.strides3(key_pool), value_pool.data_ptr(),
+                                  _lib.strides3(value_pool), pages, page_size, block_table.data_ptr(),
+                                  block_table.stride(0), block_table.shape[1], kv_len.data_ptr(), q_start.data_ptr(),
+                                  B, N, R, inter, freq, axes, num_axes, pos, pos_bytes, pos_st, _lib.stream_of(dev))
+    _lib.check(rc, "avq_paged_append")
+    return q_out
+
+
+def paged_attention(q: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor, block_table: torch.Tensor,
+                    kv_len: torch.Tensor, q_start: torch.Tensor, causal: bool = True, window: int = 0,
+                    scale: float | None = None, max_q_len: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of a packed batch's new tokens ``q [N, H, D]`` over their
+    sequences' pages (operands as in :func:`paged_append`, the new tokens' keys
+    and values appended already): ``softmax(scale q k^T) v`` with ``scale``
+    ``D ** -0.5`` by default.
+
+    Each token sees its sequence's keys, with ``causal`` those at its position
+    and before, with ``window > 0`` the last ``window`` of these.  ``H`` may be
+    a multiple of the pool's heads (query head h reads key head
+    ``h // (H // Hkv)``).  A token that sees no key gets zeros; rows behind
+    ``q_start[B]`` are left as they are in ``out``.  ``max_q_len``: the most new
+    tokens of a sequence, if known; it only steers the choice of kernels.
+    Probabilities are rounded to the dtype for the product with the values
+    (bf16, fp16), all sums are fp32.  Serving only: no gradient is recorded."""
+    lib = _lib.load()
+    _cuda(q, "query")
+    dev, dt = q.device, q.dtype
+    qs = _packed(q, "query", None, None, None)
+    N, H, D = q.shape
+    B, Hkv, pages, page_size = _pool(key_pool, value_pool, block_table, kv_len, q_start, dev, dt, D)
+    if Hkv == 0 or H == 0 or H % Hkv:
+        raise ShapeError("query heads must be a multiple of the pool's heads", expected=f"n * {Hkv}", actual=H)
+    if out is None:
+        out = torch.empty(N, H, D, dtype=dt, device=dev)
+    else:
+        _same("out", out, dev, dt)
+    os_ = _packed(out, "out", H, N, D)
+    code = _lib.dtype_code(dt)
+    ws_bytes = lib.avq_paged_attention_workspace_size(code, B, N, H, Hkv, D, max_q_len)
+    ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=dev)
+    with _on_device(dev):
+        rc = lib.avq_paged_attention(code, q.data_ptr(), qs, H, key_pool.data_ptr(), _lib.strides3(key_pool),
+                                     value_pool.data_ptr(), _lib.strides3(value_pool), Hkv, D, pages, page_size,
+                                     block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+                                     kv_len.data_ptr(), q_start.data_ptr(), B, N, causal, window,
+                                     D ** -0.5 if scale is None else scale, max_q_len, out.data_ptr(), os_,
+                                     ws.data_ptr(), ws_bytes, _lib.stream_of(dev))
+    _lib.check(rc, "avq_paged_attention")
+    return out
+
+
 __all__ = ["ForwardDiagnostics", "PreparedCodebook", "QuantState", "append", "bcar_update", "codeword_presence",
-           "dense_attention", "forward", "pass_caps", "prepare_codebook", "quantize"]
+           "dense_attention", "forward", "paged_append", "paged_attention", "pass_caps", "prepare_codebook", "quantize",
+           "rotary"]

@@ -246,6 +246,12 @@ def algorithmic_work(w, B: int, T: int | None = None, decode: bool = False, sel_
             # (read + write) and their dtype copies written, the page slots
             "append": ("hbm", G * T * (2 * D * es + 2 * 2 * D * 4 + 2 * D * es + 2 * D * es)),
             "route": ("hbm", G * M0 * 8),
+            # the dense path over a page pool: rotated q and k, the appended rows, every cached key and value, the
+            # joined pieces of the outputs
+            "rotary": ("hbm", 2 * 2 * G * T * D * es),
+            "paged_append": ("hbm", 2 * 3 * G * T * D * es),
+            "paged_attn": ("hbm", 2 * G * (S + T) * D * es),
+            "paged_combine": ("hbm", G * T * D * (4 + es)),
         }
     return {
         "parent_attn": ("tensor", 4.0 * G * T * M0 * D),          # q.P^T and e @ V (mma.sync kernel)

@@ -31,6 +31,11 @@
  *   avq_stream_extend     StreamingVQBuffer.extend, streaming_vq.py:109-229
  *   avq_dense_attention   TorchBackend.naive_attention / online_softmax_attention,
  *                         backend.py:105-156, 190-203
+ *   avq_rotary, avq_paged_append, avq_paged_attention
+ *                         no counterpart: rotary positions, and a page pool of
+ *                         ragged sequences with grouped key heads for the
+ *                         dense path (the reference's PagedKVCache, cache.py:
+ *                         262-331, keeps one page list for a whole batch)
  *   avq_device_fault      no counterpart: device-side fault record of the bounded waits
  *   avq_quantize_noalloc  no counterpart: avq_quantize with its scratch in a fixed
  *                         device array, for hosts that cannot allocate
@@ -251,11 +256,81 @@ int avq_append(int dtype, const void* k, const long long* k_strides, const void*
 /* *out = min(v[0..n)). */
 int avq_reduce_min(const int* v, int n, int* out, void* stream);
 
+/* Rotary positions: rotates q [B,Hq,T,D] and k [B,Hk,T,D] (strides as
+ * avq_quantize; Hq or Hk 0: absent) into q_out and k_out in one launch,
+ *
+ *   y_a = x_a cos t - x_b sin t,  y_b = x_a sin t + x_b cos t,
+ *   t_i = position(axis_i) * frequencies[i]
+ *
+ * for the rotary_dim / 2 pairs (a, b) = (i, i + rotary_dim/2), or with
+ * `interleaved` (2i, 2i+1); dimensions from rotary_dim on are copied.  Outputs
+ * may be their inputs (same pointer and strides).  frequencies (fp64, radians
+ * per position) and axes (NULL: axis 0) are HOST arrays of rotary_dim/2
+ * values, read during the call.  positions: device int32 / int64
+ * (position_bytes 4 / 8) with element strides {axis, b, t} (0 broadcasts), or
+ * NULL: position0 + t on every axis.  reversed: rotate by -t, which is the
+ * gradient.  Angles are fp64, products fp32, each output is rounded once.
+ * D <= 256, Hq + Hk <= 4096. */
+int avq_rotary(int dtype, const void* q, const long long* q_strides, int Hq, const void* k, const long long* k_strides,
+               int Hk, int B, int T, int D, int rotary_dim, int interleaved, const double* frequencies, const int* axes,
+               int num_axes, const void* positions, int position_bytes, const long long* position_strides,
+               long long position0, int reversed, void* q_out, const long long* q_out_strides, void* k_out,
+               const long long* k_out_strides, void* stream);
+
+/* Append a packed batch to a page pool, rotating on the way.
+ *
+ * A packed batch: N tokens, of which q_start[b] .. q_start[b+1]-1 (device
+ * int32 [B+1]) are the new tokens of sequence b; kv_len[b] (device int32) is
+ * its token count WITH them, so new token i of n has the position
+ * p = kv_len[b] - n + i.  Position p lives in slot p % page_size of page
+ * block_table[b * table_stride + p / page_size] (device int32, table_width
+ * entries a row).  Pools are [num_pages, Hkv, page_size, D] by element strides
+ * {page, head, slot}, packed operands [N, H, D] by {token, head}, unit stride
+ * along D.
+ *
+ * Writes k rotated (as avq_rotary; rotary_dim 0: unchanged) and v to their
+ * slots, and with Hq > 0 also q rotated to q_out (which may be q).  positions:
+ * NULL for p on every axis, or device integers with strides {axis, token}.
+ * Tokens behind q_start[B] are left alone.  A token whose position is negative
+ * or beyond the table's row, or whose page is not in the pool, is not written;
+ * all but the negative ones raise bit 1 of the device fault record, as do
+ * lists that are not sound (see avq_device_fault). */
+int avq_paged_append(int dtype, const void* q, const long long* q_strides, int Hq, void* q_out,
+                     const long long* q_out_strides, const void* k, const long long* k_strides, const void* v,
+                     const long long* v_strides, int Hkv, int D, void* key_pool, const long long* key_pool_strides,
+                     void* value_pool, const long long* value_pool_strides, int num_pages, int page_size,
+                     const int* block_table, long long table_stride, int table_width, const int* kv_len,
+                     const int* q_start, int B, int N, int rotary_dim, int interleaved, const double* frequencies,
+                     const int* axes, int num_axes, const void* positions, int position_bytes,
+                     const long long* position_strides, void* stream);
+
+size_t avq_paged_attention_workspace_size(int dtype, int B, int N, int H, int Hkv, int D, int max_q_len);
+
+/* Attention of a packed batch (see avq_paged_append) over its pages:
+ * out[i,h] = softmax(scale * q[i,h] . k_j) v_j over the keys j of i's sequence,
+ * with causal those at i's position and before, with window > 0 of these the
+ * last `window`.  H is a multiple of Hkv; query head h reads key head
+ * h / (H / Hkv).  A token that sees no key gets zeros; tokens behind
+ * q_start[B] are left alone.  max_q_len: a bound of the new tokens per
+ * sequence, or 0; it only steers the choice of kernels, a wrong one costs time
+ * and never the result.  Keys on pages outside the pool count as zeros and raise
+ * bit 1 of the device fault record.  D <= 256.  workspace:
+ * avq_paged_attention_workspace_size(same sizes, same max_q_len) bytes, used
+ * only during the call. */
+int avq_paged_attention(int dtype, const void* q, const long long* q_strides, int H, const void* key_pool,
+                        const long long* key_pool_strides, const void* value_pool,
+                        const long long* value_pool_strides, int Hkv, int D, int num_pages, int page_size,
+                        const int* block_table, long long table_stride, int table_width, const int* kv_len,
+                        const int* q_start, int B, int N, int causal, int window, float scale, int max_q_len, void* out,
+                        const long long* out_strides, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Read and clear the device-side fault record, after synchronizing `stream`.
- * *code receives 0, or a nonzero bit set by a kernel that abandoned a
- * bounded wait (about one second) on one of its own barriers; the kernel
- * then released its resources and returned with undefined outputs.  No
- * counterpart in the reference (its CPU kernels have no asynchronous waits). */
+ * *code receives 0, or bits: bit 0, a kernel abandoned a bounded wait (about
+ * one second) on one of its own barriers, released its resources and returned
+ * with undefined outputs; bit 1, a packed batch's device lists were not sound
+ * (a token range outside the batch, a length beyond the table's row, a page
+ * outside the pool).  No counterpart in the reference (its CPU kernels have no
+ * asynchronous waits). */
 int avq_device_fault(int* code, void* stream);
 
 /* Per-kernel device timing (no counterpart in the reference; measurement
