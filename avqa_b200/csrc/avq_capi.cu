@@ -402,11 +402,11 @@ int avq_reduce_min(const int* v, int n, int* out, void* stream) {
 int avq_device_fault(int* code, void* stream) {
   if (!code) return fail(AVQ_ERR_ARG, "avq_device_fault: null pointer");
   cudaStream_t st = (cudaStream_t)stream;
-  int rotary = 0, paged = 0;
+  int rotary = 0, paged = 0, paged_tc = 0;
   if (avq::read_device_fault(code, st) != AVQ_OK || avq::read_fault_rotary(&rotary, st) != AVQ_OK ||
-      avq::read_fault_paged(&paged, st) != AVQ_OK)
+      avq::read_fault_paged(&paged, st) != AVQ_OK || avq::read_fault_paged_tc(&paged_tc, st) != AVQ_OK)
     return fail(AVQ_ERR_CUDA, "avq_device_fault: %s", cudaGetErrorString(cudaGetLastError()));
-  *code |= rotary | paged;
+  *code |= rotary | paged | paged_tc;
   return AVQ_OK;
 }
 

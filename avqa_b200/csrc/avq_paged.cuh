@@ -108,6 +108,13 @@ struct PagedAttnArgs {
   size_t workspace_bytes;
 };
 
+// The tcgen05 kernel (bf16, fp16; head_dim 64 and 128; 16-byte rows; scale > 0) for the sequences with more than
+// row_min rows (new tokens x heads of a group).
+size_t paged_attn_tc_workspace_bytes(int B, int N, int H, int Hkv, int D, int row_min);
+template <int DT>
+int launch_paged_attention_tc(const PagedAttnArgs& a, int row_min, void* workspace, cudaStream_t st);
+int read_fault_paged_tc(int* code, cudaStream_t st);
+
 size_t paged_attn_workspace_bytes(int dtype, int B, int N, int H, int Hkv, int D, int max_q);
 template <int DT>
 int launch_paged_attention(const PagedAttnArgs& a, cudaStream_t st);

@@ -38,6 +38,9 @@ __device__ int g_fault_tables_paged;
 
 constexpr int kRows = 16, kWarps = 4, kStepKeys = 16;
 constexpr int kTargetCtas = 4 * kSms, kMinSpan = 128;
+// Rows (new tokens x heads of a group) of a sequence up to which one pass of 16-row groups over its keys is
+// taken, above which the tcgen05 kernel.
+constexpr int kFewRows = 16;
 
 struct Piece {  // what one CTA works on
   int b, group, head, span_i;  // sequence, row group, key head, index of the span
@@ -165,13 +168,18 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) 
   const float rest = isfinite(x) ? x - __uint_as_float(hi) : 0.f;
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(rest));
 }
+// d += a * b.  The tensor cores' own sums truncate: one step's products are summed there, the steps by rounded fp32
+// additions.
 __device__ __forceinline__ void mma_split(float* d, const uint32_t* ah, const uint32_t* al, float b0, float b1) {
   uint32_t h0, l0, h1, l1;
   split_tf32(b0, h0, l0);
   split_tf32(b1, h1, l1);
-  mma_tf32(d, al, h0, h1);
-  mma_tf32(d, ah, l0, l1);
-  mma_tf32(d, ah, h0, h1);
+  float x[4] = {0.f, 0.f, 0.f, 0.f};
+  mma_tf32(x, al, h0, h1);
+  mma_tf32(x, ah, l0, l1);
+  mma_tf32(x, ah, h0, h1);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) d[e] += x[e];
 }
 
 template <int DT, int DP>
@@ -489,12 +497,29 @@ __global__ void __launch_bounds__(128) combine_kernel(const PagedAttnArgs a, int
   }
 }
 
-// CTAs that hold every piece: the target, one partly filled span for each (row group, key head).
-long long most_items(int B, int N, int H, int Hkv) {
-  const long long G = H / Hkv;
-  return ((long long)N * G / kRows + B) * Hkv;
+// (row group, key head) pairs of the sequences with at most row_max rows, and the CTAs that hold every piece: the
+// target, and one partly filled span for each pair.
+long long most_items(int B, int N, int H, int Hkv, int row_max) {
+  const long long G = H / Hkv, rows = (long long)N * G;
+  return std::min(rows / kRows + std::min<long long>(B, rows),
+                  std::min<long long>(B, N) * ((row_max + (long long)kRows - 1) / kRows)) * Hkv;
 }
-long long most_pieces(int B, int N, int H, int Hkv) { return most_items(B, N, H, Hkv) + kTargetCtas; }
+long long most_pieces(int B, int N, int H, int Hkv, int row_max) {
+  return most_items(B, N, H, Hkv, row_max) + kTargetCtas;
+}
+
+// Which kernels a call launches: this file's takes the sequences with at most row_max rows, the tcgen05 kernel, where
+// it is launched too, the others.
+struct Choice {
+  bool many;
+  int row_max;
+};
+
+Choice choose(int dtype, int N, int H, int Hkv, int D, int max_q, bool operands) {
+  const long long G = H / Hkv, most = (long long)(max_q > 0 ? std::min(max_q, N) : N) * G;
+  if (dtype == DT_F32 || (D != 64 && D != 128) || !operands || most <= kFewRows) return {false, 1 << 30};
+  return {true, kFewRows};
+}
 
 int padded_dim(int D) { return D <= 64 ? 64 : (D <= 128 ? 128 : 256); }
 
@@ -506,13 +531,13 @@ bool wide_rows(const void* p, std::initializer_list<long long> strides, int elem
 }
 
 template <int DT, int DP>
-int launch_mma(const PagedAttnArgs& a, int row_max, cudaStream_t st) {
+int launch_mma(const PagedAttnArgs& a, int row_max, float* part, cudaStream_t st) {
   using T = typename Storage<DT>::T;
   const int E = (int)sizeof(T);
   const bool wide = a.D * E % 16 == 0 && wide_rows(a.kpool, {a.kps.p, a.kps.h, a.kps.s}, E) &&
                     wide_rows(a.vpool, {a.vps.p, a.vps.h, a.vps.s}, E);
-  const long long pieces = most_pieces(a.B, a.N, a.H, a.Hkv), items = most_items(a.B, a.N, a.H, a.Hkv);
-  float* part = static_cast<float*>(a.workspace);
+  const long long pieces = most_pieces(a.B, a.N, a.H, a.Hkv, row_max);
+  const long long items = most_items(a.B, a.N, a.H, a.Hkv, row_max);
   const size_t smem = mma_smem<DT, DP>();
   auto kfn = wide ? paged_attn_mma_kernel<DT, DP, true> : paged_attn_mma_kernel<DT, DP, false>;
   if (cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
@@ -525,7 +550,7 @@ int launch_mma(const PagedAttnArgs& a, int row_max, cudaStream_t st) {
   AVQ_TIMED("paged_combine", st);
   // the launch overlaps the attention kernel's end; the kernel waits for its results itself
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)items);
+  cfg.gridDim = dim3((unsigned)std::max<long long>(items, 1));
   cfg.blockDim = dim3(128);
   cfg.stream = st;
   cudaLaunchAttribute attr;
@@ -541,16 +566,36 @@ int launch_mma(const PagedAttnArgs& a, int row_max, cudaStream_t st) {
 }  // namespace
 
 size_t paged_attn_workspace_bytes(int dtype, int B, int N, int H, int Hkv, int D, int max_q) {
-  const int DP = padded_dim(D);
-  return align_up((size_t)most_pieces(B, N, H, Hkv) * kRows * (DP + 2) * sizeof(float));
+  // the operands' alignment may rule the tcgen05 kernel out: room for either choice
+  const Choice with = choose(dtype, N, H, Hkv, D, max_q, true);
+  auto few_bytes = [&](int row_max) {
+    return align_up((size_t)most_pieces(B, N, H, Hkv, row_max) * kRows * (padded_dim(D) + 2) * sizeof(float));
+  };
+  const size_t alone = few_bytes(1 << 30);
+  if (!with.many) return alone;
+  return std::max(alone, few_bytes(with.row_max) + paged_attn_tc_workspace_bytes(B, N, H, Hkv, D, with.row_max));
 }
 
 template <int DT>
 int launch_paged_attention(const PagedAttnArgs& a, cudaStream_t st) {
   if (a.B == 0 || a.N == 0) return AVQ_OK;
-  if (a.D <= 64) return launch_mma<DT, 64>(a, 1 << 30, st);
-  if (a.D <= 128) return launch_mma<DT, 128>(a, 1 << 30, st);
-  return launch_mma<DT, 256>(a, 1 << 30, st);
+  const int E = (int)sizeof(typename Storage<DT>::T);
+  const bool operands = a.scale_log2 > 0.f && wide_rows(a.q, {a.qs.t, a.qs.h}, E) &&
+                        wide_rows(a.kpool, {a.kps.p, a.kps.h, a.kps.s}, E) &&
+                        wide_rows(a.vpool, {a.vps.p, a.vps.h, a.vps.s}, E);
+  const Choice c = choose(DT, a.N, a.H, a.Hkv, a.D, a.max_q, operands);
+  char* ws = static_cast<char*>(a.workspace);
+  if constexpr (DT != DT_F32) {
+    if (c.many) {
+      const int rc = launch_paged_attention_tc<DT>(a, c.row_max, ws, st);
+      if (rc != AVQ_OK) return rc;
+      ws += paged_attn_tc_workspace_bytes(a.B, a.N, a.H, a.Hkv, a.D, c.row_max);
+    }
+  }
+  float* part = reinterpret_cast<float*>(ws);
+  if (a.D <= 64) return launch_mma<DT, 64>(a, c.row_max, part, st);
+  if (a.D <= 128) return launch_mma<DT, 128>(a, c.row_max, part, st);
+  return launch_mma<DT, 256>(a, c.row_max, part, st);
 }
 
 int read_fault_paged(int* code, cudaStream_t st) {

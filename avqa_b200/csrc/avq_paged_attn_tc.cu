@@ -1,0 +1,756 @@
+// Attention of chunks over a page pool on the tcgen05 tensor cores (bf16,
+// fp16; head_dim 64 and 128).  The operator is avq_paged_attn.cu's; this
+// kernel takes the sequences with more than kPagedFewRows rows.
+//
+// The rows of one (sequence, key head) are its (token, head of the group)
+// pairs, token by token, so that a key tile serves the whole group and short
+// chunks of many heads fill the tensor core's 128 rows.  A CTA works on 256
+// rows, two tiles of 128 that take turns: while the tensor cores multiply one
+// tile's scores or values, the other tile's threads work on its softmax.
+//
+//   warps 0-3, 4-7  softmax of tile 0 / 1, a thread per row: S from TMEM, the
+//                   running maximum, p = exp2(s - m), P to TMEM (the columns
+//                   of S), the row's sum; O is rescaled in TMEM only when the
+//                   maximum grew by more than 2^8 (the sums stay exact: P and
+//                   l refer to the same, older maximum)
+//   warp 8          issues S = Q K^T and O += P V
+//   warps 9-11      load Q, then the key and value tiles (128 keys each) by
+//                   cp.async into a ring, in the 128-byte swizzled layout that
+//                   the tensor cores read; a page may begin and end anywhere
+//                   in a tile
+//
+// Work: plan_kernel lists the (sequence, 256 rows) items and their key tiles,
+// cuts the items into pieces so that about equal shares reach every SM, and
+// the persistent CTAs fetch pieces by an atomic counter (which CTA takes a
+// piece has no influence on its result).  Pieces of one item are joined by
+// combine_tc_kernel in the order of the keys.
+//
+// Every wait is bounded (avq_tc.cuh).
+#include <cuda.h>
+
+#include <algorithm>
+
+#include "avq_mma.cuh"
+#include "avq_paged.cuh"
+#include "avq_tc.cuh"
+
+namespace avq {
+
+namespace {
+
+// Bit 0: a CTA gave up on a bounded wait; bit 1: the batch's lists are not sound.
+__device__ int g_fault_paged_tc;
+
+constexpr int TM = 128, TK = 128;  // rows of a tile, keys of a tile
+constexpr int kItemRows = 2 * TM;
+constexpr int kTcThreads = 384, kLoaders = 3, W_MMA = 8, W_LOAD = 9;
+constexpr int kMaxPieces = 8 * kSms;   // pieces of split items (each has a slot of partial sums)
+constexpr int kMaxSplit = 64;
+constexpr float kLazy = 8.f;           // log2 of the growth that rescales O
+
+template <int D> constexpr int ring_slots() { return D == 128 ? 5 : 8; }
+template <int D> constexpr int load_lag() { return D == 128 ? 2 : 5; }
+template <int D> constexpr int tile_bytes() { return TK * D * 2; }
+
+// The plan in the workspace: a header, then the items, then the pieces' items.
+struct Plan {
+  int* head;   // [0] pieces per key head, [1] the next piece to fetch, [2] items
+  int* base;   // [B + 1] first item of each sequence
+  int* seq;    // [items] sequence
+  int* part;   // index of the 256-row part in it
+  int* lo;     // first key (a multiple of TK)
+  int* tiles;  // key tiles
+  int* first;  // first piece (per key head)
+  int* split;  // pieces
+  int* of;     // [pieces] item
+};
+
+__host__ __device__ inline long long plan_ints(long long B, long long items) {
+  return 8 + (B + 1) + 6 * items + (items > kMaxPieces ? items : kMaxPieces);
+}
+__host__ __device__ inline Plan plan_at(int* p, long long B, long long items) {
+  Plan q;
+  q.head = p;
+  q.base = p + 8;
+  q.seq = q.base + B + 1;
+  q.part = q.seq + items;
+  q.lo = q.part + items;
+  q.tiles = q.lo + items;
+  q.first = q.tiles + items;
+  q.split = q.first + items;
+  q.of = q.split + items;
+  return q;
+}
+
+// Keys of a 256-row item: [lo, hi), lo a multiple of TK.
+__device__ __forceinline__ int2 item_keys(const PagedAttnArgs& a, const SeqRange& s, int part, int G) {
+  const long long r0 = (long long)part * kItemRows, r1 = min((long long)s.n * G, r0 + kItemRows) - 1;
+  int lo = 0, hi = s.len;
+  if (a.causal) hi = max(0, min(s.len, s.pos0 + (int)(r1 / G) + 1));
+  if (a.window > 0) lo = max(0, s.pos0 + (int)(r0 / G) - a.window + 1) / TK * TK;
+  return make_int2(lo, max(lo, hi));
+}
+
+// ---- the plan ---------------------------------------------------------------------------
+
+constexpr int kPlanThreads = 1024;
+
+// Exclusive prefix of v over the block; *total receives the sum.
+__device__ int block_prefix(int v, int* total) {
+  __shared__ int s_warp[kPlanThreads / 32];
+  __shared__ int s_total;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) s_warp[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    int w = s_warp[lane];
+    const int own = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += y;
+    }
+    s_warp[lane] = w - own;
+    if (lane == 31) s_total = w;
+  }
+  __syncthreads();
+  *total = s_total;
+  return s_warp[warp] + x - v;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PagedAttnArgs a, int row_min, int max_items,
+                                                            int* __restrict__ ws) {
+  const Plan p = plan_at(ws, a.B, max_items);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.H / a.Hkv;
+  const long long room = (long long)a.W * a.page_size;
+  __shared__ unsigned long long s_work;
+  __shared__ int s_most, s_pieces[kMaxSplit + 1];
+  __shared__ int s_choice;
+  asm volatile("griddepcontrol.launch_dependents;");
+  if (tid == 0) {
+    s_work = 0;
+    s_most = 1;
+  }
+  bool bad = false;
+  int items = 0;
+  for (int b0 = 0; b0 < a.B; b0 += kPlanThreads) {
+    const int b = b0 + tid;
+    int parts = 0;
+    if (b < a.B) {
+      const SeqRange s = load_seq(a.q_start, a.kv_len, b, a.N, room, &bad);
+      const long long rows = (long long)s.n * G;
+      parts = rows > row_min ? (int)((rows + kItemRows - 1) / kItemRows) : 0;
+    }
+    int total;
+    const int at = items + block_prefix(parts, &total);
+    if (b < a.B) p.base[b] = min(at, max_items);
+    items += total;
+  }
+  // token ranges that overlap could name more items than the batch has rows for
+  if (items > max_items) bad = true;
+  items = min(items, max_items);
+  if (tid == 0) {
+    p.base[a.B] = items;
+    p.head[2] = items;
+  }
+  if (bad) atomicOr(&g_fault_paged_tc, kFaultTables);
+  __syncthreads();
+  unsigned long long work = 0;
+  int most = 1;
+  for (int b = warp; b < a.B; b += kPlanThreads / 32) {
+    const int i0 = p.base[b], n = p.base[b + 1] - i0;
+    if (n == 0) continue;
+    const SeqRange s = load_seq(a.q_start, a.kv_len, b, a.N, room, &bad);
+    for (int i = lane; i < n; i += 32) {
+      const int part = n - 1 - i;  // the last rows see the most keys: longest first
+      const int2 k = item_keys(a, s, part, G);
+      const int t = max(1, (k.y - k.x + TK - 1) / TK);
+      p.seq[i0 + i] = b;
+      p.part[i0 + i] = part;
+      p.lo[i0 + i] = k.x;
+      p.tiles[i0 + i] = t;
+      work += t;
+      most = max(most, t);
+    }
+  }
+  atomicAdd(&s_work, work);
+  atomicMax(&s_most, most);
+  __syncthreads();
+  // cut the items into at most k pieces each: the k whose rounds of pieces over the SMs, with a piece's own cost of
+  // about kCost tiles (its queries, its first keys, its sums), end first
+  constexpr float kCost = 3.f;
+  for (int k = warp + 1; k <= kMaxSplit; k += kPlanThreads / 32) {
+    const int cut = (s_most + k - 1) / k;
+    int n = 0;
+    for (int i = lane; i < items; i += 32) n += (p.tiles[i] + cut - 1) / cut;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    if (lane == 0) s_pieces[k] = n;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    int best = 1;
+    float least = INFINITY;
+    for (int k = 1; k <= kMaxSplit && k <= s_most; ++k) {
+      const long long n = (long long)s_pieces[k] * a.Hkv;
+      if (k > 1 && n > kMaxPieces) break;
+      const float cost = (float)((n + kSms - 1) / kSms) * ((float)s_work / fmaxf((float)s_pieces[k], 1.f) + kCost);
+      if (cost < least) {
+        least = cost;
+        best = k;
+      }
+    }
+    s_choice = (s_most + best - 1) / best;
+  }
+  __syncthreads();
+  const int cut = s_choice;
+  int pieces = 0;
+  for (int i0 = 0; i0 < items; i0 += kPlanThreads) {
+    const int i = i0 + tid, n = i < items ? (p.tiles[i] + cut - 1) / cut : 0;
+    int total;
+    const int at = pieces + block_prefix(n, &total);
+    if (i < items) {
+      p.first[i] = at;
+      p.split[i] = n;
+      for (int s = 0; s < n; ++s) p.of[at + s] = i;
+    }
+    pieces += total;
+  }
+  if (tid == 0) {
+    p.head[0] = pieces;
+    p.head[1] = 0;
+  }
+}
+
+// ---- attention ------------------------------------------------------------------------------
+
+template <int D>
+struct TcShared {
+  static constexpr int Q = 0;
+  static constexpr int RING = 2 * tile_bytes<D>();
+  static constexpr int BARS = RING + ring_slots<D>() * tile_bytes<D>();
+  static constexpr int B_Q = 0, B_FULL = 1, B_EMPTY = B_FULL + ring_slots<D>(), B_S = B_EMPTY + ring_slots<D>(),
+                       B_P = B_S + 2, B_O = B_P + 2, B_DRAIN = B_O + 2, NBARS = B_DRAIN + 1;
+  static constexpr int MISC = BARS + NBARS * 8;
+  static constexpr int TOTAL = MISC + 32;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <int DT, int D>
+__global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const PagedAttnArgs a, int max_items,
+                                                                      int* __restrict__ plan_ws,
+                                                                      float* __restrict__ partials, int out_wide) {
+  using T = typename Storage<DT>::T;
+  using L = TcShared<D>;
+  constexpr int NR = ring_slots<D>(), LAG = load_lag<D>(), TB = tile_bytes<D>();
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  const uint32_t raw = tc::smem_addr(smem_raw);
+  unsigned char* sm = smem_raw + (((raw + 1023u) & ~1023u) - raw);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + L::BARS);
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(sm + L::MISC);
+  volatile int* abort = reinterpret_cast<volatile int*>(sm + L::MISC + 4);
+  volatile int* next = reinterpret_cast<volatile int*>(sm + L::MISC + 8);  // [2]
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.H / a.Hkv;
+  const Plan plan = plan_at(plan_ws, a.B, max_items);
+
+  if (tid == 0) {
+    tc::mbar_init(&bars[L::B_Q], kLoaders);
+    for (int i = 0; i < NR; ++i) {
+      tc::mbar_init(&bars[L::B_FULL + i], kLoaders);
+      tc::mbar_init(&bars[L::B_EMPTY + i], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      tc::mbar_init(&bars[L::B_S + t], 1);
+      tc::mbar_init(&bars[L::B_P + t], TM);
+      tc::mbar_init(&bars[L::B_O + t], 1);
+    }
+    tc::mbar_init(&bars[L::B_DRAIN], 1);
+    *abort = 0;
+    tc::fence_mbar_init();
+  }
+  if (warp == W_MMA) tc::tmem_alloc(tslot, 512);
+  tc::tc_before_sync();
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the plan
+  if (tid == 0) next[0] = atomicAdd(&plan.head[1], 1);
+  __syncthreads();
+  tc::tc_after_sync();
+  const uint32_t tbase = *tslot;
+  const int per_head = plan.head[0];
+  const long long pieces = (long long)per_head * a.Hkv;
+  const long long room = (long long)a.W * a.page_size;
+  const uint32_t col_s = tbase, col_o = tbase + 2 * TK;  // S (and P) of tile t at 128 t, O at 256 + D t
+
+  // The next piece, or false when none is left.  Every role calls it once a turn, after the CTA's barrier.
+  struct Work {
+    int piece, head, item, np, tiles, row0, rows, nt, key0;
+    SeqRange seq;
+  } w;
+  auto take = [&](int turn) {
+    w.piece = next[turn & 1];
+    if (w.piece >= pieces) return false;
+    if (tid == kTcThreads - 1) next[(turn + 1) & 1] = atomicAdd(&plan.head[1], 1);
+    w.head = w.piece / per_head;
+    const int pi = w.piece - w.head * per_head;
+    w.item = plan.of[pi];
+    w.np = plan.split[w.item];
+    // equal shares of the item's tiles
+    const int si = pi - plan.first[w.item], all = plan.tiles[w.item];
+    const int t0 = (int)((long long)all * si / w.np);
+    w.tiles = (int)((long long)all * (si + 1) / w.np) - t0;
+    bool unsound = false;  // the plan reported it
+    w.seq = load_seq(a.q_start, a.kv_len, plan.seq[w.item], a.N, room, &unsound);
+    w.row0 = plan.part[w.item] * kItemRows;
+    w.rows = w.seq.n * G - w.row0;
+    w.nt = w.rows > TM ? 2 : 1;
+    w.key0 = plan.lo[w.item] + t0 * TK;
+    return true;
+  };
+  // The end of a turn: false in every thread when one gave up.
+  auto turn_over = [&]() {
+    const bool go_on = !__syncthreads_or(*abort != 0);
+    tc::tc_after_sync();
+    return go_on;
+  };
+
+  // the launch's 384 x 168 registers: 208 for each softmax thread, 88 for the others
+  if (warp >= W_MMA) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  if (warp >= W_LOAD) {
+    // ---- loaders ----
+    const int lw = warp - W_LOAD;
+    int ring = 0;  // ring tiles so far
+    for (int turn = 0; take(turn); ++turn) {
+      const SeqRange seq = w.seq;
+      const int head = w.head, rows = w.rows, nt = w.nt, row0 = w.row0, tiles = w.tiles, key0 = w.key0;
+      bool bad = false;
+      const int2 keys = item_keys(a, seq, row0 / kItemRows, G);
+      constexpr int CPR = D / 8, RPI = 32 / CPR;               // 16-byte chunks of a row, rows of a warp's copy
+      constexpr int NI = (TK / RPI + kLoaders - 1) / kLoaders;  // copies of a tile by one warp
+      const int sub = lane / CPR, chunk = lane % CPR;
+      const uint32_t col = (uint32_t)((chunk >> 3) * TM * 128);
+      int signalled = 0, issued = 0;  // unit 0: Q, unit u: ring tile u - 1 of this piece
+      auto signal_to = [&](int n) {   // copies of units below n have landed
+        tc::fence_async_smem();
+        __syncwarp();
+        for (; signalled < n; ++signalled)
+          if (lane == 0)
+            tc::mbar_arrive(signalled == 0 ? &bars[L::B_Q] : &bars[L::B_FULL + (ring + signalled - 1) % NR]);
+      };
+      {
+        const T* q = static_cast<const T*>(a.q);
+        for (int r = lw * RPI + sub; r < nt * TM; r += kLoaders * RPI) {
+          const bool ok = r < rows;
+          const int tok = seq.q0 + (row0 + (ok ? r : 0)) / G, h = head * G + (row0 + (ok ? r : 0)) % G;
+          cp_async16(sm + L::Q + (r / TM) * TB + col + (r % TM) * 128 + (((chunk & 7) ^ (r & 7)) << 4),
+                     q + (long long)tok * a.qs.t + (long long)h * a.qs.h + chunk * 8, ok);
+        }
+        cp_async_commit();
+        issued = 1;
+      }
+      const int* row_table = a.table + (long long)plan.seq[w.item] * a.table_stride;
+      const T* kbase = static_cast<const T*>(a.kpool) + (long long)head * a.kps.h;
+      const T* vbase = static_cast<const T*>(a.vpool) + (long long)head * a.vps.h;
+      long long off[2][2];  // [key, value][the first 32 rows of the warp's list, the rest]
+      bool ok = true;
+      for (int i = 0; ok && i < 2 * tiles; ++i) {
+        const int is_v = i & 1, slot = (ring + i) % NR, use = (ring + i) / NR;
+        if (!is_v) {
+          // the warp's rows of this tile: row q of its list is row (lw + 3 (q / RPI)) RPI + q % RPI
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            const int q = hf * 32 + lane, r = (lw + kLoaders * (q / RPI)) * RPI + q % RPI;
+            const int key = key0 + (i >> 1) * TK + r;
+            off[0][hf] = off[1][hf] = -1;
+            if (r < TK && key < keys.y) {
+              const int page = row_table[key / a.page_size], s = key % a.page_size;
+              if (page >= 0 && page < a.num_pages) {
+                off[0][hf] = (long long)page * a.kps.p + (long long)s * a.kps.s;
+                off[1][hf] = (long long)page * a.vps.p + (long long)s * a.vps.s;
+              } else {
+                bad = true;
+              }
+            }
+          }
+        }
+        if (use > 0 && !tc::mbar_try(&bars[L::B_EMPTY + slot], (use - 1) & 1)) {
+          cp_async_wait<0>();  // nothing more can start: hand over what has
+          signal_to(issued);
+          ok = tc::mbar_wait(&bars[L::B_EMPTY + slot], (use - 1) & 1, abort);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+        }
+        unsigned char* dst = sm + L::RING + slot * TB + col;
+        const T* base = is_v ? vbase : kbase;
+#pragma unroll
+        for (int x = 0; x < NI; ++x) {
+          const int g = lw + kLoaders * x;  // copy g of the tile: rows g RPI ..
+          const int q = x * RPI + sub;
+          const long long o = __shfl_sync(0xffffffffu, is_v ? off[1][(x * RPI) >> 5] : off[0][(x * RPI) >> 5], q & 31);
+          const int r = g * RPI + sub;
+          if (g < TK / RPI)
+            cp_async16(dst + r * 128 + (((chunk & 7) ^ (r & 7)) << 4), base + (o >= 0 ? o + chunk * 8 : 0), o >= 0);
+        }
+        cp_async_commit();
+        ++issued;
+        if (issued > LAG) {
+          cp_async_wait<LAG>();
+          signal_to(issued - LAG);
+        }
+      }
+      cp_async_wait<0>();
+      signal_to(issued);
+      ring += 2 * tiles;
+      if (bad) atomicOr(&g_fault_paged_tc, kFaultTables);
+      if (!turn_over()) break;
+    }
+  } else if (warp == W_MMA) {
+    // ---- MMA issuer ----
+    int ring = 0, q_phase = 0;
+    int count[2] = {0, 0};  // P tiles of each row tile so far
+    for (int turn = 0; take(turn); ++turn) {
+      const int nt = w.nt, tiles = w.tiles;
+      if (lane == 0) {
+        const int fmt = DT == DT_BF16 ? 1 : 0;
+        const uint32_t id_s = tc::idesc_f16(fmt, TM, TK, false), id_o = tc::idesc_f16(fmt, TM, D, true);
+        const uint32_t qa = tc::smem_addr(sm + L::Q), ra = tc::smem_addr(sm + L::RING);
+        auto tile_ready = [&](int i) {
+          const int n = ring + i;
+          return tc::mbar_wait(&bars[L::B_FULL + n % NR], (n / NR) & 1, abort);
+        };
+        auto issue_s = [&](int t, int i) {
+          const uint32_t kb = ra + ((ring + i) % NR) * TB;
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t o = (kk >> 2) * TM * 128 + (kk & 3) * 32;
+            tc::mma_ss(col_s + t * TK, tc::sdesc_sw128(qa + t * TB + o, 16, 1024), tc::sdesc_sw128(kb + o, 16, 1024),
+                       id_s, kk > 0);
+          }
+          tc::mma_commit(&bars[L::B_S + t]);
+        };
+        bool ok = tc::mbar_wait(&bars[L::B_Q], q_phase & 1, abort) && tile_ready(0);
+        if (ok) {
+          tc::tc_after_sync();
+          for (int t = 0; t < nt; ++t) issue_s(t, 0);
+          tc::mma_commit(&bars[L::B_EMPTY + ring % NR]);
+        }
+        for (int j = 0; ok && j < tiles; ++j) {
+          if (!(ok = tile_ready(2 * j + 1))) break;
+          const uint32_t vb = ra + ((ring + 2 * j + 1) % NR) * TB;
+          for (int t = 0; ok && t < nt; ++t) {
+            // P of this tile is in TMEM, and every thread is done with S
+            if (!(ok = tc::mbar_wait(&bars[L::B_P + t], (count[t] + j) & 1, abort))) break;
+            tc::tc_after_sync();
+#pragma unroll
+            for (int kk = 0; kk < TK / 16; ++kk)
+              tc::mma_ts(col_o + t * D, col_s + t * TK + kk * 8, tc::sdesc_sw128(vb + kk * 16 * 128, TK * 128, 1024),
+                         id_o, j > 0 || kk > 0);
+            if (t == nt - 1) tc::mma_commit(&bars[L::B_EMPTY + (ring + 2 * j + 1) % NR]);
+            if (j + 1 < tiles) {
+              // the scores of the next keys take the columns of P: the tensor cores work in the order of issue
+              if (t == 0) {
+                if (!(ok = tile_ready(2 * j + 2))) break;
+                tc::tc_after_sync();
+              }
+              issue_s(t, 2 * j + 2);
+              if (t == nt - 1) tc::mma_commit(&bars[L::B_EMPTY + (ring + 2 * j + 2) % NR]);
+            } else {
+              tc::mma_commit(&bars[L::B_O + t]);
+            }
+          }
+        }
+        if (!ok) {  // let what was issued finish before the CTA leaves
+          tc::mma_commit(&bars[L::B_DRAIN]);
+          const long long since = clock64();
+          while (!tc::mbar_try(&bars[L::B_DRAIN], 0) && clock64() - since < tc::kWaitCycles / 8) {
+          }
+        }
+      }
+      __syncwarp();
+      ring += 2 * tiles;
+      ++q_phase;
+      for (int t = 0; t < 2; ++t)
+        if (t < nt) count[t] += tiles;
+      if (!turn_over()) break;
+    }
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    // ---- softmax of tile t: this thread's row is lane (tid % 128) of the tile ----
+    const int t = warp >> 2, r = t * TM + (tid & 127);
+    int s_count = 0, o_phase = 0;  // S tiles and pieces of this row tile so far
+    for (int turn = 0; take(turn); ++turn) {
+      if (t >= w.nt) {
+        if (!turn_over()) break;
+        continue;
+      }
+      const SeqRange seq = w.seq;
+      const int head = w.head, rows = w.rows, row0 = w.row0, tiles = w.tiles, key0 = w.key0, np = w.np;
+      const uint32_t lanes = (uint32_t)(warp & 3) << 21;
+      const uint32_t s_at = col_s + t * TK + lanes, o_at = col_o + t * D + lanes;
+      int first = 0, last = INT_MAX;  // visible keys; rows behind the last one need no mask
+      if (r < rows) {
+        const int pos = seq.pos0 + (row0 + r) / G;
+        last = a.causal ? (pos < 0 ? 0 : min(seq.len, pos + 1)) : seq.len;
+        first = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+      }
+      float m = -INFINITY, l = 0.f;
+      bool ok = true;
+      for (int j = 0; j < tiles; ++j) {
+        ok = tc::mbar_wait(&bars[L::B_S + t], (s_count + j) & 1, abort);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        tc::tc_after_sync();
+        uint32_t s[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tc::tmem_ld32(s_at + c * 32, s[c]);
+        tc::tmem_wait_ld();
+        const int k0 = key0 + j * TK;
+        if (__any_sync(0xffffffffu, k0 < first || last - k0 < TK)) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const int key = k0 + c * 32 + e;
+              if (key < first || key >= last) s[c][e] = 0xff800000u;  // -inf
+            }
+        }
+        float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) x[c] = fmaxf(x[c], __uint_as_float(s[c][e]));
+        const float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * a.scale_log2;
+        // (the maximum of a row whose keys are all hidden so far stays -inf, and -inf - -inf is no growth)
+        if (__any_sync(0xffffffffu, mx > m + kLazy || (m == -INFINITY && mx > m))) {
+          const float mn = fmaxf(m, mx), f = mn > m ? ex2(m - mn) : 1.f;
+          m = mn;
+          l *= f;
+          if (j > 0) {
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              tc::tmem_ld32(o_at + c * 32, o);
+              tc::tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tc::tmem_st32(o_at + c * 32, o);
+            }
+          }
+        }
+        const float sub = m == -INFINITY ? 0.f : m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float p0 = ex2(fmaf(__uint_as_float(s[c][e]), a.scale_log2, -sub));
+            const float p1 = ex2(fmaf(__uint_as_float(s[c][e + 1]), a.scale_log2, -sub));
+            sum[c] += p0 + p1;
+            pk[e / 2] = pack2<DT>(p0, p1);
+          }
+          tc::tmem_st16(s_at + c * 16, pk);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tc::tmem_wait_st();
+        tc::tc_before_sync();
+        tc::mbar_arrive(&bars[L::B_P + t]);
+      }
+      if (ok) {
+        ok = tc::mbar_wait(&bars[L::B_O + t], o_phase & 1, abort);
+        ok = __all_sync(0xffffffffu, ok);
+      }
+      if (ok) {
+        tc::tc_after_sync();
+        const bool whole = np == 1;
+        // a row that sees no key is zero; one whose keys all score -inf is 0 / 0
+        const float f = whole ? (last > first ? 1.f / l : 0.f) : 1.f;
+        T* dst = nullptr;
+        float* pd = nullptr;
+        if (r < rows) {
+          if (whole) {
+            const int tok = seq.q0 + (row0 + r) / G, h = head * G + (row0 + r) % G;
+            dst = static_cast<T*>(a.out) + (long long)tok * a.os.t + (long long)h * a.os.h;
+          } else {
+            pd = partials + (long long)w.piece * (kItemRows * (D + 2));
+            pd[kItemRows * D + r] = m;
+            pd[kItemRows * (D + 1) + r] = l;
+            pd += (long long)r * D;
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          tc::tmem_ld32(o_at + c * 32, o);
+          tc::tmem_wait_ld();
+          if (dst) {
+            if (last <= first) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = 0;
+            }
+            if (out_wide) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 8) {
+                uint4 y;
+                y.x = pack2<DT>(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 1]) * f);
+                y.y = pack2<DT>(__uint_as_float(o[e + 2]) * f, __uint_as_float(o[e + 3]) * f);
+                y.z = pack2<DT>(__uint_as_float(o[e + 4]) * f, __uint_as_float(o[e + 5]) * f);
+                y.w = pack2<DT>(__uint_as_float(o[e + 6]) * f, __uint_as_float(o[e + 7]) * f);
+                *reinterpret_cast<uint4*>(dst + c * 32 + e) = y;
+              }
+            } else {
+              for (int e = 0; e < 32; ++e) dst[c * 32 + e] = from_f<DT>(__uint_as_float(o[e]) * f);
+            }
+          } else if (pd) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<uint4*>(pd + c * 32 + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
+        }
+        tc::tc_before_sync();
+      }
+      s_count += tiles;
+      ++o_phase;
+      if (!turn_over()) break;
+    }
+  }
+  __syncthreads();
+  if (warp == W_MMA) tc::tmem_free(tbase, 512);
+  if (tid == 0 && *abort) atomicOr(&g_fault_paged_tc, 1);
+}
+
+// Joins an item's pieces: a block per (item, 32 rows), in the order of the keys.
+constexpr int kJoinRows = 32;
+
+template <int DT, int D>
+__global__ void __launch_bounds__(256) combine_tc_kernel(const PagedAttnArgs a, int max_items,
+                                                         int* __restrict__ plan_ws,
+                                                         const float* __restrict__ partials) {
+  using T = typename Storage<DT>::T;
+  const Plan plan = plan_at(plan_ws, a.B, max_items);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int item = blockIdx.x, head = blockIdx.y, G = a.H / a.Hkv;
+  if (item >= plan.head[2]) return;
+  const int np = plan.split[item];
+  if (np <= 1) return;
+  bool bad = false;
+  const SeqRange seq = load_seq(a.q_start, a.kv_len, plan.seq[item], a.N, (long long)a.W * a.page_size, &bad);
+  const int row0 = plan.part[item] * kItemRows, rows = min(kItemRows, seq.n * G - row0);
+  const long long stride = kItemRows * (D + 2);
+  const float* base = partials + ((long long)head * plan.head[0] + plan.first[item]) * stride;
+  for (int i = threadIdx.x; i < kJoinRows * (D / 4); i += 256) {
+    const int r = blockIdx.z * kJoinRows + i / (D / 4), d = i % (D / 4) * 4;
+    if (r >= rows) break;
+    float M = -INFINITY;
+    for (int s = 0; s < np; ++s) M = fmaxf(M, base[s * stride + kItemRows * D + r]);
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < np; ++s) {
+      const float* w = base + s * stride;
+      const float m = w[kItemRows * D + r], ls = w[kItemRows * (D + 1) + r];
+      const float4 o = *reinterpret_cast<const float4*>(w + (long long)r * D + d);
+      if (m == -INFINITY && ls == 0.f) continue;  // a piece whose keys this row does not see
+      const float f = m == -INFINITY ? 0.f : ex2(m - M);
+      x.x = fmaf(o.x, f, x.x);
+      x.y = fmaf(o.y, f, x.y);
+      x.z = fmaf(o.z, f, x.z);
+      x.w = fmaf(o.w, f, x.w);
+      l = fmaf(ls, f, l);
+    }
+    const int pos = seq.pos0 + (row0 + r) / G;
+    const int last = a.causal ? (pos < 0 ? 0 : min(seq.len, pos + 1)) : seq.len;
+    const int first = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+    const float inv = 1.f / l;
+    const int tok = seq.q0 + (row0 + r) / G, h = head * G + (row0 + r) % G;
+    T* dst = static_cast<T*>(a.out) + (long long)tok * a.os.t + (long long)h * a.os.h + d;
+    const float y[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) dst[e] = from_f<DT>(last > first ? y[e] : 0.f);
+  }
+}
+
+long long most_items(int B, int N, int G, int row_min) {
+  const long long rows = (long long)N * G;
+  return rows / kItemRows + std::min<long long>(B, rows / (row_min + 1)) + 1;
+}
+size_t plan_bytes(int B, long long items) { return align_up((size_t)plan_ints(B, items) * sizeof(int)); }
+
+}  // namespace
+
+size_t paged_attn_tc_workspace_bytes(int B, int N, int H, int Hkv, int D, int row_min) {
+  const long long items = most_items(B, N, H / Hkv, row_min);
+  const long long slots = std::min<long long>(kMaxPieces, items * Hkv * kMaxSplit);
+  return plan_bytes(B, items) + align_up((size_t)slots * kItemRows * (D + 2) * sizeof(float));
+}
+
+template <int DT>
+int launch_paged_attention_tc(const PagedAttnArgs& a, int row_min, void* workspace, cudaStream_t st) {
+  const long long items = most_items(a.B, a.N, a.H / a.Hkv, row_min);
+  int* ws = static_cast<int*>(workspace);
+  float* partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan_bytes(a.B, items));
+  using T = typename Storage<DT>::T;
+  const bool wide = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.os.t % 8 == 0 && a.os.h % 8 == 0;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  auto go = [&](auto kfn, auto joinfn, int D, int total) -> int {
+    {
+      AVQ_TIMED("paged_plan", st);
+      plan_kernel<<<1, kPlanThreads, 0, st>>>(a, row_min, (int)items, ws);
+      if (cudaPeekAtLastError() != cudaSuccess) return AVQ_ERR_CUDA;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    {
+      AVQ_TIMED("paged_attn_tc", st);
+      const int smem = total + 1024;
+      if (cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+        return AVQ_ERR_CUDA;
+      cfg.gridDim = dim3(kSms);
+      cfg.blockDim = dim3(kTcThreads);
+      cfg.dynamicSmemBytes = smem;
+      if (cudaLaunchKernelEx(&cfg, kfn, a, (int)items, ws, partials, (int)wide) != cudaSuccess) return AVQ_ERR_CUDA;
+    }
+    AVQ_TIMED("paged_combine_tc", st);
+    cfg.gridDim = dim3((unsigned)std::min<long long>(items, kMaxPieces), a.Hkv, kItemRows / kJoinRows);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = 0;
+    return cudaLaunchKernelEx(&cfg, joinfn, a, (int)items, ws, (const float*)partials) == cudaSuccess ? AVQ_OK
+                                                                                                      : AVQ_ERR_CUDA;
+  };
+  if (a.D == 64)
+    return go(paged_attn_tc_kernel<DT, 64>, combine_tc_kernel<DT, 64>, 64, TcShared<64>::TOTAL);
+  return go(paged_attn_tc_kernel<DT, 128>, combine_tc_kernel<DT, 128>, 128, TcShared<128>::TOTAL);
+}
+
+int read_fault_paged_tc(int* code, cudaStream_t st) {
+  int zero = 0;
+  if (cudaMemcpyFromSymbolAsync(code, g_fault_paged_tc, sizeof(int), 0, cudaMemcpyDeviceToHost, st) != cudaSuccess ||
+      cudaMemcpyToSymbolAsync(g_fault_paged_tc, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st) != cudaSuccess ||
+      cudaStreamSynchronize(st) != cudaSuccess)
+    return AVQ_ERR_CUDA;
+  return AVQ_OK;
+}
+
+template int launch_paged_attention_tc<DT_BF16>(const PagedAttnArgs&, int, void*, cudaStream_t);
+template int launch_paged_attention_tc<DT_F16>(const PagedAttnArgs&, int, void*, cudaStream_t);
+
+}  // namespace avq
