@@ -6,6 +6,7 @@ missing, every CUDA call raises :class:`BackendError`.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from pathlib import Path
 
@@ -118,16 +119,25 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+@functools.lru_cache(maxsize=4096)
+def longs(*values: int) -> ctypes.Array:
+    """A C array of ``values``; the library only reads it, so calls share one."""
+    return (ctypes.c_longlong * len(values))(*values)
+
+
 def strides3(t: torch.Tensor) -> ctypes.Array:
     """Element strides (b, h, s) of a 4-D ``[B, H, S, D]`` view with unit d-stride."""
-    if t.dim() != 4 or (t.shape[-1] > 1 and t.stride(3) != 1):
+    st = t.stride()
+    if len(st) != 4 or (st[3] != 1 and t.shape[3] > 1):
         raise BackendError("operand must be a 4-D view with a contiguous last dimension",
-                           {"shape": tuple(t.shape), "stride": tuple(t.stride())})
-    return (ctypes.c_longlong * 3)(t.stride(0), t.stride(1), t.stride(2))
+                           {"shape": tuple(t.shape), "stride": tuple(st)})
+    return longs(st[0], st[1], st[2])
 
 
 def stream_of(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """Handle of the current stream of ``device``."""
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 def dtype_code(dt: torch.dtype) -> int:

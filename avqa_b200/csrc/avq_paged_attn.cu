@@ -37,7 +37,7 @@ namespace {
 __device__ int g_fault_tables_paged;
 
 constexpr int kRows = 16, kWarps = 4, kStepKeys = 16;
-constexpr int kTargetCtas = 4 * kSms, kMinSpan = 128;
+constexpr int kTargetCtas = 16 * kSms, kMinSpan = 128;
 // Rows (new tokens x heads of a group) of a sequence up to which one pass of 16-row groups over its keys is
 // taken, above which the tcgen05 kernel.
 constexpr int kFewRows = 16;
@@ -184,11 +184,12 @@ __device__ __forceinline__ void mma_split(float* d, const uint32_t* ah, const ui
 
 template <int DT, int DP>
 constexpr int stage_elems() { return 2 * kStepKeys * (DP + Operand<DT>::kPad); }
-// Stages of a warp's ring: as many as leave room for two CTAs on an SM (one for the widest rows).
+// Stages of a warp's ring: two or three, so that three CTAs or more share an SM and one's first loads overlap the
+// others' streams (the widest rows: one stage, one CTA).
 template <int DT, int DP>
 constexpr int ring_stages() {
   const int row = DP * (int)sizeof(typename Storage<DT>::T);
-  return row <= 128 ? 5 : (row <= 256 ? 3 : (row <= 512 ? 2 : 1));
+  return row <= 128 ? 3 : (row <= 512 ? 2 : 1);
 }
 template <int DT, int DP>
 constexpr size_t mma_smem() {
@@ -200,7 +201,7 @@ constexpr size_t mma_smem() {
 
 template <int DT, int DP, bool WIDE>
 __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const PagedAttnArgs a, int row_max,
-                                                                     float* __restrict__ part) {
+                                                                     int q_wide, float* __restrict__ part) {
   using T = typename Storage<DT>::T;
   constexpr int LDS = DP + Operand<DT>::kPad, NT = DP / 8, STAGES = ring_stages<DT, DP>();
   constexpr int EPC = 16 / (int)sizeof(T), CPR = DP / EPC;  // elements of a 16-byte chunk, chunks of a row
@@ -215,15 +216,26 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
   T* ring = sq + kRows * LDS + warp * STAGES * stage_elems<DT, DP>();       // this warp's stages
   const int row0 = p.group * kRows, nrow = min(kRows, p.seq.n * G - row0);
 
-  for (int i = tid; i < kRows * DP; i += kWarps * 32) {
-    const int r = i / DP, d = i - r * DP;
-    T x = from_f<DT>(0.f);
-    if (r < nrow && d < a.D) {
-      const int tok = p.seq.q0 + (row0 + r) / G, h = p.head * G + (row0 + r) % G;
-      x = static_cast<const T*>(a.q)[(long long)tok * a.qs.t + (long long)h * a.qs.h + d];
+  if (q_wide) {
+    for (int i = tid; i < kRows * CPR; i += kWarps * 32) {
+      const int r = i / CPR, c = (i - r * CPR) * EPC;
+      const bool ok = r < nrow && c < a.D;
+      const int tok = p.seq.q0 + (row0 + (ok ? r : 0)) / G, h = p.head * G + (row0 + (ok ? r : 0)) % G;
+      cp_async16(sq + r * LDS + c,
+                 static_cast<const T*>(a.q) + (long long)tok * a.qs.t + (long long)h * a.qs.h + (ok ? c : 0), ok);
     }
-    sq[r * LDS + d] = x;
+  } else {
+    for (int i = tid; i < kRows * DP; i += kWarps * 32) {
+      const int r = i / DP, d = i - r * DP;
+      T x = from_f<DT>(0.f);
+      if (r < nrow && d < a.D) {
+        const int tok = p.seq.q0 + (row0 + r) / G, h = p.head * G + (row0 + r) % G;
+        x = static_cast<const T*>(a.q)[(long long)tok * a.qs.t + (long long)h * a.qs.h + d];
+      }
+      sq[r * LDS + d] = x;
+    }
   }
+  cp_async_commit();
 
   // the keys that any row of the group sees
   const int ra = lane >> 2, rb = ra + 8;
@@ -278,6 +290,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) load(i);
 
+  cp_async_wait<STAGES - 1>();  // the queries
   __syncthreads();
   uint32_t qf[DT == DT_F32 ? 1 : DP / 16][4];
   if constexpr (DT != DT_F32) {
@@ -436,7 +449,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
   __syncthreads();
   for (int i = tid; i < nrow * DP; i += kWarps * 32) {
     const int r = i / DP, d = i - r * DP;
-    if (d >= a.D) continue;
+    if (d >= a.D && p.nspan == 1) continue;
     float x = 0.f, l = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
@@ -462,38 +475,100 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
   }
 }
 
-// Joins the spans of one (sequence, key head, row group).
+// Joins the spans of one (sequence, key head, row group): a warp per row, or several where the rows are few, each on
+// every so-manieth span, with a row of partial sums in one load of the warp.
+constexpr int kJoinWarps = 8;
+
 template <int DT, int DP>
-__global__ void __launch_bounds__(128) combine_kernel(const PagedAttnArgs a, int row_max, long long pieces,
-                                                      const float* __restrict__ part) {
+__global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const PagedAttnArgs a, int row_max, long long pieces,
+                                                                  const float* __restrict__ part) {
   using T = typename Storage<DT>::T;
-  const int G = a.H / a.Hkv;
+  constexpr int VW = DP >= 128 ? 4 : 2, NV = DP / (32 * VW);  // floats of a lane's vector, vectors of a lane
+  __shared__ float s_x[kJoinWarps][DP];
+  __shared__ float s_l[kJoinWarps];
+  const int G = a.H / a.Hkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   long long slot = 0;
   const Piece p = find_piece(a, row_max, blockIdx.x, false, false, &slot);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   if (!p.found || p.nspan == 1) return;
   const int stride = p.lo, row0 = p.group * kRows, nrow = min(kRows, p.seq.n * G - row0);
   // token ranges that overlap could name more pieces than there are slots
   if (slot + (long long)(p.nspan - 1) * stride >= pieces) return;
   const long long step = (long long)stride * (kRows * (DP + 2));
   const float* base = part + slot * (kRows * (DP + 2));
-  for (int i = threadIdx.x; i < nrow * DP; i += 128) {
-    const int r = i / DP, d = i - r * DP;
-    if (d >= a.D) continue;
-    float M = -INFINITY;
-    for (int s = 0; s < p.nspan; ++s) M = fmaxf(M, base[s * step + kRows * DP + r]);
-    float x = 0.f, l = 0.f;
-    for (int s = 0; s < p.nspan; ++s) {
-      const float* w = base + s * step;
-      const float m = w[kRows * DP + r], f = m == -INFINITY ? 0.f : exp2f(m - M);
-      // a span whose rows saw nothing (or only -inf) adds nothing
-      if (m == -INFINITY && w[kRows * DP + kRows + r] == 0.f) continue;
-      x = fmaf(w[r * DP + d], f, x);
-      l = fmaf(w[kRows * DP + kRows + r], f, l);
+  const int per_row = nrow >= kJoinWarps ? 1 : kJoinWarps / nrow;  // warps of a row
+  const int share = warp % per_row;
+  for (int r = warp / per_row; r < nrow || per_row > 1; r += kJoinWarps / per_row) {
+    const bool mine = r < nrow && warp < nrow * per_row;
+    float x[NV][VW], l = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < VW; ++e) x[i][e] = 0.f;
+    if (mine) {
+      const float* bm = base + kRows * DP + r;
+      float M = -INFINITY;
+      for (int s = lane; s < p.nspan; s += 32) M = fmaxf(M, bm[s * step]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+#pragma unroll 4
+      for (int s = share; s < p.nspan; s += per_row) {
+        const float m = bm[s * step], ls = bm[s * step + kRows];
+        const float* w = base + s * step + r * DP;
+        float y[NV][VW];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          if constexpr (VW == 4) {
+            const float4 v = *reinterpret_cast<const float4*>(w + (i * 32 + lane) * 4);
+            y[i][0] = v.x;
+            y[i][1] = v.y;
+            y[i][2] = v.z;
+            y[i][3] = v.w;
+          } else {
+            const float2 v = *reinterpret_cast<const float2*>(w + lane * 2);
+            y[i][0] = v.x;
+            y[i][1] = v.y;
+          }
+        }
+        // a span whose keys the row does not see (or that all score -inf) adds nothing
+        if (m == -INFINITY && ls == 0.f) continue;
+        const float f = m == -INFINITY ? 0.f : exp2f(m - M);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int e = 0; e < VW; ++e) x[i][e] = fmaf(y[i][e], f, x[i][e]);
+        l = fmaf(ls, f, l);
+      }
     }
-    const int tok = p.seq.q0 + (row0 + r) / G, h = p.head * G + (row0 + r) % G;
-    const int2 v = visible(a, p.seq.pos0 + (row0 + r) / G, p.seq.len);
-    static_cast<T*>(a.out)[(long long)tok * a.os.t + (long long)h * a.os.h + d] = from_f<DT>(v.y > v.x ? x / l : 0.f);
+    if (per_row > 1) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < VW; ++e) s_x[warp][(i * 32 + lane) * VW + e] = x[i][e];
+      if (lane == 0) s_l[warp] = l;
+      __syncthreads();
+      if (mine && share == 0)
+        for (int w = 1; w < per_row; ++w) {
+#pragma unroll
+          for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < VW; ++e) x[i][e] += s_x[warp + w][(i * 32 + lane) * VW + e];
+          l += s_l[warp + w];
+        }
+    }
+    if (mine && share == 0) {
+      const int tok = p.seq.q0 + (row0 + r) / G, h = p.head * G + (row0 + r) % G;
+      const int2 v = visible(a, p.seq.pos0 + (row0 + r) / G, p.seq.len);
+      T* dst = static_cast<T*>(a.out) + (long long)tok * a.os.t + (long long)h * a.os.h;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < VW; ++e) {
+          const int d = (i * 32 + lane) * VW + e;
+          if (d < a.D) dst[d] = from_f<DT>(v.y > v.x ? x[i][e] / l : 0.f);
+        }
+    }
+    if (per_row > 1) break;  // all rows have a warp
   }
 }
 
@@ -536,6 +611,7 @@ int launch_mma(const PagedAttnArgs& a, int row_max, float* part, cudaStream_t st
   const int E = (int)sizeof(T);
   const bool wide = a.D * E % 16 == 0 && wide_rows(a.kpool, {a.kps.p, a.kps.h, a.kps.s}, E) &&
                     wide_rows(a.vpool, {a.vps.p, a.vps.h, a.vps.s}, E);
+  const bool q_wide = a.D * E % 16 == 0 && wide_rows(a.q, {a.qs.t, a.qs.h}, E);
   const long long pieces = most_pieces(a.B, a.N, a.H, a.Hkv, row_max);
   const long long items = most_items(a.B, a.N, a.H, a.Hkv, row_max);
   const size_t smem = mma_smem<DT, DP>();
@@ -544,14 +620,14 @@ int launch_mma(const PagedAttnArgs& a, int row_max, float* part, cudaStream_t st
     return AVQ_ERR_CUDA;
   {
     AVQ_TIMED("paged_attn", st);
-    kfn<<<(unsigned)pieces, kWarps * 32, smem, st>>>(a, row_max, part);
+    kfn<<<(unsigned)pieces, kWarps * 32, smem, st>>>(a, row_max, (int)q_wide, part);
     if (cudaPeekAtLastError() != cudaSuccess) return AVQ_ERR_CUDA;
   }
   AVQ_TIMED("paged_combine", st);
   // the launch overlaps the attention kernel's end; the kernel waits for its results itself
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)std::max<long long>(items, 1));
-  cfg.blockDim = dim3(128);
+  cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.stream = st;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;

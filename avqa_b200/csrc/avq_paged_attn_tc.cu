@@ -14,10 +14,12 @@
 //                   maximum grew by more than 2^8 (the sums stay exact: P and
 //                   l refer to the same, older maximum)
 //   warp 8          issues S = Q K^T and O += P V
-//   warps 9-11      load Q, then the key and value tiles (128 keys each) by
-//                   cp.async into a ring, in the 128-byte swizzled layout that
-//                   the tensor cores read; a page may begin and end anywhere
-//                   in a tile
+//   warps 9-11      load Q, then the key and value tiles (128 keys each) into
+//                   a ring, in the 128-byte swizzled layout that the tensor
+//                   cores read: warp 9 by TMA where whole pages fill a tile or
+//                   whole tiles a page (page sizes 8, 16, .. 128 and multiples
+//                   of 128), else all three by cp.async, where a page may begin
+//                   and end anywhere in a tile
 //
 // Work: plan_kernel lists the (sequence, 256 rows) items and their key tiles,
 // cuts the items into pieces so that about equal shares reach every SM, and
@@ -29,6 +31,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <cstring>
 
 #include "avq_mma.cuh"
 #include "avq_paged.cuh"
@@ -49,7 +52,6 @@ constexpr int kMaxSplit = 64;
 constexpr float kLazy = 8.f;           // log2 of the growth that rescales O
 
 template <int D> constexpr int ring_slots() { return D == 128 ? 5 : 8; }
-template <int D> constexpr int load_lag() { return D == 128 ? 2 : 5; }
 template <int D> constexpr int tile_bytes() { return TK * D * 2; }
 
 // The plan in the workspace: a header, then the items, then the pieces' items.
@@ -236,8 +238,11 @@ struct TcShared {
   static constexpr int Q = 0;
   static constexpr int RING = 2 * tile_bytes<D>();
   static constexpr int BARS = RING + ring_slots<D>() * tile_bytes<D>();
+  // queries; tiles full and empty; scores, probabilities and sums of each row tile; the last value tile's rows;
+  // what is in flight when a wait was given up
   static constexpr int B_Q = 0, B_FULL = 1, B_EMPTY = B_FULL + ring_slots<D>(), B_S = B_EMPTY + ring_slots<D>(),
-                       B_P = B_S + 2, B_O = B_P + 2, B_DRAIN = B_O + 2, NBARS = B_DRAIN + 1;
+                       B_P = B_S + 2, B_O = B_P + 2, B_TAIL = B_O + 2,
+                       B_DRAIN = B_TAIL + 1, NBARS = B_DRAIN + 1;
   static constexpr int MISC = BARS + NBARS * 8;
   static constexpr int TOTAL = MISC + 32;
 };
@@ -248,13 +253,19 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-template <int DT, int D>
-__global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const PagedAttnArgs a, int max_items,
+struct PoolMaps {  // a pool as a 4-D tensor map: d, and slots, heads and pages in the coordinates x, y and z
+  CUtensorMap k, v;
+  int4 kpos, vpos;
+};
+
+template <int DT, int D, bool TMA>
+__global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __grid_constant__ PoolMaps maps,
+                                                                      const PagedAttnArgs a, int max_items,
                                                                       int* __restrict__ plan_ws,
                                                                       float* __restrict__ partials, int out_wide) {
   using T = typename Storage<DT>::T;
   using L = TcShared<D>;
-  constexpr int NR = ring_slots<D>(), LAG = load_lag<D>(), TB = tile_bytes<D>();
+  constexpr int NR = ring_slots<D>(), TB = tile_bytes<D>();
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   const uint32_t raw = tc::smem_addr(smem_raw);
   unsigned char* sm = smem_raw + (((raw + 1023u) & ~1023u) - raw);
@@ -266,9 +277,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const Page
   const Plan plan = plan_at(plan_ws, a.B, max_items);
 
   if (tid == 0) {
-    tc::mbar_init(&bars[L::B_Q], kLoaders);
+    tc::mbar_init(&bars[L::B_Q], kLoaders * 32);
     for (int i = 0; i < NR; ++i) {
-      tc::mbar_init(&bars[L::B_FULL + i], kLoaders);
+      tc::mbar_init(&bars[L::B_FULL + i], TMA ? 1 : kLoaders * 32);
       tc::mbar_init(&bars[L::B_EMPTY + i], 1);
     }
     for (int t = 0; t < 2; ++t) {
@@ -276,6 +287,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const Page
       tc::mbar_init(&bars[L::B_P + t], TM);
       tc::mbar_init(&bars[L::B_O + t], 1);
     }
+    tc::mbar_init(&bars[L::B_TAIL], 1);
     tc::mbar_init(&bars[L::B_DRAIN], 1);
     *abort = 0;
     tc::fence_mbar_init();
@@ -331,7 +343,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const Page
   if (warp >= W_LOAD) {
     // ---- loaders ----
     const int lw = warp - W_LOAD;
-    int ring = 0;  // ring tiles so far
+    int ring = 0, tails = 0;  // ring tiles, tiles with a tail so far
     for (int turn = 0; take(turn); ++turn) {
       const SeqRange seq = w.seq;
       const int head = w.head, rows = w.rows, nt = w.nt, row0 = w.row0, tiles = w.tiles, key0 = w.key0;
@@ -341,14 +353,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const Page
       constexpr int NI = (TK / RPI + kLoaders - 1) / kLoaders;  // copies of a tile by one warp
       const int sub = lane / CPR, chunk = lane % CPR;
       const uint32_t col = (uint32_t)((chunk >> 3) * TM * 128);
-      int signalled = 0, issued = 0;  // unit 0: Q, unit u: ring tile u - 1 of this piece
-      auto signal_to = [&](int n) {   // copies of units below n have landed
-        tc::fence_async_smem();
-        __syncwarp();
-        for (; signalled < n; ++signalled)
-          if (lane == 0)
-            tc::mbar_arrive(signalled == 0 ? &bars[L::B_Q] : &bars[L::B_FULL + (ring + signalled - 1) % NR]);
-      };
       {
         const T* q = static_cast<const T*>(a.q);
         for (int r = lw * RPI + sub; r < nt * TM; r += kLoaders * RPI) {
@@ -357,61 +361,115 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const Page
           cp_async16(sm + L::Q + (r / TM) * TB + col + (r % TM) * 128 + (((chunk & 7) ^ (r & 7)) << 4),
                      q + (long long)tok * a.qs.t + (long long)h * a.qs.h + chunk * 8, ok);
         }
-        cp_async_commit();
-        issued = 1;
+        tc::cp_async_arrive(&bars[L::B_Q]);
       }
       const int* row_table = a.table + (long long)plan.seq[w.item] * a.table_stride;
-      const T* kbase = static_cast<const T*>(a.kpool) + (long long)head * a.kps.h;
-      const T* vbase = static_cast<const T*>(a.vpool) + (long long)head * a.vps.h;
-      long long off[2][2];  // [key, value][the first 32 rows of the warp's list, the rest]
       bool ok = true;
-      for (int i = 0; ok && i < 2 * tiles; ++i) {
-        const int is_v = i & 1, slot = (ring + i) % NR, use = (ring + i) / NR;
-        if (!is_v) {
-          // the warp's rows of this tile: row q of its list is row (lw + 3 (q / RPI)) RPI + q % RPI
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            const int q = hf * 32 + lane, r = (lw + kLoaders * (q / RPI)) * RPI + q % RPI;
-            const int key = key0 + (i >> 1) * TK + r;
-            off[0][hf] = off[1][hf] = -1;
-            if (r < TK && key < keys.y) {
-              const int page = row_table[key / a.page_size], s = key % a.page_size;
-              if (page >= 0 && page < a.num_pages) {
-                off[0][hf] = (long long)page * a.kps.p + (long long)s * a.kps.s;
-                off[1][hf] = (long long)page * a.vps.p + (long long)s * a.vps.s;
-              } else {
-                bad = true;
+      if constexpr (TMA) {
+        if (lw == 0) {
+          // lane x brings one box of a tile: 64 columns of the rows of one page, or of the tile where the page is larger
+          const int R = min(a.page_size, TK), boxes = TK / R * (D / 64);
+          const int row = lane / (D / 64) * R, half = lane % (D / 64);
+          int page = 0, in_page = 0, i = 0;
+          for (; ok && i < 2 * tiles; ++i) {
+            const int is_v = i & 1, slot = (ring + i) % NR, use = (ring + i) / NR, k0 = key0 + (i >> 1) * TK;
+            if (!is_v && lane < boxes) {
+              const int key = k0 + row;
+              page = a.num_pages;  // outside the map: reads as zeros
+              in_page = key % a.page_size;
+              if (key < keys.y) {
+                const int p = row_table[key / a.page_size];
+                if (p >= 0 && p < a.num_pages) page = p;
+                else bad = true;
+              }
+            }
+            if (use > 0) {
+              ok = tc::mbar_wait(&bars[L::B_EMPTY + slot], (use - 1) & 1, abort);
+              ok = __all_sync(0xffffffffu, ok);
+              if (!ok) break;
+            }
+            // the last keys' page goes on behind them: those value rows become zeros before the tensor cores see them
+            const bool tail = is_v && keys.y - k0 < TK && keys.y % R != 0;
+            uint64_t* full = &bars[L::B_FULL + slot];
+            uint64_t* bar = tail ? &bars[L::B_TAIL] : full;
+            unsigned char* dst = sm + L::RING + slot * TB;
+            if (lane == 0) tc::mbar_expect_tx(bar, TB);
+            __syncwarp();
+            if (lane < boxes) {
+              const int4 pos = is_v ? maps.vpos : maps.kpos;
+              int c[4];
+              c[0] = half * 64;
+              c[pos.x] = in_page;
+              c[pos.y] = head;
+              c[pos.z] = page;
+              tc::tma_load_4d(dst + half * TM * 128 + row * 128, is_v ? &maps.v : &maps.k, c[0], c[1], c[2], c[3], bar);
+            }
+            if (tail) {
+              ok = tc::mbar_wait(bar, tails & 1, abort);
+              ok = __all_sync(0xffffffffu, ok);
+              if (!ok) break;
+              ++tails;
+              const int r0 = max(0, keys.y - k0), r1 = min(TK, (r0 + R - 1) / R * R);
+              for (int x = lane; x < (r1 - r0) * (D / 8); x += 32) {
+                const int r = r0 + x / (D / 8), c = x % (D / 8);
+                *reinterpret_cast<uint4*>(dst + (c >> 3) * TM * 128 + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+              }
+              tc::fence_async_smem();
+              __syncwarp();
+              if (lane == 0) tc::mbar_arrive(full);
+            }
+          }
+          if (!ok)  // let the copies in flight land before the CTA leaves
+            for (int u = max(0, ring + i - NR); u < ring + i; ++u) {
+              const long long since = clock64();
+              while (!tc::mbar_try(&bars[L::B_FULL + u % NR], (u / NR) & 1) && clock64() - since < tc::kWaitCycles / 8) {
+              }
+            }
+        }
+      } else {
+        const T* kbase = static_cast<const T*>(a.kpool) + (long long)head * a.kps.h;
+        const T* vbase = static_cast<const T*>(a.vpool) + (long long)head * a.vps.h;
+        long long off[2][2];  // [key, value][the first 32 rows of the warp's list, the rest]
+        for (int i = 0; ok && i < 2 * tiles; ++i) {
+          const int is_v = i & 1, slot = (ring + i) % NR, use = (ring + i) / NR;
+          if (!is_v) {
+            // the warp's rows of this tile: row q of its list is row (lw + 3 (q / RPI)) RPI + q % RPI
+  #pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+              const int q = hf * 32 + lane, r = (lw + kLoaders * (q / RPI)) * RPI + q % RPI;
+              const int key = key0 + (i >> 1) * TK + r;
+              off[0][hf] = off[1][hf] = -1;
+              if (r < TK && key < keys.y) {
+                const int page = row_table[key / a.page_size], s = key % a.page_size;
+                if (page >= 0 && page < a.num_pages) {
+                  off[0][hf] = (long long)page * a.kps.p + (long long)s * a.kps.s;
+                  off[1][hf] = (long long)page * a.vps.p + (long long)s * a.vps.s;
+                } else {
+                  bad = true;
+                }
               }
             }
           }
-        }
-        if (use > 0 && !tc::mbar_try(&bars[L::B_EMPTY + slot], (use - 1) & 1)) {
-          cp_async_wait<0>();  // nothing more can start: hand over what has
-          signal_to(issued);
-          ok = tc::mbar_wait(&bars[L::B_EMPTY + slot], (use - 1) & 1, abort);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-        }
-        unsigned char* dst = sm + L::RING + slot * TB + col;
-        const T* base = is_v ? vbase : kbase;
-#pragma unroll
-        for (int x = 0; x < NI; ++x) {
-          const int g = lw + kLoaders * x;  // copy g of the tile: rows g RPI ..
-          const int q = x * RPI + sub;
-          const long long o = __shfl_sync(0xffffffffu, is_v ? off[1][(x * RPI) >> 5] : off[0][(x * RPI) >> 5], q & 31);
-          const int r = g * RPI + sub;
-          if (g < TK / RPI)
-            cp_async16(dst + r * 128 + (((chunk & 7) ^ (r & 7)) << 4), base + (o >= 0 ? o + chunk * 8 : 0), o >= 0);
-        }
-        cp_async_commit();
-        ++issued;
-        if (issued > LAG) {
-          cp_async_wait<LAG>();
-          signal_to(issued - LAG);
+          if (use > 0) {
+            ok = tc::mbar_wait(&bars[L::B_EMPTY + slot], (use - 1) & 1, abort);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+          }
+          unsigned char* dst = sm + L::RING + slot * TB + col;
+          const T* base = is_v ? vbase : kbase;
+  #pragma unroll
+          for (int x = 0; x < NI; ++x) {
+            const int g = lw + kLoaders * x;  // copy g of the tile: rows g RPI ..
+            const int q = x * RPI + sub;
+            const long long o = __shfl_sync(0xffffffffu, is_v ? off[1][(x * RPI) >> 5] : off[0][(x * RPI) >> 5], q & 31);
+            const int r = g * RPI + sub;
+            if (g < TK / RPI)
+              cp_async16(dst + r * 128 + (((chunk & 7) ^ (r & 7)) << 4), base + (o >= 0 ? o + chunk * 8 : 0), o >= 0);
+          }
+          tc::cp_async_arrive(&bars[L::B_FULL + slot]);  // arrives when this thread's copies have landed
         }
       }
-      cp_async_wait<0>();
-      signal_to(issued);
+      asm volatile("cp.async.wait_all;" ::: "memory");
       ring += 2 * tiles;
       if (bad) atomicOr(&g_fault_paged_tc, kFaultTables);
       if (!turn_over()) break;
@@ -440,14 +498,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const Page
           }
           tc::mma_commit(&bars[L::B_S + t]);
         };
+        // the copies are the loaders' own (generic proxy); the tensor cores read through the async proxy, which the
+        // fence after each wait puts behind them
         bool ok = tc::mbar_wait(&bars[L::B_Q], q_phase & 1, abort) && tile_ready(0);
         if (ok) {
+          tc::fence_async_smem();
           tc::tc_after_sync();
           for (int t = 0; t < nt; ++t) issue_s(t, 0);
           tc::mma_commit(&bars[L::B_EMPTY + ring % NR]);
         }
         for (int j = 0; ok && j < tiles; ++j) {
           if (!(ok = tile_ready(2 * j + 1))) break;
+          tc::fence_async_smem();
           const uint32_t vb = ra + ((ring + 2 * j + 1) % NR) * TB;
           for (int t = 0; ok && t < nt; ++t) {
             // P of this tile is in TMEM, and every thread is done with S
@@ -462,7 +524,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const Page
               // the scores of the next keys take the columns of P: the tensor cores work in the order of issue
               if (t == 0) {
                 if (!(ok = tile_ready(2 * j + 2))) break;
-                tc::tc_after_sync();
+                tc::fence_async_smem();
               }
               issue_s(t, 2 * j + 2);
               if (t == nt - 1) tc::mma_commit(&bars[L::B_EMPTY + (ring + 2 * j + 2) % NR]);
@@ -685,6 +747,30 @@ __global__ void __launch_bounds__(256) combine_tc_kernel(const PagedAttnArgs a, 
   }
 }
 
+// A pool as a tensor map with boxes of 64 columns and the rows of a page (of a tile, where the page is larger); false
+// where pages and tiles do not fit each other, or the layout cannot be mapped.
+bool pool_map(CUtensorMap* m, int dt, const void* pool, PoolStrides s, const PagedAttnArgs& a, int4* pos) {
+  const int ps = a.page_size;
+  if (!(ps >= 8 && TK % ps == 0) && ps % TK != 0) return false;
+  struct Dim {
+    long long stride, extent;
+    int which;  // 1 slot, 2 head, 3 page
+  } dd[3] = {{s.s, ps, 1}, {s.h, a.Hkv, 2}, {s.p, a.num_pages, 3}};
+  std::sort(dd, dd + 3, [](const Dim& x, const Dim& y) { return x.stride < y.stride; });
+  cuuint64_t dims[4] = {(cuuint64_t)a.D, 0, 0, 0}, str[3];
+  cuuint32_t box[4] = {64, 1, 1, 1};
+  int at[4] = {0, 0, 0, 0};
+  for (int i = 0; i < 3; ++i) {
+    if (dd[i].stride <= 0 || dd[i].extent <= 0) return false;
+    dims[i + 1] = (cuuint64_t)dd[i].extent;
+    str[i] = (cuuint64_t)dd[i].stride * 2;
+    at[dd[i].which] = i + 1;
+    if (dd[i].which == 1) box[i + 1] = (cuuint32_t)std::min(ps, TK);
+  }
+  *pos = make_int4(at[1], at[2], at[3], 0);
+  return tc::encode16(m, dt, 4, pool, dims, str, box);
+}
+
 long long most_items(int B, int N, int G, int row_min) {
   const long long rows = (long long)N * G;
   return rows / kItemRows + std::min<long long>(B, rows / (row_min + 1)) + 1;
@@ -709,7 +795,11 @@ int launch_paged_attention_tc(const PagedAttnArgs& a, int row_min, void* workspa
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
-  auto go = [&](auto kfn, auto joinfn, int D, int total) -> int {
+  PoolMaps maps;
+  std::memset(&maps, 0, sizeof(maps));
+  const bool tma = pool_map(&maps.k, DT, a.kpool, a.kps, a, &maps.kpos) &&
+                   pool_map(&maps.v, DT, a.vpool, a.vps, a, &maps.vpos);
+  auto go = [&](auto kfn, auto joinfn, int total) -> int {
     {
       AVQ_TIMED("paged_plan", st);
       plan_kernel<<<1, kPlanThreads, 0, st>>>(a, row_min, (int)items, ws);
@@ -727,7 +817,8 @@ int launch_paged_attention_tc(const PagedAttnArgs& a, int row_min, void* workspa
       cfg.gridDim = dim3(kSms);
       cfg.blockDim = dim3(kTcThreads);
       cfg.dynamicSmemBytes = smem;
-      if (cudaLaunchKernelEx(&cfg, kfn, a, (int)items, ws, partials, (int)wide) != cudaSuccess) return AVQ_ERR_CUDA;
+      if (cudaLaunchKernelEx(&cfg, kfn, maps, a, (int)items, ws, partials, (int)wide) != cudaSuccess)
+        return AVQ_ERR_CUDA;
     }
     AVQ_TIMED("paged_combine_tc", st);
     cfg.gridDim = dim3((unsigned)std::min<long long>(items, kMaxPieces), a.Hkv, kItemRows / kJoinRows);
@@ -737,8 +828,10 @@ int launch_paged_attention_tc(const PagedAttnArgs& a, int row_min, void* workspa
                                                                                                       : AVQ_ERR_CUDA;
   };
   if (a.D == 64)
-    return go(paged_attn_tc_kernel<DT, 64>, combine_tc_kernel<DT, 64>, 64, TcShared<64>::TOTAL);
-  return go(paged_attn_tc_kernel<DT, 128>, combine_tc_kernel<DT, 128>, 128, TcShared<128>::TOTAL);
+    return go(tma ? paged_attn_tc_kernel<DT, 64, true> : paged_attn_tc_kernel<DT, 64, false>, combine_tc_kernel<DT, 64>,
+              TcShared<64>::TOTAL);
+  return go(tma ? paged_attn_tc_kernel<DT, 128, true> : paged_attn_tc_kernel<DT, 128, false>,
+            combine_tc_kernel<DT, 128>, TcShared<128>::TOTAL);
 }
 
 int read_fault_paged_tc(int* code, cudaStream_t st) {

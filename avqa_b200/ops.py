@@ -11,8 +11,8 @@ from __future__ import annotations
 
 from dataclasses import dataclass
 
-import contextlib
 import ctypes
+import functools
 
 import torch
 
@@ -325,27 +325,33 @@ def forward(q: torch.Tensor, cb: PreparedCodebook, st: QuantState, P: int, passe
 _POSITION_BYTES = {torch.int32: 4, torch.int64: 8}
 
 
-_HERE = contextlib.nullcontext()
+def _call(what: str, fn, dev: torch.device, *args) -> None:
+    """``fn(*args, stream)`` on the current stream of ``dev`` (made current where it is not: a
+    launch goes to the current device), its status checked."""
+    index = dev.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _lib.stream_of(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _lib.stream_of(dev))
+    if rc:
+        _lib.check(rc, what)
 
 
-def _on_device(dev: torch.device):
-    """A guard that makes ``dev`` current where it is not (a launch goes to the current device)."""
-    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
-
-
-def _same(name: str, t: torch.Tensor, dev: torch.device, dtype: torch.dtype | None = None) -> None:
+def _same(name: str, t: torch.Tensor, dev: torch.device, dtype: torch.dtype) -> None:
     if t.device != dev:
         raise DeviceError(f"{name} must be on the same device", expected=str(dev), actual=str(t.device))
-    if dtype is not None and t.dtype != dtype:
+    if t.dtype != dtype:
         raise DtypeError(f"{name} has the wrong dtype", expected=str(dtype), actual=str(t.dtype))
 
 
 def _positions_operand(positions: torch.Tensor | None, axes: int, B: int, T: int, dev: torch.device):
-    """(pointer, bytes, ctypes strides {axis, b, t}) of positions ``[T]``, ``[B, T]`` with one
-    axis, or ``[axes, T]`` / ``[axes, B, T]``."""
+    """(pointer, bytes, strides (axis, b, t)) of positions ``[T]``, ``[B, T]`` with one axis, or
+    ``[axes, T]`` / ``[axes, B, T]``."""
     if positions is None:
-        return None, 0, None
-    _same("positions", positions, dev)
+        return None, 0, (0, 0, 0)
+    if positions.device != dev:
+        raise DeviceError("positions must be on the same device", expected=str(dev), actual=str(positions.device))
     nbytes = _POSITION_BYTES.get(positions.dtype)
     if nbytes is None:
         raise DtypeError("positions must be int32 or int64", expected="int32 | int64", actual=str(positions.dtype))
@@ -364,7 +370,7 @@ def _positions_operand(positions: torch.Tensor | None, axes: int, B: int, T: int
         strides = (st[0], st[1] if shape[1] > 1 else 0, st[2])
     if not ok:
         raise ShapeError("positions do not fit the tokens", expected=f"[{T}] or [{axes} axes, {B}, {T}]", actual=shape)
-    return positions.data_ptr(), nbytes, (ctypes.c_longlong * 3)(*strides)
+    return positions.data_ptr(), nbytes, strides
 
 
 def rotary(embedding, q: torch.Tensor, k: torch.Tensor | None = None, positions: torch.Tensor | None = None,
@@ -374,58 +380,73 @@ def rotary(embedding, q: torch.Tensor, k: torch.Tensor | None = None, positions:
     ``reverse``) into new tensors; no gradient is recorded here."""
     lib = _lib.load()
     _cuda(q, "query")
-    dev = q.device
+    dev, dt = q.device, q.dtype
     B, H, T, D = q.shape
+    if D != embedding.head_dim:
+        raise ShapeError("the rotary embedding's head_dim differs from the query's", expected=embedding.head_dim,
+                         actual=D)
     q_out = torch.empty_like(q)
     kp = ks = kop = kos = k_out = None
     Hk = 0
     if k is not None:
-        _same("key", k, dev, q.dtype)
+        _same("key", k, dev, dt)
+        Bk, Hk, Tk, Dk = k.shape
+        if Bk != B or Tk != T or Dk != D:
+            raise ShapeError("key must have the query's batch, tokens and head_dim", expected=(B, "Hk", T, D),
+                             actual=tuple(k.shape))
         k_out = torch.empty_like(k)
-        kp, ks, kop, kos, Hk = k.data_ptr(), _lib.strides3(k), k_out.data_ptr(), _lib.strides3(k_out), k.shape[1]
+        kp, ks, kop, kos = k.data_ptr(), _lib.strides3(k), k_out.data_ptr(), _lib.strides3(k_out)
     pos, pos_bytes, pos_strides = _positions_operand(positions, embedding.num_axes, B, T, dev)
-    with _on_device(dev):
-        rc = lib.avq_rotary(_lib.dtype_code(q.dtype), q.data_ptr(), _lib.strides3(q), H, kp, ks, Hk, B, T, D,
-                            embedding.rotary_dim, embedding.interleaved, embedding.c_frequencies, embedding.c_axes,
-                            embedding.num_axes, pos, pos_bytes, pos_strides, offset, reverse, q_out.data_ptr(),
-                            _lib.strides3(q_out), kop, kos, _lib.stream_of(dev))
-    _lib.check(rc, "avq_rotary")
+    _call("avq_rotary", lib.avq_rotary, dev, _lib.dtype_code(dt), q.data_ptr(), _lib.strides3(q), H, kp, ks, Hk, B, T,
+          D, embedding.rotary_dim, embedding.interleaved, embedding.c_frequencies, embedding.c_axes,
+          embedding.num_axes, pos, pos_bytes, _lib.longs(*pos_strides), offset, reverse, q_out.data_ptr(),
+          _lib.strides3(q_out), kop, kos)
     return q_out, k_out
 
 
-def _packed(t: torch.Tensor, name: str, heads: int | None, tokens: int | None, dim: int | None):
-    """Element strides (token, head) of a packed ``[N, H, D]`` operand."""
-    shape = t.shape
-    if t.dim() != 3 or (heads is not None and shape[1] != heads) or (tokens is not None and shape[0] != tokens) or (
-            dim is not None and shape[2] != dim):
+def _packed(t: torch.Tensor, name: str, heads: int, tokens: int, dim: int) -> ctypes.Array:
+    """Element strides (token, head) of a packed ``[tokens, heads, dim]`` operand."""
+    if t.shape != (tokens, heads, dim):
         raise ShapeError(f"{name} must be packed [tokens, heads, head_dim]", expected=(tokens, heads, dim),
-                         actual=tuple(shape))
-    if shape[2] > 1 and t.stride(2) != 1:
-        raise BackendError(f"{name} must have a contiguous last dimension", {"stride": tuple(t.stride())})
-    return (ctypes.c_longlong * 2)(t.stride(0), t.stride(1))
+                         actual=tuple(t.shape))
+    st = t.stride()
+    if st[2] != 1 and dim > 1:
+        raise BackendError(f"{name} must have a contiguous last dimension", {"stride": st})
+    return _lib.longs(st[0], st[1])
+
+
+def _packed_shape(t: torch.Tensor, name: str) -> torch.Size:
+    if t.dim() != 3:
+        raise ShapeError(f"{name} must be packed [tokens, heads, head_dim]", expected="[N, H, D]",
+                         actual=tuple(t.shape))
+    return t.shape
 
 
 def _pool(key_pool: torch.Tensor, value_pool: torch.Tensor, block_table: torch.Tensor, kv_len: torch.Tensor,
-          q_start: torch.Tensor, dev: torch.device, dtype: torch.dtype, D: int) -> tuple[int, int, int, int]:
-    """Check a page pool and a batch's lists; (batch, heads, pages, page size)."""
-    if key_pool.dim() != 4 or key_pool.shape[3] != D or value_pool.shape != key_pool.shape:
+          q_start: torch.Tensor, dev: torch.device, dtype: torch.dtype, D: int) -> tuple:
+    """Check a page pool and a batch's lists; (heads, the C calls' arguments from key_pool to
+    q_start without the leading sizes, batch)."""
+    shape = key_pool.shape
+    if len(shape) != 4 or shape[3] != D or value_pool.shape != shape:
         raise ShapeError("pools must be [pages, heads, page_size, head_dim], the values' like the keys'",
                          expected=("pages", "heads", "page_size", D),
                          actual=(tuple(key_pool.shape), tuple(value_pool.shape)))
-    for name, t in (("key_pool", key_pool), ("value_pool", value_pool)):
-        _same(name, t, dev, dtype)
-    for name, t in (("block_table", block_table), ("kv_len", kv_len), ("q_start", q_start)):
-        _same(name, t, dev, torch.int32)
-    B = kv_len.shape[0] if kv_len.dim() == 1 else -1
-    if block_table.dim() != 2 or tuple(q_start.shape) != (B + 1,) or block_table.shape[0] != B:
+    _same("key_pool", key_pool, dev, dtype)
+    _same("value_pool", value_pool, dev, dtype)
+    _same("block_table", block_table, dev, torch.int32)
+    _same("kv_len", kv_len, dev, torch.int32)
+    _same("q_start", q_start, dev, torch.int32)
+    table, lens = block_table.shape, kv_len.shape
+    if len(table) != 2 or len(lens) != 1 or table[0] != lens[0] or q_start.shape != (lens[0] + 1,):
         raise ShapeError("the batch's lists disagree: block_table [B, W], kv_len [B], q_start [B + 1]",
                          expected=("[B, W]", "[B]", "[B + 1]"),
-                         actual=(tuple(block_table.shape), tuple(kv_len.shape), tuple(q_start.shape)))
-    if (block_table.shape[1] > 1 and block_table.stride(1) != 1) or (B > 1 and kv_len.stride(0) != 1) or (
-            q_start.stride(0) != 1):
+                         actual=(tuple(table), tuple(lens), tuple(q_start.shape)))
+    row, col = block_table.stride()
+    if (col != 1 and table[1] > 1) or (lens[0] > 1 and kv_len.stride(0) != 1) or q_start.stride(0) != 1:
         raise BackendError("the batch's lists must be contiguous along their last dimension")
-    pages, heads, page_size, _ = key_pool.shape
-    return B, heads, pages, page_size
+    return shape[1], (key_pool.data_ptr(), _lib.strides3(key_pool), value_pool.data_ptr(),
+                      _lib.strides3(value_pool)), (shape[0], shape[2], block_table.data_ptr(), row, table[1],
+                                                   kv_len.data_ptr(), q_start.data_ptr(), lens[0])
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor,
@@ -447,22 +468,24 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, key_pool: torch.Tensor, value
     lib = _lib.load()
     _cuda(k, "key")
     dev, dt = k.device, k.dtype
-    ks = _packed(k, "key", None, None, None)
-    N, Hkv, D = k.shape
+    N, Hkv, D = _packed_shape(k, "key")
+    ks = _packed(k, "key", Hkv, N, D)
     _same("value", v, dev, dt)
     vs = _packed(v, "value", Hkv, N, D)
-    B, heads, pages, page_size = _pool(key_pool, value_pool, block_table, kv_len, q_start, dev, dt, D)
+    heads, pools, lists = _pool(key_pool, value_pool, block_table, kv_len, q_start, dev, dt, D)
     if heads != Hkv:
         raise ShapeError("the pool's heads differ from the keys'", expected=heads, actual=Hkv)
     H, qp, qs, qop, qos = 0, None, None, None, None
     if q is not None:
         _same("query", q, dev, dt)
-        qs = _packed(q, "query", None, N, D)
+        H = _packed_shape(q, "query")[1]
+        qs = _packed(q, "query", H, N, D)
         if q_out is None:
             q_out = torch.empty_like(q)
-        _same("q_out", q_out, dev, dt)
-        qos = _packed(q_out, "q_out", q.shape[1], N, D)
-        H, qp, qop = q.shape[1], q.data_ptr(), q_out.data_ptr()
+        else:
+            _same("q_out", q_out, dev, dt)
+        qos = _packed(q_out, "q_out", H, N, D)
+        qp, qop = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise BackendError("q_out needs q")
     R, inter, freq, axes, num_axes = 0, False, None, None, 1
@@ -474,17 +497,16 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, key_pool: torch.Tensor, value
         freq, axes = rotary.c_frequencies, rotary.c_axes
     elif positions is not None:
         raise BackendError("positions need a rotary embedding")
-    pos, pos_bytes, pos_st = _positions_operand(positions, num_axes, 1, N, dev)
-    if pos_st is not None:
-        pos_st = (ctypes.c_longlong * 2)(pos_st[0], pos_st[2])
-    with _on_device(dev):
-        rc = lib.avq_paged_append(_lib.dtype_code(dt), qp, qs, H, qop, qos, k.data_ptr(), ks, v.data_ptr(), vs, Hkv, D,
-                                  key_pool.data_ptr(), _lib.strides3(key_pool), value_pool.data_ptr(),
-                                  _lib.strides3(value_pool), pages, page_size, block_table.data_ptr(),
-                                  block_table.stride(0), block_table.shape[1], kv_len.data_ptr(), q_start.data_ptr(),
-                                  B, N, R, inter, freq, axes, num_axes, pos, pos_bytes, pos_st, _lib.stream_of(dev))
-    _lib.check(rc, "avq_paged_append")
+    pos, pos_bytes, pos_strides = _positions_operand(positions, num_axes, 1, N, dev)
+    _call("avq_paged_append", lib.avq_paged_append, dev, _lib.dtype_code(dt), qp, qs, H, qop, qos, k.data_ptr(), ks,
+          v.data_ptr(), vs, Hkv, D, *pools, *lists, N, R, inter, freq, axes, num_axes, pos, pos_bytes,
+          _lib.longs(pos_strides[0], pos_strides[2]))
     return q_out
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_workspace(code: int, B: int, N: int, H: int, Hkv: int, D: int, max_q_len: int) -> int:
+    return max(1, _lib.load().avq_paged_attention_workspace_size(code, B, N, H, Hkv, D, max_q_len))
 
 
 def paged_attention(q: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor, block_table: torch.Tensor,
@@ -506,27 +528,23 @@ def paged_attention(q: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.T
     lib = _lib.load()
     _cuda(q, "query")
     dev, dt = q.device, q.dtype
-    qs = _packed(q, "query", None, None, None)
-    N, H, D = q.shape
-    B, Hkv, pages, page_size = _pool(key_pool, value_pool, block_table, kv_len, q_start, dev, dt, D)
+    N, H, D = _packed_shape(q, "query")
+    qs = _packed(q, "query", H, N, D)
+    Hkv, pools, lists = _pool(key_pool, value_pool, block_table, kv_len, q_start, dev, dt, D)
     if Hkv == 0 or H == 0 or H % Hkv:
         raise ShapeError("query heads must be a multiple of the pool's heads", expected=f"n * {Hkv}", actual=H)
     if out is None:
-        out = torch.empty(N, H, D, dtype=dt, device=dev)
+        out = torch.empty((N, H, D), dtype=dt, device=dev)
     else:
         _same("out", out, dev, dt)
-    os_ = _packed(out, "out", H, N, D)
+    if scale is None:
+        scale = D ** -0.5 if D else 1.0
     code = _lib.dtype_code(dt)
-    ws_bytes = lib.avq_paged_attention_workspace_size(code, B, N, H, Hkv, D, max_q_len)
-    ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=dev)
-    with _on_device(dev):
-        rc = lib.avq_paged_attention(code, q.data_ptr(), qs, H, key_pool.data_ptr(), _lib.strides3(key_pool),
-                                     value_pool.data_ptr(), _lib.strides3(value_pool), Hkv, D, pages, page_size,
-                                     block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
-                                     kv_len.data_ptr(), q_start.data_ptr(), B, N, causal, window,
-                                     D ** -0.5 if scale is None else scale, max_q_len, out.data_ptr(), os_,
-                                     ws.data_ptr(), ws_bytes, _lib.stream_of(dev))
-    _lib.check(rc, "avq_paged_attention")
+    ws_bytes = _attention_workspace(code, lists[-1], N, H, Hkv, D, max_q_len)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    _call("avq_paged_attention", lib.avq_paged_attention, dev, code, q.data_ptr(), qs, H, *pools, Hkv, D, *lists, N,
+          causal, window, scale, max_q_len, out.data_ptr(),
+          _packed(out, "out", H, N, D), ws.data_ptr(), ws_bytes)
     return out
 
 

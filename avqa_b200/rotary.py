@@ -75,12 +75,9 @@ class RotaryEmbedding:
         Differentiable in ``q`` and ``k``: the gradient is the rotation by the
         negative angle.
         """
-        if q.dim() != 4 or q.shape[-1] != self.head_dim:
-            raise ShapeError("query must be [B, H, T, head_dim]", expected=self.head_dim, actual=tuple(q.shape))
-        if k is not None and (k.dim() != 4 or k.shape[-1] != self.head_dim or k.shape[0] != q.shape[0]
-                              or k.shape[2] != q.shape[2]):
-            raise ShapeError("key must have the query's batch, tokens and head_dim",
-                             expected=(q.shape[0], "Hk", q.shape[2], q.shape[3]), actual=tuple(k.shape))
+        if q.dim() != 4 or (k is not None and k.dim() != 4):
+            raise ShapeError("query and key must be [B, H, T, head_dim]", expected=4,
+                             actual=(tuple(q.shape), None if k is None else tuple(k.shape)))
         if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
             out = _Rotate.apply(self, positions, offset, False, q, k)
             return out[0] if k is None else out
