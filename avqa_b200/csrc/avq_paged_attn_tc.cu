@@ -32,6 +32,7 @@
 
 #include <algorithm>
 #include <cstring>
+#include <type_traits>
 
 #include "avq_mma.cuh"
 #include "avq_paged.cuh"
@@ -238,14 +239,34 @@ struct TcShared {
   static constexpr int Q = 0;
   static constexpr int RING = 2 * tile_bytes<D>();
   static constexpr int BARS = RING + ring_slots<D>() * tile_bytes<D>();
-  // queries; tiles full and empty; scores, probabilities and sums of each row tile; the last value tile's rows;
+  // queries; tiles full and empty; scores, probabilities (of the first 64 keys, of the others) and sums of each row tile; the last value tile's rows;
   // what is in flight when a wait was given up
   static constexpr int B_Q = 0, B_FULL = 1, B_EMPTY = B_FULL + ring_slots<D>(), B_S = B_EMPTY + ring_slots<D>(),
-                       B_P = B_S + 2, B_O = B_P + 2, B_TAIL = B_O + 2,
+                       B_P = B_S + 2, B_O = B_P + 4, B_TAIL = B_O + 2,
                        B_DRAIN = B_TAIL + 1, NBARS = B_DRAIN + 1;
   static constexpr int MISC = BARS + NBARS * 8;
   static constexpr int TOTAL = MISC + 32;
 };
+
+// max of three, a NaN wins.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+__device__ __forceinline__ float max2(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmov.b64 rc, {%6, %7};\n\t"
+      "fma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -253,10 +274,71 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// The two words of a 128-byte-swizzled matrix descriptor (avq_tc.cuh, sdesc_sw128).  Only the address, in the low word,
+// changes from one multiplication to the next; kept apart, a step of it is one 32-bit addition (with the whole
+// descriptor formed for each multiplication the issuing thread took 100 cycles for each, the tensor cores' 64).
+constexpr uint32_t kDescHigh = 64u | (1u << 14) | (2u << 29);
+constexpr uint32_t kDescRows = 1u << 16;                  // K-major rows
+constexpr uint32_t kDescCols = (TK * 128 / 16) << 16;     // MN-major: the 64-column blocks lie TK * 128 bytes apart
+
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(r));
+  return r != 0;
+}
+__device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t kind) { return (addr >> 4) | kind; }
+__device__ __forceinline__ void mma_ss_low(uint32_t d, uint32_t a_low, uint32_t b_low, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{ .reg .pred p; .reg .b64 a, b; setp.ne.b32 p, %4, 0; mov.b64 a, {%1, %5}; mov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p; }" ::"r"(d),
+      "r"(a_low), "r"(b_low), "r"(idesc), "r"((uint32_t)acc), "n"(kDescHigh)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts_low(uint32_t d, uint32_t a, uint32_t b_low, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{ .reg .pred p; .reg .b64 b; setp.ne.b32 p, %4, 0; mov.b64 b, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p; }" ::"r"(d),
+      "r"(a), "r"(b_low), "r"(idesc), "r"((uint32_t)acc), "n"(kDescHigh)
+      : "memory");
+}
+
 struct PoolMaps {  // a pool as a 4-D tensor map: d, and slots, heads and pages in the coordinates x, y and z
   CUtensorMap k, v;
   int4 kpos, vpos;
 };
+
+// exp2 of a pair on the fused multiply-adds: x = n + f with |f| <= 1/2 (n in the low bits of x + 1.5 2^23), 2^f by a
+// polynomial (least maximum relative error on the interval: 2^-13.7 of degree 3 for bf16, 2^-18.5 of degree 4 for
+// fp16, far below the rounding of P), n added to the exponent.  From -126 down it stays at about 2^-126, so it
+// serves tiles without hidden keys.
+template <int DT>
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+  constexpr float kMagic = 12582912.f;
+  x.x = fmaxf(x.x, -126.f);
+  x.y = fmaxf(x.y, -126.f);
+  const float2 magic = make_float2(kMagic, kMagic);
+  const float2 r = add_f32x2(x, magic);
+  const float2 n = add_f32x2(r, make_float2(-kMagic, -kMagic));
+  const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
+  float2 p;
+  auto both = [](float c) { return make_float2(c, c); };
+  if (DT == DT_BF16) {
+    p = fma2(f, both(0.0551716238f), both(0.2426111251f));
+    p = fma2(p, f, both(0.6932609677f));
+    p = fma2(p, f, both(0.9999280572f));
+  } else {
+    p = fma2(f, both(0.0095700966f), both(0.0559178591f));
+    p = fma2(p, f, both(0.2402474433f));
+    p = fma2(p, f, both(0.6931217909f));
+    p = fma2(p, f, both(0.9999992847f));
+  }
+  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(r.x) << 23)),
+                     __int_as_float(__float_as_int(p.y) + (__float_as_int(r.y) << 23)));
+}
+// The pairs of eight that take the polynomial: three of eight even out the exponential unit (8 cycles an
+// instruction and warp) and the instruction slots.
+constexpr uint32_t kPolyPairs = 0x00;
 
 template <int DT, int D, bool TMA>
 __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __grid_constant__ PoolMaps maps,
@@ -284,7 +366,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
     }
     for (int t = 0; t < 2; ++t) {
       tc::mbar_init(&bars[L::B_S + t], 1);
-      tc::mbar_init(&bars[L::B_P + t], TM);
+      tc::mbar_init(&bars[L::B_P + 2 * t], TM);
+      tc::mbar_init(&bars[L::B_P + 2 * t + 1], TM);
       tc::mbar_init(&bars[L::B_O + t], 1);
     }
     tc::mbar_init(&bars[L::B_TAIL], 1);
@@ -371,6 +454,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
           const int R = min(a.page_size, TK), boxes = TK / R * (D / 64);
           const int row = lane / (D / 64) * R, half = lane % (D / 64);
           int page = 0, in_page = 0, i = 0;
+          // the table entry of this lane's box, read one key tile ahead
+          auto look_up = [&](int k0) {
+            const int key = k0 + row;
+            return lane < boxes && key < keys.y ? row_table[key / a.page_size] : -1;
+          };
+          int ahead = look_up(key0);
           for (; ok && i < 2 * tiles; ++i) {
             const int is_v = i & 1, slot = (ring + i) % NR, use = (ring + i) / NR, k0 = key0 + (i >> 1) * TK;
             if (!is_v && lane < boxes) {
@@ -378,11 +467,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
               page = a.num_pages;  // outside the map: reads as zeros
               in_page = key % a.page_size;
               if (key < keys.y) {
-                const int p = row_table[key / a.page_size];
-                if (p >= 0 && p < a.num_pages) page = p;
+                if (ahead >= 0 && ahead < a.num_pages) page = ahead;
                 else bad = true;
               }
             }
+            if (!is_v && i + 2 < 2 * tiles) ahead = look_up(k0 + TK);
             if (use > 0) {
               ok = tc::mbar_wait(&bars[L::B_EMPTY + slot], (use - 1) & 1, abort);
               ok = __all_sync(0xffffffffu, ok);
@@ -474,77 +563,91 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
       if (bad) atomicOr(&g_fault_paged_tc, kFaultTables);
       if (!turn_over()) break;
     }
-  } else if (warp == W_MMA) {
-    // ---- MMA issuer ----
+  } else {
+    // ---- MMA issuer: the whole warp runs the loop, so that the descriptors stay in uniform registers (formed by one
+    // lane on its own each multiplication took longer to issue than to compute); one elected lane issues ----
     int ring = 0, q_phase = 0;
     int count[2] = {0, 0};  // P tiles of each row tile so far
     for (int turn = 0; take(turn); ++turn) {
-      const int nt = w.nt, tiles = w.tiles;
-      if (lane == 0) {
-        const int fmt = DT == DT_BF16 ? 1 : 0;
-        const uint32_t id_s = tc::idesc_f16(fmt, TM, TK, false), id_o = tc::idesc_f16(fmt, TM, D, true);
-        const uint32_t qa = tc::smem_addr(sm + L::Q), ra = tc::smem_addr(sm + L::RING);
-        auto tile_ready = [&](int i) {
-          const int n = ring + i;
-          return tc::mbar_wait(&bars[L::B_FULL + n % NR], (n / NR) & 1, abort);
-        };
-        auto issue_s = [&](int t, int i) {
-          const uint32_t kb = ra + ((ring + i) % NR) * TB;
+      const int nt = __shfl_sync(0xffffffffu, w.nt, 0), tiles = __shfl_sync(0xffffffffu, w.tiles, 0);
+      const int fmt = DT == DT_BF16 ? 1 : 0;
+      const uint32_t id_s = tc::idesc_f16(fmt, TM, TK, false), id_o = tc::idesc_f16(fmt, TM, D, true);
+      auto tile_ready = [&](int i) {
+        const int n = ring + i;
+        return tc::mbar_wait(&bars[L::B_FULL + n % NR], (n / NR) & 1, abort);
+      };
+      auto empty = [&](int i) { return &bars[L::B_EMPTY + (ring + i) % NR]; };
+      const uint32_t q_low = desc_low(tc::smem_addr(sm + L::Q), kDescRows);
+      const uint32_t r_low = desc_low(tc::smem_addr(sm + L::RING), 0);
+      auto issue_s = [&](int t, int i) {
+        const uint32_t k_low = r_low + kDescRows + ((ring + i) % NR) * (TB / 16), qt = q_low + t * (TB / 16);
+        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t o = (kk >> 2) * TM * 128 + (kk & 3) * 32;
-            tc::mma_ss(col_s + t * TK, tc::sdesc_sw128(qa + t * TB + o, 16, 1024), tc::sdesc_sw128(kb + o, 16, 1024),
-                       id_s, kk > 0);
+            const uint32_t o = ((kk >> 2) * TM * 128 + (kk & 3) * 32) / 16;
+            mma_ss_low(col_s + t * TK, qt + o, k_low + o, id_s, kk > 0);
           }
           tc::mma_commit(&bars[L::B_S + t]);
-        };
-        // the copies are the loaders' own (generic proxy); the tensor cores read through the async proxy, which the
-        // fence after each wait puts behind them
-        bool ok = tc::mbar_wait(&bars[L::B_Q], q_phase & 1, abort) && tile_ready(0);
-        if (ok) {
-          tc::fence_async_smem();
-          tc::tc_after_sync();
-          for (int t = 0; t < nt; ++t) issue_s(t, 0);
-          tc::mma_commit(&bars[L::B_EMPTY + ring % NR]);
+          if (t == nt - 1) tc::mma_commit(empty(i));
         }
-        for (int j = 0; ok && j < tiles; ++j) {
-          if (!(ok = tile_ready(2 * j + 1))) break;
-          tc::fence_async_smem();
-          const uint32_t vb = ra + ((ring + 2 * j + 1) % NR) * TB;
-          for (int t = 0; ok && t < nt; ++t) {
-            // P of this tile is in TMEM, and every thread is done with S
-            if (!(ok = tc::mbar_wait(&bars[L::B_P + t], (count[t] + j) & 1, abort))) break;
-            tc::tc_after_sync();
+        __syncwarp();
+      };
+      // cp.async writes through the generic proxy; the tensor cores read through the async proxy, which a fence after
+      // each wait puts behind those writes
+      bool ok = tc::mbar_wait(&bars[L::B_Q], q_phase & 1, abort) && tile_ready(0);
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok) {
+        tc::fence_async_smem();
+        tc::tc_after_sync();
+        issue_s(0, 0);
+        if (nt > 1) issue_s(1, 0);
+      }
+      for (int j = 0; ok && j < tiles; ++j) {
+        ok = __all_sync(0xffffffffu, tile_ready(2 * j + 1));
+        if (!ok) break;
+        if constexpr (!TMA) tc::fence_async_smem();
+        const uint32_t v_low = r_low + kDescCols + ((ring + 2 * j + 1) % NR) * (TB / 16);
 #pragma unroll
-            for (int kk = 0; kk < TK / 16; ++kk)
-              tc::mma_ts(col_o + t * D, col_s + t * TK + kk * 8, tc::sdesc_sw128(vb + kk * 16 * 128, TK * 128, 1024),
-                         id_o, j > 0 || kk > 0);
-            if (t == nt - 1) tc::mma_commit(&bars[L::B_EMPTY + (ring + 2 * j + 1) % NR]);
-            if (j + 1 < tiles) {
-              // the scores of the next keys take the columns of P: the tensor cores work in the order of issue
-              if (t == 0) {
-                if (!(ok = tile_ready(2 * j + 2))) break;
-                tc::fence_async_smem();
-              }
-              issue_s(t, 2 * j + 2);
-              if (t == nt - 1) tc::mma_commit(&bars[L::B_EMPTY + (ring + 2 * j + 2) % NR]);
-            } else {
-              tc::mma_commit(&bars[L::B_O + t]);
+        for (int t = 0; t < 2; ++t) {
+          if (t >= nt) break;
+          // P of this tile's first 64 keys is in TMEM, and every thread is done with S; then P of the others
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(&bars[L::B_P + 2 * t + hf], (count[t] + j) & 1, abort));
+            if (!ok) break;
+            tc::tc_after_sync();
+            if (elect_one()) {
+#pragma unroll
+              for (int kk = hf * (TK / 32); kk < (hf + 1) * (TK / 32); ++kk)
+                mma_ts_low(col_o + t * D, col_s + t * TK + kk * 8, v_low + kk * (16 * 128 / 16), id_o, j > 0 || kk > 0);
+              if (hf == 1 && t == nt - 1) tc::mma_commit(empty(2 * j + 1));
+              if (hf == 1 && j + 1 == tiles) tc::mma_commit(&bars[L::B_O + t]);
             }
+            __syncwarp();
+          }
+          if (!ok) break;
+          if (j + 1 < tiles) {
+            // the scores of the next keys take the columns of P: the tensor cores work in the order of issue
+            if (t == 0) {
+              ok = __all_sync(0xffffffffu, tile_ready(2 * j + 2));
+              if (!ok) break;
+              if constexpr (!TMA) tc::fence_async_smem();
+            }
+            issue_s(t, 2 * j + 2);
           }
         }
-        if (!ok) {  // let what was issued finish before the CTA leaves
-          tc::mma_commit(&bars[L::B_DRAIN]);
-          const long long since = clock64();
-          while (!tc::mbar_try(&bars[L::B_DRAIN], 0) && clock64() - since < tc::kWaitCycles / 8) {
-          }
+      }
+      if (!ok) {  // let what was issued finish before the CTA leaves
+        if (elect_one()) tc::mma_commit(&bars[L::B_DRAIN]);
+        const long long since = clock64();
+        while (!tc::mbar_try(&bars[L::B_DRAIN], 0) && clock64() - since < tc::kWaitCycles / 8) {
         }
       }
       __syncwarp();
       ring += 2 * tiles;
       ++q_phase;
-      for (int t = 0; t < 2; ++t)
-        if (t < nt) count[t] += tiles;
+      count[0] += tiles;
+      if (nt > 1) count[1] += tiles;
       if (!turn_over()) break;
     }
   }
@@ -582,7 +685,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         for (int c = 0; c < 4; ++c) tc::tmem_ld32(s_at + c * 32, s[c]);
         tc::tmem_wait_ld();
         const int k0 = key0 + j * TK;
-        if (__any_sync(0xffffffffu, k0 < first || last - k0 < TK)) {
+        const bool hidden = __any_sync(0xffffffffu, k0 < first || last - k0 < TK);
+        if (hidden) {
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -591,15 +695,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
               if (key < first || key >= last) s[c][e] = 0xff800000u;  // -inf
             }
         }
-        float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        auto at = [&](int c, int e) { return __uint_as_float(s[c][e]); };
+        float x[4];
 #pragma unroll
-        for (int e = 0; e < 32; ++e)
+        for (int c = 0; c < 4; ++c) x[c] = max2(at(c, 0), at(c, 1));
 #pragma unroll
-          for (int c = 0; c < 4; ++c) x[c] = fmaxf(x[c], __uint_as_float(s[c][e]));
-        const float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * a.scale_log2;
-        // (the maximum of a row whose keys are all hidden so far stays -inf, and -inf - -inf is no growth)
-        if (__any_sync(0xffffffffu, mx > m + kLazy || (m == -INFINITY && mx > m))) {
-          const float mn = fmaxf(m, mx), f = mn > m ? ex2(m - mn) : 1.f;
+        for (int e = 2; e < 32; e += 2)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) x[c] = max3(x[c], at(c, e), at(c, e + 1));
+        const float mx = max2(max3(x[0], x[1], x[2]), x[3]) * a.scale_log2;
+        // (the maximum of a row whose keys are all hidden so far stays -inf, which is no growth; a NaN is)
+        if (__any_sync(0xffffffffu, !(mx <= m + kLazy))) {
+          float mn = max2(m, mx);
+          if (mn == INFINITY) mn = NAN;  // a softmax over +inf
+          const float f = mn == m ? 1.f : ex2(m - mn);
           m = mn;
           l *= f;
           if (j > 0) {
@@ -614,24 +723,34 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             }
           }
         }
-        const float sub = m == -INFINITY ? 0.f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const float sub = m == -INFINITY ? 0.f : -m;
+        const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), sub2 = make_float2(sub, sub);
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        // P to TMEM by 32 keys; the tensor cores may start on the first 64.  Hidden keys need zeros: no polynomial
+        auto exps = [&](auto exact) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t pk[16];
+          for (int c = 0; c < 4; ++c) {
+            uint32_t pk[16];
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float p0 = ex2(fmaf(__uint_as_float(s[c][e]), a.scale_log2, -sub));
-            const float p1 = ex2(fmaf(__uint_as_float(s[c][e + 1]), a.scale_log2, -sub));
-            sum[c] += p0 + p1;
-            pk[e / 2] = pack2<DT>(p0, p1);
+            for (int e = 0; e < 16; ++e) {
+              const float2 y = fma2(make_float2(at(c, 2 * e), at(c, 2 * e + 1)), scale2, sub2);
+              float2 p;
+              if (!exact.value && ((kPolyPairs >> (e & 7)) & 1)) p = ex2_poly<DT>(y);
+              else p = make_float2(ex2(y.x), ex2(y.y));
+              sum[e & 1] = add_f32x2(sum[e & 1], p);
+              pk[e] = pack2<DT>(p.x, p.y);
+            }
+            tc::tmem_st16(s_at + c * 16, pk);
+            if (c & 1) {
+              tc::tmem_wait_st();
+              tc::tc_before_sync();
+              tc::mbar_arrive(&bars[L::B_P + 2 * t + (c >> 1)]);
+            }
           }
-          tc::tmem_st16(s_at + c * 16, pk);
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tc::tmem_wait_st();
-        tc::tc_before_sync();
-        tc::mbar_arrive(&bars[L::B_P + t]);
+        };
+        if (hidden) exps(std::true_type{});
+        else exps(std::false_type{});
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       }
       if (ok) {
         ok = tc::mbar_wait(&bars[L::B_O + t], o_phase & 1, abort);
@@ -641,7 +760,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         tc::tc_after_sync();
         const bool whole = np == 1;
         // a row that sees no key is zero; one whose keys all score -inf is 0 / 0
-        const float f = whole ? (last > first ? 1.f / l : 0.f) : 1.f;
+        const float f = whole ? (last > first ? (m == -INFINITY ? NAN : 1.f / l) : 0.f) : 1.f;
         T* dst = nullptr;
         float* pd = nullptr;
         if (r < rows) {

@@ -14,6 +14,8 @@ one rounding to the dtype is off, relative to the value.
   - p is rounded to the dtype (fp32 operands: split into tf32 parts, whose
     products are off by 2^-21 at most, in the scores too); below fp16's normal
     range by 2^-25 of the largest probability instead;
+  - the tcgen05 kernel takes some exponentials from a polynomial, within 2^-13
+    (bf16) or 2^-18 (fp16) of exp2; in p and in l;
   - the fp32 sums over L keys: L 2^-24;
   - each of these acts on sum p |v| / l at most, twice where it is in the
     numerator and in l;
@@ -70,6 +72,7 @@ def attention64(q, key_pool, value_pool, block_table, kv_len, q_start, causal=Tr
     rows = torch.zeros(N, dtype=torch.bool, device=q.device)
     dt = q.dtype
     part = 2.0 ** -21 if dt == torch.float32 else half(dt)
+    poly = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -13, torch.float16: 2.0 ** -18}[dt]
     table, lens, starts = block_table.tolist(), kv_len.tolist(), q_start.tolist()
     for b, L in enumerate(lens):
         at, end = starts[b], starts[b + 1]
@@ -101,7 +104,7 @@ def attention64(q, key_pool, value_pool, block_table, kv_len, q_start, causal=Tr
         weight = torch.where(some, p @ v.abs() / l, torch.zeros_like(o))
         few = torch.where(some, seen.double() @ v.abs() / l, torch.zeros_like(o)) * \
             (2.0 ** -25 if dt == torch.float16 else 2.0 ** -126)
-        e = weight * (part + 2 * ds + (L + 64) * 2.0 ** -24) + few
+        e = weight * (part + 2 * ds + 2 * poly + (L + 64) * 2.0 ** -24) + few
         e = e + (o.abs() + e) * half(dt) + tiny(dt)
         out[at:end], bound[at:end] = o.transpose(0, 1), e.transpose(0, 1)
     return out, bound, rows
