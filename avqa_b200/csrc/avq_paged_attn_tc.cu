@@ -16,15 +16,15 @@
 //   warp 8          issues S = Q K^T and O += P V
 //   warps 9-11      load Q, then the key and value tiles (128 keys each) into
 //                   a ring, in the 128-byte swizzled layout that the tensor
-//                   cores read: warp 9 by TMA where whole pages fill a tile or
-//                   whole tiles a page (page sizes 8, 16, .. 128 and multiples
-//                   of 128), else all three by cp.async, where a page may begin
-//                   and end anywhere in a tile
+//                   cores read: warps 9 and 10 by TMA where whole pages fill a
+//                   tile or whole tiles a page (page sizes 8, 16, .. 128 and
+//                   multiples of 128), else all three by cp.async, where a page
+//                   may begin and end anywhere in a tile
 //
 // Work: plan_kernel lists the (sequence, 256 rows) items and their key tiles,
-// cuts the items into pieces so that about equal shares reach every SM, and
-// the persistent CTAs fetch pieces by an atomic counter (which CTA takes a
-// piece has no influence on its result).  Pieces of one item are joined by
+// cuts the (key head, item) pairs into pieces that get smaller toward the end,
+// and the persistent CTAs fetch pieces by an atomic counter (which CTA takes a
+// piece has no influence on its result).  Pieces of one pair are joined by
 // combine_tc_kernel in the order of the keys.
 //
 // Every wait is bounded (avq_tc.cuh).
@@ -48,40 +48,46 @@ __device__ int g_fault_paged_tc;
 constexpr int TM = 128, TK = 128;  // rows of a tile, keys of a tile
 constexpr int kItemRows = 2 * TM;
 constexpr int kTcThreads = 384, kLoaders = 3, W_MMA = 8, W_LOAD = 9;
-constexpr int kMaxPieces = 8 * kSms;   // pieces of split items (each has a slot of partial sums)
-constexpr int kMaxSplit = 64;
+constexpr int kMaxSlots = 8 * kSms;    // pieces of split pairs, each with a slot of partial sums
 constexpr float kLazy = 8.f;           // log2 of the growth that rescales O
 
 template <int D> constexpr int ring_slots() { return D == 128 ? 5 : 8; }
 template <int D> constexpr int tile_bytes() { return TK * D * 2; }
 
-// The plan in the workspace: a header, then the items, then the pieces' items.
-struct Plan {
-  int* head;   // [0] pieces per key head, [1] the next piece to fetch, [2] items
-  int* base;   // [B + 1] first item of each sequence
-  int* seq;    // [items] sequence
-  int* part;   // index of the 256-row part in it
-  int* lo;     // first key (a multiple of TK)
-  int* tiles;  // key tiles
-  int* first;  // first piece (per key head)
-  int* split;  // pieces
-  int* of;     // [pieces] item
+// What a CTA needs to know of a piece.
+struct __align__(16) PieceWork {
+  int head, seq, row0, rows;      // key head, sequence; first row in it, rows from there on
+  int key0, tiles, pieces, slot;  // first key, key tiles; pieces of its pair, its slot of partial sums
+  int q0, pos0, len, end;         // the sequence's first token and that one's position, its keys; keys that the rows see
 };
 
-__host__ __device__ inline long long plan_ints(long long B, long long items) {
-  return 8 + (B + 1) + 6 * items + (items > kMaxPieces ? items : kMaxPieces);
+// The plan in the workspace: a header; the pieces; the items; the (key head, item) pairs, head by head.
+struct Plan {
+  int* head;         // [0] pieces, [1] the next piece to fetch, [2] items
+  PieceWork* piece;  // [pieces]
+  int* base;         // [B + 1] first item of each sequence
+  int* seq;          // [items] sequence
+  int* part;         // index of the 256-row part in it
+  int* tiles;        // key tiles
+  int* sum;          // key tiles of the items before
+  int* split;        // [pairs] pieces
+  int* slot;         // [pairs] first slot of partial sums, where there are several pieces
+};
+
+__host__ __device__ inline long long plan_ints(long long B, long long items, long long Hkv) {
+  return 8 + (items * Hkv + kMaxSlots) * (long long)(sizeof(PieceWork) / 4) + (B + 1) + 4 * items + 2 * items * Hkv;
 }
-__host__ __device__ inline Plan plan_at(int* p, long long B, long long items) {
+__host__ __device__ inline Plan plan_at(int* p, long long B, long long items, long long Hkv) {
   Plan q;
   q.head = p;
-  q.base = p + 8;
+  q.piece = reinterpret_cast<PieceWork*>(p + 8);
+  q.base = reinterpret_cast<int*>(q.piece + items * Hkv + kMaxSlots);
   q.seq = q.base + B + 1;
   q.part = q.seq + items;
-  q.lo = q.part + items;
-  q.tiles = q.lo + items;
-  q.first = q.tiles + items;
-  q.split = q.first + items;
-  q.of = q.split + items;
+  q.tiles = q.part + items;
+  q.sum = q.tiles + items;
+  q.split = q.sum + items;
+  q.slot = q.split + items * Hkv;
   return q;
 }
 
@@ -130,17 +136,10 @@ __device__ int block_prefix(int v, int* total) {
 
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PagedAttnArgs a, int row_min, int max_items,
                                                             int* __restrict__ ws) {
-  const Plan p = plan_at(ws, a.B, max_items);
+  const Plan p = plan_at(ws, a.B, max_items, a.Hkv);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.H / a.Hkv;
   const long long room = (long long)a.W * a.page_size;
-  __shared__ unsigned long long s_work;
-  __shared__ int s_most, s_pieces[kMaxSplit + 1];
-  __shared__ int s_choice;
   asm volatile("griddepcontrol.launch_dependents;");
-  if (tid == 0) {
-    s_work = 0;
-    s_most = 1;
-  }
   bool bad = false;
   int items = 0;
   for (int b0 = 0; b0 < a.B; b0 += kPlanThreads) {
@@ -165,8 +164,6 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PagedAttnArgs 
   }
   if (bad) atomicOr(&g_fault_paged_tc, kFaultTables);
   __syncthreads();
-  unsigned long long work = 0;
-  int most = 1;
   for (int b = warp; b < a.B; b += kPlanThreads / 32) {
     const int i0 = p.base[b], n = p.base[b + 1] - i0;
     if (n == 0) continue;
@@ -174,57 +171,71 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PagedAttnArgs 
     for (int i = lane; i < n; i += 32) {
       const int part = n - 1 - i;  // the last rows see the most keys: longest first
       const int2 k = item_keys(a, s, part, G);
-      const int t = max(1, (k.y - k.x + TK - 1) / TK);
       p.seq[i0 + i] = b;
       p.part[i0 + i] = part;
-      p.lo[i0 + i] = k.x;
-      p.tiles[i0 + i] = t;
-      work += t;
-      most = max(most, t);
+      p.tiles[i0 + i] = max(1, (k.y - k.x + TK - 1) / TK);
     }
   }
-  atomicAdd(&s_work, work);
-  atomicMax(&s_most, most);
   __syncthreads();
-  // cut the items into at most k pieces each: the k whose rounds of pieces over the SMs, with a piece's own cost of
-  // about kCost tiles (its queries, its first keys, its sums), end first
-  constexpr float kCost = 3.f;
-  for (int k = warp + 1; k <= kMaxSplit; k += kPlanThreads / 32) {
-    const int cut = (s_most + k - 1) / k;
-    int n = 0;
-    for (int i = lane; i < items; i += 32) n += (p.tiles[i] + cut - 1) / cut;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-    if (lane == 0) s_pieces[k] = n;
-  }
-  __syncthreads();
-  if (tid == 0) {
-    int best = 1;
-    float least = INFINITY;
-    for (int k = 1; k <= kMaxSplit && k <= s_most; ++k) {
-      const long long n = (long long)s_pieces[k] * a.Hkv;
-      if (k > 1 && n > kMaxPieces) break;
-      const float cost = (float)((n + kSms - 1) / kSms) * ((float)s_work / fmaxf((float)s_pieces[k], 1.f) + kCost);
-      if (cost < least) {
-        least = cost;
-        best = k;
-      }
-    }
-    s_choice = (s_most + best - 1) / best;
-  }
-  __syncthreads();
-  const int cut = s_choice;
-  int pieces = 0;
+  int head_tiles = 0;  // key tiles of one head
   for (int i0 = 0; i0 < items; i0 += kPlanThreads) {
-    const int i = i0 + tid, n = i < items ? (p.tiles[i] + cut - 1) / cut : 0;
+    const int i = i0 + tid;
     int total;
+    const int at = head_tiles + block_prefix(i < items ? p.tiles[i] : 0, &total);
+    if (i < items) p.sum[i] = at;
+    head_tiles += total;
+  }
+  // The pairs in order, each cut so that no piece is larger than an SM's share of the work that is left from its
+  // sequence and head on, so that the SMs finish together, nor than a quarter of an SM's whole share: CTAs that read
+  // the same keys then do so at about the same time (whole shares: 1095 us for 256 queries x 64 heads over 131072 keys,
+  // quarters 1018, sixths 1062, where the pieces' own cost shows).  Pieces below an eighth of the share or kLeast tiles
+  // are not made.
+  constexpr long long kLeast = 16;
+  const long long work = (long long)head_tiles * a.Hkv;
+  const long long least = max(kLeast, work / (8 * kSms)), top = max(least, work / (4 * kSms));
+  const int pairs = items * a.Hkv;
+  int pieces = 0, slots = 0;
+  for (int c0 = 0; c0 < pairs; c0 += kPlanThreads) {
+    const int c = c0 + tid;
+    int n = 0, head = 0, i = 0;
+    if (c < pairs) {
+      head = c / items;
+      i = c - head * items;
+      const long long left = work - (long long)head * head_tiles - p.sum[p.base[p.seq[i]]];
+      const long long most = min(top, max(least, (left + kSms - 1) / kSms));
+      n = (int)((p.tiles[i] + most - 1) / most);
+    }
+    int total, total_slots;
+    const int slot = slots + block_prefix(n > 1 ? n : 0, &total_slots);
+    if (n > 1 && slot + n > kMaxSlots) n = 1;  // no room for its partial sums (not with the cuts above)
     const int at = pieces + block_prefix(n, &total);
-    if (i < items) {
-      p.first[i] = at;
-      p.split[i] = n;
-      for (int s = 0; s < n; ++s) p.of[at + s] = i;
+    if (c < pairs) {
+      PieceWork w;
+      const SeqRange s = load_seq(a.q_start, a.kv_len, p.seq[i], a.N, room, &bad);
+      const int2 k = item_keys(a, s, p.part[i], G);
+      w.head = head;
+      w.seq = p.seq[i];
+      w.row0 = p.part[i] * kItemRows;
+      w.rows = s.n * G - w.row0;
+      w.pieces = n;
+      w.q0 = s.q0;
+      w.pos0 = s.pos0;
+      w.len = s.len;
+      w.end = k.y;
+      const int all = p.tiles[i];
+      for (int x = 0, t = 0; x < n; ++x) {  // equal shares of the pair's tiles
+        const int next = (int)((long long)all * (x + 1) / n);
+        w.key0 = k.x + t * TK;
+        w.tiles = next - t;
+        w.slot = slot + x;
+        p.piece[at + x] = w;
+        t = next;
+      }
+      p.split[c] = n;
+      p.slot[c] = slot;
     }
     pieces += total;
+    slots += total_slots;
   }
   if (tid == 0) {
     p.head[0] = pieces;
@@ -244,8 +255,9 @@ struct TcShared {
   static constexpr int B_Q = 0, B_FULL = 1, B_EMPTY = B_FULL + ring_slots<D>(), B_S = B_EMPTY + ring_slots<D>(),
                        B_P = B_S + 2, B_O = B_P + 4, B_TAIL = B_O + 2,
                        B_DRAIN = B_TAIL + 1, NBARS = B_DRAIN + 1;
-  static constexpr int MISC = BARS + NBARS * 8;
-  static constexpr int TOTAL = MISC + 32;
+  static constexpr int MISC = (BARS + NBARS * 8 + 15) / 16 * 16;
+  static constexpr int WORK = MISC + 16;  // two pieces
+  static constexpr int TOTAL = WORK + 2 * (int)sizeof(PieceWork);
 };
 
 // max of three, a NaN wins.
@@ -354,9 +366,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + L::BARS);
   uint32_t* tslot = reinterpret_cast<uint32_t*>(sm + L::MISC);
   volatile int* abort = reinterpret_cast<volatile int*>(sm + L::MISC + 4);
-  volatile int* next = reinterpret_cast<volatile int*>(sm + L::MISC + 8);  // [2]
+  PieceWork* works = reinterpret_cast<PieceWork*>(sm + L::WORK);  // this turn's piece and the next
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.H / a.Hkv;
-  const Plan plan = plan_at(plan_ws, a.B, max_items);
+  const Plan plan = plan_at(plan_ws, a.B, max_items, a.Hkv);
 
   if (tid == 0) {
     tc::mbar_init(&bars[L::B_Q], kLoaders * 32);
@@ -379,39 +391,23 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
   tc::tc_before_sync();
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the plan
-  if (tid == 0) next[0] = atomicAdd(&plan.head[1], 1);
+  const int pieces = plan.head[0];
+  // Fetches the piece of a turn: tiles 0 when none is left.
+  auto fetch = [&](int turn) {
+    const int piece = atomicAdd(&plan.head[1], 1);
+    PieceWork none{};
+    works[turn & 1] = piece < pieces ? plan.piece[piece] : none;
+  };
+  if (tid == kTcThreads - 1) fetch(0);
   __syncthreads();
   tc::tc_after_sync();
   const uint32_t tbase = *tslot;
-  const int per_head = plan.head[0];
-  const long long pieces = (long long)per_head * a.Hkv;
-  const long long room = (long long)a.W * a.page_size;
   const uint32_t col_s = tbase, col_o = tbase + 2 * TK;  // S (and P) of tile t at 128 t, O at 256 + D t
-
-  // The next piece, or false when none is left.  Every role calls it once a turn, after the CTA's barrier.
-  struct Work {
-    int piece, head, item, np, tiles, row0, rows, nt, key0;
-    SeqRange seq;
-  } w;
+  // The piece of a turn, or false when none is left.  Every role calls it once a turn, after the CTA's barrier.
+  PieceWork w;
   auto take = [&](int turn) {
-    w.piece = next[turn & 1];
-    if (w.piece >= pieces) return false;
-    if (tid == kTcThreads - 1) next[(turn + 1) & 1] = atomicAdd(&plan.head[1], 1);
-    w.head = w.piece / per_head;
-    const int pi = w.piece - w.head * per_head;
-    w.item = plan.of[pi];
-    w.np = plan.split[w.item];
-    // equal shares of the item's tiles
-    const int si = pi - plan.first[w.item], all = plan.tiles[w.item];
-    const int t0 = (int)((long long)all * si / w.np);
-    w.tiles = (int)((long long)all * (si + 1) / w.np) - t0;
-    bool unsound = false;  // the plan reported it
-    w.seq = load_seq(a.q_start, a.kv_len, plan.seq[w.item], a.N, room, &unsound);
-    w.row0 = plan.part[w.item] * kItemRows;
-    w.rows = w.seq.n * G - w.row0;
-    w.nt = w.rows > TM ? 2 : 1;
-    w.key0 = plan.lo[w.item] + t0 * TK;
-    return true;
+    w = works[turn & 1];
+    return w.tiles > 0;
   };
   // The end of a turn: false in every thread when one gave up.
   auto turn_over = [&]() {
@@ -428,10 +424,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
     const int lw = warp - W_LOAD;
     int ring = 0, tails = 0;  // ring tiles, tiles with a tail so far
     for (int turn = 0; take(turn); ++turn) {
-      const SeqRange seq = w.seq;
-      const int head = w.head, rows = w.rows, nt = w.nt, row0 = w.row0, tiles = w.tiles, key0 = w.key0;
+      const int head = w.head, rows = w.rows, nt = rows > TM ? 2 : 1, row0 = w.row0, tiles = w.tiles, key0 = w.key0;
+      const int end = w.end;
       bool bad = false;
-      const int2 keys = item_keys(a, seq, row0 / kItemRows, G);
       constexpr int CPR = D / 8, RPI = 32 / CPR;               // 16-byte chunks of a row, rows of a warp's copy
       constexpr int NI = (TK / RPI + kLoaders - 1) / kLoaders;  // copies of a tile by one warp
       const int sub = lane / CPR, chunk = lane % CPR;
@@ -440,65 +435,62 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         const T* q = static_cast<const T*>(a.q);
         for (int r = lw * RPI + sub; r < nt * TM; r += kLoaders * RPI) {
           const bool ok = r < rows;
-          const int tok = seq.q0 + (row0 + (ok ? r : 0)) / G, h = head * G + (row0 + (ok ? r : 0)) % G;
+          const int tok = w.q0 + (row0 + (ok ? r : 0)) / G, h = head * G + (row0 + (ok ? r : 0)) % G;
           cp_async16(sm + L::Q + (r / TM) * TB + col + (r % TM) * 128 + (((chunk & 7) ^ (r & 7)) << 4),
                      q + (long long)tok * a.qs.t + (long long)h * a.qs.h + chunk * 8, ok);
         }
         tc::cp_async_arrive(&bars[L::B_Q]);
       }
-      const int* row_table = a.table + (long long)plan.seq[w.item] * a.table_stride;
+      const int* row_table = a.table + (long long)w.seq * a.table_stride;
       bool ok = true;
       if constexpr (TMA) {
-        if (lw == 0) {
-          // lane x brings one box of a tile: 64 columns of the rows of one page, or of the tile where the page is larger
+        // The first warp brings the keys, the second the values; lane x of it one box of a tile: 64 columns of the rows
+        // of one page, or of the tile where the page is larger.  (The lanes' copies are issued one after the other, about
+        // 130 cycles each: with 16-token pages one warp for both took 4500 cycles a step, the tensor cores 3300.)
+        if (lw < 2) {
+          const bool is_v = lw == 1;
+          const CUtensorMap* map = is_v ? &maps.v : &maps.k;
+          const int4 pos = is_v ? maps.vpos : maps.kpos;
           const int R = min(a.page_size, TK), boxes = TK / R * (D / 64);
           const int row = lane / (D / 64) * R, half = lane % (D / 64);
-          int page = 0, in_page = 0, i = 0;
-          // the table entry of this lane's box, read one key tile ahead
+          // the table entry of this lane's box, read one tile ahead
           auto look_up = [&](int k0) {
             const int key = k0 + row;
-            return lane < boxes && key < keys.y ? row_table[key / a.page_size] : -1;
+            return lane < boxes && key < end ? row_table[key / a.page_size] : -1;
           };
-          int ahead = look_up(key0);
-          for (; ok && i < 2 * tiles; ++i) {
-            const int is_v = i & 1, slot = (ring + i) % NR, use = (ring + i) / NR, k0 = key0 + (i >> 1) * TK;
-            if (!is_v && lane < boxes) {
-              const int key = k0 + row;
-              page = a.num_pages;  // outside the map: reads as zeros
-              in_page = key % a.page_size;
-              if (key < keys.y) {
-                if (ahead >= 0 && ahead < a.num_pages) page = ahead;
-                else bad = true;
-              }
+          int ahead = look_up(key0), j = 0;
+          for (; ok && j < tiles; ++j) {
+            const int i = ring + 2 * j + lw, slot = i % NR, use = i / NR, k0 = key0 + j * TK;
+            const int key = k0 + row, in_page = key % a.page_size;
+            int page = a.num_pages;  // outside the map: reads as zeros
+            if (lane < boxes && key < end) {
+              if (ahead >= 0 && ahead < a.num_pages) page = ahead;
+              else bad = true;
             }
-            if (!is_v && i + 2 < 2 * tiles) ahead = look_up(k0 + TK);
+            if (j + 1 < tiles) ahead = look_up(k0 + TK);
             if (use > 0) {
               ok = tc::mbar_wait(&bars[L::B_EMPTY + slot], (use - 1) & 1, abort);
               ok = __all_sync(0xffffffffu, ok);
               if (!ok) break;
             }
             // the last keys' page goes on behind them: those value rows become zeros before the tensor cores see them
-            const bool tail = is_v && keys.y - k0 < TK && keys.y % R != 0;
+            const bool tail = is_v && end - k0 < TK && end % R != 0;
             uint64_t* full = &bars[L::B_FULL + slot];
             uint64_t* bar = tail ? &bars[L::B_TAIL] : full;
             unsigned char* dst = sm + L::RING + slot * TB;
             if (lane == 0) tc::mbar_expect_tx(bar, TB);
             __syncwarp();
             if (lane < boxes) {
-              const int4 pos = is_v ? maps.vpos : maps.kpos;
-              int c[4];
-              c[0] = half * 64;
-              c[pos.x] = in_page;
-              c[pos.y] = head;
-              c[pos.z] = page;
-              tc::tma_load_4d(dst + half * TM * 128 + row * 128, is_v ? &maps.v : &maps.k, c[0], c[1], c[2], c[3], bar);
+              auto coordinate = [&](int d) { return d == pos.x ? in_page : (d == pos.y ? head : page); };
+              tc::tma_load_4d(dst + half * TM * 128 + row * 128, map, half * 64, coordinate(1), coordinate(2),
+                              coordinate(3), bar);
             }
             if (tail) {
               ok = tc::mbar_wait(bar, tails & 1, abort);
               ok = __all_sync(0xffffffffu, ok);
               if (!ok) break;
               ++tails;
-              const int r0 = max(0, keys.y - k0), r1 = min(TK, (r0 + R - 1) / R * R);
+              const int r0 = max(0, end - k0), r1 = min(TK, (r0 + R - 1) / R * R);
               for (int x = lane; x < (r1 - r0) * (D / 8); x += 32) {
                 const int r = r0 + x / (D / 8), c = x % (D / 8);
                 *reinterpret_cast<uint4*>(dst + (c >> 3) * TM * 128 + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
@@ -509,9 +501,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             }
           }
           if (!ok)  // let the copies in flight land before the CTA leaves
-            for (int u = max(0, ring + i - NR); u < ring + i; ++u) {
+            for (int u = max(0, j - NR); u < j; ++u) {
+              const int i = ring + 2 * u + lw;
               const long long since = clock64();
-              while (!tc::mbar_try(&bars[L::B_FULL + u % NR], (u / NR) & 1) && clock64() - since < tc::kWaitCycles / 8) {
+              while (!tc::mbar_try(&bars[L::B_FULL + i % NR], (i / NR) & 1) && clock64() - since < tc::kWaitCycles / 8) {
               }
             }
         }
@@ -528,7 +521,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
               const int q = hf * 32 + lane, r = (lw + kLoaders * (q / RPI)) * RPI + q % RPI;
               const int key = key0 + (i >> 1) * TK + r;
               off[0][hf] = off[1][hf] = -1;
-              if (r < TK && key < keys.y) {
+              if (r < TK && key < end) {
                 const int page = row_table[key / a.page_size], s = key % a.page_size;
                 if (page >= 0 && page < a.num_pages) {
                   off[0][hf] = (long long)page * a.kps.p + (long long)s * a.kps.s;
@@ -560,6 +553,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
       ring += 2 * tiles;
+      if (tid == kTcThreads - 1) fetch(turn + 1);
       if (bad) atomicOr(&g_fault_paged_tc, kFaultTables);
       if (!turn_over()) break;
     }
@@ -569,7 +563,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
     int ring = 0, q_phase = 0;
     int count[2] = {0, 0};  // P tiles of each row tile so far
     for (int turn = 0; take(turn); ++turn) {
-      const int nt = __shfl_sync(0xffffffffu, w.nt, 0), tiles = __shfl_sync(0xffffffffu, w.tiles, 0);
+      const int nt = __shfl_sync(0xffffffffu, w.rows > TM ? 2 : 1, 0), tiles = __shfl_sync(0xffffffffu, w.tiles, 0);
       const int fmt = DT == DT_BF16 ? 1 : 0;
       const uint32_t id_s = tc::idesc_f16(fmt, TM, TK, false), id_o = tc::idesc_f16(fmt, TM, D, true);
       auto tile_ready = [&](int i) {
@@ -656,19 +650,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
     // ---- softmax of tile t: this thread's row is lane (tid % 128) of the tile ----
     const int t = warp >> 2, r = t * TM + (tid & 127);
     int s_count = 0, o_phase = 0;  // S tiles and pieces of this row tile so far
-    for (int turn = 0; take(turn); ++turn) {
-      if (t >= w.nt) {
+    for (int turn = 0; works[turn & 1].tiles > 0; ++turn) {
+      // (read again at the end: few registers are left beside a row of scores)
+      const PieceWork& w = works[turn & 1];
+      if (t * TM >= w.rows) {
         if (!turn_over()) break;
         continue;
       }
-      const SeqRange seq = w.seq;
-      const int head = w.head, rows = w.rows, row0 = w.row0, tiles = w.tiles, key0 = w.key0, np = w.np;
+      const int tiles = w.tiles, key0 = w.key0;
       const uint32_t lanes = (uint32_t)(warp & 3) << 21;
       const uint32_t s_at = col_s + t * TK + lanes, o_at = col_o + t * D + lanes;
       int first = 0, last = INT_MAX;  // visible keys; rows behind the last one need no mask
-      if (r < rows) {
-        const int pos = seq.pos0 + (row0 + r) / G;
-        last = a.causal ? (pos < 0 ? 0 : min(seq.len, pos + 1)) : seq.len;
+      if (r < w.rows) {
+        const int pos = w.pos0 + (w.row0 + r) / G;
+        last = a.causal ? (pos < 0 ? 0 : min(w.len, pos + 1)) : w.len;
         first = a.window > 0 ? max(0, pos - a.window + 1) : 0;
       }
       float m = -INFINITY, l = 0.f;
@@ -758,49 +753,65 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
       }
       if (ok) {
         tc::tc_after_sync();
-        const bool whole = np == 1;
+        const bool whole = w.pieces == 1;
+        const int rows = w.rows, row0 = w.row0, head = w.head;
         // a row that sees no key is zero; one whose keys all score -inf is 0 / 0
         const float f = whole ? (last > first ? (m == -INFINITY ? NAN : 1.f / l) : 0.f) : 1.f;
-        T* dst = nullptr;
-        float* pd = nullptr;
-        if (r < rows) {
-          if (whole) {
-            const int tok = seq.q0 + (row0 + r) / G, h = head * G + (row0 + r) % G;
-            dst = static_cast<T*>(a.out) + (long long)tok * a.os.t + (long long)h * a.os.h;
-          } else {
-            pd = partials + (long long)w.piece * (kItemRows * (D + 2));
+        if (whole) {
+          // through this row tile's queries, whose multiplications are over: 16-byte chunk c of a row at c ^ row % 8, then
+          // whole rows to memory
+          unsigned char* stage = sm + L::Q + t * TB + (warp & 3) * 32 * (D * 2);
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tc::tmem_ld32(o_at + c * 32, o);
+            tc::tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              uint32_t y[4];
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const float y0 = __uint_as_float(o[e + 2 * x]) * f, y1 = __uint_as_float(o[e + 2 * x + 1]) * f;
+                y[x] = last > first ? pack2<DT>(y0, y1) : 0u;
+              }
+              *reinterpret_cast<uint4*>(stage + lane * (D * 2) + (((c * 4 + e / 8) ^ (lane & 7)) << 4)) =
+                  make_uint4(y[0], y[1], y[2], y[3]);
+            }
+          }
+          __syncwarp();
+          constexpr int CPR = D / 8;
+          for (int x = lane; x < 32 * CPR; x += 32) {
+            const int rr = x / CPR, c = x % CPR, at_row = t * TM + (warp & 3) * 32 + rr;
+            if (at_row < rows) {
+              const uint4 y = *reinterpret_cast<const uint4*>(stage + rr * (D * 2) + ((c ^ (rr & 7)) << 4));
+              const int tok = w.q0 + (row0 + at_row) / G, h = head * G + (row0 + at_row) % G;
+              T* dst = static_cast<T*>(a.out) + (long long)tok * a.os.t + (long long)h * a.os.h + c * 8;
+              if (out_wide) {
+                *reinterpret_cast<uint4*>(dst) = y;
+              } else {
+                const T* e = reinterpret_cast<const T*>(&y);
+                for (int i = 0; i < 8; ++i) dst[i] = e[i];
+              }
+            }
+          }
+        } else {
+          // four columns of 256 rows side by side: a warp's stores are contiguous
+          float* pd = partials + (long long)w.slot * (kItemRows * (D + 2));
+          if (r < rows) {
             pd[kItemRows * D + r] = m;
             pd[kItemRows * (D + 1) + r] = l;
-            pd += (long long)r * D;
           }
-        }
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          tc::tmem_ld32(o_at + c * 32, o);
-          tc::tmem_wait_ld();
-          if (dst) {
-            if (last <= first) {
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tc::tmem_ld32(o_at + c * 32, o);
+            tc::tmem_wait_ld();
+            if (r < rows) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = 0;
+              for (int e = 0; e < 32; e += 4)
+                *reinterpret_cast<uint4*>(pd + ((c * 8 + e / 4) * kItemRows + r) * 4) =
+                    make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
             }
-            if (out_wide) {
-#pragma unroll
-              for (int e = 0; e < 32; e += 8) {
-                uint4 y;
-                y.x = pack2<DT>(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 1]) * f);
-                y.y = pack2<DT>(__uint_as_float(o[e + 2]) * f, __uint_as_float(o[e + 3]) * f);
-                y.z = pack2<DT>(__uint_as_float(o[e + 4]) * f, __uint_as_float(o[e + 5]) * f);
-                y.w = pack2<DT>(__uint_as_float(o[e + 6]) * f, __uint_as_float(o[e + 7]) * f);
-                *reinterpret_cast<uint4*>(dst + c * 32 + e) = y;
-              }
-            } else {
-              for (int e = 0; e < 32; ++e) dst[c * 32 + e] = from_f<DT>(__uint_as_float(o[e]) * f);
-            }
-          } else if (pd) {
-#pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<uint4*>(pd + c * 32 + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
           }
         }
         tc::tc_before_sync();
@@ -815,54 +826,89 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
   if (tid == 0 && *abort) atomicOr(&g_fault_paged_tc, 1);
 }
 
-// Joins an item's pieces: a block per (item, 32 rows), in the order of the keys.
+// Joins a pair's pieces: a block per (pair, 32 rows), in the order of the keys.
 constexpr int kJoinRows = 32;
 
 template <int DT, int D>
 __global__ void __launch_bounds__(256) combine_tc_kernel(const PagedAttnArgs a, int max_items,
                                                          int* __restrict__ plan_ws,
-                                                         const float* __restrict__ partials) {
+                                                         const float* __restrict__ partials, int out_wide) {
   using T = typename Storage<DT>::T;
-  const Plan plan = plan_at(plan_ws, a.B, max_items);
+  const Plan plan = plan_at(plan_ws, a.B, max_items, a.Hkv);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int item = blockIdx.x, head = blockIdx.y, G = a.H / a.Hkv;
-  if (item >= plan.head[2]) return;
-  const int np = plan.split[item];
+  const int items = plan.head[2], pair = blockIdx.x, G = a.H / a.Hkv;
+  if (pair >= items * a.Hkv) return;
+  const int np = plan.split[pair], head = pair / items, item = pair - head * items;
   if (np <= 1) return;
   bool bad = false;
   const SeqRange seq = load_seq(a.q_start, a.kv_len, plan.seq[item], a.N, (long long)a.W * a.page_size, &bad);
   const int row0 = plan.part[item] * kItemRows, rows = min(kItemRows, seq.n * G - row0);
   const long long stride = kItemRows * (D + 2);
-  const float* base = partials + ((long long)head * plan.head[0] + plan.first[item]) * stride;
-  for (int i = threadIdx.x; i < kJoinRows * (D / 4); i += 256) {
-    const int r = blockIdx.z * kJoinRows + i / (D / 4), d = i % (D / 4) * 4;
-    if (r >= rows) break;
-    float M = -INFINITY;
-    for (int s = 0; s < np; ++s) M = fmaxf(M, base[s * stride + kItemRows * D + r]);
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.f;
-#pragma unroll 4
-    for (int s = 0; s < np; ++s) {
-      const float* w = base + s * stride;
-      const float m = w[kItemRows * D + r], ls = w[kItemRows * (D + 1) + r];
-      const float4 o = *reinterpret_cast<const float4*>(w + (long long)r * D + d);
-      if (m == -INFINITY && ls == 0.f) continue;  // a piece whose keys this row does not see
-      const float f = m == -INFINITY ? 0.f : ex2(m - M);
-      x.x = fmaf(o.x, f, x.x);
-      x.y = fmaf(o.y, f, x.y);
-      x.z = fmaf(o.z, f, x.z);
-      x.w = fmaf(o.w, f, x.w);
-      l = fmaf(ls, f, l);
-    }
-    const int pos = seq.pos0 + (row0 + r) / G;
-    const int last = a.causal ? (pos < 0 ? 0 : min(seq.len, pos + 1)) : seq.len;
-    const int first = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-    const float inv = 1.f / l;
-    const int tok = seq.q0 + (row0 + r) / G, h = head * G + (row0 + r) % G;
-    T* dst = static_cast<T*>(a.out) + (long long)tok * a.os.t + (long long)h * a.os.h + d;
-    const float y[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
+  const float* base = partials + (long long)plan.slot[pair] * stride;
+  // the pieces' weights, a warp for four rows
+  __shared__ float weight[kSms][kJoinRows];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r0 = blockIdx.y * kJoinRows;
+  if (r0 >= rows) return;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) dst[e] = from_f<DT>(last > first ? y[e] : 0.f);
+  for (int x = 0; x < kJoinRows / 8; ++x) {
+    const int row = warp * (kJoinRows / 8) + x, r = min(r0 + row, rows - 1);
+    const float* bm = base + kItemRows * D + r;
+    float M = -INFINITY;
+    for (int s = lane; s < np; s += 32) M = fmaxf(M, bm[s * stride]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    float sum = 0.f;
+    for (int s = lane; s < np; s += 32) {
+      const float m = bm[s * stride], l = bm[s * stride + kItemRows];
+      // a piece whose keys the row does not see (or that all score -inf) has no weight; a NaN stays one
+      const float f = m == -INFINITY ? 0.f : ex2(m - M);
+      weight[s][row] = f;
+      if (f != 0.f) sum = fmaf(l, f, sum);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    for (int s = lane; s < np; s += 32) weight[s][row] *= 1.f / sum;  // (no weight at all: 0 / 0)
+  }
+  __syncthreads();
+  const int r = r0 + lane;
+  if (r >= rows) return;
+  const int pos = seq.pos0 + (row0 + r) / G;
+  const int last = a.causal ? (pos < 0 ? 0 : min(seq.len, pos + 1)) : seq.len;
+  const int first = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+  constexpr int NC = D / 4 / 8;  // a thread's groups of four columns
+  float4 x[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) x[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = 0; s < np; ++s) {
+    const float f = weight[s][lane];
+    float4 o[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      o[c] = *reinterpret_cast<const float4*>(base + s * stride + ((warp * NC + c) * kItemRows + r) * 4);
+    if (f == 0.f) continue;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      x[c].x = fmaf(o[c].x, f, x[c].x);
+      x[c].y = fmaf(o[c].y, f, x[c].y);
+      x[c].z = fmaf(o[c].z, f, x[c].z);
+      x[c].w = fmaf(o[c].w, f, x[c].w);
+    }
+  }
+  const int tok = seq.q0 + (row0 + r) / G, h = head * G + (row0 + r) % G;
+  T* dst = static_cast<T*>(a.out) + (long long)tok * a.os.t + (long long)h * a.os.h + warp * NC * 4;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const float y[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
+    T e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = from_f<DT>(last > first ? y[i] : 0.f);
+    if (out_wide) {
+      *reinterpret_cast<uint2*>(dst + c * 4) = *reinterpret_cast<const uint2*>(e);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) dst[c * 4 + i] = e[i];
+    }
   }
 }
 
@@ -894,21 +940,22 @@ long long most_items(int B, int N, int G, int row_min) {
   const long long rows = (long long)N * G;
   return rows / kItemRows + std::min<long long>(B, rows / (row_min + 1)) + 1;
 }
-size_t plan_bytes(int B, long long items) { return align_up((size_t)plan_ints(B, items) * sizeof(int)); }
+size_t plan_bytes(int B, long long items, int Hkv) {
+  return align_up((size_t)plan_ints(B, items, Hkv) * sizeof(int));
+}
 
 }  // namespace
 
 size_t paged_attn_tc_workspace_bytes(int B, int N, int H, int Hkv, int D, int row_min) {
   const long long items = most_items(B, N, H / Hkv, row_min);
-  const long long slots = std::min<long long>(kMaxPieces, items * Hkv * kMaxSplit);
-  return plan_bytes(B, items) + align_up((size_t)slots * kItemRows * (D + 2) * sizeof(float));
+  return plan_bytes(B, items, Hkv) + align_up((size_t)kMaxSlots * kItemRows * (D + 2) * sizeof(float));
 }
 
 template <int DT>
 int launch_paged_attention_tc(const PagedAttnArgs& a, int row_min, void* workspace, cudaStream_t st) {
   const long long items = most_items(a.B, a.N, a.H / a.Hkv, row_min);
   int* ws = static_cast<int*>(workspace);
-  float* partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan_bytes(a.B, items));
+  float* partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan_bytes(a.B, items, a.Hkv));
   using T = typename Storage<DT>::T;
   const bool wide = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.os.t % 8 == 0 && a.os.h % 8 == 0;
   cudaLaunchAttribute attr;
@@ -940,10 +987,10 @@ int launch_paged_attention_tc(const PagedAttnArgs& a, int row_min, void* workspa
         return AVQ_ERR_CUDA;
     }
     AVQ_TIMED("paged_combine_tc", st);
-    cfg.gridDim = dim3((unsigned)std::min<long long>(items, kMaxPieces), a.Hkv, kItemRows / kJoinRows);
+    cfg.gridDim = dim3((unsigned)(items * a.Hkv), kItemRows / kJoinRows);
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 0;
-    return cudaLaunchKernelEx(&cfg, joinfn, a, (int)items, ws, (const float*)partials) == cudaSuccess ? AVQ_OK
+    return cudaLaunchKernelEx(&cfg, joinfn, a, (int)items, ws, (const float*)partials, (int)wide) == cudaSuccess ? AVQ_OK
                                                                                                       : AVQ_ERR_CUDA;
   };
   if (a.D == 64)
