@@ -36,7 +36,8 @@ namespace {
 
 __device__ int g_fault_tables_paged;
 
-constexpr int kRows = 16, kWarps = 4, kStepKeys = 16;
+constexpr int kRows = 16, kWarps = 4;
+constexpr int kSpanUnit = 128;  // spans are multiples of a CTA's largest step
 constexpr int kTargetCtas = 16 * kSms, kMinSpan = 128;
 // Rows (new tokens x heads of a group) of a sequence up to which one pass of 16-row groups over its keys is
 // taken, above which the tcgen05 kernel.
@@ -79,7 +80,7 @@ __device__ Piece find_piece(const PagedAttnArgs& a, int row_max, long long at, b
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   if (report && bad) atomicOr(&g_fault_tables_paged, kFaultTables);
   long long span = (total + kTargetCtas - 1) / kTargetCtas;
-  span = (max(span, (long long)kMinSpan) + kWarps * kStepKeys - 1) / (kWarps * kStepKeys) * (kWarps * kStepKeys);
+  span = (max(span, (long long)kMinSpan) + kSpanUnit - 1) / kSpanUnit * kSpanUnit;
   Piece p;
   p.found = false;
   long long before = 0, slots = 0;  // pieces and partial slots of the sequences before
@@ -182,15 +183,16 @@ __device__ __forceinline__ void mma_split(float* d, const uint32_t* ah, const ui
   for (int e = 0; e < 4; ++e) d[e] += x[e];
 }
 
+// Keys of a warp's step: 8 KB of keys and values, 16 keys at least (a step's shuffles, votes and address
+// arithmetic are the same for 32 keys as for 16).
 template <int DT, int DP>
-constexpr int stage_elems() { return 2 * kStepKeys * (DP + Operand<DT>::kPad); }
-// Stages of a warp's ring: two or three, so that three CTAs or more share an SM and one's first loads overlap the
-// others' streams (the widest rows: one stage, one CTA).
+constexpr int step_keys() { return DP * (int)sizeof(typename Storage<DT>::T) <= 128 ? 32 : 16; }
 template <int DT, int DP>
-constexpr int ring_stages() {
-  const int row = DP * (int)sizeof(typename Storage<DT>::T);
-  return row <= 128 ? 3 : (row <= 512 ? 2 : 1);
-}
+constexpr int stage_elems() { return 2 * step_keys<DT, DP>() * (DP + Operand<DT>::kPad); }
+// Stages of a warp's ring: two, so that three CTAs or more share an SM and one's first loads overlap the others'
+// streams (the widest rows: one stage, one CTA).
+template <int DT, int DP>
+constexpr int ring_stages() { return DP * (int)sizeof(typename Storage<DT>::T) <= 512 ? 2 : 1; }
 template <int DT, int DP>
 constexpr size_t mma_smem() {
   const size_t T = sizeof(typename Storage<DT>::T);
@@ -199,10 +201,18 @@ constexpr size_t mma_smem() {
   return std::max(ring, merge) + (size_t)kRows * (DP + Operand<DT>::kPad) * T;
 }
 
-template <int DT, int DP, bool WIDE>
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// WIDE: 16-byte copies.  SAME: the pools have the same strides, so a key's and its value's places do too.
+template <int DT, int DP, bool WIDE, bool SAME>
 __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const PagedAttnArgs a, int row_max,
                                                                      int q_wide, float* __restrict__ part) {
   using T = typename Storage<DT>::T;
+  constexpr int KS = step_keys<DT, DP>(), NK = KS / 8;  // keys of a step, in columns of 8
   constexpr int LDS = DP + Operand<DT>::kPad, NT = DP / 8, STAGES = ring_stages<DT, DP>();
   constexpr int EPC = 16 / (int)sizeof(T), CPR = DP / EPC;  // elements of a 16-byte chunk, chunks of a row
   extern __shared__ __align__(128) unsigned char smem_raw[];
@@ -244,44 +254,51 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
   const int2 vf = visible(a, p.seq.pos0 + row0 / G, p.seq.len);
   const int2 vl = visible(a, p.seq.pos0 + (row0 + nrow - 1) / G, p.seq.len);
   const int lo = max(p.lo, vf.x), hi = min(p.hi, vl.y);
-  const int steps = hi > lo ? (hi - lo + kWarps * kStepKeys - 1) / (kWarps * kStepKeys) : 0;
+  const int steps = hi > lo ? (hi - lo + kWarps * KS - 1) / (kWarps * KS) : 0;
+  // keys in [every_lo, every_hi) are visible to every row
+  const int every_lo = vl.x, every_hi = min(hi, vf.y);
   const T* kbase = static_cast<const T*>(a.kpool) + (long long)p.head * a.kps.h;
   const T* vbase = static_cast<const T*>(a.vpool) + (long long)p.head * a.vps.h;
   const int* row_table = a.table + (long long)p.b * a.table_stride;
   bool bad = false;
 
-  // One stage: 16 keys and their values.  Keys outside the span, and pages outside the pool, read as zeros.
+  // One stage: KS keys and their values.  Keys outside the span, and pages outside the pool, read as zeros.
   auto load = [&](int step) {
-    const int k0 = lo + (step * kWarps + warp) * kStepKeys;
+    const int k0 = lo + (step * kWarps + warp) * KS;
     T* dst = ring + (step % STAGES) * stage_elems<DT, DP>();
     // each lane looks up one key; the chunks' lanes take the address from it
-    const int key = k0 + (lane & 15);
+    const int key = k0 + (lane % KS);
     long long ko = -1, vo = -1;
     if (step < steps && key < hi) {
       const int page = row_table[key / a.page_size], s = key % a.page_size;
       if (page >= 0 && page < a.num_pages) {
         ko = (long long)page * a.kps.p + (long long)s * a.kps.s;
-        vo = (long long)page * a.vps.p + (long long)s * a.vps.s;
+        vo = SAME ? ko : (long long)page * a.vps.p + (long long)s * a.vps.s;
       } else {
         bad = true;
       }
     }
     if constexpr (WIDE) {
+      const int c = lane % CPR * EPC;
+      T* d = dst + lane / CPR * LDS + c;
 #pragma unroll
-      for (int i = 0; i < kStepKeys * CPR / 32; ++i) {
-        const int x = i * 32 + lane, r = x / CPR, c = (x % CPR) * EPC;
-        const long long k_at = __shfl_sync(0xffffffffu, ko, r), v_at = __shfl_sync(0xffffffffu, vo, r);
-        const bool ok = k_at >= 0 && c < a.D;
-        cp_async16(dst + r * LDS + c, kbase + (ok ? k_at + c : 0), ok);
-        cp_async16(dst + (kStepKeys + r) * LDS + c, vbase + (ok ? v_at + c : 0), ok);
+      for (int i = 0; i < KS * CPR / 32; ++i) {
+        const int r = CPR <= 32 ? i * (32 / CPR) + lane / CPR : i / (CPR / 32);
+        const int cc = CPR <= 32 ? c : (i % (CPR / 32) * 32 + lane) * EPC;
+        T* to = CPR <= 32 ? d + i * (32 / CPR) * LDS : dst + r * LDS + cc;
+        const long long k_at = __shfl_sync(0xffffffffu, ko, r);
+        const long long v_at = SAME ? k_at : __shfl_sync(0xffffffffu, vo, r);
+        const bool ok = k_at >= 0 && cc < a.D;
+        cp_async16(to, kbase + (ok ? k_at + cc : 0), ok);
+        cp_async16(to + KS * LDS, vbase + (ok ? v_at + cc : 0), ok);
       }
     } else {
-      for (int r = 0; r < kStepKeys; ++r) {
+      for (int r = 0; r < KS; ++r) {
         const long long k_at = __shfl_sync(0xffffffffu, ko, r), v_at = __shfl_sync(0xffffffffu, vo, r);
         for (int c = lane; c < DP; c += 32) {
           const bool ok = k_at >= 0 && c < a.D;
           dst[r * LDS + c] = ok ? kbase[k_at + c] : from_f<DT>(0.f);
-          dst[(kStepKeys + r) * LDS + c] = ok ? vbase[v_at + c] : from_f<DT>(0.f);
+          dst[(KS + r) * LDS + c] = ok ? vbase[v_at + c] : from_f<DT>(0.f);
         }
       }
     }
@@ -309,18 +326,21 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
     cp_async_wait<STAGES - 1>();
     __syncwarp();
     const T* sk = ring + (step % STAGES) * stage_elems<DT, DP>();
-    const T* sv = sk + kStepKeys * LDS;
-    float s[2][4];
+    const T* sv = sk + KS * LDS;
+    float s[NK][4];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+    for (int j = 0; j < NK; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
     if constexpr (DT != DT_F32) {
 #pragma unroll
       for (int kk = 0; kk < DP / 16; ++kk) {
-        uint32_t b0, b1, b2, b3;
         const int qd = lane >> 3;
-        ldsm_x4(b0, b1, b2, b3, sk + ((qd >> 1) * 8 + (lane & 7)) * LDS + kk * 16 + (qd & 1) * 8);
-        mma16816<DT>(s[0], qf[kk], b0, b1);
-        mma16816<DT>(s[1], qf[kk], b2, b3);
+#pragma unroll
+        for (int j = 0; j < NK; j += 2) {
+          uint32_t b0, b1, b2, b3;
+          ldsm_x4(b0, b1, b2, b3, sk + (j * 8 + (qd >> 1) * 8 + (lane & 7)) * LDS + kk * 16 + (qd & 1) * 8);
+          mma16816<DT>(s[j], qf[kk], b0, b1);
+          mma16816<DT>(s[j + 1], qf[kk], b2, b3);
+        }
       }
     } else {
 #pragma unroll 4
@@ -332,24 +352,32 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
         split_tf32(to_f(sq[r * LDS + c + 4]), ah[2], al[2]);
         split_tf32(to_f(sq[(r + 8) * LDS + c + 4]), ah[3], al[3]);
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < NK; ++j)
           mma_split(s[j], ah, al, to_f(sk[(j * 8 + r) * LDS + c]), to_f(sk[(j * 8 + r) * LDS + c + 4]));
       }
     }
-    const int k0 = lo + (step * kWarps + warp) * kStepKeys;
+#pragma unroll
+    for (int j = 0; j < NK; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[j][e] *= a.scale_log2;
+    const int k0 = lo + (step * kWarps + warp) * KS;
+    if (k0 < every_lo || k0 + KS > every_hi) {
+#pragma unroll
+      for (int j = 0; j < NK; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = k0 + j * 8 + ct + (e & 1);
+          const int2 v = e >= 2 ? vb : va;
+          if (key < v.x || key >= min(v.y, hi)) s[j][e] = -INFINITY;
+        }
+    }
+    // (fmaxf drops a NaN score; its probability is NaN and carries it into the sum)
     float ta = -INFINITY, tb = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int key = k0 + j * 8 + ct + (e & 1);
-        const int2 v = e >= 2 ? vb : va;
-        const bool seen = key >= v.x && key < min(v.y, hi);
-        s[j][e] = seen ? s[j][e] * a.scale_log2 : -INFINITY;
-        if (e >= 2) tb = fmaxf(tb, s[j][e]);
-        else ta = fmaxf(ta, s[j][e]);
-        // (fmaxf drops a NaN score; its probability is NaN and carries it into the sum)
-      }
+    for (int j = 0; j < NK; ++j) {
+      ta = fmaxf(ta, fmaxf(s[j][0], s[j][1]));
+      tb = fmaxf(tb, fmaxf(s[j][2], s[j][3]));
+    }
 #pragma unroll
     for (int of = 1; of <= 2; of <<= 1) {
       ta = fmaxf(ta, __shfl_xor_sync(0xffffffffu, ta, of));
@@ -357,7 +385,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
     }
     const float na = fmaxf(ma, ta), nb = fmaxf(mb, tb);
     if (__any_sync(0xffffffffu, na > ma || nb > mb)) {
-      const float ca = na > ma ? exp2f(ma - na) : 1.f, cb = nb > mb ? exp2f(mb - nb) : 1.f;
+      const float ca = na > ma ? ex2(ma - na) : 1.f, cb = nb > mb ? ex2(mb - nb) : 1.f;
       la *= ca;
       lb *= cb;
 #pragma unroll
@@ -373,29 +401,32 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
     // a row with no visible key so far keeps probabilities of zero
     const float xa = ma == -INFINITY ? 0.f : ma, xb = mb == -INFINITY ? 0.f : mb;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      s[j][0] = exp2f(s[j][0] - xa);
-      s[j][1] = exp2f(s[j][1] - xa);
-      s[j][2] = exp2f(s[j][2] - xb);
-      s[j][3] = exp2f(s[j][3] - xb);
+    for (int j = 0; j < NK; ++j) {
+      s[j][0] = ex2(s[j][0] - xa);
+      s[j][1] = ex2(s[j][1] - xa);
+      s[j][2] = ex2(s[j][2] - xb);
+      s[j][3] = ex2(s[j][3] - xb);
       la += s[j][0] + s[j][1];
       lb += s[j][2] + s[j][3];
     }
     if constexpr (DT != DT_F32) {
-      const uint32_t pf[4] = {pack2<DT>(s[0][0], s[0][1]), pack2<DT>(s[0][2], s[0][3]), pack2<DT>(s[1][0], s[1][1]),
-                              pack2<DT>(s[1][2], s[1][3])};
 #pragma unroll
-      for (int jj = 0; jj < NT / 2; ++jj) {
-        uint32_t b0, b1, b2, b3;
-        const int qd = lane >> 3;
-        ldsm_x4_t(b0, b1, b2, b3, sv + ((qd & 1) * 8 + (lane & 7)) * LDS + jj * 16 + (qd >> 1) * 8);
-        mma16816<DT>(o[2 * jj], pf, b0, b1);
-        mma16816<DT>(o[2 * jj + 1], pf, b2, b3);
+      for (int j = 0; j < NK; j += 2) {
+        const uint32_t pf[4] = {pack2<DT>(s[j][0], s[j][1]), pack2<DT>(s[j][2], s[j][3]),
+                                pack2<DT>(s[j + 1][0], s[j + 1][1]), pack2<DT>(s[j + 1][2], s[j + 1][3])};
+#pragma unroll
+        for (int jj = 0; jj < NT / 2; ++jj) {
+          uint32_t b0, b1, b2, b3;
+          const int qd = lane >> 3;
+          ldsm_x4_t(b0, b1, b2, b3, sv + (j * 8 + (qd & 1) * 8 + (lane & 7)) * LDS + jj * 16 + (qd >> 1) * 8);
+          mma16816<DT>(o[2 * jj], pf, b0, b1);
+          mma16816<DT>(o[2 * jj + 1], pf, b2, b3);
+        }
       }
     } else {
       // the k index t of the fragment stands for key 2t, t + 4 for key 2t + 1: the accumulators' own layout
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < NK; ++j) {
         uint32_t ph[4], pl[4];
         split_tf32(s[j][0], ph[0], pl[0]);
         split_tf32(s[j][2], ph[1], pl[1]);
@@ -434,7 +465,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
     Ma = fmaxf(Ma, sm[w * kRows + ra]);
     Mb = fmaxf(Mb, sm[w * kRows + rb]);
   }
-  const float fa = ma == -INFINITY ? 0.f : exp2f(ma - Ma), fb = mb == -INFINITY ? 0.f : exp2f(mb - Mb);
+  const float fa = ma == -INFINITY ? 0.f : ex2(ma - Ma), fb = mb == -INFINITY ? 0.f : ex2(mb - Mb);
   // (a maximum of +inf gives NaN here and in the probabilities, as a softmax over +inf does)
   if ((lane & 3) == 0) {
     sl[warp * kRows + ra] = la * fa;
@@ -532,7 +563,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const PagedAtt
         }
         // a span whose keys the row does not see (or that all score -inf) adds nothing
         if (m == -INFINITY && ls == 0.f) continue;
-        const float f = m == -INFINITY ? 0.f : exp2f(m - M);
+        const float f = m == -INFINITY ? 0.f : ex2(m - M);
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -615,7 +646,9 @@ int launch_mma(const PagedAttnArgs& a, int row_max, float* part, cudaStream_t st
   const long long pieces = most_pieces(a.B, a.N, a.H, a.Hkv, row_max);
   const long long items = most_items(a.B, a.N, a.H, a.Hkv, row_max);
   const size_t smem = mma_smem<DT, DP>();
-  auto kfn = wide ? paged_attn_mma_kernel<DT, DP, true> : paged_attn_mma_kernel<DT, DP, false>;
+  const bool same = a.kps.p == a.vps.p && a.kps.s == a.vps.s;
+  auto kfn = !wide ? paged_attn_mma_kernel<DT, DP, false, false>
+                   : (same ? paged_attn_mma_kernel<DT, DP, true, true> : paged_attn_mma_kernel<DT, DP, true, false>);
   if (cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return AVQ_ERR_CUDA;
   {

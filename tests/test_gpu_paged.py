@@ -90,6 +90,7 @@ CASES = {
     "window": ("bf16", 4, 2, 64, 16, [50, 1, 3], [400, 90, 3], dict(window=33)),
     "window_one": ("bf16", 2, 1, 128, 16, [70], [200], dict(window=1)),
     "scale": ("f16", 2, 2, 64, 16, [3], [77], dict(scale=0.7)),
+    "scale_zero": ("f16", 2, 2, 64, 16, [3, 40], [77, 60], dict(scale=0.0)),
     "negative_scale": ("bf16", 2, 2, 64, 16, [3], [77], dict(scale=-0.2)),
     "wide_group": ("bf16", 40, 1, 128, 32, [1, 2, 9], [500, 40, 9], {}),
     "group_of_three": ("bf16", 9, 3, 64, 16, [1, 20], [129, 61], {}),
