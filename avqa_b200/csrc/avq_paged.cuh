@@ -15,9 +15,23 @@
 // device fault word that avq_device_fault reports.
 #pragma once
 
+#include <atomic>
+
 #include "avq_kernels.cuh"
 
 namespace avq {
+
+// Allows a kernel its dynamic shared memory, once a device (`done`: the kernel's own record, a bit per device).
+inline bool allow_smem(const void* kernel, size_t bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+  if (bit && (done.load(std::memory_order_relaxed) & bit)) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess)
+    return false;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return true;
+}
 
 constexpr int kFaultTables = 2;  // bit 1 of the device fault record (bit 0: an abandoned wait)
 constexpr int kSms = 148;

@@ -647,10 +647,12 @@ int launch_mma(const PagedAttnArgs& a, int row_max, float* part, cudaStream_t st
   const long long items = most_items(a.B, a.N, a.H, a.Hkv, row_max);
   const size_t smem = mma_smem<DT, DP>();
   const bool same = a.kps.p == a.vps.p && a.kps.s == a.vps.s;
-  auto kfn = !wide ? paged_attn_mma_kernel<DT, DP, false, false>
-                   : (same ? paged_attn_mma_kernel<DT, DP, true, true> : paged_attn_mma_kernel<DT, DP, true, false>);
-  if (cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return AVQ_ERR_CUDA;
+  const int variant = !wide ? 0 : (same ? 2 : 1);
+  auto kfn = variant == 0 ? paged_attn_mma_kernel<DT, DP, false, false>
+                          : (variant == 1 ? paged_attn_mma_kernel<DT, DP, true, false>
+                                          : paged_attn_mma_kernel<DT, DP, true, true>);
+  static std::atomic<unsigned long long> allowed[3];
+  if (!allow_smem((const void*)kfn, smem, allowed[variant])) return AVQ_ERR_CUDA;
   {
     AVQ_TIMED("paged_attn", st);
     kfn<<<(unsigned)pieces, kWarps * 32, smem, st>>>(a, row_max, (int)q_wide, part);

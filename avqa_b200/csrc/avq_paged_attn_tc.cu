@@ -978,8 +978,8 @@ int launch_paged_attention_tc(const PagedAttnArgs& a, int row_min, void* workspa
     {
       AVQ_TIMED("paged_attn_tc", st);
       const int smem = total + 1024;
-      if (cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-        return AVQ_ERR_CUDA;
+      static std::atomic<unsigned long long> allowed[4];
+      if (!allow_smem((const void*)kfn, smem, allowed[(a.D == 64 ? 0 : 2) + tma])) return AVQ_ERR_CUDA;
       cfg.gridDim = dim3(kSms);
       cfg.blockDim = dim3(kTcThreads);
       cfg.dynamicSmemBytes = smem;

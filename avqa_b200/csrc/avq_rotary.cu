@@ -18,7 +18,9 @@
 // What bounds it: memory.  Every row is read and written once; a block forms
 // the sines and cosines of its few tokens once, in shared memory, and all
 // heads of the tokens use them.  A task is one pair of vectors of a row (16
-// bytes each where the layout allows it), four tasks of a thread in flight.
+// bytes each where the layout allows it); a thread keeps its task and walks
+// the rows, two in flight.  Small blocks, ten to an SM: one's prologue (the
+// positions, the angles) overlaps the others' copies.
 #include <algorithm>
 
 #include "avq_paged.cuh"
@@ -29,15 +31,18 @@ namespace {
 
 __device__ int g_fault_tables_rotary;
 
-constexpr int kThreads = 256, kUnroll = 4, kMaxTokens = 16;
+constexpr int kThreads = 128, kMaxTokens = 16;
 
-// n / d for n * d < 2^32: one multiplication by ceil(2^32 / d).
+// n / d for n * d < 2^32: one multiplication by floor(2^32 / d) + 1 (d > 1).
 struct Div {
   uint32_t m;
   int d;
   __device__ int operator()(int n) const { return d == 1 ? n : (int)__umulhi((uint32_t)n, m); }
 };
-Div make_div(int d) { return Div{d == 1 ? 0u : (uint32_t)(((1ull << 32) + d - 1) / d), d}; }
+
+// 51 registers a thread: at D = 128 (bf16, 64 heads, 8192 tokens) 47.6 us, 5.6 TB/s; three blocks of 256 threads took
+// 50.9, six of them, which spill, 63.0.
+constexpr int kMinBlocks = 10;
 
 template <int BYTES> struct Raw;
 template <> struct Raw<16> { using T = uint4; };
@@ -50,12 +55,11 @@ struct Geometry {
   int block_tokens;      // tokens of a block
   int head_step;         // heads of a block (grid.y slices)
   int rot_tasks, tasks;  // tasks of a row that rotate, all tasks of a row
-  Div by_tasks;
 };
 
 
-template <int DT, int VEC, bool PAGED>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotarySpec spec, const RotaryArgs a,
+template <int DT, int VEC, bool PAGED, int kUnroll>
+__global__ void __launch_bounds__(kThreads, kMinBlocks) rotary_kernel(const __grid_constant__ RotarySpec spec, const RotaryArgs a,
                                                           const PagedAppendArgs p, const Geometry g) {
   using T = typename Storage<DT>::T;
   using V = typename Raw<VEC * (int)sizeof(T)>::T;
@@ -146,95 +150,101 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
   }
   __syncthreads();
 
-  const int row_tasks = g.tasks * (h1 - h0), total = nt * row_tasks;
-  for (int base = tid; base < total; base += kThreads * kUnroll) {
-    V lo[kUnroll], hi[kUnroll];
-    const T* src[kUnroll];
-    T* dst[kUnroll];
-    int off0[kUnroll], off1[kUnroll], rot[kUnroll];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const int x = base + u * kThreads;
-      dst[u] = nullptr;
-      if (x >= total) continue;
-      const int row = g.by_tasks(x), v = x - row * g.tasks;
-      const int t = row / (h1 - h0), h = h0 + row - t * (h1 - h0);
-      if (PAGED && s_state[t] == 0) continue;
-      bool copy = false;
-      if (h < a.q.heads) {
-        src[u] = static_cast<const T*>(a.q.src) + s_src_q[t] + (long long)h * a.q.sh;
-        dst[u] = static_cast<T*>(a.q.dst) + s_dst_q[t] + (long long)h * a.q.dh;
-      } else if constexpr (PAGED) {
-        if (s_state[t] != 2) continue;
-        const int hk = h - a.q.heads;
-        copy = hk >= p.Hkv;
-        if (!copy) {
-          src[u] = static_cast<const T*>(p.k) + s_src_k[t] + (long long)hk * p.ks.h;
-          dst[u] = static_cast<T*>(p.kpool) + s_dst_k[t] + (long long)hk * p.kps.h;
-        } else {
-          src[u] = static_cast<const T*>(p.v) + s_src_v[t] + (long long)(hk - p.Hkv) * p.vs.h;
-          dst[u] = static_cast<T*>(p.vpool) + s_dst_v[t] + (long long)(hk - p.Hkv) * p.vps.h;
-        }
-      } else {
-        const int hk = h - a.q.heads;
-        src[u] = static_cast<const T*>(a.k.src) + s_src_k[t] + (long long)hk * a.k.sh;
-        dst[u] = static_cast<T*>(a.k.dst) + s_dst_k[t] + (long long)hk * a.k.dh;
-      }
-      rot[u] = -1;
-      if (!copy && v < g.rot_tasks) {
-        off0[u] = spec.interleaved ? 2 * v * VEC : v * VEC;
-        off1[u] = spec.interleaved ? off0[u] + VEC : spec.pairs + v * VEC;
-        rot[u] = slot(t, v, 0);
-      } else {
-        off0[u] = copy ? 2 * v * VEC : 2 * spec.pairs + 2 * (v - g.rot_tasks) * VEC;
-        off1[u] = off0[u] + VEC;
-      }
-      if (off0[u] >= a.D) {
-        dst[u] = nullptr;
-        continue;
-      }
-      lo[u] = *reinterpret_cast<const V*>(src[u] + off0[u]);
-      if (off1[u] < a.D) hi[u] = *reinterpret_cast<const V*>(src[u] + off1[u]);
+  // A thread keeps its task v of a row and walks rows (token, head) of one operand after the other, kUnroll at a time.
+  const int rows_at_once = kThreads / g.tasks, v = tid % g.tasks, first = tid / g.tasks;
+  if (first >= rows_at_once) return;
+  auto walk = [&](const T* src, T* dst, const long long* src_at, const long long* dst_at, long long src_h, long long dst_h,
+                  int begin, int end, bool rotates, int state) {
+    const int n = end - begin;  // heads
+    if (n <= 0) return;
+    const bool rot = rotates && v < g.rot_tasks;
+    int off0, off1;
+    if (rot) {
+      off0 = spec.interleaved ? 2 * v * VEC : v * VEC;
+      off1 = spec.interleaved ? off0 + VEC : spec.pairs + v * VEC;
+    } else {
+      off0 = rotates ? 2 * spec.pairs + 2 * (v - g.rot_tasks) * VEC : 2 * v * VEC;
+      off1 = off0 + VEC;
     }
+    if (off0 >= a.D) return;
+    const bool two = off1 < a.D;
+    const Div by_heads = {(uint32_t)(n == 1 ? 0u : 0xffffffffu / (uint32_t)n + 1u), n};
+    for (int row = first; row < nt * n; row += kUnroll * rows_at_once) {
+      V lo[kUnroll], hi[kUnroll];
+      T* to[kUnroll];
+      int tok[kUnroll];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      if (!dst[u]) continue;
-      if (rot[u] >= 0) {
-        T* x0 = reinterpret_cast<T*>(&lo[u]);
-        T* x1 = reinterpret_cast<T*>(&hi[u]);
-        const float2* r = cs + rot[u];
-        if (!spec.interleaved) {
+      for (int u = 0; u < kUnroll; ++u) {
+        const int x = row + u * rows_at_once, t = by_heads(x), h = begin + x - t * n;
+        to[u] = nullptr;
+        if (x >= nt * n || (PAGED && s_state[t] < state)) continue;
+        const T* from = src + src_at[t] + h * src_h;
+        to[u] = dst + dst_at[t] + h * dst_h;
+        tok[u] = t;
+        lo[u] = *reinterpret_cast<const V*>(from + off0);
+        if (two) hi[u] = *reinterpret_cast<const V*>(from + off1);
+      }
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            const float2 w = VEC == 1 ? r[0] : r[(i >> 1) * g.rot_tasks * 2 + (i & 1)];
-            const float xa = to_f(x0[i]), xb = to_f(x1[i]);
-            x0[i] = from_f<DT>(xa * w.x - xb * w.y);
-            x1[i] = from_f<DT>(xa * w.y + xb * w.x);
+      for (int u = 0; u < kUnroll; ++u) {
+        if (!to[u]) continue;
+        if (rot) {
+          T* x0 = reinterpret_cast<T*>(&lo[u]);
+          T* x1 = reinterpret_cast<T*>(&hi[u]);
+          const float2* r = cs + slot(tok[u], v, 0);
+          float2 w[VEC];
+          if constexpr (VEC == 1) {
+            w[0] = r[0];
+          } else {
+#pragma unroll
+            for (int i = 0; i < VEC; i += 2) {
+              const float4 y = *reinterpret_cast<const float4*>(r + (i >> 1) * g.rot_tasks * 2);
+              w[i] = make_float2(y.x, y.y);
+              w[i + 1] = make_float2(y.z, y.w);
+            }
           }
-        } else {
-          T e[2 * VEC];
+          if (!spec.interleaved) {
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            e[i] = x0[i];
-            e[VEC + i] = x1[i];
-          }
+            for (int i = 0; i < VEC; ++i) {
+              const float xa = to_f(x0[i]), xb = to_f(x1[i]);
+              x0[i] = from_f<DT>(xa * w[i].x - xb * w[i].y);
+              x1[i] = from_f<DT>(xa * w[i].y + xb * w[i].x);
+            }
+          } else {
+            T e[2 * VEC];
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            const float2 w = VEC == 1 ? r[0] : r[(i >> 1) * g.rot_tasks * 2 + (i & 1)];
-            const float xa = to_f(e[2 * i]), xb = to_f(e[2 * i + 1]);
-            e[2 * i] = from_f<DT>(xa * w.x - xb * w.y);
-            e[2 * i + 1] = from_f<DT>(xa * w.y + xb * w.x);
-          }
+            for (int i = 0; i < VEC; ++i) {
+              e[i] = x0[i];
+              e[VEC + i] = x1[i];
+            }
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            x0[i] = e[i];
-            x1[i] = e[VEC + i];
+            for (int i = 0; i < VEC; ++i) {
+              const float xa = to_f(e[2 * i]), xb = to_f(e[2 * i + 1]);
+              e[2 * i] = from_f<DT>(xa * w[i].x - xb * w[i].y);
+              e[2 * i + 1] = from_f<DT>(xa * w[i].y + xb * w[i].x);
+            }
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+              x0[i] = e[i];
+              x1[i] = e[VEC + i];
+            }
           }
         }
+        *reinterpret_cast<V*>(to[u] + off0) = lo[u];
+        if (two) *reinterpret_cast<V*>(to[u] + off1) = hi[u];
       }
-      *reinterpret_cast<V*>(dst[u] + off0[u]) = lo[u];
-      if (off1[u] < a.D) *reinterpret_cast<V*>(dst[u] + off1[u]) = hi[u];
     }
+  };
+  const int hq = a.q.heads;
+  walk(static_cast<const T*>(a.q.src), static_cast<T*>(a.q.dst), s_src_q, s_dst_q, a.q.sh, a.q.dh, min(h0, hq),
+       min(h1, hq), true, 1);
+  if constexpr (PAGED) {
+    walk(static_cast<const T*>(p.k), static_cast<T*>(p.kpool), s_src_k, s_dst_k, p.ks.h, p.kps.h,
+         min(max(h0 - hq, 0), p.Hkv), min(max(h1 - hq, 0), p.Hkv), true, 2);
+    walk(static_cast<const T*>(p.v), static_cast<T*>(p.vpool), s_src_v, s_dst_v, p.vs.h, p.vps.h,
+         max(h0 - hq - p.Hkv, 0), max(h1 - hq - p.Hkv, 0), false, 2);
+  } else {
+    walk(static_cast<const T*>(a.k.src), static_cast<T*>(a.k.dst), s_src_k, s_dst_k, a.k.sh, a.k.dh, max(h0 - hq, 0),
+         max(h1 - hq, 0), true, 2);
   }
 }
 
@@ -256,13 +266,12 @@ Geometry geometry(const RotarySpec& spec, int D, int tokens, int heads, int vec)
   g.tokens = tokens;
   g.rot_tasks = spec.pairs / vec;
   g.tasks = g.rot_tasks + (D - 2 * spec.pairs + 2 * vec - 1) / (2 * vec);
-  g.by_tasks = make_div(g.tasks);
   // as many tokens as keep one sine and cosine to a thread; fewer tokens, and slices of the heads, where the call
   // would otherwise leave SMs without a block
   int bt = std::max(1, std::min(kMaxTokens, kThreads / std::max(spec.pairs, 16)));
   while (bt > 1 && (tokens + bt - 1) / bt < 2 * kSms) bt >>= 1;
   const int blocks = (tokens + bt - 1) / bt;
-  const int most = std::max(1, (heads * g.tasks * bt + kThreads - 1) / kThreads);
+  const int most = std::max(1, heads * g.tasks * bt / 32);
   const int slices = std::max(1, std::min(most, 2 * kSms / std::max(blocks, 1)));
   g.block_tokens = bt;
   g.head_step = (heads + slices - 1) / slices;
@@ -275,16 +284,17 @@ int go(const RotarySpec& spec, const RotaryArgs& a, const PagedAppendArgs& p, in
   const Geometry g = geometry(spec, a.D, tokens, heads, vec);
   const dim3 grid((tokens + g.block_tokens - 1) / g.block_tokens, (heads + g.head_step - 1) / g.head_step);
   const size_t smem = std::max<size_t>(16, (size_t)g.block_tokens * spec.pairs * sizeof(float2));
+  constexpr int U = 2;
   auto run = [&](auto kfn) { kfn<<<grid, kThreads, smem, st>>>(spec, a, p, g); };
   if constexpr (DT == DT_F32) {
-    if (vec == 4) run(rotary_kernel<DT, 4, PAGED>);
-    else if (vec == 2) run(rotary_kernel<DT, 2, PAGED>);
-    else run(rotary_kernel<DT, 1, PAGED>);
+    if (vec == 4) run(rotary_kernel<DT, 4, PAGED, U>);
+    else if (vec == 2) run(rotary_kernel<DT, 2, PAGED, U>);
+    else run(rotary_kernel<DT, 1, PAGED, U>);
   } else {
-    if (vec == 8) run(rotary_kernel<DT, 8, PAGED>);
-    else if (vec == 4) run(rotary_kernel<DT, 4, PAGED>);
-    else if (vec == 2) run(rotary_kernel<DT, 2, PAGED>);
-    else run(rotary_kernel<DT, 1, PAGED>);
+    if (vec == 8) run(rotary_kernel<DT, 8, PAGED, U>);
+    else if (vec == 4) run(rotary_kernel<DT, 4, PAGED, U>);
+    else if (vec == 2) run(rotary_kernel<DT, 2, PAGED, U>);
+    else run(rotary_kernel<DT, 1, PAGED, U>);
   }
   return cudaPeekAtLastError() == cudaSuccess ? AVQ_OK : AVQ_ERR_CUDA;
 }

@@ -339,7 +339,7 @@ def _call(what: str, fn, dev: torch.device, *args) -> None:
 
 
 def _same(name: str, t: torch.Tensor, dev: torch.device, dtype: torch.dtype) -> None:
-    if t.device != dev:
+    if t.get_device() != dev.index:
         raise DeviceError(f"{name} must be on the same device", expected=str(dev), actual=str(t.device))
     if t.dtype != dtype:
         raise DtypeError(f"{name} has the wrong dtype", expected=str(dtype), actual=str(t.dtype))
@@ -431,11 +431,16 @@ def _pool(key_pool: torch.Tensor, value_pool: torch.Tensor, block_table: torch.T
         raise ShapeError("pools must be [pages, heads, page_size, head_dim], the values' like the keys'",
                          expected=("pages", "heads", "page_size", D),
                          actual=(tuple(key_pool.shape), tuple(value_pool.shape)))
-    _same("key_pool", key_pool, dev, dtype)
-    _same("value_pool", value_pool, dev, dtype)
-    _same("block_table", block_table, dev, torch.int32)
-    _same("kv_len", kv_len, dev, torch.int32)
-    _same("q_start", q_start, dev, torch.int32)
+    at = dev.index
+    if not (key_pool.dtype is dtype and value_pool.dtype is dtype and block_table.dtype is torch.int32
+            and kv_len.dtype is torch.int32 and q_start.dtype is torch.int32 and key_pool.get_device() == at
+            and value_pool.get_device() == at and block_table.get_device() == at and kv_len.get_device() == at
+            and q_start.get_device() == at):  # which one it is
+        _same("key_pool", key_pool, dev, dtype)
+        _same("value_pool", value_pool, dev, dtype)
+        _same("block_table", block_table, dev, torch.int32)
+        _same("kv_len", kv_len, dev, torch.int32)
+        _same("q_start", q_start, dev, torch.int32)
     table, lens = block_table.shape, kv_len.shape
     if len(table) != 2 or len(lens) != 1 or table[0] != lens[0] or q_start.shape != (lens[0] + 1,):
         raise ShapeError("the batch's lists disagree: block_table [B, W], kv_len [B], q_start [B + 1]",
@@ -506,7 +511,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, key_pool: torch.Tensor, value
 
 @functools.lru_cache(maxsize=4096)
 def _attention_workspace(code: int, B: int, N: int, H: int, Hkv: int, D: int, max_q_len: int) -> int:
-    return max(1, _lib.load().avq_paged_attention_workspace_size(code, B, N, H, Hkv, D, max_q_len))
+    """Bytes of scratch, a multiple of 256."""
+    return max(256, _lib.load().avq_paged_attention_workspace_size(code, B, N, H, Hkv, D, max_q_len))
 
 
 def paged_attention(q: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor, block_table: torch.Tensor,
@@ -534,14 +540,14 @@ def paged_attention(q: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.T
     if Hkv == 0 or H == 0 or H % Hkv:
         raise ShapeError("query heads must be a multiple of the pool's heads", expected=f"n * {Hkv}", actual=H)
     if out is None:
-        out = torch.empty((N, H, D), dtype=dt, device=dev)
+        out = q.new_empty((N, H, D))
     else:
         _same("out", out, dev, dt)
     if scale is None:
         scale = D ** -0.5 if D else 1.0
     code = _lib.dtype_code(dt)
     ws_bytes = _attention_workspace(code, lists[-1], N, H, Hkv, D, max_q_len)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    ws = kv_len.new_empty(ws_bytes // 4)
     _call("avq_paged_attention", lib.avq_paged_attention, dev, code, q.data_ptr(), qs, H, *pools, Hkv, D, *lists, N,
           causal, window, scale, max_q_len, out.data_ptr(),
           _packed(out, "out", H, N, D), ws.data_ptr(), ws_bytes)
