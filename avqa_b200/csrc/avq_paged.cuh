@@ -127,6 +127,8 @@ struct PagedAttnArgs {
 size_t paged_attn_tc_workspace_bytes(int B, int N, int H, int Hkv, int D, int row_min);
 template <int DT>
 int launch_paged_attention_tc(const PagedAttnArgs& a, int row_min, void* workspace, cudaStream_t st);
+template <int DT>
+int launch_paged_combine_tc(const PagedAttnArgs& a, int row_min, void* workspace, cudaStream_t st);
 int read_fault_paged_tc(int* code, cudaStream_t st);
 
 size_t paged_attn_workspace_bytes(int dtype, int B, int N, int H, int Hkv, int D, int max_q);

@@ -38,7 +38,10 @@ __device__ int g_fault_tables_paged;
 
 constexpr int kRows = 16, kWarps = 4;
 constexpr int kSpanUnit = 128;  // spans are multiples of a CTA's largest step
-constexpr int kTargetCtas = 16 * kSms, kMinSpan = 128;
+// About three rounds of the CTAs that the SMs hold at once: less fills the last round badly, more pays a CTA's own cost
+// too often (32 sequences of up to 32768 keys, 8 heads of 128: 508 us at 4 per SM, 446 at 8, 455 at 16; 9 of up to
+// 9000, 16 heads of 64: 51, 47 and 61).
+constexpr int kTargetCtas = 8 * kSms, kMinSpan = 128;
 // Rows (new tokens x heads of a group) of a sequence up to which one pass of 16-row groups over its keys is
 // taken, above which the tcgen05 kernel.
 constexpr int kFewRows = 16;
@@ -65,9 +68,10 @@ __device__ __forceinline__ int first_key(const PagedAttnArgs& a, const SeqRange&
 }
 
 // Finds the piece of index `at`: a (sequence, key head, span, row group) when `spans`, else a
-// (sequence, key head, row group) with every span of it.  Each warp does the same work.
-__device__ Piece find_piece(const PagedAttnArgs& a, int row_max, long long at, bool spans, bool report,
-                            long long* first_slot) {
+// (sequence, key head, row group) with every span of it.  Each warp does the same work.  *slot receives the piece's
+// slot of partial sums (without `spans` that of its first span, the others `stride` apart).
+__device__ Piece find_piece(const PagedAttnArgs& a, int row_max, int at, bool spans, bool report, int* slot,
+                            int* stride) {
   const int lane = threadIdx.x & 31, G = a.H / a.Hkv;
   const long long room = (long long)a.W * a.page_size;
   bool bad = false;
@@ -79,11 +83,13 @@ __device__ Piece find_piece(const PagedAttnArgs& a, int row_max, long long at, b
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   if (report && bad) atomicOr(&g_fault_tables_paged, kFaultTables);
-  long long span = (total + kTargetCtas - 1) / kTargetCtas;
-  span = (max(span, (long long)kMinSpan) + kSpanUnit - 1) / kSpanUnit * kSpanUnit;
+  const unsigned span =
+      (unsigned)min((max((total + kTargetCtas - 1) / kTargetCtas, (long long)kMinSpan) + kSpanUnit - 1) / kSpanUnit *
+                        kSpanUnit,
+                    (long long)(1 << 30));
   Piece p;
   p.found = false;
-  long long before = 0, slots = 0;  // pieces and partial slots of the sequences before
+  unsigned before = 0, slots = 0;  // pieces and partial slots of the sequences before
   for (int b0 = 0; b0 < a.B; b0 += 32) {
     const int b = b0 + lane;
     SeqRange s{0, 0, 0, 0};
@@ -93,42 +99,41 @@ __device__ Piece find_piece(const PagedAttnArgs& a, int row_max, long long at, b
       s = load_seq(a.q_start, a.kv_len, b, a.N, room, &ignore);
       groups = row_groups(a, G, s.n, row_max);
       f = first_key(a, s);
-      ns = max(1, (int)((s.len - f + span - 1) / span));
+      ns = max(1, (int)(((unsigned)(s.len - f) + span - 1) / span));
     }
-    const long long mine = (long long)groups * a.Hkv * ns, count = spans ? mine : (long long)groups * a.Hkv;
-    long long pre = count, pre_slots = mine;
+    const unsigned mine = (unsigned)groups * a.Hkv * ns, count = spans ? mine : (unsigned)groups * a.Hkv;
+    unsigned pre = count, pre_slots = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long x = __shfl_up_sync(0xffffffffu, pre, o), y = __shfl_up_sync(0xffffffffu, pre_slots, o);
+      const unsigned x = __shfl_up_sync(0xffffffffu, pre, o), y = __shfl_up_sync(0xffffffffu, pre_slots, o);
       if (lane >= o) {
         pre += x;
         pre_slots += y;
       }
     }
-    const unsigned hit = __ballot_sync(0xffffffffu, before + pre > at);
+    const unsigned hit = __ballot_sync(0xffffffffu, before + pre > (unsigned)at);
     if (hit) {
       const int src = __ffs(hit) - 1;
-      const long long rel = at - before - __shfl_sync(0xffffffffu, pre - count, src);
-      const long long base = slots + __shfl_sync(0xffffffffu, pre_slots - mine, src);
+      const unsigned rel = (unsigned)at - before - __shfl_sync(0xffffffffu, pre - count, src);
+      const unsigned base = slots + __shfl_sync(0xffffffffu, pre_slots - mine, src);
       p.b = b0 + src;
       p.seq.q0 = __shfl_sync(0xffffffffu, s.q0, src);
       p.seq.n = __shfl_sync(0xffffffffu, s.n, src);
       p.seq.len = __shfl_sync(0xffffffffu, s.len, src);
       p.seq.pos0 = __shfl_sync(0xffffffffu, s.pos0, src);
       p.nspan = __shfl_sync(0xffffffffu, ns, src);
-      groups = __shfl_sync(0xffffffffu, groups, src);
+      const unsigned n_groups = __shfl_sync(0xffffffffu, groups, src);
       f = __shfl_sync(0xffffffffu, f, src);
       // row groups of one span lie side by side: they read the same keys
-      p.group = (int)(rel % groups);
-      const int rest = (int)(rel / groups);
-      p.span_i = spans ? rest % p.nspan : 0;
-      p.head = spans ? rest / p.nspan : rest;
-      p.lo = (int)min((long long)p.seq.len, f + p.span_i * span);
-      p.hi = (int)min((long long)p.seq.len, f + (p.span_i + 1) * span);
+      const unsigned rest = n_groups == 1 ? rel : rel / n_groups;
+      p.group = (int)(rel - rest * n_groups);
+      p.head = (int)(spans ? rest / (unsigned)p.nspan : rest);
+      p.span_i = spans ? (int)(rest - (unsigned)p.head * p.nspan) : 0;
+      p.lo = (int)min((unsigned)p.seq.len, f + p.span_i * span);
+      p.hi = (int)min((unsigned)p.seq.len, f + (p.span_i + 1) * span);
       p.found = true;
-      if (first_slot) *first_slot = base + ((long long)p.head * p.nspan) * groups + p.group;
-      // the slot of span i is first_slot + i * groups
-      if (first_slot && !spans) p.lo = groups;  // the stride, for the caller that walks the spans
+      *slot = (int)(base + ((unsigned)p.head * p.nspan + p.span_i) * n_groups + p.group);
+      *stride = (int)n_groups;
       return p;
     }
     before += __shfl_sync(0xffffffffu, pre, 31);
@@ -207,10 +212,12 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// WIDE: 16-byte copies.  SAME: the pools have the same strides, so a key's and its value's places do too.
+// WIDE: 16-byte copies.  SAME: the pools have the same strides, so that a key's place is its value's, and are below
+// 2^32 chunks of 16 bytes.
 template <int DT, int DP, bool WIDE, bool SAME>
 __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const PagedAttnArgs a, int row_max,
-                                                                     int q_wide, float* __restrict__ part) {
+                                                                     int q_wide, int beside,
+                                                                     float* __restrict__ part) {
   using T = typename Storage<DT>::T;
   constexpr int KS = step_keys<DT, DP>(), NK = KS / 8;  // keys of a step, in columns of 8
   constexpr int LDS = DP + Operand<DT>::kPad, NT = DP / 8, STAGES = ring_stages<DT, DP>();
@@ -218,10 +225,16 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
   extern __shared__ __align__(128) unsigned char smem_raw[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.H / a.Hkv;
   asm volatile("griddepcontrol.launch_dependents;");
-  long long slot = 0;
-  const Piece p = find_piece(a, row_max, blockIdx.x, true, blockIdx.x == 0 && warp == 0, &slot);
-  if (!p.found) return;
-  slot += (long long)p.span_i * row_groups(a, G, p.seq.n, row_max);
+  int slot = 0, slot_stride = 0;
+  const Piece p = find_piece(a, row_max, blockIdx.x, true, blockIdx.x == 0 && warp == 0, &slot, &slot_stride);
+  // a grid that runs beside another ends after it, so that what waits for this one has waited for both
+  auto leave = [&]() {
+    if (beside && blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+  };
+  if (!p.found) {
+    leave();
+    return;
+  }
   T* sq = reinterpret_cast<T*>(smem_raw);                                  // [kRows][LDS]
   T* ring = sq + kRows * LDS + warp * STAGES * stage_elems<DT, DP>();       // this warp's stages
   const int row0 = p.group * kRows, nrow = min(kRows, p.seq.n * G - row0);
@@ -262,35 +275,53 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
   const int* row_table = a.table + (long long)p.b * a.table_stride;
   bool bad = false;
 
-  // One stage: KS keys and their values.  Keys outside the span, and pages outside the pool, read as zeros.
+  // One stage: KS keys and their values.  Keys outside the span, and pages outside the pool, read as zeros.  Each lane
+  // looks up one key, its table entry one stage ahead, and the chunks' lanes take the place from it; the stages come in
+  // order, so the page and the slot only step on.
+  const int step_pages = kWarps * KS / a.page_size, step_slots = kWarps * KS - step_pages * a.page_size;
+  int key = lo + warp * KS + lane % KS, page_at = key / a.page_size, in_page = key - page_at * a.page_size;
+  int ahead = key < hi ? row_table[page_at] : -1;
   auto load = [&](int step) {
-    const int k0 = lo + (step * kWarps + warp) * KS;
     T* dst = ring + (step % STAGES) * stage_elems<DT, DP>();
-    // each lane looks up one key; the chunks' lanes take the address from it
-    const int key = k0 + (lane % KS);
     long long ko = -1, vo = -1;
-    if (step < steps && key < hi) {
-      const int page = row_table[key / a.page_size], s = key % a.page_size;
-      if (page >= 0 && page < a.num_pages) {
-        ko = (long long)page * a.kps.p + (long long)s * a.kps.s;
-        vo = SAME ? ko : (long long)page * a.vps.p + (long long)s * a.vps.s;
+    if (key < hi) {
+      if (ahead >= 0 && ahead < a.num_pages) {
+        ko = (long long)ahead * a.kps.p + (long long)in_page * a.kps.s;
+        if (!SAME) vo = (long long)ahead * a.vps.p + (long long)in_page * a.vps.s;
       } else {
         bad = true;
       }
     }
+    key += kWarps * KS;
+    page_at += step_pages;
+    in_page += step_slots;
+    if (in_page >= a.page_size) {
+      in_page -= a.page_size;
+      ++page_at;
+    }
+    ahead = key < hi ? row_table[page_at] : -1;
     if constexpr (WIDE) {
       const int c = lane % CPR * EPC;
+      const bool in_row = c < a.D;  // (rows of up to 32 chunks)
       T* d = dst + lane / CPR * LDS + c;
+      const uint32_t chunk = SAME ? (uint32_t)(ko / EPC) : 0u;  // the place in 16-byte chunks; all ones: none
 #pragma unroll
       for (int i = 0; i < KS * CPR / 32; ++i) {
         const int r = CPR <= 32 ? i * (32 / CPR) + lane / CPR : i / (CPR / 32);
         const int cc = CPR <= 32 ? c : (i % (CPR / 32) * 32 + lane) * EPC;
         T* to = CPR <= 32 ? d + i * (32 / CPR) * LDS : dst + r * LDS + cc;
-        const long long k_at = __shfl_sync(0xffffffffu, ko, r);
-        const long long v_at = SAME ? k_at : __shfl_sync(0xffffffffu, vo, r);
-        const bool ok = k_at >= 0 && cc < a.D;
-        cp_async16(to, kbase + (ok ? k_at + cc : 0), ok);
-        cp_async16(to + KS * LDS, vbase + (ok ? v_at + cc : 0), ok);
+        if constexpr (SAME) {
+          const uint32_t at = __shfl_sync(0xffffffffu, ko < 0 ? 0xffffffffu : chunk, r);
+          const bool ok = at != 0xffffffffu && (CPR <= 32 ? in_row : cc < a.D);
+          const long long off = ok ? (long long)at * EPC + cc : 0;
+          cp_async16(to, kbase + off, ok);
+          cp_async16(to + KS * LDS, vbase + off, ok);
+        } else {
+          const long long k_at = __shfl_sync(0xffffffffu, ko, r), v_at = __shfl_sync(0xffffffffu, vo, r);
+          const bool ok = k_at >= 0 && cc < a.D;
+          cp_async16(to, kbase + (ok ? k_at + cc : 0), ok);
+          cp_async16(to + KS * LDS, vbase + (ok ? v_at + cc : 0), ok);
+        }
       }
     } else {
       for (int r = 0; r < KS; ++r) {
@@ -475,7 +506,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
   for (int j = 0; j < NT; ++j) {
     float* w = so + (warp * kRows + ra) * DP + j * 8 + ct;
     *reinterpret_cast<float2*>(w) = make_float2(o[j][0] * fa, o[j][1] * fa);
-    *reinterpret_cast<float2*>(w + 8 * DP) = make_float2(o[j][2] * fb, o[j][3] * fb);
+    if (nrow > 8) *reinterpret_cast<float2*>(w + 8 * DP) = make_float2(o[j][2] * fb, o[j][3] * fb);
   }
   __syncthreads();
   for (int i = tid; i < nrow * DP; i += kWarps * 32) {
@@ -494,7 +525,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
       static_cast<T*>(a.out)[(long long)tok * a.os.t + (long long)h * a.os.h + d] =
           from_f<DT>(v.y > v.x ? x / l : 0.f);
     } else {
-      float* w = part + slot * (kRows * (DP + 2));
+      float* w = part + (long long)slot * (kRows * (DP + 2));
       w[r * DP + d] = x;
       if (d == 0) {
         float M = sm[r];
@@ -504,6 +535,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
       }
     }
   }
+  leave();
 }
 
 // Joins the spans of one (sequence, key head, row group): a warp per row, or several where the rows are few, each on
@@ -518,15 +550,16 @@ __global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const PagedAtt
   __shared__ float s_x[kJoinWarps][DP];
   __shared__ float s_l[kJoinWarps];
   const int G = a.H / a.Hkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the lists are older than the attention kernel, which this launch may overtake
+  int slot = 0, stride = 0;
+  const Piece p = find_piece(a, row_max, blockIdx.x, false, false, &slot, &stride);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  long long slot = 0;
-  const Piece p = find_piece(a, row_max, blockIdx.x, false, false, &slot);
   if (!p.found || p.nspan == 1) return;
-  const int stride = p.lo, row0 = p.group * kRows, nrow = min(kRows, p.seq.n * G - row0);
+  const int row0 = p.group * kRows, nrow = min(kRows, p.seq.n * G - row0);
   // token ranges that overlap could name more pieces than there are slots
-  if (slot + (long long)(p.nspan - 1) * stride >= pieces) return;
+  if (slot < 0 || slot + (long long)(p.nspan - 1) * stride >= pieces) return;
   const long long step = (long long)stride * (kRows * (DP + 2));
-  const float* base = part + slot * (kRows * (DP + 2));
+  const float* base = part + (long long)slot * (kRows * (DP + 2));
   const int per_row = nrow >= kJoinWarps ? 1 : kJoinWarps / nrow;  // warps of a row
   const int share = warp % per_row;
   for (int r = warp / per_row; r < nrow || per_row > 1; r += kJoinWarps / per_row) {
@@ -637,7 +670,7 @@ bool wide_rows(const void* p, std::initializer_list<long long> strides, int elem
 }
 
 template <int DT, int DP>
-int launch_mma(const PagedAttnArgs& a, int row_max, float* part, cudaStream_t st) {
+int launch_mma(const PagedAttnArgs& a, int row_max, bool beside, void* tc_workspace, float* part, cudaStream_t st) {
   using T = typename Storage<DT>::T;
   const int E = (int)sizeof(T);
   const bool wide = a.D * E % 16 == 0 && wide_rows(a.kpool, {a.kps.p, a.kps.h, a.kps.s}, E) &&
@@ -646,28 +679,42 @@ int launch_mma(const PagedAttnArgs& a, int row_max, float* part, cudaStream_t st
   const long long pieces = most_pieces(a.B, a.N, a.H, a.Hkv, row_max);
   const long long items = most_items(a.B, a.N, a.H, a.Hkv, row_max);
   const size_t smem = mma_smem<DT, DP>();
-  const bool same = a.kps.p == a.vps.p && a.kps.s == a.vps.s;
+  const long long extent = (long long)std::max(a.num_pages - 1, 0) * a.kps.p + (long long)(a.page_size - 1) * a.kps.s;
+  const bool same = a.kps.p == a.vps.p && a.kps.s == a.vps.s && a.kps.p >= 0 && a.kps.s >= 0 &&
+                    extent / (16 / E) < 0xffffffffll;
   const int variant = !wide ? 0 : (same ? 2 : 1);
   auto kfn = variant == 0 ? paged_attn_mma_kernel<DT, DP, false, false>
                           : (variant == 1 ? paged_attn_mma_kernel<DT, DP, true, false>
                                           : paged_attn_mma_kernel<DT, DP, true, true>);
   static std::atomic<unsigned long long> allowed[3];
   if (!allow_smem((const void*)kfn, smem, allowed[variant])) return AVQ_ERR_CUDA;
-  {
-    AVQ_TIMED("paged_attn", st);
-    kfn<<<(unsigned)pieces, kWarps * 32, smem, st>>>(a, row_max, (int)q_wide, part);
-    if (cudaPeekAtLastError() != cudaSuccess) return AVQ_ERR_CUDA;
-  }
-  AVQ_TIMED("paged_combine", st);
-  // the launch overlaps the attention kernel's end; the kernel waits for its results itself
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)std::max<long long>(items, 1));
-  cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.stream = st;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
+  {
+    AVQ_TIMED("paged_attn", st);
+    // beside the tcgen05 kernel, whose SMs it takes over one by one (it needs nothing of its)
+    const long long room = ((long long)a.W * a.page_size + kMinSpan - 1) / kMinSpan;
+    cfg.gridDim = dim3((unsigned)std::min(pieces, items * std::max(room, 1ll)));
+    cfg.blockDim = dim3(kWarps * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.numAttrs = beside ? 1 : 0;
+    if (cudaLaunchKernelEx(&cfg, kfn, a, row_max, (int)q_wide, (int)beside, part) != cudaSuccess) return AVQ_ERR_CUDA;
+  }
+  if constexpr (DT != DT_F32 && DP <= 128) {
+    if (beside) {
+      const int rc = launch_paged_combine_tc<DT>(a, row_max, tc_workspace, st);
+      if (rc != AVQ_OK) return rc;
+    }
+  }
+  AVQ_TIMED("paged_combine", st);
+  // the launch overlaps the attention kernel's end; the kernel waits for its results itself
+  cfg.gridDim = dim3((unsigned)std::max<long long>(items, 1));
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, combine_kernel<DT, DP>, a, row_max, pieces, (const float*)part) == cudaSuccess
              ? AVQ_OK
@@ -704,9 +751,9 @@ int launch_paged_attention(const PagedAttnArgs& a, cudaStream_t st) {
     }
   }
   float* part = reinterpret_cast<float*>(ws);
-  if (a.D <= 64) return launch_mma<DT, 64>(a, c.row_max, part, st);
-  if (a.D <= 128) return launch_mma<DT, 128>(a, c.row_max, part, st);
-  return launch_mma<DT, 256>(a, c.row_max, part, st);
+  if (a.D <= 64) return launch_mma<DT, 64>(a, c.row_max, c.many, a.workspace, part, st);
+  if (a.D <= 128) return launch_mma<DT, 128>(a, c.row_max, c.many, a.workspace, part, st);
+  return launch_mma<DT, 256>(a, c.row_max, c.many, a.workspace, part, st);
 }
 
 int read_fault_paged(int* code, cudaStream_t st) {

@@ -940,6 +940,10 @@ long long most_items(int B, int N, int G, int row_min) {
   const long long rows = (long long)N * G;
   return rows / kItemRows + std::min<long long>(B, rows / (row_min + 1)) + 1;
 }
+// Whether an output row takes 16-byte stores.
+bool out_rows_wide(const PagedAttnArgs& a) {
+  return reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.os.t % 8 == 0 && a.os.h % 8 == 0;
+}
 size_t plan_bytes(int B, long long items, int Hkv) {
   return align_up((size_t)plan_ints(B, items, Hkv) * sizeof(int));
 }
@@ -956,8 +960,6 @@ int launch_paged_attention_tc(const PagedAttnArgs& a, int row_min, void* workspa
   const long long items = most_items(a.B, a.N, a.H / a.Hkv, row_min);
   int* ws = static_cast<int*>(workspace);
   float* partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan_bytes(a.B, items, a.Hkv));
-  using T = typename Storage<DT>::T;
-  const bool wide = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.os.t % 8 == 0 && a.os.h % 8 == 0;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
@@ -965,7 +967,7 @@ int launch_paged_attention_tc(const PagedAttnArgs& a, int row_min, void* workspa
   std::memset(&maps, 0, sizeof(maps));
   const bool tma = pool_map(&maps.k, DT, a.kpool, a.kps, a, &maps.kpos) &&
                    pool_map(&maps.v, DT, a.vpool, a.vps, a, &maps.vpos);
-  auto go = [&](auto kfn, auto joinfn, int total) -> int {
+  auto go = [&](auto kfn, int total) -> int {
     {
       AVQ_TIMED("paged_plan", st);
       plan_kernel<<<1, kPlanThreads, 0, st>>>(a, row_min, (int)items, ws);
@@ -983,21 +985,36 @@ int launch_paged_attention_tc(const PagedAttnArgs& a, int row_min, void* workspa
       cfg.gridDim = dim3(kSms);
       cfg.blockDim = dim3(kTcThreads);
       cfg.dynamicSmemBytes = smem;
-      if (cudaLaunchKernelEx(&cfg, kfn, maps, a, (int)items, ws, partials, (int)wide) != cudaSuccess)
+      if (cudaLaunchKernelEx(&cfg, kfn, maps, a, (int)items, ws, partials, (int)out_rows_wide(a)) != cudaSuccess)
         return AVQ_ERR_CUDA;
     }
-    AVQ_TIMED("paged_combine_tc", st);
-    cfg.gridDim = dim3((unsigned)(items * a.Hkv), kItemRows / kJoinRows);
-    cfg.blockDim = dim3(256);
-    cfg.dynamicSmemBytes = 0;
-    return cudaLaunchKernelEx(&cfg, joinfn, a, (int)items, ws, (const float*)partials, (int)wide) == cudaSuccess ? AVQ_OK
-                                                                                                      : AVQ_ERR_CUDA;
+    return AVQ_OK;
   };
   if (a.D == 64)
-    return go(tma ? paged_attn_tc_kernel<DT, 64, true> : paged_attn_tc_kernel<DT, 64, false>, combine_tc_kernel<DT, 64>,
-              TcShared<64>::TOTAL);
-  return go(tma ? paged_attn_tc_kernel<DT, 128, true> : paged_attn_tc_kernel<DT, 128, false>,
-            combine_tc_kernel<DT, 128>, TcShared<128>::TOTAL);
+    return go(tma ? paged_attn_tc_kernel<DT, 64, true> : paged_attn_tc_kernel<DT, 64, false>, TcShared<64>::TOTAL);
+  return go(tma ? paged_attn_tc_kernel<DT, 128, true> : paged_attn_tc_kernel<DT, 128, false>, TcShared<128>::TOTAL);
+}
+
+template <int DT>
+int launch_paged_combine_tc(const PagedAttnArgs& a, int row_min, void* workspace, cudaStream_t st) {
+  const long long items = most_items(a.B, a.N, a.H / a.Hkv, row_min);
+  int* ws = static_cast<int*>(workspace);
+  const float* partials =
+      reinterpret_cast<const float*>(static_cast<char*>(workspace) + plan_bytes(a.B, items, a.Hkv));
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cfg.gridDim = dim3((unsigned)(items * a.Hkv), kItemRows / kJoinRows);
+  cfg.blockDim = dim3(256);
+  AVQ_TIMED("paged_combine_tc", st);
+  return cudaLaunchKernelEx(&cfg, a.D == 64 ? combine_tc_kernel<DT, 64> : combine_tc_kernel<DT, 128>, a, (int)items, ws,
+                            partials, (int)out_rows_wide(a)) == cudaSuccess
+             ? AVQ_OK
+             : AVQ_ERR_CUDA;
 }
 
 int read_fault_paged_tc(int* code, cudaStream_t st) {
@@ -1011,5 +1028,7 @@ int read_fault_paged_tc(int* code, cudaStream_t st) {
 
 template int launch_paged_attention_tc<DT_BF16>(const PagedAttnArgs&, int, void*, cudaStream_t);
 template int launch_paged_attention_tc<DT_F16>(const PagedAttnArgs&, int, void*, cudaStream_t);
+template int launch_paged_combine_tc<DT_BF16>(const PagedAttnArgs&, int, void*, cudaStream_t);
+template int launch_paged_combine_tc<DT_F16>(const PagedAttnArgs&, int, void*, cudaStream_t);
 
 }  // namespace avq
