@@ -325,33 +325,40 @@ def forward(q: torch.Tensor, cb: PreparedCodebook, st: QuantState, P: int, passe
 _POSITION_BYTES = {torch.int32: 4, torch.int64: 8}
 
 
-def _call(what: str, fn, dev: torch.device, *args) -> None:
-    """``fn(*args, stream)`` on the current stream of ``dev`` (made current where it is not: a
-    launch goes to the current device), its status checked."""
-    index = dev.index
+def _call(what: str, fn, index: int, *args) -> None:
+    """``fn(*args, stream)`` on the current stream of device ``index`` (made current where it is
+    not: a launch goes to the current device), its status checked."""
     if index == torch.cuda.current_device():
-        rc = fn(*args, _lib.stream_of(dev))
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, _lib.stream_of(dev))
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _lib.check(rc, what)
 
 
-def _same(name: str, t: torch.Tensor, dev: torch.device, dtype: torch.dtype) -> None:
-    if t.get_device() != dev.index:
-        raise DeviceError(f"{name} must be on the same device", expected=str(dev), actual=str(t.device))
+def _cuda_index(t: torch.Tensor, name: str) -> int:
+    index = t.get_device()
+    if index < 0:
+        _cuda(t, name)
+    return index
+
+
+def _same(name: str, t: torch.Tensor, index: int, dtype: torch.dtype) -> None:
+    if t.get_device() != index:
+        raise DeviceError(f"{name} must be on the same device", expected=f"cuda:{index}", actual=str(t.device))
     if t.dtype != dtype:
         raise DtypeError(f"{name} has the wrong dtype", expected=str(dtype), actual=str(t.dtype))
 
 
-def _positions_operand(positions: torch.Tensor | None, axes: int, B: int, T: int, dev: torch.device):
+def _positions_operand(positions: torch.Tensor | None, axes: int, B: int, T: int, index: int):
     """(pointer, bytes, strides (axis, b, t)) of positions ``[T]``, ``[B, T]`` with one axis, or
     ``[axes, T]`` / ``[axes, B, T]``."""
     if positions is None:
         return None, 0, (0, 0, 0)
-    if positions.device != dev:
-        raise DeviceError("positions must be on the same device", expected=str(dev), actual=str(positions.device))
+    if positions.get_device() != index:
+        raise DeviceError("positions must be on the same device", expected=f"cuda:{index}",
+                          actual=str(positions.device))
     nbytes = _POSITION_BYTES.get(positions.dtype)
     if nbytes is None:
         raise DtypeError("positions must be int32 or int64", expected="int32 | int64", actual=str(positions.dtype))
@@ -379,8 +386,7 @@ def rotary(embedding, q: torch.Tensor, k: torch.Tensor | None = None, positions:
     :class:`~avqa_b200.rotary.RotaryEmbedding` (by the negative angle with
     ``reverse``) into new tensors; no gradient is recorded here."""
     lib = _lib.load()
-    _cuda(q, "query")
-    dev, dt = q.device, q.dtype
+    at, dt = _cuda_index(q, "query"), q.dtype
     B, H, T, D = q.shape
     if D != embedding.head_dim:
         raise ShapeError("the rotary embedding's head_dim differs from the query's", expected=embedding.head_dim,
@@ -389,15 +395,15 @@ def rotary(embedding, q: torch.Tensor, k: torch.Tensor | None = None, positions:
     kp = ks = kop = kos = k_out = None
     Hk = 0
     if k is not None:
-        _same("key", k, dev, dt)
+        _same("key", k, at, dt)
         Bk, Hk, Tk, Dk = k.shape
         if Bk != B or Tk != T or Dk != D:
             raise ShapeError("key must have the query's batch, tokens and head_dim", expected=(B, "Hk", T, D),
                              actual=tuple(k.shape))
         k_out = torch.empty_like(k)
         kp, ks, kop, kos = k.data_ptr(), _lib.strides3(k), k_out.data_ptr(), _lib.strides3(k_out)
-    pos, pos_bytes, pos_strides = _positions_operand(positions, embedding.num_axes, B, T, dev)
-    _call("avq_rotary", lib.avq_rotary, dev, _lib.dtype_code(dt), q.data_ptr(), _lib.strides3(q), H, kp, ks, Hk, B, T,
+    pos, pos_bytes, pos_strides = _positions_operand(positions, embedding.num_axes, B, T, at)
+    _call("avq_rotary", lib.avq_rotary, at, _lib.dtype_code(dt), q.data_ptr(), _lib.strides3(q), H, kp, ks, Hk, B, T,
           D, embedding.rotary_dim, embedding.interleaved, embedding.c_frequencies, embedding.c_axes,
           embedding.num_axes, pos, pos_bytes, _lib.longs(*pos_strides), offset, reverse, q_out.data_ptr(),
           _lib.strides3(q_out), kop, kos)
@@ -422,36 +428,40 @@ def _packed_shape(t: torch.Tensor, name: str) -> torch.Size:
     return t.shape
 
 
-def _pool(key_pool: torch.Tensor, value_pool: torch.Tensor, block_table: torch.Tensor, kv_len: torch.Tensor,
-          q_start: torch.Tensor, dev: torch.device, dtype: torch.dtype, D: int) -> tuple:
-    """Check a page pool and a batch's lists; (heads, the C calls' arguments from key_pool to
-    q_start without the leading sizes, batch)."""
-    shape = key_pool.shape
-    if len(shape) != 4 or shape[3] != D or value_pool.shape != shape:
+@functools.lru_cache(maxsize=4096)
+def _pool_layout(keys: tuple, key_strides: tuple, values: tuple, value_strides: tuple, table: tuple,
+                 table_strides: tuple, lens: tuple, len_strides: tuple, starts: tuple, start_strides: tuple,
+                 D: int) -> tuple:
+    """Check a pool's and a batch's shapes and strides; (heads, the pools' stride arrays, pages,
+    page size, table row stride and width, batch).  The same layouts come again on every step."""
+    if len(keys) != 4 or keys[3] != D or values != keys:
         raise ShapeError("pools must be [pages, heads, page_size, head_dim], the values' like the keys'",
-                         expected=("pages", "heads", "page_size", D),
-                         actual=(tuple(key_pool.shape), tuple(value_pool.shape)))
-    at = dev.index
-    if not (key_pool.dtype is dtype and value_pool.dtype is dtype and block_table.dtype is torch.int32
-            and kv_len.dtype is torch.int32 and q_start.dtype is torch.int32 and key_pool.get_device() == at
+                         expected=("pages", "heads", "page_size", D), actual=(tuple(keys), tuple(values)))
+    if D > 1 and (key_strides[3] != 1 or value_strides[3] != 1):
+        raise BackendError("pools must have a contiguous last dimension",
+                           {"stride": (tuple(key_strides), tuple(value_strides))})
+    if len(table) != 2 or len(lens) != 1 or table[0] != lens[0] or tuple(starts) != (lens[0] + 1,):
+        raise ShapeError("the batch's lists disagree: block_table [B, W], kv_len [B], q_start [B + 1]",
+                         expected=("[B, W]", "[B]", "[B + 1]"), actual=(tuple(table), tuple(lens), tuple(starts)))
+    if (table_strides[1] != 1 and table[1] > 1) or (len_strides[0] != 1 and lens[0] > 1) or start_strides[0] != 1:
+        raise BackendError("the batch's lists must be contiguous along their last dimension")
+    return (keys[1], _lib.longs(*key_strides[:3]), _lib.longs(*value_strides[:3]), keys[0], keys[2], table_strides[0],
+            table[1], lens[0])
+
+
+def _pool(key_pool: torch.Tensor, value_pool: torch.Tensor, block_table: torch.Tensor, kv_len: torch.Tensor,
+          q_start: torch.Tensor, at: int, dtype: torch.dtype, D: int) -> tuple:
+    """Check a page pool and a batch's lists on device ``at``; see :func:`_pool_layout`."""
+    i32 = torch.int32
+    if not (key_pool.dtype is dtype and value_pool.dtype is dtype and block_table.dtype is i32
+            and kv_len.dtype is i32 and q_start.dtype is i32 and key_pool.get_device() == at
             and value_pool.get_device() == at and block_table.get_device() == at and kv_len.get_device() == at
             and q_start.get_device() == at):  # which one it is
-        _same("key_pool", key_pool, dev, dtype)
-        _same("value_pool", value_pool, dev, dtype)
-        _same("block_table", block_table, dev, torch.int32)
-        _same("kv_len", kv_len, dev, torch.int32)
-        _same("q_start", q_start, dev, torch.int32)
-    table, lens = block_table.shape, kv_len.shape
-    if len(table) != 2 or len(lens) != 1 or table[0] != lens[0] or q_start.shape != (lens[0] + 1,):
-        raise ShapeError("the batch's lists disagree: block_table [B, W], kv_len [B], q_start [B + 1]",
-                         expected=("[B, W]", "[B]", "[B + 1]"),
-                         actual=(tuple(table), tuple(lens), tuple(q_start.shape)))
-    row, col = block_table.stride()
-    if (col != 1 and table[1] > 1) or (lens[0] > 1 and kv_len.stride(0) != 1) or q_start.stride(0) != 1:
-        raise BackendError("the batch's lists must be contiguous along their last dimension")
-    return shape[1], (key_pool.data_ptr(), _lib.strides3(key_pool), value_pool.data_ptr(),
-                      _lib.strides3(value_pool)), (shape[0], shape[2], block_table.data_ptr(), row, table[1],
-                                                   kv_len.data_ptr(), q_start.data_ptr(), lens[0])
+        for name, t, want in (("key_pool", key_pool, dtype), ("value_pool", value_pool, dtype),
+                              ("block_table", block_table, i32), ("kv_len", kv_len, i32), ("q_start", q_start, i32)):
+            _same(name, t, at, want)
+    return _pool_layout(key_pool.shape, key_pool.stride(), value_pool.shape, value_pool.stride(), block_table.shape,
+                        block_table.stride(), kv_len.shape, kv_len.stride(), q_start.shape, q_start.stride(), D)
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor,
@@ -471,24 +481,24 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, key_pool: torch.Tensor, value
     ``[axes, N]``) replaces for the rotation only.  Tokens behind
     ``q_start[B]`` are left alone.  Serving only: no gradient is recorded."""
     lib = _lib.load()
-    _cuda(k, "key")
-    dev, dt = k.device, k.dtype
+    at, dt = _cuda_index(k, "key"), k.dtype
     N, Hkv, D = _packed_shape(k, "key")
     ks = _packed(k, "key", Hkv, N, D)
-    _same("value", v, dev, dt)
+    _same("value", v, at, dt)
     vs = _packed(v, "value", Hkv, N, D)
-    heads, pools, lists = _pool(key_pool, value_pool, block_table, kv_len, q_start, dev, dt, D)
+    heads, kst, vst, pages, page_size, row, width, B = _pool(key_pool, value_pool, block_table, kv_len, q_start, at, dt,
+                                                             D)
     if heads != Hkv:
         raise ShapeError("the pool's heads differ from the keys'", expected=heads, actual=Hkv)
     H, qp, qs, qop, qos = 0, None, None, None, None
     if q is not None:
-        _same("query", q, dev, dt)
+        _same("query", q, at, dt)
         H = _packed_shape(q, "query")[1]
         qs = _packed(q, "query", H, N, D)
         if q_out is None:
             q_out = torch.empty_like(q)
         else:
-            _same("q_out", q_out, dev, dt)
+            _same("q_out", q_out, at, dt)
         qos = _packed(q_out, "q_out", H, N, D)
         qp, qop = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
@@ -502,10 +512,11 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, key_pool: torch.Tensor, value
         freq, axes = rotary.c_frequencies, rotary.c_axes
     elif positions is not None:
         raise BackendError("positions need a rotary embedding")
-    pos, pos_bytes, pos_strides = _positions_operand(positions, num_axes, 1, N, dev)
-    _call("avq_paged_append", lib.avq_paged_append, dev, _lib.dtype_code(dt), qp, qs, H, qop, qos, k.data_ptr(), ks,
-          v.data_ptr(), vs, Hkv, D, *pools, *lists, N, R, inter, freq, axes, num_axes, pos, pos_bytes,
-          _lib.longs(pos_strides[0], pos_strides[2]))
+    pos, pos_bytes, pos_strides = _positions_operand(positions, num_axes, 1, N, at)
+    _call("avq_paged_append", lib.avq_paged_append, at, _lib.dtype_code(dt), qp, qs, H, qop, qos, k.data_ptr(), ks,
+          v.data_ptr(), vs, Hkv, D, key_pool.data_ptr(), kst, value_pool.data_ptr(), vst, pages, page_size,
+          block_table.data_ptr(), row, width, kv_len.data_ptr(), q_start.data_ptr(), B, N, R, inter, freq, axes,
+          num_axes, pos, pos_bytes, _lib.longs(pos_strides[0], pos_strides[2]))
     return q_out
 
 
@@ -532,25 +543,26 @@ def paged_attention(q: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.T
     Probabilities are rounded to the dtype for the product with the values
     (bf16, fp16), all sums are fp32.  Serving only: no gradient is recorded."""
     lib = _lib.load()
-    _cuda(q, "query")
-    dev, dt = q.device, q.dtype
+    at, dt = _cuda_index(q, "query"), q.dtype
     N, H, D = _packed_shape(q, "query")
     qs = _packed(q, "query", H, N, D)
-    Hkv, pools, lists = _pool(key_pool, value_pool, block_table, kv_len, q_start, dev, dt, D)
+    Hkv, kst, vst, pages, page_size, row, width, B = _pool(key_pool, value_pool, block_table, kv_len, q_start, at, dt,
+                                                           D)
     if Hkv == 0 or H == 0 or H % Hkv:
         raise ShapeError("query heads must be a multiple of the pool's heads", expected=f"n * {Hkv}", actual=H)
     if out is None:
         out = q.new_empty((N, H, D))
     else:
-        _same("out", out, dev, dt)
+        _same("out", out, at, dt)
     if scale is None:
         scale = D ** -0.5 if D else 1.0
     code = _lib.dtype_code(dt)
-    ws_bytes = _attention_workspace(code, lists[-1], N, H, Hkv, D, max_q_len)
+    ws_bytes = _attention_workspace(code, B, N, H, Hkv, D, max_q_len)
     ws = kv_len.new_empty(ws_bytes // 4)
-    _call("avq_paged_attention", lib.avq_paged_attention, dev, code, q.data_ptr(), qs, H, *pools, Hkv, D, *lists, N,
-          causal, window, scale, max_q_len, out.data_ptr(),
-          _packed(out, "out", H, N, D), ws.data_ptr(), ws_bytes)
+    _call("avq_paged_attention", lib.avq_paged_attention, at, code, q.data_ptr(), qs, H, key_pool.data_ptr(), kst,
+          value_pool.data_ptr(), vst, Hkv, D, pages, page_size, block_table.data_ptr(), row, width, kv_len.data_ptr(),
+          q_start.data_ptr(), B, N, causal, window, scale, max_q_len, out.data_ptr(), _packed(out, "out", H, N, D),
+          ws.data_ptr(), ws_bytes)
     return out
 
 

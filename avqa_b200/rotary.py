@@ -95,23 +95,32 @@ class _Rotate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rotary, positions, offset, reverse, q, k):
         ctx.args = (rotary, offset, reverse)
-        ctx.save_for_backward(positions)
+        if positions is not None:
+            ctx.save_for_backward(positions)
         ctx.set_materialize_grads(False)
-        q_out, k_out = ops.rotary(rotary, q, k, positions, offset, reverse)
-        return q_out, k_out
+        return ops.rotary(rotary, q, k, positions, offset, reverse)
 
     @staticmethod
     def backward(ctx, gq, gk):
         rotary, offset, reverse = ctx.args
-        (positions,) = ctx.saved_tensors
-        grads = [g if ctx.needs_input_grad[4 + i] else None for i, g in enumerate((gq, gk))]
-        have = [g for g in grads if g is not None]
+        saved = ctx.saved_tensors
+        positions = saved[0] if saved else None
+        if not ctx.needs_input_grad[4]:
+            gq = None
+        if not ctx.needs_input_grad[5]:
+            gk = None
+        # a gradient expanded along D (a sum's, say) has no unit stride there
+        have = [g if g.stride(-1) == 1 or g.shape[-1] == 1 else g.contiguous() for g in (gq, gk) if g is not None]
         if not have:
             return None, None, None, None, None, None
-        # a gradient expanded along D (a sum's, say) has no unit stride there
-        have = [g if g.stride(-1) == 1 or g.shape[-1] == 1 else g.contiguous() for g in have]
-        out = list(_Rotate.apply(rotary, positions, offset, not reverse, have[0], have[1] if len(have) > 1 else None))
-        return (None, None, None, None, *[None if g is None else out.pop(0) for g in grads])
+        second = have[1] if len(have) > 1 else None
+        if torch.is_grad_enabled():  # a gradient of this gradient is wanted
+            out = _Rotate.apply(rotary, positions, offset, not reverse, have[0], second)
+        else:
+            out = ops.rotary(rotary, have[0], second, positions, offset, not reverse)
+        if gq is None:
+            return None, None, None, None, None, out[0]
+        return None, None, None, None, out[0], out[1]
 
 
 __all__ = ["RotaryEmbedding"]
