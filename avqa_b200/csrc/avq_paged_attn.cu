@@ -26,6 +26,7 @@
 // order of the keys.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "avq_mma.cuh"
 #include "avq_paged.cuh"
@@ -36,7 +37,7 @@ namespace {
 
 __device__ int g_fault_tables_paged;
 
-constexpr int kRows = 16, kWarps = 4;
+constexpr int kWarps = 4;
 constexpr int kSpanUnit = 128;  // spans are multiples of a CTA's largest step
 // About three rounds of the CTAs that the SMs hold at once: less fills the last round badly, more pays a CTA's own cost
 // too often (32 sequences of up to 32768 keys, 8 heads of 128: 508 us at 4 per SM, 446 at 8, 455 at 16; 9 of up to
@@ -54,10 +55,11 @@ struct Piece {  // what one CTA works on
   bool found;
 };
 
-// Rows of sequence b that this kernel owns, in groups of kRows.
-__device__ __forceinline__ int row_groups(const PagedAttnArgs& a, int G, int n, int row_max) {
+// Rows of a sequence that this kernel owns, in groups of RB.
+template <int RB>
+__device__ __forceinline__ int row_groups(int G, int n, int row_max) {
   const long long rows = (long long)n * G;
-  return rows > row_max ? 0 : (int)((rows + kRows - 1) / kRows);
+  return rows > row_max ? 0 : (int)((rows + RB - 1) / RB);
 }
 
 // First key that any token of the sequence sees.
@@ -70,6 +72,7 @@ __device__ __forceinline__ int first_key(const PagedAttnArgs& a, const SeqRange&
 // Finds the piece of index `at`: a (sequence, key head, span, row group) when `spans`, else a
 // (sequence, key head, row group) with every span of it.  Each warp does the same work.  *slot receives the piece's
 // slot of partial sums (without `spans` that of its first span, the others `stride` apart).
+template <int RB>
 __device__ Piece find_piece(const PagedAttnArgs& a, int row_max, int at, bool spans, bool report, int* slot,
                             int* stride) {
   const int lane = threadIdx.x & 31, G = a.H / a.Hkv;
@@ -78,7 +81,7 @@ __device__ Piece find_piece(const PagedAttnArgs& a, int row_max, int at, bool sp
   long long total = 0;
   for (int b = lane; b < a.B; b += 32) {
     const SeqRange s = load_seq(a.q_start, a.kv_len, b, a.N, room, &bad);
-    total += (long long)row_groups(a, G, s.n, row_max) * a.Hkv * (s.len - first_key(a, s));
+    total += (long long)row_groups<RB>(G, s.n, row_max) * a.Hkv * (s.len - first_key(a, s));
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
@@ -97,7 +100,7 @@ __device__ Piece find_piece(const PagedAttnArgs& a, int row_max, int at, bool sp
     bool ignore = false;
     if (b < a.B) {
       s = load_seq(a.q_start, a.kv_len, b, a.N, room, &ignore);
-      groups = row_groups(a, G, s.n, row_max);
+      groups = row_groups<RB>(G, s.n, row_max);
       f = first_key(a, s);
       ns = max(1, (int)(((unsigned)(s.len - f) + span - 1) / span));
     }
@@ -198,12 +201,19 @@ constexpr int stage_elems() { return 2 * step_keys<DT, DP>() * (DP + Operand<DT>
 // streams (the widest rows: one stage, one CTA).
 template <int DT, int DP>
 constexpr int ring_stages() { return DP * (int)sizeof(typename Storage<DT>::T) <= 512 ? 2 : 1; }
-template <int DT, int DP>
+template <int DT, int DP, int RB>
 constexpr size_t mma_smem() {
   const size_t T = sizeof(typename Storage<DT>::T);
   const size_t ring = (size_t)kWarps * ring_stages<DT, DP>() * stage_elems<DT, DP>() * T;
-  const size_t merge = (size_t)kWarps * kRows * (DP + 2) * sizeof(float);
-  return std::max(ring, merge) + (size_t)kRows * (DP + Operand<DT>::kPad) * T;
+  const size_t merge = (size_t)kWarps * RB * (DP + 2) * sizeof(float);
+  return std::max(ring, merge) + (size_t)RB * (DP + Operand<DT>::kPad) * T;
+}
+
+// An 8 x 8 block of 16-bit values, two of a row to a lane, transposed.
+__device__ __forceinline__ uint32_t transposed8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -214,19 +224,24 @@ __device__ __forceinline__ float ex2(float x) {
 
 // WIDE: 16-byte copies.  SAME: the pools have the same strides, so that a key's place is its value's, and are below
 // 2^32 chunks of 16 bytes.
-template <int DT, int DP, bool WIDE, bool SAME>
+// RB: the rows of a group.  16 are the rows of the products S = Q K^T and O = P V; eight are the columns of the
+// transposed products (bf16, fp16), S^T = K Q^T and O^T = V^T P^T, whose 16 rows are keys and dimensions: half the
+// products and half the scores of a row tile that would be half empty.  P^T needs the other layout, which movmatrix
+// makes of each 8 x 8 block.
+template <int DT, int DP, bool WIDE, bool SAME, int RB>
 __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const PagedAttnArgs a, int row_max,
                                                                      int q_wide, int beside,
                                                                      float* __restrict__ part) {
   using T = typename Storage<DT>::T;
   constexpr int KS = step_keys<DT, DP>(), NK = KS / 8;  // keys of a step, in columns of 8
-  constexpr int LDS = DP + Operand<DT>::kPad, NT = DP / 8, STAGES = ring_stages<DT, DP>();
+  static_assert(RB == 16 || (RB == 8 && DT != DT_F32), "");
+  constexpr int LDS = DP + Operand<DT>::kPad, NT = RB == 8 ? DP / 16 : DP / 8, STAGES = ring_stages<DT, DP>();
   constexpr int EPC = 16 / (int)sizeof(T), CPR = DP / EPC;  // elements of a 16-byte chunk, chunks of a row
   extern __shared__ __align__(128) unsigned char smem_raw[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.H / a.Hkv;
   asm volatile("griddepcontrol.launch_dependents;");
   int slot = 0, slot_stride = 0;
-  const Piece p = find_piece(a, row_max, blockIdx.x, true, blockIdx.x == 0 && warp == 0, &slot, &slot_stride);
+  const Piece p = find_piece<RB>(a, row_max, blockIdx.x, true, blockIdx.x == 0 && warp == 0, &slot, &slot_stride);
   // a grid that runs beside another ends after it, so that what waits for this one has waited for both
   auto leave = [&]() {
     if (beside && blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -235,12 +250,12 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
     leave();
     return;
   }
-  T* sq = reinterpret_cast<T*>(smem_raw);                                  // [kRows][LDS]
-  T* ring = sq + kRows * LDS + warp * STAGES * stage_elems<DT, DP>();       // this warp's stages
-  const int row0 = p.group * kRows, nrow = min(kRows, p.seq.n * G - row0);
+  T* sq = reinterpret_cast<T*>(smem_raw);                                  // [RB][LDS]
+  T* ring = sq + RB * LDS + warp * STAGES * stage_elems<DT, DP>();       // this warp's stages
+  const int row0 = p.group * RB, nrow = min(RB, p.seq.n * G - row0);
 
   if (q_wide) {
-    for (int i = tid; i < kRows * CPR; i += kWarps * 32) {
+    for (int i = tid; i < RB * CPR; i += kWarps * 32) {
       const int r = i / CPR, c = (i - r * CPR) * EPC;
       const bool ok = r < nrow && c < a.D;
       const int tok = p.seq.q0 + (row0 + (ok ? r : 0)) / G, h = p.head * G + (row0 + (ok ? r : 0)) % G;
@@ -248,7 +263,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
                  static_cast<const T*>(a.q) + (long long)tok * a.qs.t + (long long)h * a.qs.h + (ok ? c : 0), ok);
     }
   } else {
-    for (int i = tid; i < kRows * DP; i += kWarps * 32) {
+    for (int i = tid; i < RB * DP; i += kWarps * 32) {
       const int r = i / DP, d = i - r * DP;
       T x = from_f<DT>(0.f);
       if (r < nrow && d < a.D) {
@@ -261,7 +276,8 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
   cp_async_commit();
 
   // the keys that any row of the group sees
-  const int ra = lane >> 2, rb = ra + 8;
+  // this thread's two rows: lane / 4 and eight on, or two neighbours
+  const int ra = RB == 8 ? (lane & 3) * 2 : lane >> 2, rb = RB == 8 ? ra + 1 : ra + 8;
   const int2 va = visible(a, p.seq.pos0 + (row0 + min(ra, nrow - 1)) / G, p.seq.len);
   const int2 vb = visible(a, p.seq.pos0 + (row0 + min(rb, nrow - 1)) / G, p.seq.len);
   const int2 vf = visible(a, p.seq.pos0 + row0 / G, p.seq.len);
@@ -340,8 +356,14 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
 
   cp_async_wait<STAGES - 1>();  // the queries
   __syncthreads();
-  uint32_t qf[DT == DT_F32 ? 1 : DP / 16][4];
-  if constexpr (DT != DT_F32) {
+  uint32_t qf[DT == DT_F32 ? 1 : DP / 16][RB == 8 ? 2 : 4];
+  if constexpr (RB == 8) {
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        qf[kk][e] = *reinterpret_cast<const uint32_t*>(sq + (lane >> 2) * LDS + kk * 16 + e * 8 + (lane & 3) * 2);
+  } else if constexpr (DT != DT_F32) {
 #pragma unroll
     for (int kk = 0; kk < DP / 16; ++kk)
       ldsm_x4(qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3], sq + (lane & 15) * LDS + kk * 16 + (lane >> 4) * 8);
@@ -351,6 +373,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
   for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
   float ma = -INFINITY, mb = -INFINITY, la = 0.f, lb = 0.f;
   const int ct = (lane & 3) * 2;
+  constexpr int kFirst = RB == 8 ? 4 : 1, kBehind = RB == 8 ? 32 : 4;  // the lanes that share a row's scores
 
   for (int step = 0; step < steps; ++step) {
     load(step + STAGES - 1);
@@ -358,10 +381,22 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
     __syncwarp();
     const T* sk = ring + (step % STAGES) * stage_elems<DT, DP>();
     const T* sv = sk + KS * LDS;
-    float s[NK][4];
+    // the scores: of columns j of 8 keys, [0, 1] row a, [2, 3] row b; transposed, of 16 keys, [0, 2] row a, [1, 3] row b
+    constexpr int NS = RB == 8 ? KS / 16 : NK;
+    constexpr int A1 = RB == 8 ? 2 : 1, B0 = RB == 8 ? 1 : 2;
+    float s[NS][4];
 #pragma unroll
-    for (int j = 0; j < NK; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
-    if constexpr (DT != DT_F32) {
+    for (int j = 0; j < NS; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+    if constexpr (RB == 8) {
+#pragma unroll
+      for (int kk = 0; kk < DP / 16; ++kk)
+#pragma unroll
+        for (int j = 0; j < NS; ++j) {
+          uint32_t ka[4];
+          ldsm_x4(ka[0], ka[1], ka[2], ka[3], sk + (j * 16 + (lane & 15)) * LDS + kk * 16 + (lane >> 4) * 8);
+          mma16816<DT>(s[j], ka, qf[kk][0], qf[kk][1]);
+        }
+    } else if constexpr (DT != DT_F32) {
 #pragma unroll
       for (int kk = 0; kk < DP / 16; ++kk) {
         const int qd = lane >> 3;
@@ -388,29 +423,29 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
       }
     }
 #pragma unroll
-    for (int j = 0; j < NK; ++j)
+    for (int j = 0; j < NS; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[j][e] *= a.scale_log2;
     const int k0 = lo + (step * kWarps + warp) * KS;
     if (k0 < every_lo || k0 + KS > every_hi) {
 #pragma unroll
-      for (int j = 0; j < NK; ++j)
+      for (int j = 0; j < NS; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int key = k0 + j * 8 + ct + (e & 1);
-          const int2 v = e >= 2 ? vb : va;
+          const int key = RB == 8 ? k0 + j * 16 + (lane >> 2) + (e >> 1) * 8 : k0 + j * 8 + ct + (e & 1);
+          const int2 v = (RB == 8 ? e & 1 : e >> 1) ? vb : va;
           if (key < v.x || key >= min(v.y, hi)) s[j][e] = -INFINITY;
         }
     }
     // (fmaxf drops a NaN score; its probability is NaN and carries it into the sum)
     float ta = -INFINITY, tb = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < NK; ++j) {
-      ta = fmaxf(ta, fmaxf(s[j][0], s[j][1]));
-      tb = fmaxf(tb, fmaxf(s[j][2], s[j][3]));
+    for (int j = 0; j < NS; ++j) {
+      ta = fmaxf(ta, fmaxf(s[j][0], s[j][A1]));
+      tb = fmaxf(tb, fmaxf(s[j][B0], s[j][3]));
     }
 #pragma unroll
-    for (int of = 1; of <= 2; of <<= 1) {
+    for (int of = kFirst; of < kBehind; of <<= 1) {
       ta = fmaxf(ta, __shfl_xor_sync(0xffffffffu, ta, of));
       tb = fmaxf(tb, __shfl_xor_sync(0xffffffffu, tb, of));
     }
@@ -422,8 +457,8 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         o[j][0] *= ca;
-        o[j][1] *= ca;
-        o[j][2] *= cb;
+        o[j][A1] *= ca;
+        o[j][B0] *= cb;
         o[j][3] *= cb;
       }
       ma = na;
@@ -432,15 +467,27 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
     // a row with no visible key so far keeps probabilities of zero
     const float xa = ma == -INFINITY ? 0.f : ma, xb = mb == -INFINITY ? 0.f : mb;
 #pragma unroll
-    for (int j = 0; j < NK; ++j) {
+    for (int j = 0; j < NS; ++j) {
       s[j][0] = ex2(s[j][0] - xa);
-      s[j][1] = ex2(s[j][1] - xa);
-      s[j][2] = ex2(s[j][2] - xb);
+      s[j][A1] = ex2(s[j][A1] - xa);
+      s[j][B0] = ex2(s[j][B0] - xb);
       s[j][3] = ex2(s[j][3] - xb);
-      la += s[j][0] + s[j][1];
-      lb += s[j][2] + s[j][3];
+      la += s[j][0] + s[j][A1];
+      lb += s[j][B0] + s[j][3];
     }
-    if constexpr (DT != DT_F32) {
+    if constexpr (RB == 8) {
+#pragma unroll
+      for (int j = 0; j < NS; ++j) {
+        const uint32_t p0 = transposed8(pack2<DT>(s[j][0], s[j][1])), p1 = transposed8(pack2<DT>(s[j][2], s[j][3]));
+#pragma unroll
+        for (int jj = 0; jj < NT; ++jj) {
+          uint32_t va4[4];
+          ldsm_x4_t(va4[0], va4[1], va4[2], va4[3],
+                    sv + (j * 16 + (lane >> 4) * 8 + (lane & 7)) * LDS + jj * 16 + ((lane >> 3) & 1) * 8);
+          mma16816<DT>(o[jj], va4, p0, p1);
+        }
+      }
+    } else if constexpr (DT != DT_F32) {
 #pragma unroll
       for (int j = 0; j < NK; j += 2) {
         const uint32_t pf[4] = {pack2<DT>(s[j][0], s[j][1]), pack2<DT>(s[j][2], s[j][3]),
@@ -474,7 +521,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
   }
   cp_async_wait<0>();
 #pragma unroll
-  for (int of = 1; of <= 2; of <<= 1) {
+  for (int of = kFirst; of < kBehind; of <<= 1) {
     la += __shfl_xor_sync(0xffffffffu, la, of);
     lb += __shfl_xor_sync(0xffffffffu, lb, of);
   }
@@ -482,29 +529,37 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
   __syncthreads();  // every warp is done with its ring
 
   // the warps' sums meet: one row's maximum, then the scaled sums
-  float* sm = reinterpret_cast<float*>(sq + kRows * LDS);  // [kWarps][kRows] maxima, then sums, then outputs
-  float* sl = sm + kWarps * kRows;
-  float* so = sl + kWarps * kRows;  // [kWarps][kRows][DP]
-  if ((lane & 3) == 0) {
-    sm[warp * kRows + ra] = ma;
-    sm[warp * kRows + rb] = mb;
+  float* sm = reinterpret_cast<float*>(sq + RB * LDS);  // [kWarps][RB] maxima, then sums, then outputs
+  float* sl = sm + kWarps * RB;
+  float* so = sl + kWarps * RB;  // [kWarps][RB][DP]
+  if (RB == 8 ? lane < 4 : (lane & 3) == 0) {
+    sm[warp * RB + ra] = ma;
+    sm[warp * RB + rb] = mb;
   }
   __syncthreads();
   float Ma = sm[ra], Mb = sm[rb];
 #pragma unroll
   for (int w = 1; w < kWarps; ++w) {
-    Ma = fmaxf(Ma, sm[w * kRows + ra]);
-    Mb = fmaxf(Mb, sm[w * kRows + rb]);
+    Ma = fmaxf(Ma, sm[w * RB + ra]);
+    Mb = fmaxf(Mb, sm[w * RB + rb]);
   }
   const float fa = ma == -INFINITY ? 0.f : ex2(ma - Ma), fb = mb == -INFINITY ? 0.f : ex2(mb - Mb);
   // (a maximum of +inf gives NaN here and in the probabilities, as a softmax over +inf does)
-  if ((lane & 3) == 0) {
-    sl[warp * kRows + ra] = la * fa;
-    sl[warp * kRows + rb] = lb * fb;
+  if (RB == 8 ? lane < 4 : (lane & 3) == 0) {
+    sl[warp * RB + ra] = la * fa;
+    sl[warp * RB + rb] = lb * fb;
   }
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
-    float* w = so + (warp * kRows + ra) * DP + j * 8 + ct;
+    if constexpr (RB == 8) {  // dimensions lane / 4 and eight on
+      float* w = so + (warp * RB + ra) * DP + j * 16 + (lane >> 2);
+      w[0] = o[j][0] * fa;
+      w[8] = o[j][2] * fa;
+      w[DP] = o[j][1] * fb;
+      w[DP + 8] = o[j][3] * fb;
+      continue;
+    }
+    float* w = so + (warp * RB + ra) * DP + j * 8 + ct;
     *reinterpret_cast<float2*>(w) = make_float2(o[j][0] * fa, o[j][1] * fa);
     if (nrow > 8) *reinterpret_cast<float2*>(w + 8 * DP) = make_float2(o[j][2] * fb, o[j][3] * fb);
   }
@@ -515,8 +570,8 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
     float x = 0.f, l = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      x += so[(w * kRows + r) * DP + d];
-      l += sl[w * kRows + r];
+      x += so[(w * RB + r) * DP + d];
+      l += sl[w * RB + r];
     }
     if (p.nspan == 1) {
       const int tok = p.seq.q0 + (row0 + r) / G, h = p.head * G + (row0 + r) % G;
@@ -525,13 +580,13 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
       static_cast<T*>(a.out)[(long long)tok * a.os.t + (long long)h * a.os.h + d] =
           from_f<DT>(v.y > v.x ? x / l : 0.f);
     } else {
-      float* w = part + (long long)slot * (kRows * (DP + 2));
+      float* w = part + (long long)slot * (RB * (DP + 2));
       w[r * DP + d] = x;
       if (d == 0) {
         float M = sm[r];
-        for (int k = 1; k < kWarps; ++k) M = fmaxf(M, sm[k * kRows + r]);
-        w[kRows * DP + r] = M;
-        w[kRows * DP + kRows + r] = l;
+        for (int k = 1; k < kWarps; ++k) M = fmaxf(M, sm[k * RB + r]);
+        w[RB * DP + r] = M;
+        w[RB * DP + RB + r] = l;
       }
     }
   }
@@ -542,7 +597,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
 // every so-manieth span, with a row of partial sums in one load of the warp.
 constexpr int kJoinWarps = 8;
 
-template <int DT, int DP>
+template <int DT, int DP, int RB>
 __global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const PagedAttnArgs a, int row_max, long long pieces,
                                                                   const float* __restrict__ part) {
   using T = typename Storage<DT>::T;
@@ -552,14 +607,14 @@ __global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const PagedAtt
   const int G = a.H / a.Hkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // the lists are older than the attention kernel, which this launch may overtake
   int slot = 0, stride = 0;
-  const Piece p = find_piece(a, row_max, blockIdx.x, false, false, &slot, &stride);
+  const Piece p = find_piece<RB>(a, row_max, blockIdx.x, false, false, &slot, &stride);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (!p.found || p.nspan == 1) return;
-  const int row0 = p.group * kRows, nrow = min(kRows, p.seq.n * G - row0);
+  const int row0 = p.group * RB, nrow = min(RB, p.seq.n * G - row0);
   // token ranges that overlap could name more pieces than there are slots
   if (slot < 0 || slot + (long long)(p.nspan - 1) * stride >= pieces) return;
-  const long long step = (long long)stride * (kRows * (DP + 2));
-  const float* base = part + (long long)slot * (kRows * (DP + 2));
+  const long long step = (long long)stride * (RB * (DP + 2));
+  const float* base = part + (long long)slot * (RB * (DP + 2));
   const int per_row = nrow >= kJoinWarps ? 1 : kJoinWarps / nrow;  // warps of a row
   const int share = warp % per_row;
   for (int r = warp / per_row; r < nrow || per_row > 1; r += kJoinWarps / per_row) {
@@ -570,14 +625,14 @@ __global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const PagedAtt
 #pragma unroll
       for (int e = 0; e < VW; ++e) x[i][e] = 0.f;
     if (mine) {
-      const float* bm = base + kRows * DP + r;
+      const float* bm = base + RB * DP + r;
       float M = -INFINITY;
       for (int s = lane; s < p.nspan; s += 32) M = fmaxf(M, bm[s * step]);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
 #pragma unroll 4
       for (int s = share; s < p.nspan; s += per_row) {
-        const float m = bm[s * step], ls = bm[s * step + kRows];
+        const float m = bm[s * step], ls = bm[s * step + RB];
         const float* w = base + s * step + r * DP;
         float y[NV][VW];
 #pragma unroll
@@ -638,13 +693,13 @@ __global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const PagedAtt
 
 // (row group, key head) pairs of the sequences with at most row_max rows, and the CTAs that hold every piece: the
 // target, and one partly filled span for each pair.
-long long most_items(int B, int N, int H, int Hkv, int row_max) {
+long long most_items(int B, int N, int H, int Hkv, int row_max, int group) {
   const long long G = H / Hkv, rows = (long long)N * G;
-  return std::min(rows / kRows + std::min<long long>(B, rows),
-                  std::min<long long>(B, N) * ((row_max + (long long)kRows - 1) / kRows)) * Hkv;
+  return std::min(rows / group + std::min<long long>(B, rows),
+                  std::min<long long>(B, N) * ((row_max + (long long)group - 1) / group)) * Hkv;
 }
-long long most_pieces(int B, int N, int H, int Hkv, int row_max) {
-  return most_items(B, N, H, Hkv, row_max) + kTargetCtas;
+long long most_pieces(int B, int N, int H, int Hkv, int row_max, int group) {
+  return most_items(B, N, H, Hkv, row_max, group) + kTargetCtas;
 }
 
 // Which kernels a call launches: this file's takes the sequences with at most row_max rows, the tcgen05 kernel, where
@@ -652,12 +707,15 @@ long long most_pieces(int B, int N, int H, int Hkv, int row_max) {
 struct Choice {
   bool many;
   int row_max;
+  int group;  // rows of a group in this file's kernel
 };
 
 Choice choose(int dtype, int N, int H, int Hkv, int D, int max_q, bool operands) {
   const long long G = H / Hkv, most = (long long)(max_q > 0 ? std::min(max_q, N) : N) * G;
-  if (dtype == DT_F32 || (D != 64 && D != 128) || !operands || most <= kFewRows) return {false, 1 << 30};
-  return {true, kFewRows};
+  const bool many = most > kFewRows && dtype != DT_F32 && (D == 64 || D == 128) && operands;
+  // groups of eight where the sequences that come here have no more rows: beside the tcgen05 kernel, single tokens
+  const int group = dtype != DT_F32 && operands && (many ? G : most) <= 8 ? 8 : 16;
+  return {many, many ? kFewRows : 1 << 30, group};
 }
 
 int padded_dim(int D) { return D <= 64 ? 64 : (D <= 128 ? 128 : 256); }
@@ -669,23 +727,24 @@ bool wide_rows(const void* p, std::initializer_list<long long> strides, int elem
   return true;
 }
 
-template <int DT, int DP>
-int launch_mma(const PagedAttnArgs& a, int row_max, bool beside, void* tc_workspace, float* part, cudaStream_t st) {
+template <int DT, int DP, int RB>
+int launch_mma(const PagedAttnArgs& a, const Choice& c, void* tc_workspace, float* part, cudaStream_t st) {
   using T = typename Storage<DT>::T;
-  const int E = (int)sizeof(T);
+  const int E = (int)sizeof(T), row_max = c.row_max;
+  const bool beside = c.many;
   const bool wide = a.D * E % 16 == 0 && wide_rows(a.kpool, {a.kps.p, a.kps.h, a.kps.s}, E) &&
                     wide_rows(a.vpool, {a.vps.p, a.vps.h, a.vps.s}, E);
   const bool q_wide = a.D * E % 16 == 0 && wide_rows(a.q, {a.qs.t, a.qs.h}, E);
-  const long long pieces = most_pieces(a.B, a.N, a.H, a.Hkv, row_max);
-  const long long items = most_items(a.B, a.N, a.H, a.Hkv, row_max);
-  const size_t smem = mma_smem<DT, DP>();
+  const long long pieces = most_pieces(a.B, a.N, a.H, a.Hkv, row_max, RB);
+  const long long items = most_items(a.B, a.N, a.H, a.Hkv, row_max, RB);
+  const size_t smem = mma_smem<DT, DP, RB>();
   const long long extent = (long long)std::max(a.num_pages - 1, 0) * a.kps.p + (long long)(a.page_size - 1) * a.kps.s;
   const bool same = a.kps.p == a.vps.p && a.kps.s == a.vps.s && a.kps.p >= 0 && a.kps.s >= 0 &&
                     extent / (16 / E) < 0xffffffffll;
   const int variant = !wide ? 0 : (same ? 2 : 1);
-  auto kfn = variant == 0 ? paged_attn_mma_kernel<DT, DP, false, false>
-                          : (variant == 1 ? paged_attn_mma_kernel<DT, DP, true, false>
-                                          : paged_attn_mma_kernel<DT, DP, true, true>);
+  auto kfn = variant == 0 ? paged_attn_mma_kernel<DT, DP, false, false, RB>
+                          : (variant == 1 ? paged_attn_mma_kernel<DT, DP, true, false, RB>
+                                          : paged_attn_mma_kernel<DT, DP, true, true, RB>);
   static std::atomic<unsigned long long> allowed[3];
   if (!allow_smem((const void*)kfn, smem, allowed[variant])) return AVQ_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
@@ -716,7 +775,7 @@ int launch_mma(const PagedAttnArgs& a, int row_max, bool beside, void* tc_worksp
   cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, combine_kernel<DT, DP>, a, row_max, pieces, (const float*)part) == cudaSuccess
+  return cudaLaunchKernelEx(&cfg, combine_kernel<DT, DP, RB>, a, row_max, pieces, (const float*)part) == cudaSuccess
              ? AVQ_OK
              : AVQ_ERR_CUDA;
 }
@@ -724,11 +783,14 @@ int launch_mma(const PagedAttnArgs& a, int row_max, bool beside, void* tc_worksp
 }  // namespace
 
 size_t paged_attn_workspace_bytes(int dtype, int B, int N, int H, int Hkv, int D, int max_q) {
-  // the operands' alignment may rule the tcgen05 kernel out: room for either choice
-  const Choice with = choose(dtype, N, H, Hkv, D, max_q, true);
+  // the operands' alignment decides between kernels too: room for any choice
   auto few_bytes = [&](int row_max) {
-    return align_up((size_t)most_pieces(B, N, H, Hkv, row_max) * kRows * (padded_dim(D) + 2) * sizeof(float));
+    size_t most = 0;
+    for (int group : {8, 16})
+      most = std::max(most, (size_t)most_pieces(B, N, H, Hkv, row_max, group) * group);
+    return align_up(most * (padded_dim(D) + 2) * sizeof(float));
   };
+  const Choice with = choose(dtype, N, H, Hkv, D, max_q, true);
   const size_t alone = few_bytes(1 << 30);
   if (!with.many) return alone;
   return std::max(alone, few_bytes(with.row_max) + paged_attn_tc_workspace_bytes(B, N, H, Hkv, D, with.row_max));
@@ -751,9 +813,16 @@ int launch_paged_attention(const PagedAttnArgs& a, cudaStream_t st) {
     }
   }
   float* part = reinterpret_cast<float*>(ws);
-  if (a.D <= 64) return launch_mma<DT, 64>(a, c.row_max, c.many, a.workspace, part, st);
-  if (a.D <= 128) return launch_mma<DT, 128>(a, c.row_max, c.many, a.workspace, part, st);
-  return launch_mma<DT, 256>(a, c.row_max, c.many, a.workspace, part, st);
+  auto go = [&](auto group) -> int {
+    constexpr int RB = decltype(group)::value;
+    if (a.D <= 64) return launch_mma<DT, 64, RB>(a, c, a.workspace, part, st);
+    if (a.D <= 128) return launch_mma<DT, 128, RB>(a, c, a.workspace, part, st);
+    return launch_mma<DT, 256, RB>(a, c, a.workspace, part, st);
+  };
+  if constexpr (DT != DT_F32) {
+    if (c.group == 8) return go(std::integral_constant<int, 8>{});
+  }
+  return go(std::integral_constant<int, 16>{});
 }
 
 int read_fault_paged(int* code, cudaStream_t st) {
