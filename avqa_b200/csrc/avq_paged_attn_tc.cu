@@ -560,21 +560,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
   } else {
     // ---- MMA issuer: the whole warp runs the loop, so that the descriptors stay in uniform registers (formed by one
     // lane on its own each multiplication took longer to issue than to compute); one elected lane issues ----
-    int ring = 0, q_phase = 0;
-    int count[2] = {0, 0};  // P tiles of each row tile so far
+    int slot = 0, q_phase = 0;
+    uint32_t ring_phase = 0;         // of the ring's slots from `slot` on, until it wraps
+    uint32_t p_phase[2] = {0, 0};    // of each row tile's P
+    const int fmt = DT == DT_BF16 ? 1 : 0;
+    const uint32_t id_s = tc::idesc_f16(fmt, TM, TK, false), id_o = tc::idesc_f16(fmt, TM, D, true);
+    const uint32_t q_low = desc_low(tc::smem_addr(sm + L::Q), kDescRows);
+    const uint32_t r_low = desc_low(tc::smem_addr(sm + L::RING), 0);
     for (int turn = 0; take(turn); ++turn) {
       const int nt = __shfl_sync(0xffffffffu, w.rows > TM ? 2 : 1, 0), tiles = __shfl_sync(0xffffffffu, w.tiles, 0);
-      const int fmt = DT == DT_BF16 ? 1 : 0;
-      const uint32_t id_s = tc::idesc_f16(fmt, TM, TK, false), id_o = tc::idesc_f16(fmt, TM, D, true);
-      auto tile_ready = [&](int i) {
-        const int n = ring + i;
-        return tc::mbar_wait(&bars[L::B_FULL + n % NR], (n / NR) & 1, abort);
+      auto agree = [&](bool ok) { return (bool)__all_sync(0xffffffffu, ok); };
+      auto step_on = [&](int& at, uint32_t& phase) {
+        if (++at == NR) {
+          at = 0;
+          phase ^= 1;
+        }
       };
-      auto empty = [&](int i) { return &bars[L::B_EMPTY + (ring + i) % NR]; };
-      const uint32_t q_low = desc_low(tc::smem_addr(sm + L::Q), kDescRows);
-      const uint32_t r_low = desc_low(tc::smem_addr(sm + L::RING), 0);
-      auto issue_s = [&](int t, int i) {
-        const uint32_t k_low = r_low + kDescRows + ((ring + i) % NR) * (TB / 16), qt = q_low + t * (TB / 16);
+      auto issue_s = [&](int t, int at) {
+        const uint32_t k_low = r_low + kDescRows + at * (TB / 16), qt = q_low + t * (TB / 16);
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
@@ -582,53 +585,56 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             mma_ss_low(col_s + t * TK, qt + o, k_low + o, id_s, kk > 0);
           }
           tc::mma_commit(&bars[L::B_S + t]);
-          if (t == nt - 1) tc::mma_commit(empty(i));
+          if (t == nt - 1) tc::mma_commit(&bars[L::B_EMPTY + at]);
         }
         __syncwarp();
       };
       // cp.async writes through the generic proxy; the tensor cores read through the async proxy, which a fence after
       // each wait puts behind those writes
-      bool ok = tc::mbar_wait(&bars[L::B_Q], q_phase & 1, abort) && tile_ready(0);
-      ok = __all_sync(0xffffffffu, ok);
+      bool ok = agree(tc::mbar_wait(&bars[L::B_Q], q_phase & 1, abort) &&
+                      tc::mbar_wait(&bars[L::B_FULL + slot], ring_phase, abort));
       if (ok) {
         tc::fence_async_smem();
         tc::tc_after_sync();
-        issue_s(0, 0);
-        if (nt > 1) issue_s(1, 0);
+        issue_s(0, slot);
+        if (nt > 1) issue_s(1, slot);
+        step_on(slot, ring_phase);
       }
       for (int j = 0; ok && j < tiles; ++j) {
-        ok = __all_sync(0xffffffffu, tile_ready(2 * j + 1));
-        if (!ok) break;
-        if constexpr (!TMA) tc::fence_async_smem();
-        const uint32_t v_low = r_low + kDescCols + ((ring + 2 * j + 1) % NR) * (TB / 16);
+        // the values of these keys and the next keys
+        const int v_at = slot;
+        const uint32_t v_phase = ring_phase;
+        step_on(slot, ring_phase);
+        const int k_at = slot;
+        const uint32_t k_phase = ring_phase;
+        const bool more = j + 1 < tiles;
+        if (more) step_on(slot, ring_phase);
+        ok = tc::mbar_wait(&bars[L::B_FULL + v_at], v_phase, abort) &&
+             (!more || tc::mbar_wait(&bars[L::B_FULL + k_at], k_phase, abort));
+        const uint32_t v_low = r_low + kDescCols + v_at * (TB / 16);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           if (t >= nt) break;
           // P of this tile's first 64 keys is in TMEM, and every thread is done with S; then P of the others
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {
-            ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(&bars[L::B_P + 2 * t + hf], (count[t] + j) & 1, abort));
+            ok = agree(ok && tc::mbar_wait(&bars[L::B_P + 2 * t + hf], p_phase[t], abort));
             if (!ok) break;
+            if constexpr (!TMA) tc::fence_async_smem();
             tc::tc_after_sync();
             if (elect_one()) {
 #pragma unroll
               for (int kk = hf * (TK / 32); kk < (hf + 1) * (TK / 32); ++kk)
                 mma_ts_low(col_o + t * D, col_s + t * TK + kk * 8, v_low + kk * (16 * 128 / 16), id_o, j > 0 || kk > 0);
-              if (hf == 1 && t == nt - 1) tc::mma_commit(empty(2 * j + 1));
-              if (hf == 1 && j + 1 == tiles) tc::mma_commit(&bars[L::B_O + t]);
+              if (hf == 1 && t == nt - 1) tc::mma_commit(&bars[L::B_EMPTY + v_at]);
+              if (hf == 1 && !more) tc::mma_commit(&bars[L::B_O + t]);
             }
             __syncwarp();
           }
           if (!ok) break;
-          if (j + 1 < tiles) {
-            // the scores of the next keys take the columns of P: the tensor cores work in the order of issue
-            if (t == 0) {
-              ok = __all_sync(0xffffffffu, tile_ready(2 * j + 2));
-              if (!ok) break;
-              if constexpr (!TMA) tc::fence_async_smem();
-            }
-            issue_s(t, 2 * j + 2);
-          }
+          p_phase[t] ^= 1;
+          // the scores of the next keys take the columns of P: the tensor cores work in the order of issue
+          if (more) issue_s(t, k_at);
         }
       }
       if (!ok) {  // let what was issued finish before the CTA leaves
@@ -638,10 +644,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         }
       }
       __syncwarp();
-      ring += 2 * tiles;
       ++q_phase;
-      count[0] += tiles;
-      if (nt > 1) count[1] += tiles;
       if (!turn_over()) break;
     }
   }
