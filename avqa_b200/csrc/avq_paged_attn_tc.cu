@@ -136,7 +136,19 @@ __device__ int block_prefix(int v, int* total) {
 
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PagedAttnArgs a, int row_min, int max_items,
                                                             int* __restrict__ ws) {
-  const Plan p = plan_at(ws, a.B, max_items, a.Hkv);
+  Plan p = plan_at(ws, a.B, max_items, a.Hkv);
+  // what the plan itself reads again stays in shared memory where it fits (a round trip to memory for each of the plan's
+  // steps would be most of its time); the joining kernel reads `seq` and `part` from the workspace
+  constexpr int kHeld = 1024;
+  __shared__ int s_base[kHeld + 1], s_seq[kHeld], s_part[kHeld], s_tiles[kHeld], s_sum[kHeld];
+  int *const out_seq = p.seq, *const out_part = p.part;
+  if (a.B <= kHeld && max_items <= kHeld) {
+    p.base = s_base;
+    p.seq = s_seq;
+    p.part = s_part;
+    p.tiles = s_tiles;
+    p.sum = s_sum;
+  }
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.H / a.Hkv;
   const long long room = (long long)a.W * a.page_size;
   asm volatile("griddepcontrol.launch_dependents;");
@@ -171,8 +183,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PagedAttnArgs 
     for (int i = lane; i < n; i += 32) {
       const int part = n - 1 - i;  // the last rows see the most keys: longest first
       const int2 k = item_keys(a, s, part, G);
-      p.seq[i0 + i] = b;
-      p.part[i0 + i] = part;
+      p.seq[i0 + i] = out_seq[i0 + i] = b;
+      p.part[i0 + i] = out_part[i0 + i] = part;
       p.tiles[i0 + i] = max(1, (k.y - k.x + TK - 1) / TK);
     }
   }
