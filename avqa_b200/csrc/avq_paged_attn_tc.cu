@@ -360,9 +360,11 @@ __device__ __forceinline__ float2 ex2_poly(float2 x) {
   return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(r.x) << 23)),
                      __int_as_float(__float_as_int(p.y) + (__float_as_int(r.y) << 23)));
 }
-// The pairs of eight that take the polynomial: three of eight even out the exponential unit (8 cycles an
-// instruction and warp) and the instruction slots.
-constexpr uint32_t kPolyPairs = 0x00;
+// The pairs of eight that take the polynomial.  At head_dim 64 the softmax bounds the kernel and the exponential unit the
+// softmax: a quarter there (4 prompts of about 2048 tokens over 8192: 576 us with none, 559 a quarter, 590 three
+// eighths).  At head_dim 128 the tensor cores and the power they draw bound it, and the polynomial's instructions only
+// cost (256 queries over 131072 keys: 1012 us with none, 1015 a quarter, 1080 three eighths).
+template <int D> constexpr uint32_t poly_pairs() { return D == 64 ? 0x12u : 0u; }
 
 template <int DT, int D, bool TMA>
 __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __grid_constant__ PoolMaps maps,
@@ -745,7 +747,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             for (int e = 0; e < 16; ++e) {
               const float2 y = fma2(make_float2(at(c, 2 * e), at(c, 2 * e + 1)), scale2, sub2);
               float2 p;
-              if (!exact.value && ((kPolyPairs >> (e & 7)) & 1)) p = ex2_poly<DT>(y);
+              if (!exact.value && ((poly_pairs<D>() >> (e & 7)) & 1)) p = ex2_poly<DT>(y);
               else p = make_float2(ex2(y.x), ex2(y.y));
               sum[e & 1] = add_f32x2(sum[e & 1], p);
               pk[e] = pack2<DT>(p.x, p.y);
