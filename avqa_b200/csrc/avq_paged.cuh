@@ -158,4 +158,57 @@ __device__ __forceinline__ SeqRange load_seq(const int* q_start, const int* kv_l
   return s;
 }
 
+// Keys visible to the token at position pos: [first, last).
+__device__ __forceinline__ int2 visible(const PagedAttnArgs& a, int pos, int len) {
+  int last = len, first = 0;
+  if (a.causal) last = pos < 0 ? 0 : min(len, pos + 1);
+  if (a.window > 0) first = max(0, pos - a.window + 1);
+  return make_int2(first, last);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// A product over a tile of rows takes every key of its tile or span for every row, those that a row does not see with a
+// probability of zero; where such a key's value is not finite, that makes 0 * inf = NaN of the row.  This is the row
+// again, key by key over [lo, hi) and its own visible keys, by one warp: its sums before division (the lanes' dimensions
+// lane, lane + 32, ..), its maximum (times log2 e) and its sum.  Rows that need it are rare, and its speed does not count.
+template <int DT, int DP>
+__device__ void row_alone(const PagedAttnArgs& a, const int* row_table, int head, const typename Storage<DT>::T* q,
+                          int lo, int hi, float (&x)[DP / 32], float* m_out, float* l_out) {
+  using T = typename Storage<DT>::T;
+  const int lane = threadIdx.x & 31;
+  float m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < DP / 32; ++i) x[i] = 0.f;
+  for (int key = lo; key < hi; ++key) {
+    const int page = row_table[key / a.page_size], s = key % a.page_size;
+    const bool have = page >= 0 && page < a.num_pages;  // a page outside the pool reads as zeros
+    const T* k = static_cast<const T*>(a.kpool) + (have ? page * a.kps.p + head * a.kps.h + s * a.kps.s : 0);
+    const T* v = static_cast<const T*>(a.vpool) + (have ? page * a.vps.p + head * a.vps.h + s * a.vps.s : 0);
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) {
+      const int d = i * 32 + lane;
+      if (d < a.D && have) dot = fmaf(to_f(q[d]), to_f(k[d]), dot);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    const float score = dot * a.scale_log2, mn = fmaxf(m, score), base = mn == -INFINITY ? 0.f : mn;
+    const float f = mn > m ? ex2(m - base) : 1.f, p = ex2(score - base);
+    l = l * f + p;
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) {
+      const int d = i * 32 + lane;
+      x[i] = fmaf(d < a.D && have ? to_f(v[d]) : 0.f, p, x[i] * f);
+    }
+    m = mn;
+  }
+  *m_out = m;
+  *l_out = l;
+}
+
 }  // namespace avq

@@ -38,6 +38,7 @@ namespace {
 __device__ int g_fault_tables_paged;
 
 constexpr int kWarps = 4;
+constexpr int kMaxGroup = 16;   // rows of a group, at most
 constexpr int kSpanUnit = 128;  // spans are multiples of a CTA's largest step
 // About three rounds of the CTAs that the SMs hold at once: less fills the last round badly, more pays a CTA's own cost
 // too often (32 sequences of up to 32768 keys, 8 heads of 128: 508 us at 4 per SM, 446 at 8, 455 at 16; 9 of up to
@@ -104,8 +105,10 @@ __device__ Piece find_piece(const PagedAttnArgs& a, int row_max, int at, bool sp
       f = first_key(a, s);
       ns = max(1, (int)(((unsigned)(s.len - f) + span - 1) / span));
     }
+    // (only cut sequences need slots: at most twice the target, as ceil(x) < 2 x for x > 1)
     const unsigned mine = (unsigned)groups * a.Hkv * ns, count = spans ? mine : (unsigned)groups * a.Hkv;
-    unsigned pre = count, pre_slots = mine;
+    const unsigned slotted = ns > 1 ? mine : 0u;
+    unsigned pre = count, pre_slots = slotted;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const unsigned x = __shfl_up_sync(0xffffffffu, pre, o), y = __shfl_up_sync(0xffffffffu, pre_slots, o);
@@ -118,7 +121,7 @@ __device__ Piece find_piece(const PagedAttnArgs& a, int row_max, int at, bool sp
     if (hit) {
       const int src = __ffs(hit) - 1;
       const unsigned rel = (unsigned)at - before - __shfl_sync(0xffffffffu, pre - count, src);
-      const unsigned base = slots + __shfl_sync(0xffffffffu, pre_slots - mine, src);
+      const unsigned base = slots + __shfl_sync(0xffffffffu, pre_slots - slotted, src);
       p.b = b0 + src;
       p.seq.q0 = __shfl_sync(0xffffffffu, s.q0, src);
       p.seq.n = __shfl_sync(0xffffffffu, s.n, src);
@@ -143,14 +146,6 @@ __device__ Piece find_piece(const PagedAttnArgs& a, int row_max, int at, bool sp
     slots += __shfl_sync(0xffffffffu, pre_slots, 31);
   }
   return p;
-}
-
-// Keys visible to the token at position pos: [first, last).
-__device__ __forceinline__ int2 visible(const PagedAttnArgs& a, int pos, int len) {
-  int last = len, first = 0;
-  if (a.causal) last = pos < 0 ? 0 : min(len, pos + 1);
-  if (a.window > 0) first = max(0, pos - a.window + 1);
-  return make_int2(first, last);
 }
 
 // ---- operands -----------------------------------------------------------------------
@@ -213,12 +208,6 @@ constexpr size_t mma_smem() {
 __device__ __forceinline__ uint32_t transposed8(uint32_t x) {
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-  return y;
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -564,6 +553,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
     if (nrow > 8) *reinterpret_cast<float2*>(w + 8 * DP) = make_float2(o[j][2] * fb, o[j][3] * fb);
   }
   __syncthreads();
+  bool odd = false;  // a sum that is not finite
   for (int i = tid; i < nrow * DP; i += kWarps * 32) {
     const int r = i / DP, d = i - r * DP;
     if (d >= a.D && p.nspan == 1) continue;
@@ -573,6 +563,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
       x += so[(w * RB + r) * DP + d];
       l += sl[w * RB + r];
     }
+    odd = odd || !isfinite(x);
     if (p.nspan == 1) {
       const int tok = p.seq.q0 + (row0 + r) / G, h = p.head * G + (row0 + r) % G;
       const int2 v = visible(a, p.seq.pos0 + (row0 + r) / G, p.seq.len);
@@ -590,6 +581,28 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
       }
     }
   }
+  // rows that do not all see the same keys, and a sum that is not finite: each row again on its own
+  if ((every_lo > lo || every_hi < hi) && __syncthreads_or(odd)) {
+    for (int r = warp; r < nrow; r += kWarps) {
+      const int tok = p.seq.q0 + (row0 + r) / G, h = p.head * G + (row0 + r) % G;
+      const int2 v = visible(a, p.seq.pos0 + (row0 + r) / G, p.seq.len);
+      float x[DP / 32], M, l;
+      row_alone<DT, DP>(a, row_table, p.head, static_cast<const T*>(a.q) + (long long)tok * a.qs.t + (long long)h * a.qs.h,
+                        max(v.x, p.lo), min(v.y, p.hi), x, &M, &l);
+      T* out = static_cast<T*>(a.out) + (long long)tok * a.os.t + (long long)h * a.os.h;
+      float* w = part + (long long)slot * (RB * (DP + 2));
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i) {
+        const int d = i * 32 + lane;
+        if (p.nspan > 1) w[r * DP + d] = x[i];
+        else if (d < a.D) out[d] = from_f<DT>(v.y > v.x ? x[i] / l : 0.f);
+      }
+      if (p.nspan > 1 && lane == 0) {
+        w[RB * DP + r] = M;
+        w[RB * DP + RB + r] = l;
+      }
+    }
+  }
   leave();
 }
 
@@ -598,7 +611,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
 constexpr int kJoinWarps = 8;
 
 template <int DT, int DP, int RB>
-__global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const PagedAttnArgs a, int row_max, long long pieces,
+__global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const PagedAttnArgs a, int row_max,
                                                                   const float* __restrict__ part) {
   using T = typename Storage<DT>::T;
   constexpr int VW = DP >= 128 ? 4 : 2, NV = DP / (32 * VW);  // floats of a lane's vector, vectors of a lane
@@ -611,8 +624,6 @@ __global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const PagedAtt
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (!p.found || p.nspan == 1) return;
   const int row0 = p.group * RB, nrow = min(RB, p.seq.n * G - row0);
-  // token ranges that overlap could name more pieces than there are slots
-  if (slot < 0 || slot + (long long)(p.nspan - 1) * stride >= pieces) return;
   const long long step = (long long)stride * (RB * (DP + 2));
   const float* base = part + (long long)slot * (RB * (DP + 2));
   const int per_row = nrow >= kJoinWarps ? 1 : kJoinWarps / nrow;  // warps of a row
@@ -775,7 +786,7 @@ int launch_mma(const PagedAttnArgs& a, const Choice& c, void* tc_workspace, floa
   cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, combine_kernel<DT, DP, RB>, a, row_max, pieces, (const float*)part) == cudaSuccess
+  return cudaLaunchKernelEx(&cfg, combine_kernel<DT, DP, RB>, a, row_max, (const float*)part) == cudaSuccess
              ? AVQ_OK
              : AVQ_ERR_CUDA;
 }
@@ -783,17 +794,9 @@ int launch_mma(const PagedAttnArgs& a, const Choice& c, void* tc_workspace, floa
 }  // namespace
 
 size_t paged_attn_workspace_bytes(int dtype, int B, int N, int H, int Hkv, int D, int max_q) {
-  // the operands' alignment decides between kernels too: room for any choice
-  auto few_bytes = [&](int row_max) {
-    size_t most = 0;
-    for (int group : {8, 16})
-      most = std::max(most, (size_t)most_pieces(B, N, H, Hkv, row_max, group) * group);
-    return align_up(most * (padded_dim(D) + 2) * sizeof(float));
-  };
-  const Choice with = choose(dtype, N, H, Hkv, D, max_q, true);
-  const size_t alone = few_bytes(1 << 30);
-  if (!with.many) return alone;
-  return std::max(alone, few_bytes(with.row_max) + paged_attn_tc_workspace_bytes(B, N, H, Hkv, D, with.row_max));
+  const size_t few = align_up((size_t)2 * kTargetCtas * kMaxGroup * (padded_dim(D) + 2) * sizeof(float));
+  const Choice with = choose(dtype, N, H, Hkv, D, max_q, true);  // (the operands' alignment may still rule it out)
+  return with.many ? few + paged_attn_tc_workspace_bytes(B, N, H, Hkv, D, with.row_max) : few;
 }
 
 template <int DT>

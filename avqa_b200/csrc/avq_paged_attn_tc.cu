@@ -59,6 +59,7 @@ struct __align__(16) PieceWork {
   int head, seq, row0, rows;      // key head, sequence; first row in it, rows from there on
   int key0, tiles, pieces, slot;  // first key, key tiles; pieces of its pair, its slot of partial sums
   int q0, pos0, len, end;         // the sequence's first token and that one's position, its keys; keys that the rows see
+  int pair, unused[3];
 };
 
 // The plan in the workspace: a header; the pieces; the items; the (key head, item) pairs, head by head.
@@ -72,10 +73,11 @@ struct Plan {
   int* sum;          // key tiles of the items before
   int* split;        // [pairs] pieces
   int* slot;         // [pairs] first slot of partial sums, where there are several pieces
+  int* odd;          // [pairs] raised where a row's sums are not finite and keys that it does not see may be why
 };
 
 __host__ __device__ inline long long plan_ints(long long B, long long items, long long Hkv) {
-  return 8 + (items * Hkv + kMaxSlots) * (long long)(sizeof(PieceWork) / 4) + (B + 1) + 4 * items + 2 * items * Hkv;
+  return 8 + (items * Hkv + kMaxSlots) * (long long)(sizeof(PieceWork) / 4) + (B + 1) + 4 * items + 3 * items * Hkv;
 }
 __host__ __device__ inline Plan plan_at(int* p, long long B, long long items, long long Hkv) {
   Plan q;
@@ -88,6 +90,7 @@ __host__ __device__ inline Plan plan_at(int* p, long long B, long long items, lo
   q.sum = q.tiles + items;
   q.split = q.sum + items;
   q.slot = q.split + items * Hkv;
+  q.odd = q.slot + items * Hkv;
   return q;
 }
 
@@ -234,6 +237,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PagedAttnArgs 
       w.pos0 = s.pos0;
       w.len = s.len;
       w.end = k.y;
+      w.pair = c;
       const int all = p.tiles[i];
       for (int x = 0, t = 0; x < n; ++x) {  // equal shares of the pair's tiles
         const int next = (int)((long long)all * (x + 1) / n);
@@ -245,6 +249,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PagedAttnArgs 
       }
       p.split[c] = n;
       p.slot[c] = slot;
+      p.odd[c] = 0;
     }
     pieces += total;
     slots += total_slots;
@@ -290,12 +295,6 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
       : "=f"(d.x), "=f"(d.y)
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
   return d;
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 // The two words of a 128-byte-swizzled matrix descriptor (avq_tc.cuh, sdesc_sw128).  Only the address, in the low word,
@@ -772,6 +771,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         tc::tc_after_sync();
         const bool whole = w.pieces == 1;
         const int rows = w.rows, row0 = w.row0, head = w.head;
+        float zero = 0.f;  // NaN once a sum is not finite
         // a row that sees no key is zero; one whose keys all score -inf is 0 / 0
         const float f = whole ? (last > first ? (m == -INFINITY ? NAN : 1.f / l) : 0.f) : 1.f;
         if (whole) {
@@ -783,6 +783,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             uint32_t o[32];
             tc::tmem_ld32(o_at + c * 32, o);
             tc::tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) zero = fmaf(__uint_as_float(o[e]), 0.f, zero);
 #pragma unroll
             for (int e = 0; e < 32; e += 8) {
               uint32_t y[4];
@@ -823,6 +825,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             uint32_t o[32];
             tc::tmem_ld32(o_at + c * 32, o);
             tc::tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) zero = fmaf(__uint_as_float(o[e]), 0.f, zero);
             if (r < rows) {
 #pragma unroll
               for (int e = 0; e < 32; e += 4)
@@ -831,6 +835,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             }
           }
         }
+        // (the joining kernel then takes the pair's rows one by one)
+        if (zero != 0.f && r < rows && (first > key0 || last < min(w.end, key0 + tiles * TK))) plan.odd[w.pair] = 1;
         tc::tc_before_sync();
       }
       s_count += tiles;
@@ -856,7 +862,8 @@ __global__ void __launch_bounds__(256) combine_tc_kernel(const PagedAttnArgs a, 
   const int items = plan.head[2], pair = blockIdx.x, G = a.H / a.Hkv;
   if (pair >= items * a.Hkv) return;
   const int np = plan.split[pair], head = pair / items, item = pair - head * items;
-  if (np <= 1) return;
+  const bool odd = plan.odd[pair] != 0;
+  if (np <= 1 && !odd) return;
   bool bad = false;
   const SeqRange seq = load_seq(a.q_start, a.kv_len, plan.seq[item], a.N, (long long)a.W * a.page_size, &bad);
   const int row0 = plan.part[item] * kItemRows, rows = min(kItemRows, seq.n * G - row0);
@@ -866,6 +873,20 @@ __global__ void __launch_bounds__(256) combine_tc_kernel(const PagedAttnArgs a, 
   __shared__ float weight[kSms][kJoinRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r0 = blockIdx.y * kJoinRows;
   if (r0 >= rows) return;
+  if (odd) {
+    for (int r = r0 + warp; r < min(rows, r0 + kJoinRows); r += 8) {
+      const int tok = seq.q0 + (row0 + r) / G, h = head * G + (row0 + r) % G;
+      const int2 v = visible(a, seq.pos0 + (row0 + r) / G, seq.len);
+      float x[D / 32], m, l;
+      row_alone<DT, D>(a, a.table + (long long)plan.seq[item] * a.table_stride, head,
+                       static_cast<const T*>(a.q) + (long long)tok * a.qs.t + (long long)h * a.qs.h, v.x, v.y, x, &m, &l);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+        static_cast<T*>(a.out)[(long long)tok * a.os.t + (long long)h * a.os.h + i * 32 + lane] =
+            from_f<DT>(v.y > v.x ? x[i] / l : 0.f);
+    }
+    return;
+  }
 #pragma unroll
   for (int x = 0; x < kJoinRows / 8; ++x) {
     const int row = warp * (kJoinRows / 8) + x, r = min(r0 + row, rows - 1);

@@ -107,6 +107,14 @@ CASES = {
     "big_chunk": ("bf16", 8, 1, 128, 256, [300], [1500], {}),
     "big_chunk_f16_d64": ("f16", 4, 4, 64, 16, [260, 515], [260, 1030], {}),
     "big_window": ("bf16", 4, 2, 128, 32, [400, 3], [1700, 800], dict(window=300)),
+    "chunk_longer_than_its_cache": ("bf16", 4, 2, 64, 16, [60, 0, 33], [40, 5, 0], {}),  # rows that see nothing
+    "rows_16_and_17": ("f16", 1, 1, 64, 16, [16, 17], [200, 150], {}),
+    "rows_128_and_129": ("bf16", 2, 1, 128, 16, [64, 65], [64, 300], {}),
+    "rows_256_and_257": ("bf16", 1, 1, 128, 128, [256, 257], [400, 257], {}),
+    "page_384": ("f16", 4, 2, 64, 384, [90, 1], [1000, 385], {}),
+    "page_8": ("bf16", 4, 2, 128, 8, [40, 1], [333, 41], {}),
+    "many_sequences": ("bf16", 2, 1, 64, 16, [1] * 1100, [1 + 7 * i % 45 for i in range(1100)], {}),
+    "many_chunks": ("bf16", 1, 1, 64, 16, [20] * 1100, [20 + 7 * i % 45 for i in range(1100)], {}),
     "big_not_causal": ("bf16", 4, 2, 64, 16, [200], [700], dict(causal=False)),
 }
 
@@ -175,6 +183,48 @@ def test_attention_nan_and_infinity() -> None:
     b.q.zero_()
     b.q[..., 0] = 1
     assert torch.isnan(ops.paged_attention(b.q, *b.lists)).all()
+
+
+@pytest.mark.parametrize("dt,D,page", [("bf16", 128, 16), ("f16", 64, 24), ("bf16", 72, 16), ("f32", 64, 16)])
+@pytest.mark.parametrize("new,length,window", [(3, 40, 0), (60, 200, 0), (200, 200, 0), (200, 4000, 0), (70, 300, 50)])
+def test_attention_unseen_keys_reach_no_row(dt, D, page, new, length, window) -> None:
+    """A key or value that is not finite changes the rows that see it, and no other, whatever tile they share."""
+    b = Batch(dt, 4, 2, D, page, [new, 1], [length, 30])
+    clean = ops.paged_attention(b.q, *b.lists, window=window)
+    at = length - new + new // 2  # a token in the middle of the new ones
+    slot = int(b.block_table[0, at // page]), slice(None), at % page
+    for pool, value in ((b.value_pool, float("nan")), (b.value_pool, float("inf")), (b.key_pool, float("nan"))):
+        kept = pool[slot].clone()
+        pool[slot] = value
+        got = ops.paged_attention(b.q, *b.lists, window=window)
+        pool[slot] = kept
+        pos = length - new + torch.arange(new, device="cuda")
+        sees = torch.zeros(b.N, dtype=torch.bool, device="cuda")
+        sees[:new] = (pos >= at) & ((pos < at + window) if window else True)
+        want, bound, _ = attention64(b.q, *b.lists, window=window)
+        assert_within(got[~sees], want[~sees], bound[~sees], "rows that do not see it")
+        assert not torch.isfinite(got[sees].float()).any()
+    assert torch.equal(ops.paged_attention(b.q, *b.lists, window=window), clean)
+
+
+@pytest.mark.parametrize("new,length", [(1, 700), (40, 700)])
+def test_offsets_beyond_32_bits(new, length) -> None:
+    """Pools of more than 2^32 elements each, with the pages in use at their end."""
+    D, page = 128, 256
+    pages = 2 ** 32 // (page * D) + 8
+    b = Batch("bf16", 4, 1, D, page, [new], [length])
+    used = b.block_table[0].long()
+    key_pool, value_pool = (torch.empty(pages, 1, page, D, device="cuda", dtype=b.dt) for _ in range(2))
+    far = torch.tensor([[pages - 1 - i for i in range(len(used))]], dtype=torch.int32, device="cuda")
+    key_pool[far[0].long()], value_pool[far[0].long()] = b.key_pool[used], b.value_pool[used]
+    want = ops.paged_attention(b.q, *b.lists)
+    assert torch.equal(ops.paged_attention(b.q, key_pool, value_pool, far, b.kv_len, b.q_start), want)
+    rot = RotaryEmbedding(D)
+    ops.paged_append(b.k, b.v, *b.lists, rotary=rot)
+    ops.paged_append(b.k, b.v, key_pool, value_pool, far, b.kv_len, b.q_start, rotary=rot)
+    for big, small in ((key_pool, b.key_pool), (value_pool, b.value_pool)):
+        assert torch.equal(big[far[0].long()].view(torch.int16), small[used].view(torch.int16))
+    assert fault() == 0
 
 
 def test_attention_large_scores_do_not_overflow() -> None:
