@@ -9,13 +9,16 @@
 //
 // paged_attn_mma_kernel: the kernel of few rows (single tokens, short drafts)
 // and of every type and head width.  Its rows are the (token, head of the
-// group) pairs of one sequence and key head, 16 to a CTA, so that one read of
-// a key serves the whole group; the sequence's keys are cut into spans, a CTA
+// group) pairs of one sequence and key head, 8 or 16 to a CTA, so that one read
+// of a key serves the whole group; the sequence's keys are cut into spans, a CTA
 // each.  Memory bounds it: every key and value is read once, by cp.async into
-// a ring of each warp's own (16 keys a stage), so that no barrier joins the
-// warps until their sums meet at the end.  The span follows from the lengths,
-// which only the device knows: every CTA adds up the batch's work, takes the
-// span that cuts it into about kTargetCtas pieces, and finds its own piece.
+// a ring of each warp's own (16 or 32 keys a stage), so that no barrier joins
+// the warps until their sums meet at the end (32 sequences of up to 32768 keys,
+// 8 key heads of 128, bf16: 454 us, 6.4 TB/s).  The span follows from the
+// lengths, which only the device knows: every CTA adds up the batch's work,
+// takes the span that cuts it into about target_ctas pieces, and finds its own.
+// Few short sequences go to clusters of CTAs instead, which join their sums
+// through shared memory (one token of 4097 keys, 8 key heads: 12 us).
 //
 // The scores, the running maximum and sum, and the output are fp32.  bf16 and
 // fp16 multiply on mma.sync with the probabilities rounded to the dtype
@@ -39,14 +42,24 @@ __device__ int g_fault_tables_paged;
 
 constexpr int kWarps = 4;
 constexpr int kMaxGroup = 16;   // rows of a group, at most
-constexpr int kSpanUnit = 128;  // spans are multiples of a CTA's largest step
-// About three rounds of the CTAs that the SMs hold at once: less fills the last round badly, more pays a CTA's own cost
-// too often (32 sequences of up to 32768 keys, 8 heads of 128: 508 us at 4 per SM, 446 at 8, 455 at 16; 9 of up to
-// 9000, 16 heads of 64: 51, 47 and 61).
-constexpr int kTargetCtas = 8 * kSms, kMinSpan = 128;
+// The pieces that a batch of `total` keys (over its row groups and key heads) is cut into.  Long batches: about three
+// rounds of the CTAs that the SMs hold at once; less fills the last round badly, more pays a CTA's own cost too often (32
+// sequences of up to 32768 keys, 8 heads of 128: 503 us at 2 per SM, 454 at 8, 455 at 16).  Short ones: a single round,
+// as a CTA's first loads and its merge are then most of its time (one sequence of 16384 keys, 8 heads of 128: 18 us at 2
+// per SM, 30 at 8; of 32768 keys 34 and 44).  The two meet between 2^19 keys (55 and 63 us) and 2^20 (104 and 97).
+constexpr int kTargetCtas = 8 * kSms, kFewestCtas = 2 * kSms, kMinSpan = 128;
+constexpr long long kFewKeys = 1 << 19;
+// A cluster of eight CTAs for each (row group, key head), without a second kernel, where two CTAs to an SM hold them all
+// and the keys of a sequence are few (bf16, 8 key heads of 128: 1024 keys 7 us and in pieces 8.5, 4096 keys 11.2 and 11.4,
+// 8192 keys 16.6 and 13.5; 64 pairs of 512 keys, more than the SMs hold: 15 and 11).  fp32, whose keys cost four times as
+// much: 1024 keys 9.6 and 11.5, 2048 keys 14 and 12.
+constexpr int kCluster = 8;
+constexpr long long kClusterItems = 2 * kSms / kCluster, kClusterKeys = 4096;
 // Rows (new tokens x heads of a group) of a sequence up to which one pass of 16-row groups over its keys is
 // taken, above which the tcgen05 kernel.
 constexpr int kFewRows = 16;
+
+__host__ __device__ constexpr int target_ctas(long long total) { return total > kFewKeys ? kTargetCtas : kFewestCtas; }
 
 struct Piece {  // what one CTA works on
   int b, group, head, span_i;  // sequence, row group, key head, index of the span
@@ -70,10 +83,10 @@ __device__ __forceinline__ int first_key(const PagedAttnArgs& a, const SeqRange&
   return f > 0 ? min(f, s.len) : 0;
 }
 
-// Finds the piece of index `at`: a (sequence, key head, span, row group) when `spans`, else a
+// Finds the piece of index `at`, spans being multiples of UNIT keys (a CTA's step): a (sequence, key head, span, row group) when `spans`, else a
 // (sequence, key head, row group) with every span of it.  Each warp does the same work.  *slot receives the piece's
 // slot of partial sums (without `spans` that of its first span, the others `stride` apart).
-template <int RB>
+template <int RB, int UNIT>
 __device__ Piece find_piece(const PagedAttnArgs& a, int row_max, int at, bool spans, bool report, int* slot,
                             int* stride) {
   const int lane = threadIdx.x & 31, G = a.H / a.Hkv;
@@ -87,10 +100,10 @@ __device__ Piece find_piece(const PagedAttnArgs& a, int row_max, int at, bool sp
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   if (report && bad) atomicOr(&g_fault_tables_paged, kFaultTables);
-  const unsigned span =
-      (unsigned)min((max((total + kTargetCtas - 1) / kTargetCtas, (long long)kMinSpan) + kSpanUnit - 1) / kSpanUnit *
-                        kSpanUnit,
-                    (long long)(1 << 30));
+  const int target = target_ctas(total);
+  const unsigned span = (unsigned)min(
+      (max((total + target - 1) / target, (long long)kMinSpan) + UNIT - 1) / UNIT * UNIT,
+      (long long)(1 << 30));
   Piece p;
   p.found = false;
   unsigned before = 0, slots = 0;  // pieces and partial slots of the sequences before
@@ -165,12 +178,11 @@ __device__ __forceinline__ void mma_tf32(float* d, const uint32_t* a, uint32_t b
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// x = hi + lo + (less than 2^-22 of x), both tf32.
+// x = hi + lo + (less than 2^-22 of x), both tf32.  (An infinity leaves a NaN in the low part: rows whose sums are not
+// finite are formed again on their own.)
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
-  // an infinity or NaN is all in the high part
-  const float rest = isfinite(x) ? x - __uint_as_float(hi) : 0.f;
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(rest));
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
 }
 // d += a * b.  The tensor cores' own sums truncate: one step's products are summed there, the steps by rounded fp32
 // additions.
@@ -193,15 +205,16 @@ constexpr int step_keys() { return DP * (int)sizeof(typename Storage<DT>::T) <= 
 template <int DT, int DP>
 constexpr int stage_elems() { return 2 * step_keys<DT, DP>() * (DP + Operand<DT>::kPad); }
 // Stages of a warp's ring: two, so that three CTAs or more share an SM and one's first loads overlap the others'
-// streams (the widest rows: one stage, one CTA).
-template <int DT, int DP>
-constexpr int ring_stages() { return DP * (int)sizeof(typename Storage<DT>::T) <= 512 ? 2 : 1; }
-template <int DT, int DP, int RB>
+// streams (the widest rows: one stage, one CTA); three in a cluster, where fewer CTAs run.
+template <int DT, int DP, bool CL>
+constexpr int ring_stages() { return DP * (int)sizeof(typename Storage<DT>::T) <= 512 ? (CL && DT != DT_F32 ? 3 : 2) : 1; }
+template <int DT, int DP, int RB, bool CL>
 constexpr size_t mma_smem() {
   const size_t T = sizeof(typename Storage<DT>::T);
-  const size_t ring = (size_t)kWarps * ring_stages<DT, DP>() * stage_elems<DT, DP>() * T;
+  const size_t ring = (size_t)kWarps * ring_stages<DT, DP, CL>() * stage_elems<DT, DP>() * T;
   const size_t merge = (size_t)kWarps * RB * (DP + 2) * sizeof(float);
-  return std::max(ring, merge) + (size_t)RB * (DP + Operand<DT>::kPad) * T;
+  // the queries, in fp32 as their two parts
+  return std::max(ring, merge) + (size_t)(DT == DT_F32 ? 2 : 1) * RB * (DP + Operand<DT>::kPad) * T;
 }
 
 // An 8 x 8 block of 16-bit values, two of a row to a lane, transposed.
@@ -217,30 +230,54 @@ __device__ __forceinline__ uint32_t transposed8(uint32_t x) {
 // transposed products (bf16, fp16), S^T = K Q^T and O^T = V^T P^T, whose 16 rows are keys and dimensions: half the
 // products and half the scores of a row tile that would be half empty.  P^T needs the other layout, which movmatrix
 // makes of each 8 x 8 block.
-template <int DT, int DP, bool WIDE, bool SAME, int RB>
+// CL: the spans of a (row group, key head) are the CTAs of a cluster, in equal shares of the sequence's keys, and join
+// their sums through each other's shared memory, without a second kernel.
+__device__ __forceinline__ float peer_float(const float* p, int rank) {
+  uint32_t at;
+  float x;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(at) : "memory");
+  return x;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <int DT, int DP, bool WIDE, bool SAME, int RB, bool CL>
 __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const PagedAttnArgs a, int row_max,
                                                                      int q_wide, int beside,
                                                                      float* __restrict__ part) {
   using T = typename Storage<DT>::T;
   constexpr int KS = step_keys<DT, DP>(), NK = KS / 8;  // keys of a step, in columns of 8
   static_assert(RB == 16 || (RB == 8 && DT != DT_F32), "");
-  constexpr int LDS = DP + Operand<DT>::kPad, NT = RB == 8 ? DP / 16 : DP / 8, STAGES = ring_stages<DT, DP>();
+  constexpr int LDS = DP + Operand<DT>::kPad, NT = RB == 8 ? DP / 16 : DP / 8, STAGES = ring_stages<DT, DP, CL>();
   constexpr int EPC = 16 / (int)sizeof(T), CPR = DP / EPC;  // elements of a 16-byte chunk, chunks of a row
   extern __shared__ __align__(128) unsigned char smem_raw[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.H / a.Hkv;
   asm volatile("griddepcontrol.launch_dependents;");
   int slot = 0, slot_stride = 0;
-  const Piece p = find_piece<RB>(a, row_max, blockIdx.x, true, blockIdx.x == 0 && warp == 0, &slot, &slot_stride);
+  Piece p = find_piece<RB, kWarps * KS>(a, row_max, CL ? blockIdx.x / kCluster : blockIdx.x, !CL,
+                                        blockIdx.x == 0 && warp == 0, &slot, &slot_stride);
   // a grid that runs beside another ends after it, so that what waits for this one has waited for both
   auto leave = [&]() {
     if (beside && blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
   };
-  if (!p.found) {
+  if (!p.found) {  // (all CTAs of a cluster look for the same)
     leave();
     return;
   }
+  const int rank = blockIdx.x % kCluster;
+  if constexpr (CL) {
+    const int first = first_key(a, p.seq), each = (p.seq.len - first + kCluster - 1) / kCluster;
+    const int share = (each + kWarps * KS - 1) / (kWarps * KS) * (kWarps * KS);
+    p.lo = (int)min((long long)p.seq.len, first + (long long)rank * share);
+    p.hi = (int)min((long long)p.seq.len, p.lo + (long long)share);
+  }
+  const bool direct = !CL && p.nspan == 1;
   T* sq = reinterpret_cast<T*>(smem_raw);                                  // [RB][LDS]
-  T* ring = sq + RB * LDS + warp * STAGES * stage_elems<DT, DP>();       // this warp's stages
+  T* sq_low = sq + RB * LDS;                                               // fp32: the queries' low parts
+  T* shared = DT == DT_F32 ? sq_low + RB * LDS : sq_low;
+  T* ring = shared + warp * STAGES * stage_elems<DT, DP>();                // this warp's stages
   const int row0 = p.group * RB, nrow = min(RB, p.seq.n * G - row0);
 
   if (q_wide) {
@@ -345,6 +382,16 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
 
   cp_async_wait<STAGES - 1>();  // the queries
   __syncthreads();
+  if constexpr (DT == DT_F32) {
+    for (int i = tid; i < RB * DP; i += kWarps * 32) {
+      const int at = i / DP * LDS + i % DP;
+      uint32_t h, l;
+      split_tf32(sq[at], h, l);
+      sq[at] = __uint_as_float(h);
+      sq_low[at] = __uint_as_float(l);
+    }
+    __syncthreads();
+  }
   uint32_t qf[DT == DT_F32 ? 1 : DP / 16][RB == 8 ? 2 : 4];
   if constexpr (RB == 8) {
 #pragma unroll
@@ -402,10 +449,12 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
       for (int kk = 0; kk < DP / 8; ++kk) {
         const int c = kk * 8 + (lane & 3), r = lane >> 2;
         uint32_t ah[4], al[4];
-        split_tf32(to_f(sq[r * LDS + c]), ah[0], al[0]);
-        split_tf32(to_f(sq[(r + 8) * LDS + c]), ah[1], al[1]);
-        split_tf32(to_f(sq[r * LDS + c + 4]), ah[2], al[2]);
-        split_tf32(to_f(sq[(r + 8) * LDS + c + 4]), ah[3], al[3]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int at = (r + (e & 1) * 8) * LDS + c + (e >> 1) * 4;
+          ah[e] = __float_as_uint(to_f(sq[at]));
+          al[e] = __float_as_uint(to_f(sq_low[at]));
+        }
 #pragma unroll
         for (int j = 0; j < NK; ++j)
           mma_split(s[j], ah, al, to_f(sk[(j * 8 + r) * LDS + c]), to_f(sk[(j * 8 + r) * LDS + c + 4]));
@@ -518,7 +567,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
   __syncthreads();  // every warp is done with its ring
 
   // the warps' sums meet: one row's maximum, then the scaled sums
-  float* sm = reinterpret_cast<float*>(sq + RB * LDS);  // [kWarps][RB] maxima, then sums, then outputs
+  float* sm = reinterpret_cast<float*>(shared);  // [kWarps][RB] maxima, then sums, then outputs
   float* sl = sm + kWarps * RB;
   float* so = sl + kWarps * RB;  // [kWarps][RB][DP]
   if (RB == 8 ? lane < 4 : (lane & 3) == 0) {
@@ -553,36 +602,40 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
     if (nrow > 8) *reinterpret_cast<float2*>(w + 8 * DP) = make_float2(o[j][2] * fb, o[j][3] * fb);
   }
   __syncthreads();
+  // Where a piece's sums go: the output, its slot, or this CTA's shared memory (in place of the first warp's).
+  auto slot_at = [&]() { return part + (long long)slot * (RB * (DP + 2)); };
+  float* const x_at = CL ? so : slot_at();
+  float* const m_at = CL ? sm : slot_at() + RB * DP;
+  float* const l_at = CL ? sl : slot_at() + RB * DP + RB;
   bool odd = false;  // a sum that is not finite
   for (int i = tid; i < nrow * DP; i += kWarps * 32) {
     const int r = i / DP, d = i - r * DP;
-    if (d >= a.D && p.nspan == 1) continue;
+    if (d >= a.D && direct) continue;
     float x = 0.f, l = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       x += so[(w * RB + r) * DP + d];
-      l += sl[w * RB + r];
+      if (direct || d == 0) l += sl[w * RB + r];
     }
     odd = odd || !isfinite(x);
-    if (p.nspan == 1) {
+    if (direct) {
       const int tok = p.seq.q0 + (row0 + r) / G, h = p.head * G + (row0 + r) % G;
       const int2 v = visible(a, p.seq.pos0 + (row0 + r) / G, p.seq.len);
       // a row that sees no key is zero; one whose keys all score -inf is 0 / 0
       static_cast<T*>(a.out)[(long long)tok * a.os.t + (long long)h * a.os.h + d] =
           from_f<DT>(v.y > v.x ? x / l : 0.f);
     } else {
-      float* w = part + (long long)slot * (RB * (DP + 2));
-      w[r * DP + d] = x;
+      x_at[r * DP + d] = x;
       if (d == 0) {
         float M = sm[r];
         for (int k = 1; k < kWarps; ++k) M = fmaxf(M, sm[k * RB + r]);
-        w[RB * DP + r] = M;
-        w[RB * DP + RB + r] = l;
+        m_at[r] = M;
+        l_at[r] = l;
       }
     }
   }
-  // rows that do not all see the same keys, and a sum that is not finite: each row again on its own
-  if ((every_lo > lo || every_hi < hi) && __syncthreads_or(odd)) {
+  // rows that do not all see the same keys, or fp32's parts, and a sum that is not finite: each row again on its own
+  if ((DT == DT_F32 || every_lo > lo || every_hi < hi) && __syncthreads_or(odd)) {
     for (int r = warp; r < nrow; r += kWarps) {
       const int tok = p.seq.q0 + (row0 + r) / G, h = p.head * G + (row0 + r) % G;
       const int2 v = visible(a, p.seq.pos0 + (row0 + r) / G, p.seq.len);
@@ -590,25 +643,54 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
       row_alone<DT, DP>(a, row_table, p.head, static_cast<const T*>(a.q) + (long long)tok * a.qs.t + (long long)h * a.qs.h,
                         max(v.x, p.lo), min(v.y, p.hi), x, &M, &l);
       T* out = static_cast<T*>(a.out) + (long long)tok * a.os.t + (long long)h * a.os.h;
-      float* w = part + (long long)slot * (RB * (DP + 2));
 #pragma unroll
       for (int i = 0; i < DP / 32; ++i) {
         const int d = i * 32 + lane;
-        if (p.nspan > 1) w[r * DP + d] = x[i];
+        if (!direct) x_at[r * DP + d] = x[i];
         else if (d < a.D) out[d] = from_f<DT>(v.y > v.x ? x[i] / l : 0.f);
       }
-      if (p.nspan > 1 && lane == 0) {
-        w[RB * DP + r] = M;
-        w[RB * DP + RB + r] = l;
+      if (!direct && lane == 0) {
+        m_at[r] = M;
+        l_at[r] = l;
       }
     }
+  }
+  if constexpr (CL) {
+    cluster_sync();
+    for (int i = rank * (kWarps * 32) + tid; i < nrow * DP; i += kCluster * kWarps * 32) {
+      const int r = i / DP, d = i - r * DP;
+      if (d >= a.D) continue;
+      float m[kCluster], M = -INFINITY, x = 0.f, l = 0.f;
+#pragma unroll
+      for (int c = 0; c < kCluster; ++c) {
+        m[c] = peer_float(sm + r, c);
+        M = fmaxf(M, m[c]);
+      }
+#pragma unroll
+      for (int c = 0; c < kCluster; ++c) {
+        const float xc = peer_float(so + r * DP + d, c), lc = peer_float(sl + r, c);
+        // a share whose keys the row does not see (or that all score -inf) adds nothing
+        const float f = m[c] == -INFINITY ? 0.f : ex2(m[c] - M);
+        if (m[c] == -INFINITY && lc == 0.f) continue;
+        x = fmaf(xc, f, x);
+        l = fmaf(lc, f, l);
+      }
+      const int tok = p.seq.q0 + (row0 + r) / G, h = p.head * G + (row0 + r) % G;
+      const int2 v = visible(a, p.seq.pos0 + (row0 + r) / G, p.seq.len);
+      static_cast<T*>(a.out)[(long long)tok * a.os.t + (long long)h * a.os.h + d] =
+          from_f<DT>(v.y > v.x ? x / l : 0.f);
+    }
+    cluster_sync();  // until every peer has read
   }
   leave();
 }
 
-// Joins the spans of one (sequence, key head, row group): a warp per row, or several where the rows are few, each on
-// every so-manieth span, with a row of partial sums in one load of the warp.
+// Joins the spans of one (sequence, key head, row group), or every gridDim.y-th row of it: a warp per row, or several
+// where the rows are few, each on every so-manieth span, with a row of partial sums in one load of the warp.
 constexpr int kJoinWarps = 8;
+// CTAs up to which the rows of a pair go to several (one sequence of 32768 keys, one key head: 66 us of a call with one
+// CTA a pair, 20 with one a row).
+constexpr int kJoinCtas = 4 * kSms;
 
 template <int DT, int DP, int RB>
 __global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const PagedAttnArgs a, int row_max,
@@ -620,16 +702,19 @@ __global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const PagedAtt
   const int G = a.H / a.Hkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // the lists are older than the attention kernel, which this launch may overtake
   int slot = 0, stride = 0;
-  const Piece p = find_piece<RB>(a, row_max, blockIdx.x, false, false, &slot, &stride);
+  const Piece p = find_piece<RB, kWarps * step_keys<DT, DP>()>(a, row_max, blockIdx.x, false, false, &slot, &stride);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (!p.found || p.nspan == 1) return;
   const int row0 = p.group * RB, nrow = min(RB, p.seq.n * G - row0);
   const long long step = (long long)stride * (RB * (DP + 2));
   const float* base = part + (long long)slot * (RB * (DP + 2));
-  const int per_row = nrow >= kJoinWarps ? 1 : kJoinWarps / nrow;  // warps of a row
+  const int rows = (nrow - (int)blockIdx.y + (int)gridDim.y - 1) / (int)gridDim.y;  // of this CTA
+  if (rows <= 0) return;
+  const int per_row = rows >= kJoinWarps ? 1 : kJoinWarps / rows;  // warps of a row
   const int share = warp % per_row;
-  for (int r = warp / per_row; r < nrow || per_row > 1; r += kJoinWarps / per_row) {
-    const bool mine = r < nrow && warp < nrow * per_row;
+  for (int i_row = warp / per_row; i_row < rows || per_row > 1; i_row += kJoinWarps / per_row) {
+    const bool mine = i_row < rows && warp < rows * per_row;
+    const int r = i_row * gridDim.y + blockIdx.y;
     float x[NV][VW], l = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -702,17 +787,12 @@ __global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const PagedAtt
   }
 }
 
-// (row group, key head) pairs of the sequences with at most row_max rows, and the CTAs that hold every piece: the
-// target, and one partly filled span for each pair.
+// (row group, key head) pairs of the sequences with at most row_max rows, at most.
 long long most_items(int B, int N, int H, int Hkv, int row_max, int group) {
   const long long G = H / Hkv, rows = (long long)N * G;
   return std::min(rows / group + std::min<long long>(B, rows),
                   std::min<long long>(B, N) * ((row_max + (long long)group - 1) / group)) * Hkv;
 }
-long long most_pieces(int B, int N, int H, int Hkv, int row_max, int group) {
-  return most_items(B, N, H, Hkv, row_max, group) + kTargetCtas;
-}
-
 // Which kernels a call launches: this file's takes the sequences with at most row_max rows, the tcgen05 kernel, where
 // it is launched too, the others.
 struct Choice {
@@ -746,29 +826,44 @@ int launch_mma(const PagedAttnArgs& a, const Choice& c, void* tc_workspace, floa
   const bool wide = a.D * E % 16 == 0 && wide_rows(a.kpool, {a.kps.p, a.kps.h, a.kps.s}, E) &&
                     wide_rows(a.vpool, {a.vps.p, a.vps.h, a.vps.s}, E);
   const bool q_wide = a.D * E % 16 == 0 && wide_rows(a.q, {a.qs.t, a.qs.h}, E);
-  const long long pieces = most_pieces(a.B, a.N, a.H, a.Hkv, row_max, RB);
   const long long items = most_items(a.B, a.N, a.H, a.Hkv, row_max, RB);
-  const size_t smem = mma_smem<DT, DP, RB>();
   const long long extent = (long long)std::max(a.num_pages - 1, 0) * a.kps.p + (long long)(a.page_size - 1) * a.kps.s;
   const bool same = a.kps.p == a.vps.p && a.kps.s == a.vps.s && a.kps.p >= 0 && a.kps.s >= 0 &&
                     extent / (16 / E) < 0xffffffffll;
-  const int variant = !wide ? 0 : (same ? 2 : 1);
-  auto kfn = variant == 0 ? paged_attn_mma_kernel<DT, DP, false, false, RB>
-                          : (variant == 1 ? paged_attn_mma_kernel<DT, DP, true, false, RB>
-                                          : paged_attn_mma_kernel<DT, DP, true, true, RB>);
-  static std::atomic<unsigned long long> allowed[3];
+  const long long room = std::min((long long)a.W * a.page_size, 1ll << 31);  // keys of a sequence, at most
+  // a cluster for each (row group, key head) where they are few and their keys are: one kernel and no partial sums in
+  // memory; else spans enough to fill the SMs
+  const int variant = !wide ? 0 : (!same ? 1 : (!beside && items <= kClusterItems && room * (DT == DT_F32 ? 4 : 1) <= kClusterKeys ? 3 : 2));
+  auto kfn = variant == 0   ? paged_attn_mma_kernel<DT, DP, false, false, RB, false>
+             : variant == 1 ? paged_attn_mma_kernel<DT, DP, true, false, RB, false>
+             : variant == 2 ? paged_attn_mma_kernel<DT, DP, true, true, RB, false>
+                            : paged_attn_mma_kernel<DT, DP, true, true, RB, true>;
+  const size_t smem = variant == 3 ? mma_smem<DT, DP, RB, true>() : mma_smem<DT, DP, RB, false>();
+  static std::atomic<unsigned long long> allowed[4];
   if (!allow_smem((const void*)kfn, smem, allowed[variant])) return AVQ_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.stream = st;
   cudaLaunchAttribute attr;
+  if (variant == 3) {
+    AVQ_TIMED("paged_attn", st);
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = kCluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    cfg.gridDim = dim3((unsigned)(items * kCluster));
+    cfg.blockDim = dim3(kWarps * 32);
+    cfg.dynamicSmemBytes = smem;
+    return cudaLaunchKernelEx(&cfg, kfn, a, row_max, (int)q_wide, 0, part) == cudaSuccess ? AVQ_OK : AVQ_ERR_CUDA;
+  }
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   {
     AVQ_TIMED("paged_attn", st);
     // beside the tcgen05 kernel, whose SMs it takes over one by one (it needs nothing of its)
-    const long long room = ((long long)a.W * a.page_size + kMinSpan - 1) / kMinSpan;
-    cfg.gridDim = dim3((unsigned)std::min(pieces, items * std::max(room, 1ll)));
+    // (every piece has its CTA: the target's, and one partly filled span for each pair)
+    cfg.gridDim = dim3((unsigned)(items + std::min<long long>(target_ctas(items * room), items * (room / kMinSpan))));
     cfg.blockDim = dim3(kWarps * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.numAttrs = beside ? 1 : 0;
@@ -782,7 +877,9 @@ int launch_mma(const PagedAttnArgs& a, const Choice& c, void* tc_workspace, floa
   }
   AVQ_TIMED("paged_combine", st);
   // the launch overlaps the attention kernel's end; the kernel waits for its results itself
-  cfg.gridDim = dim3((unsigned)std::max<long long>(items, 1));
+  long long split = 1;
+  while (split < RB && items * split < kJoinCtas) split *= 2;
+  cfg.gridDim = dim3((unsigned)items, (unsigned)split);
   cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;

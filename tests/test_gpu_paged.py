@@ -132,6 +132,24 @@ def test_attention_matches_formula(name, slot_major) -> None:
     assert fault() == 0
 
 
+@pytest.mark.parametrize("dt,D", [("bf16", 128), ("f16", 64), ("bf16", 72), ("f32", 64), ("f32", 256)])
+@pytest.mark.parametrize("new,lens", [([1], [1]), ([1, 0, 1], [2, 900, 1023]), ([2, 1], [1000, 0]), ([3, 1], [2, 70])])
+@pytest.mark.parametrize("window", [0, 40])
+def test_few_short_sequences_by_either_split(dt, D, new, lens, window) -> None:
+    """Tables of different widths hold the same keys: clusters of CTAs for the narrow, spans and a join for the wide."""
+    for pages in (0, 600):
+        b = Batch(dt, 4, 2, D, 16, new, lens, width=pages)
+        b.check(f"{pages} pages to a row", window=window)
+        b.check(f"{pages} pages to a row, every key", causal=False)
+
+
+def test_many_keys_take_the_larger_count_of_pieces() -> None:
+    """More keys than a single round of CTAs takes: 16 heads of 17 sequences, with rows that see little among them."""
+    b = Batch("bf16", 16, 16, 64, 32, [1] * 17, [2300] * 15 + [1, 0])
+    b.check()
+    b.check(window=100)
+
+
 def test_attention_rows_behind_the_last_sequence_stay() -> None:
     for new, lens in (([2, 1], [40, 9]), ([200, 3], [300, 9])):
         b = Batch("bf16", 4, 2, 64, 16, new, lens)
@@ -176,6 +194,17 @@ def test_attention_nan_and_infinity() -> None:
     assert torch.isnan(out[1]).all()
     assert torch.isinf(out[2, :, 9]).all() and torch.isfinite(out[2, :, :9]).all()
     assert torch.isfinite(out[3, 0]).all() and not torch.isfinite(out[3, 1]).any()
+    b = Batch("f32", 2, 1, 64, 16, [1, 1, 1], [30, 30, 30])  # fp32: its parts of an infinity are formed again
+    b.value_pool[int(b.block_table[0, 1]), 0, 2, 9] = float("-inf")
+    b.q[2, 0, 0] = float("nan")
+    minus = b.key_pool[int(b.block_table[1, 0]), 0, 3]
+    minus.zero_()
+    minus[5] = float("-inf")
+    b.q[1, :, 5] = b.q[1, :, 5].abs() + 1  # that key scores -inf: no weight, and no NaN
+    out = ops.paged_attention(b.q, *b.lists)
+    assert (out[0, :, 9] == float("-inf")).all() and torch.isfinite(out[0, :, :9]).all()
+    assert torch.isfinite(out[1]).all()
+    assert torch.isnan(out[2, 0]).all() and torch.isfinite(out[2, 1]).all()
     # scores of -inf on every visible key: 0 / 0, as softmax over -inf
     b = Batch("f32", 1, 1, 64, 16, [1], [20])
     b.key_pool[b.block_table[0].long()] = 0
