@@ -20,7 +20,7 @@ from dataclasses import dataclass
 
 import torch
 
-from avqa_b200.exceptions import ConfigurationError, NotInitializedError, ShapeError
+from avqa_b200.exceptions import BackendError, ConfigurationError, NotInitializedError, ShapeError
 
 
 class KVCache(ABC):
@@ -245,7 +245,10 @@ class BlockKVCache(KVCache):
     def reserve(self, new: Sequence[int]) -> PagedBatch:
         """Make room for ``new[b]`` more tokens of each sequence b (a longer
         list than before starts new sequences) and return the step's lists.
-        The cache is unchanged when the pool cannot hold them."""
+        The cache is unchanged when the pool cannot hold them.  The lists are a
+        step's own: a CUDA graph captures the operators over lists made before."""
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise BackendError("a step's pages cannot be reserved while a CUDA graph is captured")
         new = [int(n) for n in new]
         if len(new) < len(self.lengths) or any(n < 0 for n in new):
             raise ShapeError("every sequence needs a number of new tokens, 0 or more", expected=len(self.lengths),

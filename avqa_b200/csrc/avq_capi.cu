@@ -429,7 +429,6 @@ int rotary_spec(const char* what, int D, int rotary_dim, int interleaved, const 
   std::memset(spec, 0, sizeof(*spec));
   spec->pairs = rotary_dim / 2;
   spec->interleaved = interleaved != 0;
-  spec->axes = num_axes;
   spec->reversed = reversed != 0;
   for (int i = 0; i < spec->pairs; ++i) {
     spec->half_turns[i] = frequencies[i] / 3.14159265358979323846;
@@ -584,7 +583,8 @@ int avq_paged_attention(int dtype, const void* q, const long long* q_strides, in
     return fail(AVQ_ERR_ARG, "avq_paged_attention: %d query heads are no multiple of %d key heads", H, Hkv);
   if (window < 0 || (window > 0 && !causal))
     return fail(AVQ_ERR_ARG, "avq_paged_attention: a window needs causal, and a size >= 0");
-  if (!std::isfinite(scale)) return fail(AVQ_ERR_ARG, "avq_paged_attention: scale must be finite");
+  const float scale_log2 = (float)((double)scale * 1.4426950408889634);
+  if (!std::isfinite(scale_log2)) return fail(AVQ_ERR_ARG, "avq_paged_attention: scale must be finite");
   if (max_q_len < 0) return fail(AVQ_ERR_ARG, "avq_paged_attention: bad max_q_len %d", max_q_len);
   if (((long long)N * H + (long long)B * Hkv) > INT_MAX / 2 || (long long)N * H * D > (1ll << 40))
     return fail(AVQ_ERR_ARG, "avq_paged_attention: N*H = %lld is too large", (long long)N * H);
@@ -616,12 +616,11 @@ int avq_paged_attention(int dtype, const void* q, const long long* q_strides, in
   a.W = table_width;
   a.causal = causal != 0;
   a.window = window;
-  a.scale_log2 = (float)((double)scale * 1.4426950408889634);
+  a.scale_log2 = scale_log2;
   a.out = out;
   a.os = st2(out_strides);
   a.max_q = max_q_len;
   a.workspace = workspace;
-  a.workspace_bytes = workspace_bytes;
   cudaStream_t st = (cudaStream_t)stream;
   switch (dtype) {
     case 0: rc = avq::launch_paged_attention<avq::DT_F32>(a, st); break;

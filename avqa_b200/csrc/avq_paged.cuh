@@ -50,7 +50,6 @@ constexpr int kMaxPairs = 128;  // head_dim <= 256
 struct RotarySpec {
   int pairs;        // R/2 rotated pairs; dimensions >= 2 * pairs pass through
   int interleaved;  // pairs (2i, 2i+1) instead of (i, i + R/2)
-  int axes;
   int reversed;     // rotate by the negative angle (the gradient)
   double half_turns[kMaxPairs];  // angle per position, in units of pi
   unsigned char axis[kMaxPairs];
@@ -87,7 +86,6 @@ struct PagedAppendArgs {
   const int* kv_len;
   const int* q_start;
   int B, N, Hkv, D, num_pages, page_size, W;
-  int rotate;
   const void* positions;  // [axes, N] by strides, or nullptr: the cache position
   int pos_bytes;
   long long pa, pt;
@@ -119,7 +117,6 @@ struct PagedAttnArgs {
   Strides2 os;
   int max_q;         // host bound of the new tokens per sequence, 0: unknown
   void* workspace;
-  size_t workspace_bytes;
 };
 
 // The tcgen05 kernel (bf16, fp16; head_dim 64 and 128; 16-byte rows; scale > 0) for the sequences with more than
@@ -158,12 +155,14 @@ __device__ __forceinline__ SeqRange load_seq(const int* q_start, const int* kv_l
   return s;
 }
 
+// First key in the window of the token at position pos (which may be negative, the window any int).
+__device__ __forceinline__ int window_start(const PagedAttnArgs& a, int pos) {
+  return a.window > 0 ? (int)max(0ll, (long long)pos + 1 - a.window) : 0;
+}
+
 // Keys visible to the token at position pos: [first, last).
 __device__ __forceinline__ int2 visible(const PagedAttnArgs& a, int pos, int len) {
-  int last = len, first = 0;
-  if (a.causal) last = pos < 0 ? 0 : min(len, pos + 1);
-  if (a.window > 0) first = max(0, pos - a.window + 1);
-  return make_int2(first, last);
+  return make_int2(window_start(a, pos), !a.causal ? len : (pos < 0 ? 0 : min(len, pos + 1)));
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -172,10 +171,10 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// A product over a tile of rows takes every key of its tile or span for every row, those that a row does not see with a
-// probability of zero; where such a key's value is not finite, that makes 0 * inf = NaN of the row.  This is the row
-// again, key by key over [lo, hi) and its own visible keys, by one warp: its sums before division (the lanes' dimensions
-// lane, lane + 32, ..), its maximum (times log2 e) and its sum.  Rows that need it are rare, and its speed does not count.
+// A product over a tile of rows takes every key of its tile or span for every row, those that a row does not see with
+// a probability of zero; where such a key's value is not finite, that makes 0 * inf = NaN of the row.  This is the row
+// again, key by key over its visible keys [lo, hi), by one warp: its sums before division (the lanes' dimensions lane,
+// lane + 32, ..), its maximum (times log2 e) and its sum.  Rows that need it are rare, and its speed does not count.
 template <int DT, int DP>
 __device__ void row_alone(const PagedAttnArgs& a, const int* row_table, int head, const typename Storage<DT>::T* q,
                           int lo, int hi, float (&x)[DP / 32], float* m_out, float* l_out) {

@@ -43,16 +43,16 @@ __device__ int g_fault_tables_paged;
 constexpr int kWarps = 4;
 constexpr int kMaxGroup = 16;   // rows of a group, at most
 // The pieces that a batch of `total` keys (over its row groups and key heads) is cut into.  Long batches: about three
-// rounds of the CTAs that the SMs hold at once; less fills the last round badly, more pays a CTA's own cost too often (32
-// sequences of up to 32768 keys, 8 heads of 128: 503 us at 2 per SM, 454 at 8, 455 at 16).  Short ones: a single round,
-// as a CTA's first loads and its merge are then most of its time (one sequence of 16384 keys, 8 heads of 128: 18 us at 2
-// per SM, 30 at 8; of 32768 keys 34 and 44).  The two meet between 2^19 keys (55 and 63 us) and 2^20 (104 and 97).
+// rounds of the CTAs that the SMs hold at once; less fills the last round badly, more pays a CTA's own cost too often
+// (32 sequences of up to 32768 keys, 8 heads of 128: 503 us at 2 per SM, 454 at 8, 455 at 16).  Short ones: a single
+// round, as a CTA's first loads and its merge are then most of its time (one sequence of 16384 keys, 8 heads of 128: 18
+// us at 2 per SM, 30 at 8; of 32768 keys 34 and 44).  The two meet between 2^19 keys (55 and 63 us) and 2^20 (104, 97).
 constexpr int kTargetCtas = 8 * kSms, kFewestCtas = 2 * kSms, kMinSpan = 128;
 constexpr long long kFewKeys = 1 << 19;
-// A cluster of eight CTAs for each (row group, key head), without a second kernel, where two CTAs to an SM hold them all
-// and the keys of a sequence are few (bf16, 8 key heads of 128: 1024 keys 7 us and in pieces 8.5, 4096 keys 11.2 and 11.4,
-// 8192 keys 16.6 and 13.5; 64 pairs of 512 keys, more than the SMs hold: 15 and 11).  fp32, whose keys cost four times as
-// much: 1024 keys 9.6 and 11.5, 2048 keys 14 and 12.
+// A cluster of eight CTAs for each (row group, key head), without a second kernel, where two CTAs to an SM hold them
+// all and the keys of a sequence are few (bf16, 8 key heads of 128: 1024 keys 7 us and in pieces 8.5, 4096 keys 11.2
+// and 11.4, 8192 keys 16.6 and 13.5; 64 pairs of 512 keys, more than the SMs hold: 15 and 11).  fp32, whose keys cost
+// four times as much: 1024 keys 9.6 and 11.5, 2048 keys 14 and 12.
 constexpr int kCluster = 8;
 constexpr long long kClusterItems = 2 * kSms / kCluster, kClusterKeys = 4096;
 // Rows (new tokens x heads of a group) of a sequence up to which one pass of 16-row groups over its keys is
@@ -78,14 +78,12 @@ __device__ __forceinline__ int row_groups(int G, int n, int row_max) {
 
 // First key that any token of the sequence sees.
 __device__ __forceinline__ int first_key(const PagedAttnArgs& a, const SeqRange& s) {
-  if (a.window <= 0) return 0;
-  const int f = s.pos0 - a.window + 1;
-  return f > 0 ? min(f, s.len) : 0;
+  return min(window_start(a, s.pos0), s.len);
 }
 
-// Finds the piece of index `at`, spans being multiples of UNIT keys (a CTA's step): a (sequence, key head, span, row group) when `spans`, else a
-// (sequence, key head, row group) with every span of it.  Each warp does the same work.  *slot receives the piece's
-// slot of partial sums (without `spans` that of its first span, the others `stride` apart).
+// Finds the piece of index `at`, spans being multiples of UNIT keys (a CTA's step): a (sequence, key head, span, row
+// group) when `spans`, else a (sequence, key head, row group) with every span of it.  Each warp does the same work.
+// *slot receives the piece's slot of partial sums (without `spans` that of its first span, the others `stride` apart).
 template <int RB, int UNIT>
 __device__ Piece find_piece(const PagedAttnArgs& a, int row_max, int at, bool spans, bool report, int* slot,
                             int* stride) {
@@ -204,10 +202,12 @@ template <int DT, int DP>
 constexpr int step_keys() { return DP * (int)sizeof(typename Storage<DT>::T) <= 128 ? 32 : 16; }
 template <int DT, int DP>
 constexpr int stage_elems() { return 2 * step_keys<DT, DP>() * (DP + Operand<DT>::kPad); }
-// Stages of a warp's ring: two, so that three CTAs or more share an SM and one's first loads overlap the others'
-// streams (the widest rows: one stage, one CTA); three in a cluster, where fewer CTAs run.
+// Stages of a warp's ring: two, so that three CTAs or more (fp32: two) share an SM and one's first loads overlap the
+// others' streams (fp32 of 129 dimensions on: one stage, one CTA); three in a cluster, where fewer CTAs run.
 template <int DT, int DP, bool CL>
-constexpr int ring_stages() { return DP * (int)sizeof(typename Storage<DT>::T) <= 512 ? (CL && DT != DT_F32 ? 3 : 2) : 1; }
+constexpr int ring_stages() {
+  return DP * (int)sizeof(typename Storage<DT>::T) > 512 ? 1 : (CL && DT != DT_F32 ? 3 : 2);
+}
 template <int DT, int DP, int RB, bool CL>
 constexpr size_t mma_smem() {
   const size_t T = sizeof(typename Storage<DT>::T);
@@ -417,7 +417,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
     __syncwarp();
     const T* sk = ring + (step % STAGES) * stage_elems<DT, DP>();
     const T* sv = sk + KS * LDS;
-    // the scores: of columns j of 8 keys, [0, 1] row a, [2, 3] row b; transposed, of 16 keys, [0, 2] row a, [1, 3] row b
+    // the scores: of columns j of 8 keys, [0, 1] row a, [2, 3] row b; transposed, of 16 keys, [0, 2] and [1, 3]
     constexpr int NS = RB == 8 ? KS / 16 : NK;
     constexpr int A1 = RB == 8 ? 2 : 1, B0 = RB == 8 ? 1 : 2;
     float s[NS][4];
@@ -640,8 +640,8 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
       const int tok = p.seq.q0 + (row0 + r) / G, h = p.head * G + (row0 + r) % G;
       const int2 v = visible(a, p.seq.pos0 + (row0 + r) / G, p.seq.len);
       float x[DP / 32], M, l;
-      row_alone<DT, DP>(a, row_table, p.head, static_cast<const T*>(a.q) + (long long)tok * a.qs.t + (long long)h * a.qs.h,
-                        max(v.x, p.lo), min(v.y, p.hi), x, &M, &l);
+      const T* q_row = static_cast<const T*>(a.q) + (long long)tok * a.qs.t + (long long)h * a.qs.h;
+      row_alone<DT, DP>(a, row_table, p.head, q_row, max(v.x, p.lo), min(v.y, p.hi), x, &M, &l);
       T* out = static_cast<T*>(a.out) + (long long)tok * a.os.t + (long long)h * a.os.h;
 #pragma unroll
       for (int i = 0; i < DP / 32; ++i) {
@@ -833,7 +833,8 @@ int launch_mma(const PagedAttnArgs& a, const Choice& c, void* tc_workspace, floa
   const long long room = std::min((long long)a.W * a.page_size, 1ll << 31);  // keys of a sequence, at most
   // a cluster for each (row group, key head) where they are few and their keys are: one kernel and no partial sums in
   // memory; else spans enough to fill the SMs
-  const int variant = !wide ? 0 : (!same ? 1 : (!beside && items <= kClusterItems && room * (DT == DT_F32 ? 4 : 1) <= kClusterKeys ? 3 : 2));
+  const bool clusters = !beside && items <= kClusterItems && room * (DT == DT_F32 ? 4 : 1) <= kClusterKeys;
+  const int variant = !wide ? 0 : (!same ? 1 : (clusters ? 3 : 2));
   auto kfn = variant == 0   ? paged_attn_mma_kernel<DT, DP, false, false, RB, false>
              : variant == 1 ? paged_attn_mma_kernel<DT, DP, true, false, RB, false>
              : variant == 2 ? paged_attn_mma_kernel<DT, DP, true, true, RB, false>

@@ -49,6 +49,7 @@ constexpr int TM = 128, TK = 128;  // rows of a tile, keys of a tile
 constexpr int kItemRows = 2 * TM;
 constexpr int kTcThreads = 384, kLoaders = 3, W_MMA = 8, W_LOAD = 9;
 constexpr int kMaxSlots = 8 * kSms;    // pieces of split pairs, each with a slot of partial sums
+constexpr int kMaxPieces = kSms;       // of a pair
 constexpr float kLazy = 8.f;           // log2 of the growth that rescales O
 
 template <int D> constexpr int ring_slots() { return D == 128 ? 5 : 8; }
@@ -58,7 +59,7 @@ template <int D> constexpr int tile_bytes() { return TK * D * 2; }
 struct __align__(16) PieceWork {
   int head, seq, row0, rows;      // key head, sequence; first row in it, rows from there on
   int key0, tiles, pieces, slot;  // first key, key tiles; pieces of its pair, its slot of partial sums
-  int q0, pos0, len, end;         // the sequence's first token and that one's position, its keys; keys that the rows see
+  int q0, pos0, len, end;         // the sequence's first token and its position; its keys, those that the rows see
   int pair, unused[3];
 };
 
@@ -97,9 +98,8 @@ __host__ __device__ inline Plan plan_at(int* p, long long B, long long items, lo
 // Keys of a 256-row item: [lo, hi), lo a multiple of TK.
 __device__ __forceinline__ int2 item_keys(const PagedAttnArgs& a, const SeqRange& s, int part, int G) {
   const long long r0 = (long long)part * kItemRows, r1 = min((long long)s.n * G, r0 + kItemRows) - 1;
-  int lo = 0, hi = s.len;
-  if (a.causal) hi = max(0, min(s.len, s.pos0 + (int)(r1 / G) + 1));
-  if (a.window > 0) lo = max(0, s.pos0 + (int)(r0 / G) - a.window + 1) / TK * TK;
+  const int lo = window_start(a, s.pos0 + (int)(r0 / G)) / TK * TK;
+  const int hi = a.causal ? max(0, min(s.len, s.pos0 + (int)(r1 / G) + 1)) : s.len;
   return make_int2(lo, max(lo, hi));
 }
 
@@ -140,8 +140,8 @@ __device__ int block_prefix(int v, int* total) {
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PagedAttnArgs a, int row_min, int max_items,
                                                             int* __restrict__ ws) {
   Plan p = plan_at(ws, a.B, max_items, a.Hkv);
-  // what the plan itself reads again stays in shared memory where it fits (a round trip to memory for each of the plan's
-  // steps would be most of its time); the joining kernel reads `seq` and `part` from the workspace
+  // what the plan itself reads again stays in shared memory where it fits (a round trip to memory for each of the
+  // plan's steps would be most of its time); the joining kernel reads `seq` and `part` from the workspace
   constexpr int kHeld = 1024;
   __shared__ int s_base[kHeld + 1], s_seq[kHeld], s_part[kHeld], s_tiles[kHeld], s_sum[kHeld];
   int *const out_seq = p.seq, *const out_part = p.part;
@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PagedAttnArgs 
   // sequence and head on, so that the SMs finish together, nor than a quarter of an SM's whole share: CTAs that read
   // the same keys then do so at about the same time (whole shares: 1095 us for 256 queries x 64 heads over 131072 keys,
   // quarters 1018, sixths 1062, where the pieces' own cost shows).  Pieces below an eighth of the share or kLeast tiles
-  // are not made.
+  // are not made, nor more pieces of a pair than there are SMs, for which the joining kernel has room.
   constexpr long long kLeast = 16;
   const long long work = (long long)head_tiles * a.Hkv;
   const long long least = max(kLeast, work / (8 * kSms)), top = max(least, work / (4 * kSms));
@@ -218,11 +218,11 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PagedAttnArgs 
       i = c - head * items;
       const long long left = work - (long long)head * head_tiles - p.sum[p.base[p.seq[i]]];
       const long long most = min(top, max(least, (left + kSms - 1) / kSms));
-      n = (int)((p.tiles[i] + most - 1) / most);
+      n = (int)min((p.tiles[i] + most - 1) / most, (long long)kMaxPieces);
     }
     int total, total_slots;
     const int slot = slots + block_prefix(n > 1 ? n : 0, &total_slots);
-    if (n > 1 && slot + n > kMaxSlots) n = 1;  // no room for its partial sums (not with the cuts above)
+    if (n > 1 && slot + n > kMaxSlots) n = 1;  // no room for its partial sums
     const int at = pieces + block_prefix(n, &total);
     if (c < pairs) {
       PieceWork w;
@@ -267,8 +267,8 @@ struct TcShared {
   static constexpr int Q = 0;
   static constexpr int RING = 2 * tile_bytes<D>();
   static constexpr int BARS = RING + ring_slots<D>() * tile_bytes<D>();
-  // queries; tiles full and empty; scores, probabilities (of the first 64 keys, of the others) and sums of each row tile; the last value tile's rows;
-  // what is in flight when a wait was given up
+  // queries; tiles full and empty; scores, probabilities (of the first 64 keys, of the others) and sums of each row
+  // tile; the last value tile's rows; what is in flight when a wait was given up
   static constexpr int B_Q = 0, B_FULL = 1, B_EMPTY = B_FULL + ring_slots<D>(), B_S = B_EMPTY + ring_slots<D>(),
                        B_P = B_S + 2, B_O = B_P + 4, B_TAIL = B_O + 2,
                        B_DRAIN = B_TAIL + 1, NBARS = B_DRAIN + 1;
@@ -359,8 +359,8 @@ __device__ __forceinline__ float2 ex2_poly(float2 x) {
   return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(r.x) << 23)),
                      __int_as_float(__float_as_int(p.y) + (__float_as_int(r.y) << 23)));
 }
-// The pairs of eight that take the polynomial.  At head_dim 64 the softmax bounds the kernel and the exponential unit the
-// softmax: a quarter there (4 prompts of about 2048 tokens over 8192: 576 us with none, 559 a quarter, 590 three
+// The pairs of eight that take the polynomial.  At head_dim 64 the softmax bounds the kernel and the exponential unit
+// the softmax: a quarter there (4 prompts of about 2048 tokens over 8192: 576 us with none, 559 a quarter, 590 three
 // eighths).  At head_dim 128 the tensor cores and the power they draw bound it, and the polynomial's instructions only
 // cost (256 queries over 131072 keys: 1012 us with none, 1015 a quarter, 1080 three eighths).
 template <int D> constexpr uint32_t poly_pairs() { return D == 64 ? 0x12u : 0u; }
@@ -431,236 +431,240 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
 
   // the launch's 384 x 168 registers: 208 for each softmax thread, 88 for the others
   if (warp >= W_MMA) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-  if (warp >= W_LOAD) {
-    // ---- loaders ----
-    const int lw = warp - W_LOAD;
-    int ring = 0, tails = 0;  // ring tiles, tiles with a tail so far
-    for (int turn = 0; take(turn); ++turn) {
-      const int head = w.head, rows = w.rows, nt = rows > TM ? 2 : 1, row0 = w.row0, tiles = w.tiles, key0 = w.key0;
-      const int end = w.end;
-      bool bad = false;
-      constexpr int CPR = D / 8, RPI = 32 / CPR;               // 16-byte chunks of a row, rows of a warp's copy
-      constexpr int NI = (TK / RPI + kLoaders - 1) / kLoaders;  // copies of a tile by one warp
-      const int sub = lane / CPR, chunk = lane % CPR;
-      const uint32_t col = (uint32_t)((chunk >> 3) * TM * 128);
-      {
-        const T* q = static_cast<const T*>(a.q);
-        for (int r = lw * RPI + sub; r < nt * TM; r += kLoaders * RPI) {
-          const bool ok = r < rows;
-          const int tok = w.q0 + (row0 + (ok ? r : 0)) / G, h = head * G + (row0 + (ok ? r : 0)) % G;
-          cp_async16(sm + L::Q + (r / TM) * TB + col + (r % TM) * 128 + (((chunk & 7) ^ (r & 7)) << 4),
-                     q + (long long)tok * a.qs.t + (long long)h * a.qs.h + chunk * 8, ok);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp >= W_LOAD) {
+      // ---- loaders ----
+      const int lw = warp - W_LOAD;
+      int ring = 0, tails = 0;  // ring tiles, tiles with a tail so far
+      for (int turn = 0; take(turn); ++turn) {
+        const int head = w.head, rows = w.rows, nt = rows > TM ? 2 : 1, row0 = w.row0, tiles = w.tiles, key0 = w.key0;
+        const int end = w.end;
+        bool bad = false;
+        constexpr int CPR = D / 8, RPI = 32 / CPR;               // 16-byte chunks of a row, rows of a warp's copy
+        constexpr int NI = (TK / RPI + kLoaders - 1) / kLoaders;  // copies of a tile by one warp
+        const int sub = lane / CPR, chunk = lane % CPR;
+        const uint32_t col = (uint32_t)((chunk >> 3) * TM * 128);
+        {
+          const T* q = static_cast<const T*>(a.q);
+          for (int r = lw * RPI + sub; r < nt * TM; r += kLoaders * RPI) {
+            const bool ok = r < rows;
+            const int tok = w.q0 + (row0 + (ok ? r : 0)) / G, h = head * G + (row0 + (ok ? r : 0)) % G;
+            cp_async16(sm + L::Q + (r / TM) * TB + col + (r % TM) * 128 + (((chunk & 7) ^ (r & 7)) << 4),
+                       q + (long long)tok * a.qs.t + (long long)h * a.qs.h + chunk * 8, ok);
+          }
+          tc::cp_async_arrive(&bars[L::B_Q]);
         }
-        tc::cp_async_arrive(&bars[L::B_Q]);
-      }
-      const int* row_table = a.table + (long long)w.seq * a.table_stride;
-      bool ok = true;
-      if constexpr (TMA) {
-        // The first warp brings the keys, the second the values; lane x of it one box of a tile: 64 columns of the rows
-        // of one page, or of the tile where the page is larger.  (The lanes' copies are issued one after the other, about
-        // 130 cycles each: with 16-token pages one warp for both took 4500 cycles a step, the tensor cores 3300.)
-        if (lw < 2) {
-          const bool is_v = lw == 1;
-          const CUtensorMap* map = is_v ? &maps.v : &maps.k;
-          const int4 pos = is_v ? maps.vpos : maps.kpos;
-          const int R = min(a.page_size, TK), boxes = TK / R * (D / 64);
-          const int row = lane / (D / 64) * R, half = lane % (D / 64);
-          // the table entry of this lane's box, read one tile ahead
-          auto look_up = [&](int k0) {
-            const int key = k0 + row;
-            return lane < boxes && key < end ? row_table[key / a.page_size] : -1;
-          };
-          int ahead = look_up(key0), j = 0;
-          for (; ok && j < tiles; ++j) {
-            const int i = ring + 2 * j + lw, slot = i % NR, use = i / NR, k0 = key0 + j * TK;
-            const int key = k0 + row, in_page = key % a.page_size;
-            int page = a.num_pages;  // outside the map: reads as zeros
-            if (lane < boxes && key < end) {
-              if (ahead >= 0 && ahead < a.num_pages) page = ahead;
-              else bad = true;
+        const int* row_table = a.table + (long long)w.seq * a.table_stride;
+        bool ok = true;
+        if constexpr (TMA) {
+          // The first warp brings the keys, the second the values; lane x of it one box of a tile: 64 columns of the
+          // rows of one page, or of the tile where the page is larger.  (The lanes' copies are issued one after the
+          // other, about 130 cycles each: with 16-token pages one warp for both took 4500 cycles a step, the tensor
+          // cores 3300.)
+          if (lw < 2) {
+            const bool is_v = lw == 1;
+            const CUtensorMap* map = is_v ? &maps.v : &maps.k;
+            const int4 pos = is_v ? maps.vpos : maps.kpos;
+            const int R = min(a.page_size, TK), boxes = TK / R * (D / 64);
+            const int row = lane / (D / 64) * R, half = lane % (D / 64);
+            // the table entry of this lane's box, read one tile ahead
+            auto look_up = [&](int k0) {
+              const int key = k0 + row;
+              return lane < boxes && key < end ? row_table[key / a.page_size] : -1;
+            };
+            int ahead = look_up(key0), j = 0;
+            for (; ok && j < tiles; ++j) {
+              const int i = ring + 2 * j + lw, slot = i % NR, use = i / NR, k0 = key0 + j * TK;
+              const int key = k0 + row, in_page = key % a.page_size;
+              int page = a.num_pages;  // outside the map: reads as zeros
+              if (lane < boxes && key < end) {
+                if (ahead >= 0 && ahead < a.num_pages) page = ahead;
+                else bad = true;
+              }
+              if (j + 1 < tiles) ahead = look_up(k0 + TK);
+              if (use > 0) {
+                ok = tc::mbar_wait(&bars[L::B_EMPTY + slot], (use - 1) & 1, abort);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+              }
+              // the last keys' page goes on behind them: those value rows become zeros before the tensor cores see them
+              const bool tail = is_v && end - k0 < TK && end % R != 0;
+              uint64_t* full = &bars[L::B_FULL + slot];
+              uint64_t* bar = tail ? &bars[L::B_TAIL] : full;
+              unsigned char* dst = sm + L::RING + slot * TB;
+              if (lane == 0) tc::mbar_expect_tx(bar, TB);
+              __syncwarp();
+              if (lane < boxes) {
+                auto coordinate = [&](int d) { return d == pos.x ? in_page : (d == pos.y ? head : page); };
+                tc::tma_load_4d(dst + half * TM * 128 + row * 128, map, half * 64, coordinate(1), coordinate(2),
+                                coordinate(3), bar);
+              }
+              if (tail) {
+                ok = tc::mbar_wait(bar, tails & 1, abort);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                ++tails;
+                const int r0 = max(0, end - k0), r1 = min(TK, (r0 + R - 1) / R * R);
+                for (int x = lane; x < (r1 - r0) * (D / 8); x += 32) {
+                  const int r = r0 + x / (D / 8), c = x % (D / 8);
+                  *reinterpret_cast<uint4*>(dst + (c >> 3) * TM * 128 + r * 128 + (c & 7) * 16) = uint4{};
+                }
+                tc::fence_async_smem();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(full);
+              }
             }
-            if (j + 1 < tiles) ahead = look_up(k0 + TK);
+            if (!ok)  // let the copies in flight land before the CTA leaves
+              for (int u = max(0, j - NR); u < j; ++u) {
+                const int i = ring + 2 * u + lw;
+                const long long since = clock64();
+                while (!tc::mbar_try(&bars[L::B_FULL + i % NR], (i / NR) & 1) &&
+                       clock64() - since < tc::kWaitCycles / 8) {
+                }
+              }
+          }
+        } else {
+          const T* kbase = static_cast<const T*>(a.kpool) + (long long)head * a.kps.h;
+          const T* vbase = static_cast<const T*>(a.vpool) + (long long)head * a.vps.h;
+          long long off[2][2];  // [key, value][the first 32 rows of the warp's list, the rest]
+          for (int i = 0; ok && i < 2 * tiles; ++i) {
+            const int is_v = i & 1, slot = (ring + i) % NR, use = (ring + i) / NR;
+            if (!is_v) {
+              // the warp's rows of this tile: row q of its list is row (lw + 3 (q / RPI)) RPI + q % RPI
+#pragma unroll
+              for (int hf = 0; hf < 2; ++hf) {
+                const int q = hf * 32 + lane, r = (lw + kLoaders * (q / RPI)) * RPI + q % RPI;
+                const int key = key0 + (i >> 1) * TK + r;
+                off[0][hf] = off[1][hf] = -1;
+                if (r < TK && key < end) {
+                  const int page = row_table[key / a.page_size], s = key % a.page_size;
+                  if (page >= 0 && page < a.num_pages) {
+                    off[0][hf] = (long long)page * a.kps.p + (long long)s * a.kps.s;
+                    off[1][hf] = (long long)page * a.vps.p + (long long)s * a.vps.s;
+                  } else {
+                    bad = true;
+                  }
+                }
+              }
+            }
             if (use > 0) {
               ok = tc::mbar_wait(&bars[L::B_EMPTY + slot], (use - 1) & 1, abort);
               ok = __all_sync(0xffffffffu, ok);
               if (!ok) break;
             }
-            // the last keys' page goes on behind them: those value rows become zeros before the tensor cores see them
-            const bool tail = is_v && end - k0 < TK && end % R != 0;
-            uint64_t* full = &bars[L::B_FULL + slot];
-            uint64_t* bar = tail ? &bars[L::B_TAIL] : full;
-            unsigned char* dst = sm + L::RING + slot * TB;
-            if (lane == 0) tc::mbar_expect_tx(bar, TB);
-            __syncwarp();
-            if (lane < boxes) {
-              auto coordinate = [&](int d) { return d == pos.x ? in_page : (d == pos.y ? head : page); };
-              tc::tma_load_4d(dst + half * TM * 128 + row * 128, map, half * 64, coordinate(1), coordinate(2),
-                              coordinate(3), bar);
-            }
-            if (tail) {
-              ok = tc::mbar_wait(bar, tails & 1, abort);
-              ok = __all_sync(0xffffffffu, ok);
-              if (!ok) break;
-              ++tails;
-              const int r0 = max(0, end - k0), r1 = min(TK, (r0 + R - 1) / R * R);
-              for (int x = lane; x < (r1 - r0) * (D / 8); x += 32) {
-                const int r = r0 + x / (D / 8), c = x % (D / 8);
-                *reinterpret_cast<uint4*>(dst + (c >> 3) * TM * 128 + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-              }
-              tc::fence_async_smem();
-              __syncwarp();
-              if (lane == 0) tc::mbar_arrive(full);
-            }
-          }
-          if (!ok)  // let the copies in flight land before the CTA leaves
-            for (int u = max(0, j - NR); u < j; ++u) {
-              const int i = ring + 2 * u + lw;
-              const long long since = clock64();
-              while (!tc::mbar_try(&bars[L::B_FULL + i % NR], (i / NR) & 1) && clock64() - since < tc::kWaitCycles / 8) {
-              }
-            }
-        }
-      } else {
-        const T* kbase = static_cast<const T*>(a.kpool) + (long long)head * a.kps.h;
-        const T* vbase = static_cast<const T*>(a.vpool) + (long long)head * a.vps.h;
-        long long off[2][2];  // [key, value][the first 32 rows of the warp's list, the rest]
-        for (int i = 0; ok && i < 2 * tiles; ++i) {
-          const int is_v = i & 1, slot = (ring + i) % NR, use = (ring + i) / NR;
-          if (!is_v) {
-            // the warp's rows of this tile: row q of its list is row (lw + 3 (q / RPI)) RPI + q % RPI
-  #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-              const int q = hf * 32 + lane, r = (lw + kLoaders * (q / RPI)) * RPI + q % RPI;
-              const int key = key0 + (i >> 1) * TK + r;
-              off[0][hf] = off[1][hf] = -1;
-              if (r < TK && key < end) {
-                const int page = row_table[key / a.page_size], s = key % a.page_size;
-                if (page >= 0 && page < a.num_pages) {
-                  off[0][hf] = (long long)page * a.kps.p + (long long)s * a.kps.s;
-                  off[1][hf] = (long long)page * a.vps.p + (long long)s * a.vps.s;
-                } else {
-                  bad = true;
-                }
-              }
-            }
-          }
-          if (use > 0) {
-            ok = tc::mbar_wait(&bars[L::B_EMPTY + slot], (use - 1) & 1, abort);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-          }
-          unsigned char* dst = sm + L::RING + slot * TB + col;
-          const T* base = is_v ? vbase : kbase;
-  #pragma unroll
-          for (int x = 0; x < NI; ++x) {
-            const int g = lw + kLoaders * x;  // copy g of the tile: rows g RPI ..
-            const int q = x * RPI + sub;
-            const long long o = __shfl_sync(0xffffffffu, is_v ? off[1][(x * RPI) >> 5] : off[0][(x * RPI) >> 5], q & 31);
-            const int r = g * RPI + sub;
-            if (g < TK / RPI)
-              cp_async16(dst + r * 128 + (((chunk & 7) ^ (r & 7)) << 4), base + (o >= 0 ? o + chunk * 8 : 0), o >= 0);
-          }
-          tc::cp_async_arrive(&bars[L::B_FULL + slot]);  // arrives when this thread's copies have landed
-        }
-      }
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      ring += 2 * tiles;
-      if (tid == kTcThreads - 1) fetch(turn + 1);
-      if (bad) atomicOr(&g_fault_paged_tc, kFaultTables);
-      if (!turn_over()) break;
-    }
-  } else {
-    // ---- MMA issuer: the whole warp runs the loop, so that the descriptors stay in uniform registers (formed by one
-    // lane on its own each multiplication took longer to issue than to compute); one elected lane issues ----
-    int slot = 0, q_phase = 0;
-    uint32_t ring_phase = 0;         // of the ring's slots from `slot` on, until it wraps
-    uint32_t p_phase[2] = {0, 0};    // of each row tile's P
-    const int fmt = DT == DT_BF16 ? 1 : 0;
-    const uint32_t id_s = tc::idesc_f16(fmt, TM, TK, false), id_o = tc::idesc_f16(fmt, TM, D, true);
-    const uint32_t q_low = desc_low(tc::smem_addr(sm + L::Q), kDescRows);
-    const uint32_t r_low = desc_low(tc::smem_addr(sm + L::RING), 0);
-    for (int turn = 0; take(turn); ++turn) {
-      const int nt = __shfl_sync(0xffffffffu, w.rows > TM ? 2 : 1, 0), tiles = __shfl_sync(0xffffffffu, w.tiles, 0);
-      auto agree = [&](bool ok) { return (bool)__all_sync(0xffffffffu, ok); };
-      auto step_on = [&](int& at, uint32_t& phase) {
-        if (++at == NR) {
-          at = 0;
-          phase ^= 1;
-        }
-      };
-      auto issue_s = [&](int t, int at) {
-        const uint32_t k_low = r_low + kDescRows + at * (TB / 16), qt = q_low + t * (TB / 16);
-        if (elect_one()) {
+            unsigned char* dst = sm + L::RING + slot * TB + col;
+            const T* base = is_v ? vbase : kbase;
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t o = ((kk >> 2) * TM * 128 + (kk & 3) * 32) / 16;
-            mma_ss_low(col_s + t * TK, qt + o, k_low + o, id_s, kk > 0);
+            for (int x = 0; x < NI; ++x) {
+              const int g = lw + kLoaders * x;  // copy g of the tile: rows g RPI ..
+              const int q = x * RPI + sub;
+              const int hf = (x * RPI) >> 5;
+              const long long o = __shfl_sync(0xffffffffu, is_v ? off[1][hf] : off[0][hf], q & 31);
+              const int r = g * RPI + sub;
+              if (g < TK / RPI)
+                cp_async16(dst + r * 128 + (((chunk & 7) ^ (r & 7)) << 4), base + (o >= 0 ? o + chunk * 8 : 0), o >= 0);
+            }
+            tc::cp_async_arrive(&bars[L::B_FULL + slot]);  // arrives when this thread's copies have landed
           }
-          tc::mma_commit(&bars[L::B_S + t]);
-          if (t == nt - 1) tc::mma_commit(&bars[L::B_EMPTY + at]);
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        ring += 2 * tiles;
+        if (tid == kTcThreads - 1) fetch(turn + 1);
+        if (bad) atomicOr(&g_fault_paged_tc, kFaultTables);
+        if (!turn_over()) break;
+      }
+    } else {
+      // ---- MMA issuer: the whole warp runs the loop, so that the descriptors stay in uniform registers (formed by one
+      // lane on its own each multiplication took longer to issue than to compute); one elected lane issues ----
+      int slot = 0, q_phase = 0;
+      uint32_t ring_phase = 0;         // of the ring's slots from `slot` on, until it wraps
+      uint32_t p_phase[2] = {0, 0};    // of each row tile's P
+      const int fmt = DT == DT_BF16 ? 1 : 0;
+      const uint32_t id_s = tc::idesc_f16(fmt, TM, TK, false), id_o = tc::idesc_f16(fmt, TM, D, true);
+      const uint32_t q_low = desc_low(tc::smem_addr(sm + L::Q), kDescRows);
+      const uint32_t r_low = desc_low(tc::smem_addr(sm + L::RING), 0);
+      for (int turn = 0; take(turn); ++turn) {
+        const int nt = __shfl_sync(0xffffffffu, w.rows > TM ? 2 : 1, 0), tiles = __shfl_sync(0xffffffffu, w.tiles, 0);
+        auto agree = [&](bool ok) { return (bool)__all_sync(0xffffffffu, ok); };
+        auto step_on = [&](int& at, uint32_t& phase) {
+          if (++at == NR) {
+            at = 0;
+            phase ^= 1;
+          }
+        };
+        auto issue_s = [&](int t, int at) {
+          const uint32_t k_low = r_low + kDescRows + at * (TB / 16), qt = q_low + t * (TB / 16);
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t o = ((kk >> 2) * TM * 128 + (kk & 3) * 32) / 16;
+              mma_ss_low(col_s + t * TK, qt + o, k_low + o, id_s, kk > 0);
+            }
+            tc::mma_commit(&bars[L::B_S + t]);
+            if (t == nt - 1) tc::mma_commit(&bars[L::B_EMPTY + at]);
+          }
+          __syncwarp();
+        };
+        // cp.async writes through the generic proxy; the tensor cores read through the async proxy, which a fence after
+        // each wait puts behind those writes
+        bool ok = agree(tc::mbar_wait(&bars[L::B_Q], q_phase & 1, abort) &&
+                        tc::mbar_wait(&bars[L::B_FULL + slot], ring_phase, abort));
+        if (ok) {
+          tc::fence_async_smem();
+          tc::tc_after_sync();
+          issue_s(0, slot);
+          if (nt > 1) issue_s(1, slot);
+          step_on(slot, ring_phase);
+        }
+        for (int j = 0; ok && j < tiles; ++j) {
+          // the values of these keys and the next keys
+          const int v_at = slot;
+          const uint32_t v_phase = ring_phase;
+          step_on(slot, ring_phase);
+          const int k_at = slot;
+          const uint32_t k_phase = ring_phase;
+          const bool more = j + 1 < tiles;
+          if (more) step_on(slot, ring_phase);
+          ok = tc::mbar_wait(&bars[L::B_FULL + v_at], v_phase, abort) &&
+               (!more || tc::mbar_wait(&bars[L::B_FULL + k_at], k_phase, abort));
+          const uint32_t v_low = r_low + kDescCols + v_at * (TB / 16);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (t >= nt) break;
+            // P of this tile's first 64 keys is in TMEM, and every thread is done with S; then P of the others
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+              ok = agree(ok && tc::mbar_wait(&bars[L::B_P + 2 * t + hf], p_phase[t], abort));
+              if (!ok) break;
+              if constexpr (!TMA) tc::fence_async_smem();
+              tc::tc_after_sync();
+              if (elect_one()) {
+#pragma unroll
+                for (int kk = hf * (TK / 32); kk < (hf + 1) * (TK / 32); ++kk)
+                  mma_ts_low(col_o + t * D, col_s + t * TK + kk * 8, v_low + kk * (16 * 128 / 16), id_o,
+                             j > 0 || kk > 0);
+                if (hf == 1 && t == nt - 1) tc::mma_commit(&bars[L::B_EMPTY + v_at]);
+                if (hf == 1 && !more) tc::mma_commit(&bars[L::B_O + t]);
+              }
+              __syncwarp();
+            }
+            if (!ok) break;
+            p_phase[t] ^= 1;
+            // the scores of the next keys take the columns of P: the tensor cores work in the order of issue
+            if (more) issue_s(t, k_at);
+          }
+        }
+        if (!ok) {  // let what was issued finish before the CTA leaves
+          if (elect_one()) tc::mma_commit(&bars[L::B_DRAIN]);
+          const long long since = clock64();
+          while (!tc::mbar_try(&bars[L::B_DRAIN], 0) && clock64() - since < tc::kWaitCycles / 8) {
+          }
         }
         __syncwarp();
-      };
-      // cp.async writes through the generic proxy; the tensor cores read through the async proxy, which a fence after
-      // each wait puts behind those writes
-      bool ok = agree(tc::mbar_wait(&bars[L::B_Q], q_phase & 1, abort) &&
-                      tc::mbar_wait(&bars[L::B_FULL + slot], ring_phase, abort));
-      if (ok) {
-        tc::fence_async_smem();
-        tc::tc_after_sync();
-        issue_s(0, slot);
-        if (nt > 1) issue_s(1, slot);
-        step_on(slot, ring_phase);
+        ++q_phase;
+        if (!turn_over()) break;
       }
-      for (int j = 0; ok && j < tiles; ++j) {
-        // the values of these keys and the next keys
-        const int v_at = slot;
-        const uint32_t v_phase = ring_phase;
-        step_on(slot, ring_phase);
-        const int k_at = slot;
-        const uint32_t k_phase = ring_phase;
-        const bool more = j + 1 < tiles;
-        if (more) step_on(slot, ring_phase);
-        ok = tc::mbar_wait(&bars[L::B_FULL + v_at], v_phase, abort) &&
-             (!more || tc::mbar_wait(&bars[L::B_FULL + k_at], k_phase, abort));
-        const uint32_t v_low = r_low + kDescCols + v_at * (TB / 16);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (t >= nt) break;
-          // P of this tile's first 64 keys is in TMEM, and every thread is done with S; then P of the others
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            ok = agree(ok && tc::mbar_wait(&bars[L::B_P + 2 * t + hf], p_phase[t], abort));
-            if (!ok) break;
-            if constexpr (!TMA) tc::fence_async_smem();
-            tc::tc_after_sync();
-            if (elect_one()) {
-#pragma unroll
-              for (int kk = hf * (TK / 32); kk < (hf + 1) * (TK / 32); ++kk)
-                mma_ts_low(col_o + t * D, col_s + t * TK + kk * 8, v_low + kk * (16 * 128 / 16), id_o, j > 0 || kk > 0);
-              if (hf == 1 && t == nt - 1) tc::mma_commit(&bars[L::B_EMPTY + v_at]);
-              if (hf == 1 && !more) tc::mma_commit(&bars[L::B_O + t]);
-            }
-            __syncwarp();
-          }
-          if (!ok) break;
-          p_phase[t] ^= 1;
-          // the scores of the next keys take the columns of P: the tensor cores work in the order of issue
-          if (more) issue_s(t, k_at);
-        }
-      }
-      if (!ok) {  // let what was issued finish before the CTA leaves
-        if (elect_one()) tc::mma_commit(&bars[L::B_DRAIN]);
-        const long long since = clock64();
-        while (!tc::mbar_try(&bars[L::B_DRAIN], 0) && clock64() - since < tc::kWaitCycles / 8) {
-        }
-      }
-      __syncwarp();
-      ++q_phase;
-      if (!turn_over()) break;
     }
-  }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ---- softmax of tile t: this thread's row is lane (tid % 128) of the tile ----
@@ -678,9 +682,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
       const uint32_t s_at = col_s + t * TK + lanes, o_at = col_o + t * D + lanes;
       int first = 0, last = INT_MAX;  // visible keys; rows behind the last one need no mask
       if (r < w.rows) {
-        const int pos = w.pos0 + (w.row0 + r) / G;
-        last = a.causal ? (pos < 0 ? 0 : min(w.len, pos + 1)) : w.len;
-        first = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+        const int2 v = visible(a, w.pos0 + (w.row0 + r) / G, w.len);
+        first = v.x;
+        last = v.y;
       }
       float m = -INFINITY, l = 0.f;
       bool ok = true;
@@ -775,8 +779,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         // a row that sees no key is zero; one whose keys all score -inf is 0 / 0
         const float f = whole ? (last > first ? (m == -INFINITY ? NAN : 1.f / l) : 0.f) : 1.f;
         if (whole) {
-          // through this row tile's queries, whose multiplications are over: 16-byte chunk c of a row at c ^ row % 8, then
-          // whole rows to memory
+          // through this row tile's queries, whose multiplications are over: 16-byte chunk c of a row at c ^ row % 8,
+          // then whole rows to memory
           unsigned char* stage = sm + L::Q + t * TB + (warp & 3) * 32 * (D * 2);
 #pragma unroll
           for (int c = 0; c < D / 32; ++c) {
@@ -870,7 +874,7 @@ __global__ void __launch_bounds__(256) combine_tc_kernel(const PagedAttnArgs a, 
   const long long stride = kItemRows * (D + 2);
   const float* base = partials + (long long)plan.slot[pair] * stride;
   // the pieces' weights, a warp for four rows
-  __shared__ float weight[kSms][kJoinRows];
+  __shared__ float weight[kMaxPieces][kJoinRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r0 = blockIdx.y * kJoinRows;
   if (r0 >= rows) return;
   if (odd) {
@@ -878,8 +882,8 @@ __global__ void __launch_bounds__(256) combine_tc_kernel(const PagedAttnArgs a, 
       const int tok = seq.q0 + (row0 + r) / G, h = head * G + (row0 + r) % G;
       const int2 v = visible(a, seq.pos0 + (row0 + r) / G, seq.len);
       float x[D / 32], m, l;
-      row_alone<DT, D>(a, a.table + (long long)plan.seq[item] * a.table_stride, head,
-                       static_cast<const T*>(a.q) + (long long)tok * a.qs.t + (long long)h * a.qs.h, v.x, v.y, x, &m, &l);
+      const T* q_row = static_cast<const T*>(a.q) + (long long)tok * a.qs.t + (long long)h * a.qs.h;
+      row_alone<DT, D>(a, a.table + (long long)plan.seq[item] * a.table_stride, head, q_row, v.x, v.y, x, &m, &l);
 #pragma unroll
       for (int i = 0; i < D / 32; ++i)
         static_cast<T*>(a.out)[(long long)tok * a.os.t + (long long)h * a.os.h + i * 32 + lane] =
@@ -910,9 +914,7 @@ __global__ void __launch_bounds__(256) combine_tc_kernel(const PagedAttnArgs a, 
   __syncthreads();
   const int r = r0 + lane;
   if (r >= rows) return;
-  const int pos = seq.pos0 + (row0 + r) / G;
-  const int last = a.causal ? (pos < 0 ? 0 : min(seq.len, pos + 1)) : seq.len;
-  const int first = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+  const int2 seen = visible(a, seq.pos0 + (row0 + r) / G, seq.len);
   constexpr int NC = D / 4 / 8;  // a thread's groups of four columns
   float4 x[NC];
 #pragma unroll
@@ -940,7 +942,7 @@ __global__ void __launch_bounds__(256) combine_tc_kernel(const PagedAttnArgs a, 
     const float y[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
     T e[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) e[i] = from_f<DT>(last > first ? y[i] : 0.f);
+    for (int i = 0; i < 4; ++i) e[i] = from_f<DT>(seen.y > seen.x ? y[i] : 0.f);
     if (out_wide) {
       *reinterpret_cast<uint2*>(dst + c * 4) = *reinterpret_cast<const uint2*>(e);
     } else {

@@ -59,8 +59,9 @@ struct Geometry {
 
 
 template <int DT, int VEC, bool PAGED, int kUnroll>
-__global__ void __launch_bounds__(kThreads, kMinBlocks) rotary_kernel(const __grid_constant__ RotarySpec spec, const RotaryArgs a,
-                                                          const PagedAppendArgs p, const Geometry g) {
+__global__ void __launch_bounds__(kThreads, kMinBlocks) rotary_kernel(const __grid_constant__ RotarySpec spec,
+                                                                      const RotaryArgs a, const PagedAppendArgs p,
+                                                                      const Geometry g) {
   using T = typename Storage<DT>::T;
   using V = typename Raw<VEC * (int)sizeof(T)>::T;
   extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -153,8 +154,8 @@ __global__ void __launch_bounds__(kThreads, kMinBlocks) rotary_kernel(const __gr
   // A thread keeps its task v of a row and walks rows (token, head) of one operand after the other, kUnroll at a time.
   const int rows_at_once = kThreads / g.tasks, v = tid % g.tasks, first = tid / g.tasks;
   if (first >= rows_at_once) return;
-  auto walk = [&](const T* src, T* dst, const long long* src_at, const long long* dst_at, long long src_h, long long dst_h,
-                  int begin, int end, bool rotates, int state) {
+  auto walk = [&](const T* src, T* dst, const long long* src_at, const long long* dst_at, long long src_h,
+                  long long dst_h, int begin, int end, bool rotates, int state) {
     const int n = end - begin;  // heads
     if (n <= 0) return;
     const bool rot = rotates && v < g.rot_tasks;

@@ -540,6 +540,7 @@ def paged_attention(q: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.T
     ``h // (H // Hkv)``).  A token that sees no key gets zeros; rows behind
     ``q_start[B]`` are left as they are in ``out``.  ``max_q_len``: the most new
     tokens of a sequence, if known; it only steers the choice of kernels.
+    ``out`` must not overlap ``q``.
     Probabilities are rounded to the dtype for the product with the values
     (bf16, fp16), all sums are fp32.  Serving only: no gradient is recorded."""
     lib = _lib.load()
@@ -548,12 +549,17 @@ def paged_attention(q: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.T
     qs = _packed(q, "query", H, N, D)
     Hkv, kst, vst, pages, page_size, row, width, B = _pool(key_pool, value_pool, block_table, kv_len, q_start, at, dt,
                                                            D)
+    if not (0 <= window < 1 << 31 and 0 <= max_q_len < 1 << 31):
+        raise BackendError("window and max_q_len must be int32 and not negative",
+                           {"window": window, "max_q_len": max_q_len})
     if Hkv == 0 or H == 0 or H % Hkv:
         raise ShapeError("query heads must be a multiple of the pool's heads", expected=f"n * {Hkv}", actual=H)
     if out is None:
         out = q.new_empty((N, H, D))
     else:
         _same("out", out, at, dt)
+        if N and out.data_ptr() == q.data_ptr():
+            raise BackendError("out must not be the query's memory")
     if scale is None:
         scale = D ** -0.5 if D else 1.0
     code = _lib.dtype_code(dt)

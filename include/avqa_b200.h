@@ -311,7 +311,7 @@ size_t avq_paged_attention_workspace_size(int dtype, int B, int N, int H, int Hk
  * with causal those at i's position and before, with window > 0 of these the
  * last `window`.  H is a multiple of Hkv; query head h reads key head
  * h / (H / Hkv).  A token that sees no key gets zeros; tokens behind
- * q_start[B] are left alone.  max_q_len: a bound of the new tokens per
+ * q_start[B] are left alone; out must not overlap q.  max_q_len: a bound of the new tokens per
  * sequence, or 0; it only steers the choice of kernels, a wrong one costs time
  * and never the result.  Keys on pages outside the pool count as zeros and raise
  * bit 1 of the device fault record.  D <= 256.  workspace:

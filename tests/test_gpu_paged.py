@@ -150,6 +150,44 @@ def test_many_keys_take_the_larger_count_of_pieces() -> None:
     b.check(window=100)
 
 
+def test_one_pair_over_more_keys_than_its_pieces_number() -> None:
+    """One key head and one row tile over 350000 keys: the most pieces that a pair may have."""
+    b = Batch("bf16", 2, 1, 64, 256, [20], [350000])
+    b.check()
+    b.check(window=330000)
+    assert fault() == 0
+
+
+@pytest.mark.parametrize("dt,D", [("bf16", 128), ("f16", 64), ("f32", 64)])
+@pytest.mark.parametrize("new,lens", [([3, 1], [1, 50]), ([60, 40], [40, 90])])
+def test_window_of_any_size(dt, D, new, lens) -> None:
+    """A window larger than every cache hides nothing, with rows before the first position too."""
+    b = Batch(dt, 4, 2, D, 16, new, lens)
+    want = b.check()
+    for window in (91, 2 ** 31 - 2, 2 ** 31 - 1):
+        b.check(f"window {window}", window=window)
+        assert torch.equal(ops.paged_attention(b.q, *b.lists, window=window) == 0, want == 0)
+
+
+def test_attention_refuses_what_it_cannot_take() -> None:
+    b = Batch("bf16", 4, 2, 64, 16, [2], [20])
+    for kw in (dict(window=2 ** 31), dict(window=-1), dict(max_q_len=2 ** 31), dict(max_q_len=-1), dict(out=b.q),
+               dict(scale=float("nan")), dict(scale=3e38), dict(window=4, causal=False)):
+        with pytest.raises(BackendError):
+            ops.paged_attention(b.q, *b.lists, **kw)
+    b.check()  # nothing is left behind
+
+
+def test_cache_refuses_to_reserve_inside_a_graph() -> None:
+    cache = BlockKVCache(4, num_heads=1, head_dim=64, dtype=torch.bfloat16)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(BackendError):
+            cache.reserve([3])
+    assert cache.lengths == [] and len(cache.free_pages) == 4
+
+
 def test_attention_rows_behind_the_last_sequence_stay() -> None:
     for new, lens in (([2, 1], [40, 9]), ([200, 3], [300, 9])):
         b = Batch("bf16", 4, 2, 64, 16, new, lens)
