@@ -14,12 +14,13 @@
 //                   maximum grew by more than 2^8 (the sums stay exact: P and
 //                   l refer to the same, older maximum)
 //   warp 8          issues S = Q K^T and O += P V
-//   warps 9-11      load Q, then the key and value tiles (128 keys each) into
-//                   a ring, in the 128-byte swizzled layout that the tensor
-//                   cores read: warps 9 and 10 by TMA where whole pages fill a
-//                   tile or whole tiles a page (page sizes 8, 16, .. 128 and
-//                   multiples of 128), else all three by cp.async, where a page
-//                   may begin and end anywhere in a tile
+//   warps 9-11      load Q (by TMA where the heads of a group divide 128, else
+//                   by cp.async) and the key and value tiles (128 keys each)
+//                   into a ring, in the 128-byte swizzled layout that the
+//                   tensor cores read: warps 9 and 10 by TMA where whole pages
+//                   fill a tile or whole tiles a page (page sizes 8, 16, .. 128
+//                   and multiples of 128), else all three by cp.async, where a
+//                   page may begin and end anywhere in a tile
 //
 // Work: plan_kernel lists the (sequence, 256 rows) items and their key tiles,
 // cuts the (key head, item) pairs into pieces that get smaller toward the end,
@@ -326,9 +327,25 @@ __device__ __forceinline__ void mma_ts_low(uint32_t d, uint32_t a, uint32_t b_lo
       : "memory");
 }
 
-struct PoolMaps {  // a pool as a 4-D tensor map: d, and slots, heads and pages in the coordinates x, y and z
-  CUtensorMap k, v;
+struct TensorMaps {
+  CUtensorMap k, v;  // a pool: d, and slots, heads and pages in the coordinates x, y and z of its `pos`
+  CUtensorMap q;     // d, heads, tokens
   int4 kpos, vpos;
+  int has_q;
+};
+
+// The (token, head of the group) pairs of rows that a thread steps through, without a division for each.
+struct RowStep {
+  int tok, h, by_tok, by_h, G;
+  __device__ RowStep(int row, int by, int g) : tok(row / g), h(row % g), by_tok(by / g), by_h(by % g), G(g) {}
+  __device__ void next() {
+    tok += by_tok;
+    h += by_h;
+    if (h >= G) {
+      h -= G;
+      ++tok;
+    }
+  }
 };
 
 // exp2 of a pair on the fused multiply-adds: x = n + f with |f| <= 1/2 (n in the low bits of x + 1.5 2^23), 2^f by a
@@ -366,7 +383,7 @@ __device__ __forceinline__ float2 ex2_poly(float2 x) {
 template <int D> constexpr uint32_t poly_pairs() { return D == 64 ? 0x12u : 0u; }
 
 template <int DT, int D, bool TMA>
-__global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __grid_constant__ PoolMaps maps,
+__global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __grid_constant__ TensorMaps maps,
                                                                       const PagedAttnArgs a, int max_items,
                                                                       int* __restrict__ plan_ws,
                                                                       float* __restrict__ partials, int out_wide) {
@@ -384,7 +401,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
   const Plan plan = plan_at(plan_ws, a.B, max_items, a.Hkv);
 
   if (tid == 0) {
-    tc::mbar_init(&bars[L::B_Q], kLoaders * 32);
+    tc::mbar_init(&bars[L::B_Q], maps.has_q ? 1 : kLoaders * 32);
     for (int i = 0; i < NR; ++i) {
       tc::mbar_init(&bars[L::B_FULL + i], TMA ? 1 : kLoaders * 32);
       tc::mbar_init(&bars[L::B_EMPTY + i], 1);
@@ -444,15 +461,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         constexpr int NI = (TK / RPI + kLoaders - 1) / kLoaders;  // copies of a tile by one warp
         const int sub = lane / CPR, chunk = lane % CPR;
         const uint32_t col = (uint32_t)((chunk >> 3) * TM * 128);
-        {
+        if (!maps.has_q) {
           const T* q = static_cast<const T*>(a.q);
-          for (int r = lw * RPI + sub; r < nt * TM; r += kLoaders * RPI) {
+          RowStep at(row0 + lw * RPI + sub, kLoaders * RPI, G);
+          for (int r = lw * RPI + sub; r < nt * TM; r += kLoaders * RPI, at.next()) {
             const bool ok = r < rows;
-            const int tok = w.q0 + (row0 + (ok ? r : 0)) / G, h = head * G + (row0 + (ok ? r : 0)) % G;
-            cp_async16(sm + L::Q + (r / TM) * TB + col + (r % TM) * 128 + (((chunk & 7) ^ (r & 7)) << 4),
-                       q + (long long)tok * a.qs.t + (long long)h * a.qs.h + chunk * 8, ok);
+            const T* from = q + (long long)(w.q0 + at.tok) * a.qs.t + (long long)(head * G + at.h) * a.qs.h + chunk * 8;
+            cp_async16(sm + L::Q + (r / TM) * TB + col + (r % TM) * 128 + (((chunk & 7) ^ (r & 7)) << 4), ok ? from : q,
+                       ok);
           }
           tc::cp_async_arrive(&bars[L::B_Q]);
+        } else if (lw == kLoaders - 1 && lane == 0) {
+          // (rows behind the piece's last one hold other tokens, or zeros: nothing of theirs is written)
+          tc::mbar_expect_tx(&bars[L::B_Q], nt * TB);
+          for (int x = 0; x < nt * (D / 64); ++x) {
+            const int t = x / (D / 64), half = x % (D / 64);
+            tc::tma_load_3d(sm + L::Q + t * TB + half * TM * 128, &maps.q, half * 64, head * G,
+                            w.q0 + (row0 + t * TM) / G, &bars[L::B_Q]);
+          }
         }
         const int* row_table = a.table + (long long)w.seq * a.table_stride;
         bool ok = true;
@@ -802,13 +828,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             }
           }
           __syncwarp();
-          constexpr int CPR = D / 8;
-          for (int x = lane; x < 32 * CPR; x += 32) {
-            const int rr = x / CPR, c = x % CPR, at_row = t * TM + (warp & 3) * 32 + rr;
-            if (at_row < rows) {
+          constexpr int CPR = D / 8, RPI = 32 / CPR;
+          const int c = lane % CPR, warp_row = t * TM + (warp & 3) * 32;
+          T* out = static_cast<T*>(a.out) + (long long)w.q0 * a.os.t + (long long)head * G * a.os.h + c * 8;
+          RowStep at(row0 + warp_row + lane / CPR, RPI, G);
+#pragma unroll 4
+          for (int rr = lane / CPR; rr < 32; rr += RPI, at.next()) {
+            if (warp_row + rr < rows) {
               const uint4 y = *reinterpret_cast<const uint4*>(stage + rr * (D * 2) + ((c ^ (rr & 7)) << 4));
-              const int tok = w.q0 + (row0 + at_row) / G, h = head * G + (row0 + at_row) % G;
-              T* dst = static_cast<T*>(a.out) + (long long)tok * a.os.t + (long long)h * a.os.h + c * 8;
+              T* dst = out + (long long)at.tok * a.os.t + (long long)at.h * a.os.h;
               if (out_wide) {
                 *reinterpret_cast<uint4*>(dst) = y;
               } else {
@@ -817,6 +845,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
               }
             }
           }
+          tc::fence_async_smem();  // the next queries may come by TMA
         } else {
           // four columns of 256 rows side by side: a warp's stores are contiguous
           float* pd = partials + (long long)w.slot * (kItemRows * (D + 2));
@@ -976,6 +1005,16 @@ bool pool_map(CUtensorMap* m, int dt, const void* pool, PoolStrides s, const Pag
   return tc::encode16(m, dt, 4, pool, dims, str, box);
 }
 
+// The queries as a tensor map whose boxes are 128 rows, tokens by heads of a group; false where these do not fit.
+bool query_map(CUtensorMap* m, int dt, const PagedAttnArgs& a) {
+  const int G = a.H / a.Hkv;
+  if (G > TM || TM % G || a.qs.h <= 0 || a.qs.t <= 0) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)a.D, (cuuint64_t)a.H, (cuuint64_t)a.N};
+  const cuuint64_t str[2] = {(cuuint64_t)a.qs.h * 2, (cuuint64_t)a.qs.t * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)(TM / G)};
+  return tc::encode16(m, dt, 3, a.q, dims, str, box);
+}
+
 long long most_items(int B, int N, int G, int row_min) {
   const long long rows = (long long)N * G;
   return rows / kItemRows + std::min<long long>(B, rows / (row_min + 1)) + 1;
@@ -1003,10 +1042,11 @@ int launch_paged_attention_tc(const PagedAttnArgs& a, int row_min, void* workspa
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
-  PoolMaps maps;
+  TensorMaps maps;
   std::memset(&maps, 0, sizeof(maps));
   const bool tma = pool_map(&maps.k, DT, a.kpool, a.kps, a, &maps.kpos) &&
                    pool_map(&maps.v, DT, a.vpool, a.vps, a, &maps.vpos);
+  maps.has_q = query_map(&maps.q, DT, a);
   auto go = [&](auto kfn, int total) -> int {
     {
       AVQ_TIMED("paged_plan", st);
