@@ -416,6 +416,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
     tc::mbar_init(&bars[L::B_DRAIN], 1);
     *abort = 0;
     tc::fence_mbar_init();
+    if (TMA) {
+      tc::tma_prefetch_desc(&maps.k);
+      tc::tma_prefetch_desc(&maps.v);
+    }
+    if (maps.has_q) tc::tma_prefetch_desc(&maps.q);
   }
   if (warp == W_MMA) tc::tmem_alloc(tslot, 512);
   tc::tc_before_sync();
@@ -800,14 +805,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
       if (ok) {
         tc::tc_after_sync();
         const bool whole = w.pieces == 1;
-        const int rows = w.rows, row0 = w.row0, head = w.head;
+        const int rows = w.rows, head = w.head;
         float zero = 0.f;  // NaN once a sum is not finite
         // a row that sees no key is zero; one whose keys all score -inf is 0 / 0
         const float f = whole ? (last > first ? (m == -INFINITY ? NAN : 1.f / l) : 0.f) : 1.f;
         if (whole) {
-          // through this row tile's queries, whose multiplications are over: 16-byte chunk c of a row at c ^ row % 8,
-          // then whole rows to memory
-          unsigned char* stage = sm + L::Q + t * TB + (warp & 3) * 32 * (D * 2);
+          const int at_row = min(w.row0 + r, w.row0 + rows - 1), tok = w.q0 + at_row / G, h = head * G + at_row % G;
+          T* dst = static_cast<T*>(a.out) + (long long)tok * a.os.t + (long long)h * a.os.h;
 #pragma unroll
           for (int c = 0; c < D / 32; ++c) {
             uint32_t o[32];
@@ -815,6 +819,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             tc::tmem_wait_ld();
 #pragma unroll
             for (int e = 0; e < 32; ++e) zero = fmaf(__uint_as_float(o[e]), 0.f, zero);
+            if (r >= rows) continue;
 #pragma unroll
             for (int e = 0; e < 32; e += 8) {
               uint32_t y[4];
@@ -823,29 +828,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
                 const float y0 = __uint_as_float(o[e + 2 * x]) * f, y1 = __uint_as_float(o[e + 2 * x + 1]) * f;
                 y[x] = last > first ? pack2<DT>(y0, y1) : 0u;
               }
-              *reinterpret_cast<uint4*>(stage + lane * (D * 2) + (((c * 4 + e / 8) ^ (lane & 7)) << 4)) =
-                  make_uint4(y[0], y[1], y[2], y[3]);
-            }
-          }
-          __syncwarp();
-          constexpr int CPR = D / 8, RPI = 32 / CPR;
-          const int c = lane % CPR, warp_row = t * TM + (warp & 3) * 32;
-          T* out = static_cast<T*>(a.out) + (long long)w.q0 * a.os.t + (long long)head * G * a.os.h + c * 8;
-          RowStep at(row0 + warp_row + lane / CPR, RPI, G);
-#pragma unroll 4
-          for (int rr = lane / CPR; rr < 32; rr += RPI, at.next()) {
-            if (warp_row + rr < rows) {
-              const uint4 y = *reinterpret_cast<const uint4*>(stage + rr * (D * 2) + ((c ^ (rr & 7)) << 4));
-              T* dst = out + (long long)at.tok * a.os.t + (long long)at.h * a.os.h;
               if (out_wide) {
-                *reinterpret_cast<uint4*>(dst) = y;
+                *reinterpret_cast<uint4*>(dst + c * 32 + e) = make_uint4(y[0], y[1], y[2], y[3]);
               } else {
-                const T* e = reinterpret_cast<const T*>(&y);
-                for (int i = 0; i < 8; ++i) dst[i] = e[i];
+                const T* one = reinterpret_cast<const T*>(y);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) dst[c * 32 + e + i] = one[i];
               }
             }
           }
-          tc::fence_async_smem();  // the next queries may come by TMA
         } else {
           // four columns of 256 rows side by side: a warp's stores are contiguous
           float* pd = partials + (long long)w.slot * (kItemRows * (D + 2));
