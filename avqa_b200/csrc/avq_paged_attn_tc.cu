@@ -106,7 +106,7 @@ __device__ __forceinline__ int2 item_keys(const PagedAttnArgs& a, const SeqRange
 
 // ---- the plan ---------------------------------------------------------------------------
 
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 256;  // (1024 take 1 us longer: their barriers)
 
 // Exclusive prefix of v over the block; *total receives the sum.
 __device__ int block_prefix(int v, int* total) {
@@ -123,14 +123,14 @@ __device__ int block_prefix(int v, int* total) {
   if (lane == 31) s_warp[warp] = x;
   __syncthreads();
   if (warp == 0) {
-    int w = s_warp[lane];
+    int w = lane < kPlanThreads / 32 ? s_warp[lane] : 0;
     const int own = w;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, w, o);
       if (lane >= o) w += y;
     }
-    s_warp[lane] = w - own;
+    if (lane < kPlanThreads / 32) s_warp[lane] = w - own;
     if (lane == 31) s_total = w;
   }
   __syncthreads();
@@ -158,18 +158,25 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PagedAttnArgs 
   asm volatile("griddepcontrol.launch_dependents;");
   bool bad = false;
   int items = 0;
+  long long beside = 0;  // what the kernel of few rows does, in key tiles that take the tensor cores as long
   for (int b0 = 0; b0 < a.B; b0 += kPlanThreads) {
     const int b = b0 + tid;
-    int parts = 0;
+    int parts = 0, few = 0;
     if (b < a.B) {
       const SeqRange s = load_seq(a.q_start, a.kv_len, b, a.N, room, &bad);
       const long long rows = (long long)s.n * G;
       parts = rows > row_min ? (int)((rows + kItemRows - 1) / kItemRows) : 0;
+      if (rows > 0 && parts == 0) {
+        const int keys = s.len - min(s.len, window_start(a, s.pos0));
+        few = (int)min((long long)keys * a.Hkv * a.D / (TK * 128), 1ll << 20);
+      }
     }
-    int total;
+    int total, total_few;
     const int at = items + block_prefix(parts, &total);
+    block_prefix(few, &total_few);
     if (b < a.B) p.base[b] = min(at, max_items);
     items += total;
+    beside += total_few;
   }
   // token ranges that overlap could name more items than the batch has rows for
   if (items > max_items) bad = true;
@@ -205,11 +212,22 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PagedAttnArgs 
   // sequence and head on, so that the SMs finish together, nor than a quarter of an SM's whole share: CTAs that read
   // the same keys then do so at about the same time (whole shares: 1095 us for 256 queries x 64 heads over 131072 keys,
   // quarters 1018, sixths 1062, where the pieces' own cost shows).  Pieces below an eighth of the share or kLeast tiles
-  // are not made, nor more pieces of a pair than there are SMs, for which the joining kernel has room.
-  constexpr long long kLeast = 16;
-  const long long work = (long long)head_tiles * a.Hkv;
-  const long long least = max(kLeast, work / (8 * kSms)), top = max(least, work / (4 * kSms));
-  const int pairs = items * a.Hkv;
+  // are not made (a piece's partial sums are twice the bytes of a key and value tile; 4 prompts of 100 tokens over 1000:
+  // 35 us at 16, 37 at 8, 44 at 4), nor more pieces of a pair than there are SMs, for which the joining kernel has room.
+  // Beside sequences of few rows the SMs that get no piece have their work: pieces are then as long as an SM's share of
+  // all of it, if one round of the SMs takes them (a chunk of 256 tokens over 30000 beside 32 single ones over 4000, 32
+  // heads over 8: 193 us, 245 cut as above; where it takes two, 512 over 8000 beside 8 over 500, 105 and 92).
+  constexpr int kLeast = 16;
+  auto capped = [](long long x) { return (int)min(x, 1ll << 30); };
+  const int work = capped((long long)head_tiles * a.Hkv), pairs = items * a.Hkv;
+  int least = max(kLeast, work / (8 * kSms)), top = max(least, work / (4 * kSms));
+  if (beside > 0 && pairs <= kSms) {
+    const int share = max(kLeast, capped(work + beside) / kSms);
+    int n = 0, total;
+    for (int i = tid; i < items; i += kPlanThreads) n += (p.tiles[i] - 1) / share + 1;
+    block_prefix(n, &total);
+    if ((long long)total * a.Hkv <= kSms) least = top = share;
+  }
   int pieces = 0, slots = 0;
   for (int c0 = 0; c0 < pairs; c0 += kPlanThreads) {
     const int c = c0 + tid;
@@ -217,9 +235,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PagedAttnArgs 
     if (c < pairs) {
       head = c / items;
       i = c - head * items;
-      const long long left = work - (long long)head * head_tiles - p.sum[p.base[p.seq[i]]];
-      const long long most = min(top, max(least, (left + kSms - 1) / kSms));
-      n = (int)min((p.tiles[i] + most - 1) / most, (long long)kMaxPieces);
+      const int left = work - capped((long long)head * head_tiles) - p.sum[p.base[p.seq[i]]];
+      const int most = min(top, max(least, (left + kSms - 1) / kSms));
+      n = min((p.tiles[i] - 1) / most + 1, kMaxPieces);
     }
     int total, total_slots;
     const int slot = slots + block_prefix(n > 1 ? n : 0, &total_slots);
