@@ -15,8 +15,9 @@
 // a ring of each warp's own (16 or 32 keys a stage), so that no barrier joins
 // the warps until their sums meet at the end (32 sequences of up to 32768 keys,
 // 8 key heads of 128, bf16: 454 us, 6.4 TB/s).  The span follows from the
-// lengths, which only the device knows: every CTA adds up the batch's work,
-// takes the span that cuts it into about target_ctas pieces, and finds its own.
+// lengths, which only the device knows: every CTA (for many sequences a kernel
+// before it) adds up the batch's work, takes the span that cuts it into about
+// target_ctas pieces, and finds its own.
 // Few short sequences go to clusters of CTAs instead, which join their sums
 // through shared memory (one token of 4097 keys, 8 key heads: 12 us).
 //
@@ -81,81 +82,200 @@ __device__ __forceinline__ int first_key(const PagedAttnArgs& a, const SeqRange&
   return min(window_start(a, s.pos0), s.len);
 }
 
-// Finds the piece of index `at`, spans being multiples of UNIT keys (a CTA's step): a (sequence, key head, span, row
-// group) when `spans`, else a (sequence, key head, row group) with every span of it.  Each warp does the same work.
-// *slot receives the piece's slot of partial sums (without `spans` that of its first span, the others `stride` apart).
+// How a sequence is cut: its row groups, the first key that it sees, its spans.
+struct Cut {
+  int groups, first, spans;
+};
+template <int RB>
+__device__ __forceinline__ Cut cut_of(const PagedAttnArgs& a, const SeqRange& s, int row_max, unsigned span) {
+  const int f = first_key(a, s);
+  return {row_groups<RB>(a.H / a.Hkv, s.n, row_max), f, max(1, (int)(((unsigned)(s.len - f) + span - 1) / span))};
+}
+// The keys of a sequence, over its row groups and key heads.
+template <int RB>
+__device__ __forceinline__ long long work_of(const PagedAttnArgs& a, const SeqRange& s, int row_max) {
+  return (long long)row_groups<RB>(a.H / a.Hkv, s.n, row_max) * a.Hkv * (s.len - first_key(a, s));
+}
+// The span that cuts a batch of so much work into about target_ctas pieces, in multiples of UNIT keys (a CTA's step).
+template <int UNIT>
+__device__ __forceinline__ unsigned span_of(long long total) {
+  const int target = target_ctas(total);
+  return (unsigned)min((max((total + target - 1) / target, (long long)kMinSpan) + UNIT - 1) / UNIT * UNIT,
+                       (long long)(1 << 30));
+}
+
+// The pieces of a long list of sequences, by lists_kernel: where each sequence's begin.  Adding up the whole list in
+// every CTA, which costs the least for a short one, takes most of a long one's time (8 key heads of 128, bf16,
+// sequences of up to 1000 keys: 64 of them 38.6 us so and 40.6 with the lists, 96 52.9 and 51.2, 256 152 and 111, 2048
+// 3754 and 729, of which the keys need 702).
+constexpr int kListed = 64;
+struct Lists {
+  unsigned* head;    // [0] the span, [1] pieces, [2] (row group, key head) pairs
+  unsigned* pieces;  // [B] pieces of the sequences before
+  unsigned* pairs;   // [B] pairs of the sequences before
+  unsigned* slots;   // [B] slots of partial sums of the sequences before
+};
+__host__ __device__ inline Lists lists_at(unsigned* p, int B) { return {p, p + 8, p + 8 + B, p + 8 + 2ll * B}; }
+size_t lists_bytes(int B) { return B > kListed ? align_up((8 + 3ull * B) * sizeof(unsigned)) : 0; }
+
+constexpr int kListThreads = 1024;
+
 template <int RB, int UNIT>
-__device__ Piece find_piece(const PagedAttnArgs& a, int row_max, int at, bool spans, bool report, int* slot,
-                            int* stride) {
-  const int lane = threadIdx.x & 31, G = a.H / a.Hkv;
+__global__ void __launch_bounds__(kListThreads) lists_kernel(const PagedAttnArgs a, int row_max, unsigned* ws) {
+  __shared__ long long s_total[kListThreads / 32];
+  __shared__ unsigned s_warp[3][kListThreads / 32];
+  const Lists out = lists_at(ws, a.B);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const long long room = (long long)a.W * a.page_size;
   bool bad = false;
   long long total = 0;
-  for (int b = lane; b < a.B; b += 32) {
-    const SeqRange s = load_seq(a.q_start, a.kv_len, b, a.N, room, &bad);
-    total += (long long)row_groups<RB>(G, s.n, row_max) * a.Hkv * (s.len - first_key(a, s));
-  }
+  for (int b = tid; b < a.B; b += kListThreads)
+    total += work_of<RB>(a, load_seq(a.q_start, a.kv_len, b, a.N, room, &bad), row_max);
+  if (bad) atomicOr(&g_fault_tables_paged, kFaultTables);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  if (report && bad) atomicOr(&g_fault_tables_paged, kFaultTables);
-  const int target = target_ctas(total);
-  const unsigned span = (unsigned)min(
-      (max((total + target - 1) / target, (long long)kMinSpan) + UNIT - 1) / UNIT * UNIT,
-      (long long)(1 << 30));
+  if (lane == 0) s_total[warp] = total;
+  __syncthreads();
+  total = 0;
+  for (int w = 0; w < kListThreads / 32; ++w) total += s_total[w];
+  const unsigned span = span_of<UNIT>(total);
+  unsigned before[3] = {0, 0, 0};  // pieces, pairs, slots of the sequences before this turn's
+  for (int b0 = 0; b0 < a.B; b0 += kListThreads) {
+    const int b = b0 + tid;
+    unsigned mine[3] = {0, 0, 0}, pre[3];
+    if (b < a.B) {
+      const Cut c = cut_of<RB>(a, load_seq(a.q_start, a.kv_len, b, a.N, room, &bad), row_max, span);
+      mine[1] = (unsigned)c.groups * a.Hkv;
+      mine[0] = mine[1] * c.spans;
+      mine[2] = c.spans > 1 ? mine[0] : 0u;
+    }
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      pre[i] = mine[i];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned x = __shfl_up_sync(0xffffffffu, pre[i], o);
+        if (lane >= o) pre[i] += x;
+      }
+      if (lane == 31) s_warp[i][warp] = pre[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const unsigned w = s_warp[i][lane];  // (as many warps as lanes)
+      unsigned x = lane < warp ? w : 0u, all = w;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        x += __shfl_xor_sync(0xffffffffu, x, o);
+        all += __shfl_xor_sync(0xffffffffu, all, o);
+      }
+      pre[i] += before[i] + x - mine[i];
+      before[i] += all;
+    }
+    __syncthreads();
+    if (b < a.B) {
+      out.pieces[b] = pre[0];
+      out.pairs[b] = pre[1];
+      out.slots[b] = pre[2];
+    }
+  }
+  if (tid == 0) {
+    out.head[0] = span;
+    out.head[1] = before[0];
+    out.head[2] = before[1];
+  }
+}
+
+// Finds the piece of index `at`: a (sequence, key head, span, row group) when `spans`, else a (sequence, key head, row
+// group) with every span of it.  Each warp does the same work, from the lists if there are any.  *slot receives the
+// piece's slot of partial sums (without `spans` that of its first span, the others `stride` apart).
+template <int RB, int UNIT>
+__device__ Piece find_piece(const PagedAttnArgs& a, int row_max, unsigned at, bool spans, bool report, unsigned* lists,
+                            int* slot, int* stride) {
+  const int lane = threadIdx.x & 31;
+  const long long room = (long long)a.W * a.page_size;
   Piece p;
   p.found = false;
-  unsigned before = 0, slots = 0;  // pieces and partial slots of the sequences before
-  for (int b0 = 0; b0 < a.B; b0 += 32) {
-    const int b = b0 + lane;
-    SeqRange s{0, 0, 0, 0};
-    int groups = 0, ns = 0, f = 0;
-    bool ignore = false;
-    if (b < a.B) {
-      s = load_seq(a.q_start, a.kv_len, b, a.N, room, &ignore);
-      groups = row_groups<RB>(G, s.n, row_max);
-      f = first_key(a, s);
-      ns = max(1, (int)(((unsigned)(s.len - f) + span - 1) / span));
+  unsigned span, rel = 0, base = 0;  // the index in the sequence's pieces, its first slot
+  Cut cut{0, 0, 0};
+  bool bad = false;
+  if (lists) {
+    const Lists l = lists_at(lists, a.B);
+    span = l.head[0];
+    if (at >= l.head[spans ? 1 : 2]) return p;
+    const unsigned* begin = spans ? l.pieces : l.pairs;
+    int lo = 0;  // the last sequence that begins at or before the index
+    for (int n = a.B; n > 1;) {
+      const int step = (n + 31) / 32, i = lane * step;
+      const int k = __popc(__ballot_sync(0xffffffffu, i < n && begin[lo + min(i, n - 1)] <= at)) - 1;
+      lo += k * step;
+      n = min(step, n - k * step);
     }
-    // (only cut sequences need slots: at most twice the target, as ceil(x) < 2 x for x > 1)
-    const unsigned mine = (unsigned)groups * a.Hkv * ns, count = spans ? mine : (unsigned)groups * a.Hkv;
-    const unsigned slotted = ns > 1 ? mine : 0u;
-    unsigned pre = count, pre_slots = slotted;
+    p.b = lo;
+    p.seq = load_seq(a.q_start, a.kv_len, lo, a.N, room, &bad);
+    cut = cut_of<RB>(a, p.seq, row_max, span);
+    rel = at - begin[lo];
+    base = l.slots[lo];
+    p.found = true;
+  } else {
+    long long total = 0;
+    for (int b = lane; b < a.B; b += 32)
+      total += work_of<RB>(a, load_seq(a.q_start, a.kv_len, b, a.N, room, &bad), row_max);
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned x = __shfl_up_sync(0xffffffffu, pre, o), y = __shfl_up_sync(0xffffffffu, pre_slots, o);
-      if (lane >= o) {
-        pre += x;
-        pre_slots += y;
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    if (report && bad) atomicOr(&g_fault_tables_paged, kFaultTables);
+    span = span_of<UNIT>(total);
+    unsigned before = 0, slots = 0;  // pieces and partial slots of the sequences before
+    for (int b0 = 0; b0 < a.B && !p.found; b0 += 32) {
+      const int b = b0 + lane;
+      SeqRange s{0, 0, 0, 0};
+      Cut c{0, 0, 0};
+      if (b < a.B) {
+        s = load_seq(a.q_start, a.kv_len, b, a.N, room, &bad);
+        c = cut_of<RB>(a, s, row_max, span);
       }
+      // (only cut sequences need slots: at most twice the target, as ceil(x) < 2 x for x > 1)
+      const unsigned mine = (unsigned)c.groups * a.Hkv * c.spans, count = spans ? mine : (unsigned)c.groups * a.Hkv;
+      const unsigned slotted = c.spans > 1 ? mine : 0u;
+      unsigned pre = count, pre_slots = slotted;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned x = __shfl_up_sync(0xffffffffu, pre, o), y = __shfl_up_sync(0xffffffffu, pre_slots, o);
+        if (lane >= o) {
+          pre += x;
+          pre_slots += y;
+        }
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, before + pre > at);
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        rel = at - before - __shfl_sync(0xffffffffu, pre - count, src);
+        base = slots + __shfl_sync(0xffffffffu, pre_slots - slotted, src);
+        p.b = b0 + src;
+        p.seq.q0 = __shfl_sync(0xffffffffu, s.q0, src);
+        p.seq.n = __shfl_sync(0xffffffffu, s.n, src);
+        p.seq.len = __shfl_sync(0xffffffffu, s.len, src);
+        p.seq.pos0 = __shfl_sync(0xffffffffu, s.pos0, src);
+        cut.groups = __shfl_sync(0xffffffffu, c.groups, src);
+        cut.first = __shfl_sync(0xffffffffu, c.first, src);
+        cut.spans = __shfl_sync(0xffffffffu, c.spans, src);
+        p.found = true;
+      }
+      before += __shfl_sync(0xffffffffu, pre, 31);
+      slots += __shfl_sync(0xffffffffu, pre_slots, 31);
     }
-    const unsigned hit = __ballot_sync(0xffffffffu, before + pre > (unsigned)at);
-    if (hit) {
-      const int src = __ffs(hit) - 1;
-      const unsigned rel = (unsigned)at - before - __shfl_sync(0xffffffffu, pre - count, src);
-      const unsigned base = slots + __shfl_sync(0xffffffffu, pre_slots - slotted, src);
-      p.b = b0 + src;
-      p.seq.q0 = __shfl_sync(0xffffffffu, s.q0, src);
-      p.seq.n = __shfl_sync(0xffffffffu, s.n, src);
-      p.seq.len = __shfl_sync(0xffffffffu, s.len, src);
-      p.seq.pos0 = __shfl_sync(0xffffffffu, s.pos0, src);
-      p.nspan = __shfl_sync(0xffffffffu, ns, src);
-      const unsigned n_groups = __shfl_sync(0xffffffffu, groups, src);
-      f = __shfl_sync(0xffffffffu, f, src);
-      // row groups of one span lie side by side: they read the same keys
-      const unsigned rest = n_groups == 1 ? rel : rel / n_groups;
-      p.group = (int)(rel - rest * n_groups);
-      p.head = (int)(spans ? rest / (unsigned)p.nspan : rest);
-      p.span_i = spans ? (int)(rest - (unsigned)p.head * p.nspan) : 0;
-      p.lo = (int)min((unsigned)p.seq.len, f + p.span_i * span);
-      p.hi = (int)min((unsigned)p.seq.len, f + (p.span_i + 1) * span);
-      p.found = true;
-      *slot = (int)(base + ((unsigned)p.head * p.nspan + p.span_i) * n_groups + p.group);
-      *stride = (int)n_groups;
-      return p;
-    }
-    before += __shfl_sync(0xffffffffu, pre, 31);
-    slots += __shfl_sync(0xffffffffu, pre_slots, 31);
+    if (!p.found) return p;
   }
+  // row groups of one span lie side by side: they read the same keys
+  const unsigned n_groups = cut.groups, rest = n_groups == 1 ? rel : rel / n_groups;
+  p.nspan = cut.spans;
+  p.group = (int)(rel - rest * n_groups);
+  p.head = (int)(spans ? rest / (unsigned)p.nspan : rest);
+  p.span_i = spans ? (int)(rest - (unsigned)p.head * p.nspan) : 0;
+  p.lo = (int)min((unsigned)p.seq.len, cut.first + p.span_i * span);
+  p.hi = (int)min((unsigned)p.seq.len, cut.first + (p.span_i + 1) * span);
+  *slot = (int)(base + ((unsigned)p.head * p.nspan + p.span_i) * n_groups + p.group);
+  *stride = (int)n_groups;
   return p;
 }
 
@@ -245,7 +365,7 @@ __device__ __forceinline__ void cluster_sync() {
 
 template <int DT, int DP, bool WIDE, bool SAME, int RB, bool CL>
 __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const PagedAttnArgs a, int row_max,
-                                                                     int q_wide, int beside,
+                                                                     int q_wide, int beside, unsigned* lists,
                                                                      float* __restrict__ part) {
   using T = typename Storage<DT>::T;
   constexpr int KS = step_keys<DT, DP>(), NK = KS / 8;  // keys of a step, in columns of 8
@@ -257,7 +377,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
   asm volatile("griddepcontrol.launch_dependents;");
   int slot = 0, slot_stride = 0;
   Piece p = find_piece<RB, kWarps * KS>(a, row_max, CL ? blockIdx.x / kCluster : blockIdx.x, !CL,
-                                        blockIdx.x == 0 && warp == 0, &slot, &slot_stride);
+                                        blockIdx.x == 0 && warp == 0, lists, &slot, &slot_stride);
   // a grid that runs beside another ends after it, so that what waits for this one has waited for both
   auto leave = [&]() {
     if (beside && blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -693,7 +813,7 @@ constexpr int kJoinWarps = 8;
 constexpr int kJoinCtas = 4 * kSms;
 
 template <int DT, int DP, int RB>
-__global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const PagedAttnArgs a, int row_max,
+__global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const PagedAttnArgs a, int row_max, unsigned* lists,
                                                                   const float* __restrict__ part) {
   using T = typename Storage<DT>::T;
   constexpr int VW = DP >= 128 ? 4 : 2, NV = DP / (32 * VW);  // floats of a lane's vector, vectors of a lane
@@ -702,7 +822,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) combine_kernel(const PagedAtt
   const int G = a.H / a.Hkv, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // the lists are older than the attention kernel, which this launch may overtake
   int slot = 0, stride = 0;
-  const Piece p = find_piece<RB, kWarps * step_keys<DT, DP>()>(a, row_max, blockIdx.x, false, false, &slot, &stride);
+  const Piece p =
+      find_piece<RB, kWarps * step_keys<DT, DP>()>(a, row_max, blockIdx.x, false, false, lists, &slot, &stride);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (!p.found || p.nspan == 1) return;
   const int row0 = p.group * RB, nrow = min(RB, p.seq.n * G - row0);
@@ -810,6 +931,9 @@ Choice choose(int dtype, int N, int H, int Hkv, int D, int max_q, bool operands)
 }
 
 int padded_dim(int D) { return D <= 64 ? 64 : (D <= 128 ? 128 : 256); }
+size_t slots_bytes(int D) {
+  return align_up((size_t)2 * kTargetCtas * kMaxGroup * (padded_dim(D) + 2) * sizeof(float));
+}
 
 bool wide_rows(const void* p, std::initializer_list<long long> strides, int elem) {
   if (reinterpret_cast<uintptr_t>(p) % 16) return false;
@@ -819,7 +943,8 @@ bool wide_rows(const void* p, std::initializer_list<long long> strides, int elem
 }
 
 template <int DT, int DP, int RB>
-int launch_mma(const PagedAttnArgs& a, const Choice& c, void* tc_workspace, float* part, cudaStream_t st) {
+int launch_mma(const PagedAttnArgs& a, const Choice& c, void* tc_workspace, float* part, unsigned* lists,
+               cudaStream_t st) {
   using T = typename Storage<DT>::T;
   const int E = (int)sizeof(T), row_max = c.row_max;
   const bool beside = c.many;
@@ -842,6 +967,17 @@ int launch_mma(const PagedAttnArgs& a, const Choice& c, void* tc_workspace, floa
   const size_t smem = variant == 3 ? mma_smem<DT, DP, RB, true>() : mma_smem<DT, DP, RB, false>();
   static std::atomic<unsigned long long> allowed[4];
   if (!allow_smem((const void*)kfn, smem, allowed[variant])) return AVQ_ERR_CUDA;
+  if (lists) {
+    AVQ_TIMED("paged_lists", st);
+    lists_kernel<RB, kWarps * step_keys<DT, DP>()><<<1, kListThreads, 0, st>>>(a, row_max, lists);
+    if (cudaPeekAtLastError() != cudaSuccess) return AVQ_ERR_CUDA;
+  }
+  if constexpr (DT != DT_F32 && DP <= 128) {
+    if (beside) {  // (its plan begins when the lists are there, and so does all that follows)
+      const int rc = launch_paged_attention_tc<DT>(a, row_max, tc_workspace, st);
+      if (rc != AVQ_OK) return rc;
+    }
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.stream = st;
   cudaLaunchAttribute attr;
@@ -855,7 +991,8 @@ int launch_mma(const PagedAttnArgs& a, const Choice& c, void* tc_workspace, floa
     cfg.gridDim = dim3((unsigned)(items * kCluster));
     cfg.blockDim = dim3(kWarps * 32);
     cfg.dynamicSmemBytes = smem;
-    return cudaLaunchKernelEx(&cfg, kfn, a, row_max, (int)q_wide, 0, part) == cudaSuccess ? AVQ_OK : AVQ_ERR_CUDA;
+    return cudaLaunchKernelEx(&cfg, kfn, a, row_max, (int)q_wide, 0, lists, part) == cudaSuccess ? AVQ_OK
+                                                                                                  : AVQ_ERR_CUDA;
   }
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
@@ -868,7 +1005,8 @@ int launch_mma(const PagedAttnArgs& a, const Choice& c, void* tc_workspace, floa
     cfg.blockDim = dim3(kWarps * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.numAttrs = beside ? 1 : 0;
-    if (cudaLaunchKernelEx(&cfg, kfn, a, row_max, (int)q_wide, (int)beside, part) != cudaSuccess) return AVQ_ERR_CUDA;
+    if (cudaLaunchKernelEx(&cfg, kfn, a, row_max, (int)q_wide, (int)beside, lists, part) != cudaSuccess)
+      return AVQ_ERR_CUDA;
   }
   if constexpr (DT != DT_F32 && DP <= 128) {
     if (beside) {
@@ -884,7 +1022,7 @@ int launch_mma(const PagedAttnArgs& a, const Choice& c, void* tc_workspace, floa
   cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, combine_kernel<DT, DP, RB>, a, row_max, (const float*)part) == cudaSuccess
+  return cudaLaunchKernelEx(&cfg, combine_kernel<DT, DP, RB>, a, row_max, lists, (const float*)part) == cudaSuccess
              ? AVQ_OK
              : AVQ_ERR_CUDA;
 }
@@ -892,7 +1030,7 @@ int launch_mma(const PagedAttnArgs& a, const Choice& c, void* tc_workspace, floa
 }  // namespace
 
 size_t paged_attn_workspace_bytes(int dtype, int B, int N, int H, int Hkv, int D, int max_q) {
-  const size_t few = align_up((size_t)2 * kTargetCtas * kMaxGroup * (padded_dim(D) + 2) * sizeof(float));
+  const size_t few = slots_bytes(D) + lists_bytes(B);
   const Choice with = choose(dtype, N, H, Hkv, D, max_q, true);  // (the operands' alignment may still rule it out)
   return with.many ? few + paged_attn_tc_workspace_bytes(B, N, H, Hkv, D, with.row_max) : few;
 }
@@ -905,20 +1043,17 @@ int launch_paged_attention(const PagedAttnArgs& a, cudaStream_t st) {
                         wide_rows(a.kpool, {a.kps.p, a.kps.h, a.kps.s}, E) &&
                         wide_rows(a.vpool, {a.vps.p, a.vps.h, a.vps.s}, E);
   const Choice c = choose(DT, a.N, a.H, a.Hkv, a.D, a.max_q, operands);
+  // the workspace: slots of partial sums, the lists, what the tcgen05 kernel needs
   char* ws = static_cast<char*>(a.workspace);
-  if constexpr (DT != DT_F32) {
-    if (c.many) {
-      const int rc = launch_paged_attention_tc<DT>(a, c.row_max, ws, st);
-      if (rc != AVQ_OK) return rc;
-      ws += paged_attn_tc_workspace_bytes(a.B, a.N, a.H, a.Hkv, a.D, c.row_max);
-    }
-  }
   float* part = reinterpret_cast<float*>(ws);
+  ws += slots_bytes(a.D);
+  unsigned* lists = a.B > kListed ? reinterpret_cast<unsigned*>(ws) : nullptr;
+  ws += lists_bytes(a.B);
   auto go = [&](auto group) -> int {
     constexpr int RB = decltype(group)::value;
-    if (a.D <= 64) return launch_mma<DT, 64, RB>(a, c, a.workspace, part, st);
-    if (a.D <= 128) return launch_mma<DT, 128, RB>(a, c, a.workspace, part, st);
-    return launch_mma<DT, 256, RB>(a, c, a.workspace, part, st);
+    if (a.D <= 64) return launch_mma<DT, 64, RB>(a, c, ws, part, lists, st);
+    if (a.D <= 128) return launch_mma<DT, 128, RB>(a, c, ws, part, lists, st);
+    return launch_mma<DT, 256, RB>(a, c, ws, part, lists, st);
   };
   if constexpr (DT != DT_F32) {
     if (c.group == 8) return go(std::integral_constant<int, 8>{});

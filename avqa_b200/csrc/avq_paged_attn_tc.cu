@@ -212,8 +212,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PagedAttnArgs 
   // sequence and head on, so that the SMs finish together, nor than a quarter of an SM's whole share: CTAs that read
   // the same keys then do so at about the same time (whole shares: 1095 us for 256 queries x 64 heads over 131072 keys,
   // quarters 1018, sixths 1062, where the pieces' own cost shows).  Pieces below an eighth of the share or kLeast tiles
-  // are not made (a piece's partial sums are twice the bytes of a key and value tile; 4 prompts of 100 tokens over 1000:
-  // 35 us at 16, 37 at 8, 44 at 4), nor more pieces of a pair than there are SMs, for which the joining kernel has room.
+  // are not made (a piece's partial sums are twice the bytes of a key and value tile; 4 prompts of 100 tokens over
+  // 1000: 35 us at 16, 37 at 8, 44 at 4), nor more pieces of a pair than there are SMs, for which the joining kernel
+  // has room.
   // Beside sequences of few rows the SMs that get no piece have their work: pieces are then as long as an SM's share of
   // all of it, if one round of the SMs takes them (a chunk of 256 tokens over 30000 beside 32 single ones over 4000, 32
   // heads over 8: 193 us, 245 cut as above; where it takes two, 512 over 8000 beside 8 over 500, 105 and 92).

@@ -253,6 +253,7 @@ def algorithmic_work(w, B: int, T: int | None = None, decode: bool = False, sel_
             "paged_attn": ("hbm", 2 * G * (S + T) * D * es),
             "paged_combine": ("hbm", G * T * D * (4 + es)),
             "paged_attn_tc": ("tensor", 4.0 * G * T * (S + T) * D),
+            "paged_lists": ("hbm", 20 * B),
             "paged_plan": ("hbm", 12 * B),
             "paged_combine_tc": ("hbm", G * T * D * (4 + es)),
         }

@@ -158,6 +158,35 @@ def test_one_pair_over_more_keys_than_its_pieces_number() -> None:
     assert fault() == 0
 
 
+@pytest.mark.parametrize("dt,D", [("bf16", 128), ("f16", 64), ("f32", 40)])
+@pytest.mark.parametrize("B", [64, 65, 300, 1025])
+@pytest.mark.parametrize("chunk", [1, 40])
+def test_long_lists_of_sequences(dt, D, B, chunk) -> None:
+    """Sequences of all kinds by the hundreds: empty ones, ones longer than a span, none seen, beside chunks or not."""
+    r = random.Random(B)
+    new = [r.choice([0, 1, 1, 1, 2]) for _ in range(B)]
+    new[B // 2] = chunk
+    lens = [r.choice([0, 1, 5, 17, 40]) + n for n in new]
+    lens[B // 3], lens[B - 1] = 2000, 700
+    b = Batch(dt, 4, 2, D, 16, new, lens, seed=B)
+    b.check()
+    b.check("window", window=30)
+    assert fault() == 0
+    lens = b.kv_len.clone()
+    b.kv_len[5] = 1 << 30  # beyond the table's row
+    ops.paged_attention(b.q, *b.lists)
+    assert fault() == 2
+    b.kv_len.copy_(lens)
+    want = b.check()
+    b.q_start[:B // 4] = b.q_start[B // 4].clone()  # the first quarter has no tokens any more
+    out = torch.full_like(want, 7.0)
+    ops.paged_attention(b.q, *b.lists, out=out)
+    first = int(b.q_start[B // 4])
+    assert (out[:first] == 7.0).all()
+    rest, bound, _ = attention64(b.q, *b.lists)
+    assert_within(out[first:], rest[first:], bound[first:], "a quarter without tokens")
+
+
 @pytest.mark.parametrize("dt,D", [("bf16", 128), ("f16", 64), ("f32", 64)])
 @pytest.mark.parametrize("new,lens", [([3, 1], [1, 50]), ([60, 40], [40, 90])])
 def test_window_of_any_size(dt, D, new, lens) -> None:
