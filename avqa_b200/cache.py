@@ -239,6 +239,7 @@ class BlockKVCache(KVCache):
         self.lengths: list[int] = []  # tokens of each sequence
         self.pages: list[list[int]] = []  # its pages, in order
         self.free_pages = list(range(num_pages - 1, -1, -1))
+        self._table = torch.zeros(0, 1, dtype=torch.int32)  # the pages as the steps' table rows, on the host
 
     # -- sequences ---------------------------------------------------------------
 
@@ -260,18 +261,25 @@ class BlockKVCache(KVCache):
             raise NotInitializedError(f"paged KV cache is full ({self.num_pages} pages)",
                                       {"needed": sum(more), "free": len(self.free_pages)})
         self.pages.extend([] for _ in range(len(new) - len(self.pages)))
-        for b, n in enumerate(more):
-            self.pages[b].extend(self.free_pages.pop() for _ in range(n))
-        self.lengths = grown
         B, W = len(new), max([1, *need])
+        if self._table.shape[0] < B or self._table.shape[1] < W:
+            table = torch.zeros(max(B, self._table.shape[0]), max(W, 2 * self._table.shape[1]), dtype=torch.int32)
+            table[:self._table.shape[0], :self._table.shape[1]] = self._table
+            self._table = table
+        for b, n in enumerate(more):
+            if n > 0:
+                old = len(self.pages[b])
+                self.pages[b].extend(self.free_pages.pop() for _ in range(n))
+                self._table[b, old:old + n] = torch.tensor(self.pages[b][old:], dtype=torch.int32)
+        self.lengths = grown
         starts = [0]
         for n in new:
             starts.append(starts[-1] + n)
-        rows = [p + [0] * (W - len(p)) for p in self.pages]
-        # one copy carries all lists
-        flat = torch.tensor([x for row in rows for x in row] + self.lengths + starts, dtype=torch.int32)
-        if self.device.type == "cuda":
-            flat = flat.pin_memory().to(self.device, non_blocking=True)
+        # one copy carries all lists; its host memory is the step's own, as the copy may still run when the next begins
+        flat = torch.empty(B * W + 2 * B + 1, dtype=torch.int32, pin_memory=self.device.type == "cuda")
+        flat[:B * W].view(B, W).copy_(self._table[:B, :W])
+        flat[B * W:] = torch.tensor(grown + starts, dtype=torch.int32)
+        flat = flat.to(self.device, non_blocking=True)
         return PagedBatch(flat[:B * W].view(B, W), flat[B * W:B * W + B], flat[B * W + B:], max([0, *new]),
                           starts[-1])
 
