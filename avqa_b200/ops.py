@@ -380,6 +380,27 @@ def _positions_operand(positions: torch.Tensor | None, axes: int, B: int, T: int
     return positions.data_ptr(), nbytes, strides
 
 
+@functools.lru_cache(maxsize=4096)
+def _rotary_layout(q: tuple, q_strides: tuple, q_out_strides: tuple, k: tuple | None, k_strides: tuple | None,
+                   k_out_strides: tuple | None, head_dim: int) -> tuple:
+    """Check the shapes and strides of a rotation; (B, heads of q and k, T, D, stride arrays of
+    q, k and their outputs).  The same layouts come again on every step."""
+    if len(q) != 4:
+        raise ShapeError("query and key must be [B, H, T, head_dim]", expected=4, actual=tuple(q))
+    B, H, T, D = q
+    if D != head_dim:
+        raise ShapeError("the rotary embedding's head_dim differs from the query's", expected=head_dim, actual=D)
+    if k is not None and (len(k) != 4 or k[0] != B or k[2] != T or k[3] != D):
+        raise ShapeError("key must have the query's batch, tokens and head_dim", expected=(B, "Hk", T, D),
+                         actual=tuple(k))
+    arrays = []
+    for st in (q_strides, k_strides, q_out_strides, k_out_strides):
+        if st is not None and st[3] != 1 and D > 1:
+            raise BackendError("operand must be a 4-D view with a contiguous last dimension", {"stride": tuple(st)})
+        arrays.append(None if st is None else _lib.longs(*st[:3]))
+    return B, H, 0 if k is None else k[1], T, D, *arrays
+
+
 def rotary(embedding, q: torch.Tensor, k: torch.Tensor | None = None, positions: torch.Tensor | None = None,
            offset: int = 0, reverse: bool = False) -> tuple[torch.Tensor, torch.Tensor | None]:
     """Rotate ``q [B, H, T, D]`` and ``k [B, Hk, T, D]`` (or ``None``) by a
@@ -387,26 +408,21 @@ def rotary(embedding, q: torch.Tensor, k: torch.Tensor | None = None, positions:
     ``reverse``) into new tensors; no gradient is recorded here."""
     lib = _lib.load()
     at, dt = _cuda_index(q, "query"), q.dtype
-    B, H, T, D = q.shape
-    if D != embedding.head_dim:
-        raise ShapeError("the rotary embedding's head_dim differs from the query's", expected=embedding.head_dim,
-                         actual=D)
     q_out = torch.empty_like(q)
-    kp = ks = kop = kos = k_out = None
-    Hk = 0
-    if k is not None:
+    kp = kop = k_out = None
+    if k is None:
+        B, H, Hk, T, D, qs, ks, qos, kos = _rotary_layout(q.shape, q.stride(), q_out.stride(), None, None, None,
+                                                          embedding.head_dim)
+    else:
         _same("key", k, at, dt)
-        Bk, Hk, Tk, Dk = k.shape
-        if Bk != B or Tk != T or Dk != D:
-            raise ShapeError("key must have the query's batch, tokens and head_dim", expected=(B, "Hk", T, D),
-                             actual=tuple(k.shape))
         k_out = torch.empty_like(k)
-        kp, ks, kop, kos = k.data_ptr(), _lib.strides3(k), k_out.data_ptr(), _lib.strides3(k_out)
+        kp, kop = k.data_ptr(), k_out.data_ptr()
+        B, H, Hk, T, D, qs, ks, qos, kos = _rotary_layout(q.shape, q.stride(), q_out.stride(), k.shape, k.stride(),
+                                                          k_out.stride(), embedding.head_dim)
     pos, pos_bytes, pos_strides = _positions_operand(positions, embedding.num_axes, B, T, at)
-    _call("avq_rotary", lib.avq_rotary, at, _lib.dtype_code(dt), q.data_ptr(), _lib.strides3(q), H, kp, ks, Hk, B, T,
-          D, embedding.rotary_dim, embedding.interleaved, embedding.c_frequencies, embedding.c_axes,
-          embedding.num_axes, pos, pos_bytes, _lib.longs(*pos_strides), offset, reverse, q_out.data_ptr(),
-          _lib.strides3(q_out), kop, kos)
+    _call("avq_rotary", lib.avq_rotary, at, _lib.dtype_code(dt), q.data_ptr(), qs, H, kp, ks, Hk, B, T, D,
+          embedding.rotary_dim, embedding.interleaved, embedding.c_frequencies, embedding.c_axes, embedding.num_axes,
+          pos, pos_bytes, _lib.longs(*pos_strides), offset, reverse, q_out.data_ptr(), qos, kop, kos)
     return q_out, k_out
 
 
@@ -526,6 +542,17 @@ def _attention_workspace(code: int, B: int, N: int, H: int, Hkv: int, D: int, ma
     return max(256, _lib.load().avq_paged_attention_workspace_size(code, B, N, H, Hkv, D, max_q_len))
 
 
+@functools.lru_cache(maxsize=4096)
+def _query_layout(q: tuple, strides: tuple) -> tuple:
+    """Check a packed query; (N, H, D, its stride array, that of a contiguous output)."""
+    if len(q) != 3:
+        raise ShapeError("query must be packed [tokens, heads, head_dim]", expected="[N, H, D]", actual=tuple(q))
+    N, H, D = q
+    if strides[2] != 1 and D > 1:
+        raise BackendError("query must have a contiguous last dimension", {"stride": tuple(strides)})
+    return N, H, D, _lib.longs(strides[0], strides[1]), _lib.longs(H * D, D)
+
+
 def paged_attention(q: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.Tensor, block_table: torch.Tensor,
                     kv_len: torch.Tensor, q_start: torch.Tensor, causal: bool = True, window: int = 0,
                     scale: float | None = None, max_q_len: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -545,8 +572,7 @@ def paged_attention(q: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.T
     (bf16, fp16), all sums are fp32.  Serving only: no gradient is recorded."""
     lib = _lib.load()
     at, dt = _cuda_index(q, "query"), q.dtype
-    N, H, D = _packed_shape(q, "query")
-    qs = _packed(q, "query", H, N, D)
+    N, H, D, qs, os = _query_layout(q.shape, q.stride())
     Hkv, kst, vst, pages, page_size, row, width, B = _pool(key_pool, value_pool, block_table, kv_len, q_start, at, dt,
                                                            D)
     if not (0 <= window < 1 << 31 and 0 <= max_q_len < 1 << 31):
@@ -560,6 +586,7 @@ def paged_attention(q: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.T
         _same("out", out, at, dt)
         if N and out.data_ptr() == q.data_ptr():
             raise BackendError("out must not be the query's memory")
+        os = _packed(out, "out", H, N, D)
     if scale is None:
         scale = D ** -0.5 if D else 1.0
     code = _lib.dtype_code(dt)
@@ -567,8 +594,7 @@ def paged_attention(q: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.T
     ws = kv_len.new_empty(ws_bytes // 4)
     _call("avq_paged_attention", lib.avq_paged_attention, at, code, q.data_ptr(), qs, H, key_pool.data_ptr(), kst,
           value_pool.data_ptr(), vst, Hkv, D, pages, page_size, block_table.data_ptr(), row, width, kv_len.data_ptr(),
-          q_start.data_ptr(), B, N, causal, window, scale, max_q_len, out.data_ptr(), _packed(out, "out", H, N, D),
-          ws.data_ptr(), ws_bytes)
+          q_start.data_ptr(), B, N, causal, window, scale, max_q_len, out.data_ptr(), os, ws.data_ptr(), ws_bytes)
     return out
 
 
