@@ -218,16 +218,23 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PagedAttnArgs 
   // Beside sequences of few rows the SMs that get no piece have their work: pieces are then as long as an SM's share of
   // all of it, if one round of the SMs takes them (a chunk of 256 tokens over 30000 beside 32 single ones over 4000, 32
   // heads over 8: 193 us, 245 cut as above; where it takes two, 512 over 8000 beside 8 over 500, 105 and 92).
+  // Without them a few pairs are cut into as many equal pieces as half a round of the SMs takes, or a round where they
+  // are cut anyway, down to half of kLeast (64 tokens over 8000, 32 heads over 8: 53 us as above, 42 so; over 20000 63
+  // and 58; 3 prompts of 100 over 3000 48 and 43).
   constexpr int kLeast = 16;
   auto capped = [](long long x) { return (int)min(x, 1ll << 30); };
   const int work = capped((long long)head_tiles * a.Hkv), pairs = items * a.Hkv;
   int least = max(kLeast, work / (8 * kSms)), top = max(least, work / (4 * kSms));
-  if (beside > 0 && pairs <= kSms) {
-    const int share = max(kLeast, capped(work + beside) / kSms);
+  if (pairs <= kSms) {
+    const int even = beside > 0 ? max(kLeast, capped(work + beside) / kSms) : max(kLeast / 2, work / kSms + 1);
     int n = 0, total;
-    for (int i = tid; i < items; i += kPlanThreads) n += (p.tiles[i] - 1) / share + 1;
+    bool cut = beside > 0;
+    for (int i = tid; i < items; i += kPlanThreads) {
+      n += (p.tiles[i] - 1) / even + 1;
+      cut = cut || p.tiles[i] > kLeast;
+    }
     block_prefix(n, &total);
-    if ((long long)total * a.Hkv <= kSms) least = top = share;
+    if ((long long)total * a.Hkv <= (__syncthreads_or(cut) ? kSms : kSms / 2)) least = top = even;
   }
   int pieces = 0, slots = 0;
   for (int c0 = 0; c0 < pairs; c0 += kPlanThreads) {
