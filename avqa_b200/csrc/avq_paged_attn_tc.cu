@@ -208,6 +208,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PagedAttnArgs 
     if (i < items) p.sum[i] = at;
     head_tiles += total;
   }
+  __syncthreads();  // (the cuts below read the sums of other warps' items)
   // The pairs in order, each cut so that no piece is larger than an SM's share of the work that is left from its
   // sequence and head on, so that the SMs finish together, nor than a quarter of an SM's whole share: CTAs that read
   // the same keys then do so at about the same time (whole shares: 1095 us for 256 queries x 64 heads over 131072 keys,
