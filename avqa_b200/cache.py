@@ -260,18 +260,19 @@ class BlockKVCache(KVCache):
         if sum(more) > len(self.free_pages):
             raise NotInitializedError(f"paged KV cache is full ({self.num_pages} pages)",
                                       {"needed": sum(more), "free": len(self.free_pages)})
-        self.pages.extend([] for _ in range(len(new) - len(self.pages)))
         B, W = len(new), max([1, *need])
-        if self._table.shape[0] < B or self._table.shape[1] < W:
-            table = torch.zeros(max(B, self._table.shape[0]), max(W, 2 * self._table.shape[1]), dtype=torch.int32)
-            table[:self._table.shape[0], :self._table.shape[1]] = self._table
+        rows, width = self._table.shape
+        if rows < B or width < W:  # only what is short grows; no sequence can hold more than the pool
+            table = torch.zeros(rows if rows >= B else max(B, 2 * rows),
+                                width if width >= W else min(max(W, 2 * width), self.num_pages), dtype=torch.int32)
+            table[:rows, :width] = self._table
             self._table = table
+        free, taken = len(self.free_pages), {}
         for b, n in enumerate(more):
             if n > 0:
-                old = len(self.pages[b])
-                self.pages[b].extend(self.free_pages.pop() for _ in range(n))
-                self._table[b, old:old + n] = torch.tensor(self.pages[b][old:], dtype=torch.int32)
-        self.lengths = grown
+                taken[b] = self.free_pages[free - n:free][::-1]
+                free -= n
+                self._table[b, need[b] - n:need[b]] = torch.tensor(taken[b], dtype=torch.int32)
         starts = [0]
         for n in new:
             starts.append(starts[-1] + n)
@@ -280,6 +281,12 @@ class BlockKVCache(KVCache):
         flat[:B * W].view(B, W).copy_(self._table[:B, :W])
         flat[B * W:] = torch.tensor(grown + starts, dtype=torch.int32)
         flat = flat.to(self.device, non_blocking=True)
+        # nothing can fail any more
+        del self.free_pages[free:]
+        self.pages.extend([] for _ in range(B - len(self.pages)))
+        for b, pages in taken.items():
+            self.pages[b].extend(pages)
+        self.lengths = grown
         return PagedBatch(flat[:B * W].view(B, W), flat[B * W:B * W + B], flat[B * W + B:], max([0, *new]),
                           starts[-1])
 

@@ -1,0 +1,54 @@
+"""The block cache's bookkeeping over many sequences and after refusals, without a GPU."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from avqa_b200 import BlockKVCache
+
+
+def _cache(**kw):
+    return BlockKVCache(**{**dict(num_pages=6, page_size=4, num_heads=2, head_dim=8, device="cpu"), **kw})
+
+
+def _whole(c) -> bool:
+    """Every page of the pool is held once, and the table's rows are the sequences' pages."""
+    held = [p for pages in c.pages for p in pages]
+    return sorted(held + c.free_pages) == list(range(c.num_pages)) and \
+        all(c._table[b, :len(p)].tolist() == p for b, p in enumerate(c.pages))
+
+
+@pytest.mark.parametrize("tokens", [1, 9])
+def test_host_table_stays_small_as_sequences_come_one_by_one(tokens) -> None:
+    c = _cache(num_pages=1000)
+    for n in range(1, 301):
+        batch = c.reserve([0] * (n - 1) + [tokens])
+        need = -(-tokens // 4)
+        assert batch.block_table.shape == (n, need) and batch.block_table.tolist() == c.pages
+        assert c._table.numel() <= 2 * n * 2 * need  # each side at most doubled
+    assert _whole(c)
+
+
+def test_host_table_grows_with_one_sequence_up_to_the_pool() -> None:
+    c = _cache(num_pages=50)
+    for n in range(50):
+        c.reserve([4])
+        assert c._table.shape[0] == 1 and n < c._table.shape[1] <= min(50, 2 * (n + 1))
+    assert c.pages == [list(range(50))] and c.free_pages == [] and _whole(c)
+
+
+@pytest.mark.parametrize("call", ["empty", "zeros"])
+def test_a_step_whose_memory_cannot_be_had_changes_nothing(call, monkeypatch) -> None:
+    c = _cache()
+    c.reserve([5, 1])
+    before = list(c.lengths), [list(p) for p in c.pages], list(c.free_pages)
+
+    def refuse(*args, **kw):
+        raise RuntimeError("out of memory")
+
+    monkeypatch.setattr(torch, call, refuse)
+    with pytest.raises(RuntimeError):
+        c.reserve([4, 1, 2])
+    monkeypatch.undo()
+    assert (c.lengths, c.pages, c.free_pages) == before and _whole(c)
+    assert c.reserve([4, 1, 2]).kv_len.tolist() == [9, 2, 2] and _whole(c)
