@@ -385,14 +385,35 @@ class BlockKVCache(KVCache):
                 "key_pages": self.key_pool[used].clone(), "value_pages": self.value_pool[used].clone()}
 
     def load_state_dict(self, state: dict[str, torch.Tensor]) -> None:
+        """Hold a saved cache's sequences instead; one that does not fit is refused and changes nothing."""
         for name in ("page_size", "num_heads", "head_dim"):
             if name in state and int(state[name]) != getattr(self, name):
                 raise ShapeError(f"{name} mismatch", expected=getattr(self, name), actual=int(state[name]))
-        self.reset()
-        self.reserve(state["lengths"].tolist())
+        lengths = [int(n) for n in state["lengths"].tolist()]
+        if any(n < 0 for n in lengths):
+            raise ShapeError("a saved length is negative", expected="0 or more", actual=lengths)
+        need = sum(-(-n // self.page_size) for n in lengths)
+        if need > self.num_pages:
+            raise NotInitializedError(f"the saved sequences do not fit the paged KV cache ({self.num_pages} pages)",
+                                      {"needed": need, "pages": self.num_pages})
+        want = (need, *self.key_pool.shape[1:])
+        saved = []
+        for name in ("key_pages", "value_pages"):
+            if tuple(state[name].shape) != want:
+                raise ShapeError(f"{name} do not fit the saved lengths", expected=want, actual=tuple(state[name].shape))
+            saved.append(state[name].to(device=self.device, dtype=self.dtype))
+        kept = self.lengths, self.pages, self.free_pages
+        self.lengths, self.pages, self.free_pages = [], [], list(range(self.num_pages - 1, -1, -1))
+        try:
+            self.reserve(lengths)
+        except Exception:  # the cache keeps what it held
+            self.lengths, self.pages, self.free_pages = kept
+            for b, pages in enumerate(self.pages):
+                self._table[b, :len(pages)] = torch.tensor(pages, dtype=torch.int32)
+            raise
+        self.quant_states.clear()
         used = [p for pages in self.pages for p in pages]
-        self.key_pool[used] = state["key_pages"].to(device=self.device, dtype=self.dtype)
-        self.value_pool[used] = state["value_pages"].to(device=self.device, dtype=self.dtype)
+        self.key_pool[used], self.value_pool[used] = saved
 
     @property
     def size(self) -> int:

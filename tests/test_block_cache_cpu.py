@@ -4,7 +4,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from avqa_b200 import BlockKVCache
+from avqa_b200 import BlockKVCache, NotInitializedError, ShapeError
 
 
 def _cache(**kw):
@@ -52,3 +52,38 @@ def test_a_step_whose_memory_cannot_be_had_changes_nothing(call, monkeypatch) ->
     monkeypatch.undo()
     assert (c.lengths, c.pages, c.free_pages) == before and _whole(c)
     assert c.reserve([4, 1, 2]).kv_len.tolist() == [9, 2, 2] and _whole(c)
+
+
+def test_a_state_that_does_not_fit_changes_nothing(monkeypatch) -> None:
+    big = _cache(num_pages=12)
+    big.reserve([30, 9])
+    big.key_pool.copy_(torch.randn_like(big.key_pool))
+    state = big.state_dict()
+    c = _cache()
+    c.reserve([5, 9])
+    c.key_pool.copy_(torch.randn_like(c.key_pool))
+    before = list(c.lengths), [list(p) for p in c.pages], list(c.free_pages), c.key_pool.clone()
+
+    def same() -> bool:
+        return (c.lengths, c.pages, c.free_pages) == before[:3] and torch.equal(c.key_pool, before[3]) and _whole(c)
+
+    with pytest.raises(NotInitializedError):
+        c.load_state_dict(state)
+    assert same()
+    small = _cache()
+    small.reserve([4, 1])
+    for bad in (dict(lengths=torch.tensor([5, 1])), dict(lengths=torch.tensor([8, -3])),
+                dict(key_pages=small.key_pool[:1]), dict(value_pages=small.value_pool[:2, :1])):
+        with pytest.raises(ShapeError):
+            c.load_state_dict({**small.state_dict(), **bad})
+        assert same()
+    real = c.reserve
+    monkeypatch.setattr(c, "reserve", lambda new: (real(new), 1 / 0))  # fails when the lists have changed already
+    with pytest.raises(ZeroDivisionError):
+        c.load_state_dict(small.state_dict())
+    monkeypatch.undo()
+    assert same()
+    c.load_state_dict(small.state_dict())
+    assert c.lengths == [4, 1] and _whole(c)
+    c.load_state_dict(_cache().state_dict())  # an empty one
+    assert c.lengths == [] and len(c.free_pages) == 6
