@@ -205,8 +205,7 @@ def cuda_run_pipeline(m, query: torch.Tensor, key: torch.Tensor, value: torch.Te
     dense = not c.refinement.enabled or c.execution.mode == "reference"
     if isinstance(kv_cache, BlockKVCache):
         if not dense:
-            raise BackendError("the quantized path does not attend over a BlockKVCache; use a PagedKVCache, or "
-                               "execution.mode = 'reference'")
+            refuse_block_cache(kv_cache)
         return block_dense_path(m, q, k, v, mask, kv_cache, chunk_size, positions)
     q, k = rotated(m, q, k, kv_cache, positions)
     m.sync_codebook_device(q)
@@ -408,10 +407,19 @@ def _cache_states(kv_cache) -> dict:
     return states
 
 
+def refuse_block_cache(kv_cache) -> None:
+    """The quantized path extends a state over one common length by raw keys; a
+    :class:`~avqa_b200.cache.BlockKVCache` rotates its keys and its sequences come and go."""
+    if isinstance(kv_cache, BlockKVCache):
+        raise BackendError("the quantized path does not attend over a BlockKVCache; use a PagedKVCache, or "
+                           "execution.mode = 'reference'")
+
+
 def resolve_quantization(m, k: torch.Tensor, v: torch.Tensor, cb: ops.PreparedCodebook,
                          kv_cache=None) -> ops.QuantState:
     """Quantize ``k``/``v`` -- or, with a cache, extend the cache's device state
     (resolve_kv_cache, attention_module.py:350-367, then the quantizer)."""
+    refuse_block_cache(kv_cache)
     if kv_cache is None:
         st = ops.quantize(k, v, cb)
         m.last_keys = k.detach()
@@ -448,4 +456,4 @@ def resolve_quantization(m, k: torch.Tensor, v: torch.Tensor, cb: ops.PreparedCo
 
 
 __all__ = ["AVQAttention", "block_dense_path", "codeword_mask", "cuda_run_pipeline", "global_min_valid", "hvaq_mode",
-           "query_chunks", "resolve_quantization", "rotated"]
+           "query_chunks", "refuse_block_cache", "resolve_quantization", "rotated"]

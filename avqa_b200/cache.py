@@ -287,6 +287,7 @@ class BlockKVCache(KVCache):
         for b, pages in taken.items():
             self.pages[b].extend(pages)
         self.lengths = grown
+        self.quant_states.clear()  # whatever covered the pages does no longer
         return PagedBatch(flat[:B * W].view(B, W), flat[B * W:B * W + B], flat[B * W + B:], max([0, *new]),
                           starts[-1])
 
@@ -297,6 +298,7 @@ class BlockKVCache(KVCache):
         self.free_pages.extend(reversed(self.pages[sequence]))
         self.pages[sequence] = []
         self.lengths[sequence] = 0
+        self.quant_states.clear()
 
     # -- packed steps --------------------------------------------------------------
 
@@ -411,7 +413,6 @@ class BlockKVCache(KVCache):
             for b, pages in enumerate(self.pages):
                 self._table[b, :len(pages)] = torch.tensor(pages, dtype=torch.int32)
             raise
-        self.quant_states.clear()
         used = [p for pages in self.pages for p in pages]
         self.key_pool[used], self.value_pool[used] = saved
 

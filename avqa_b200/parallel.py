@@ -54,7 +54,8 @@ class CudaShardCompute:
 
     def quantize(self, k, v, kv_cache=None):
         """Quantize the keys -- or, with a KV cache of this rank's heads,
-        extend the cache's quantized state by the new tokens (decode)."""
+        extend the cache's quantized state by the new tokens (decode).  A
+        ``BlockKVCache`` is refused."""
         if kv_cache is None:
             st = self.ops.quantize(k, v, self.cb)
         else:

@@ -4,7 +4,8 @@ from __future__ import annotations
 import pytest
 import torch
 
-from avqa_b200 import BlockKVCache, NotInitializedError, ShapeError
+from avqa_b200 import BackendError, BlockKVCache, NotInitializedError, RotaryEmbedding, ShapeError, ops
+from avqa_b200.parallel import CudaShardCompute, ShardedAVQAttention
 
 
 def _cache(**kw):
@@ -87,3 +88,28 @@ def test_a_state_that_does_not_fit_changes_nothing(monkeypatch) -> None:
     assert c.lengths == [4, 1] and _whole(c)
     c.load_state_dict(_cache().state_dict())  # an empty one
     assert c.lengths == [] and len(c.free_pages) == 6
+
+
+@pytest.mark.parametrize("rotary", [None, RotaryEmbedding(8)])
+def test_the_sharded_quantized_path_refuses_the_cache(rotary) -> None:
+    """A quantized state of raw keys would ignore the cache's rotation, and outlive the sequences it covers."""
+    sharded = ShardedAVQAttention.__new__(ShardedAVQAttention)
+    sharded.h0, sharded.h1, sharded.D, sharded.world = 0, 2, 8, 1
+    sharded.compute = CudaShardCompute.__new__(CudaShardCompute)
+    sharded.compute.ops, sharded.compute.cb = ops, object()
+    c = _cache(rotary=rotary)
+    c.reserve([3])
+    x = torch.zeros(1, 1, 16)
+    with pytest.raises(BackendError, match="BlockKVCache"):
+        sharded.forward(x, x, x, kv_cache=c)
+    assert c.lengths == [3]
+
+
+@pytest.mark.parametrize("change", [lambda c: c.reserve([1, 0]), lambda c: c.release(1), lambda c: c.reset(),
+                                    lambda c: c.load_state_dict(c.state_dict())])
+def test_what_changes_the_pages_drops_the_states_over_them(change) -> None:
+    c = _cache()
+    c.reserve([5, 2])
+    c.quant_states["a module's"] = object()
+    change(c)
+    assert c.quant_states == {}
