@@ -447,9 +447,9 @@ avq::PoolStrides pst(const long long* s) { return avq::PoolStrides{s[0], s[1], s
 int paged_sizes(const char* what, int B, int N, int Hkv, int num_pages, int page_size, int table_width) {
   if (B < 0 || N < 0 || Hkv <= 0 || num_pages < 0 || page_size <= 0 || table_width < 0)
     return fail(AVQ_ERR_ARG, "%s: bad sizes", what);
-  if ((long long)page_size * table_width > INT_MAX)
-    return fail(AVQ_ERR_ARG, "%s: page_size * table width %lld exceeds INT_MAX", what,
-                (long long)page_size * table_width);
+  if ((long long)page_size * table_width > avq::kMaxRoom)
+    return fail(AVQ_ERR_ARG, "%s: page_size * table width %lld exceeds %lld", what,
+                (long long)page_size * table_width, avq::kMaxRoom);
   return AVQ_OK;
 }
 

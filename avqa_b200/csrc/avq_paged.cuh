@@ -35,6 +35,9 @@ inline bool allow_smem(const void* kernel, size_t bytes, std::atomic<unsigned lo
 
 constexpr int kFaultTables = 2;  // bit 1 of the device fault record (bit 0: an abandoned wait)
 constexpr int kSms = 148;
+// Tokens that a table's row may hold.  The kernels count keys in 32 bits and step past a sequence's last key by up to
+// five steps of 128 keys (loads that are asked for ahead, the rest of a tile), which must not wrap.
+constexpr long long kMaxRoom = 0x7fffffffll - 65536;
 
 struct Strides2 {  // element strides of a packed [N, H, D] operand (token, head)
   long long t, h;
@@ -150,7 +153,7 @@ __device__ __forceinline__ SeqRange load_seq(const int* q_start, const int* kv_l
   s.q0 = sound ? a : 0;
   s.n = sound ? e - a : 0;
   s.len = len < 0 ? 0 : (len > room ? (int)room : len);
-  s.pos0 = len - s.n;
+  s.pos0 = (int)min((long long)max(len, 0), kMaxRoom) - s.n;
   *bad = *bad || !sound || len < 0 || len > room;
   return s;
 }

@@ -284,9 +284,9 @@ int avq_rotary(int dtype, const void* q, const long long* q_strides, int Hq, con
  * its token count WITH them, so new token i of n has the position
  * p = kv_len[b] - n + i.  Position p lives in slot p % page_size of page
  * block_table[b * table_stride + p / page_size] (device int32, table_width
- * entries a row).  Pools are [num_pages, Hkv, page_size, D] by element strides
- * {page, head, slot}, packed operands [N, H, D] by {token, head}, unit stride
- * along D.
+ * entries a row, page_size * table_width at most 2^31 - 65537).  Pools are
+ * [num_pages, Hkv, page_size, D] by element strides {page, head, slot}, packed
+ * operands [N, H, D] by {token, head}, unit stride along D.
  *
  * Writes k rotated (as avq_rotary; rotary_dim 0: unchanged) and v to their
  * slots, and with Hq > 0 also q rotated to q_out (which may be q).  positions:

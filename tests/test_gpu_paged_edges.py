@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from avqa_b200 import ops
-from paged_reference import assert_within, attention64
+from paged_reference import DTYPES, assert_within, attention64, half
 from test_gpu_paged import Batch, fault
 
 pytestmark = pytest.mark.gpu
@@ -21,3 +21,24 @@ def test_many_cut_pairs_give_the_same_bits_again(dt, D) -> None:
     for _ in range(30):
         assert torch.equal(ops.paged_attention(b.q, *b.lists), first)
     assert fault() == 0
+
+
+@pytest.mark.parametrize("dt,D", [("bf16", 64), ("bf16", 128), ("f16", 72), ("f32", 64)])
+@pytest.mark.parametrize("new", [1, 20])
+@pytest.mark.parametrize("less", [0, 1, 127, 65536])
+def test_the_longest_sequence_that_a_table_may_hold(dt, D, new, less) -> None:
+    """A window at the end of 2^31 - 65537 tokens, which all lie on one page whose slots are the same row."""
+    room = 2 ** 31 - 65537
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q = torch.randn(new, 4, D, generator=g, device="cuda").to(DTYPES[dt])
+    k, v = (torch.randn(1, 2, 1, D, generator=g, device="cuda").to(DTYPES[dt]) for _ in range(2))
+    lists = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([[0]], [room - less], [0, new])]
+    pools = [x.expand(-1, -1, room, -1) for x in (k, v)]
+    got = ops.paged_attention(q, *pools, *lists, window=300)
+    # every key scores the same: the values' own row, which each sum's roundings reach
+    want = v[0, :, 0].double().repeat_interleave(2, 0).expand(new, -1, -1)
+    assert_within(got, want, want.abs() * 4 * half(DTYPES[dt]) + want.abs() * 400 * 2.0 ** -24, "one row everywhere")
+    assert fault() == 0
+    lists[1] -= room  # no keys at all, and fewer than none
+    assert (ops.paged_attention(q, *pools, *lists, window=300) == 0).all()
+    assert fault() == (2 if less else 0)
