@@ -61,7 +61,8 @@ struct __align__(16) PieceWork {
   int head, seq, row0, rows;      // key head, sequence; first row in it, rows from there on
   int key0, tiles, pieces, slot;  // first key, key tiles; pieces of its pair, its slot of partial sums
   int q0, pos0, len, end;         // the sequence's first token and its position; its keys, those that the rows see
-  int pair, unused[3];
+  int pair, first;                // first key that any row sees, in the tile of the pair's first key
+  int unused[2];
 };
 
 // The plan in the workspace: a header; the pieces; the items; the (key head, item) pairs, head by head.
@@ -265,6 +266,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PagedAttnArgs 
       w.pos0 = s.pos0;
       w.len = s.len;
       w.end = k.y;
+      w.first = window_start(a, s.pos0 + w.row0 / G);
       w.pair = c;
       const int all = p.tiles[i];
       for (int x = 0, t = 0; x < n; ++x) {  // equal shares of the pair's tiles
@@ -487,7 +489,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
       int ring = 0, tails = 0;  // ring tiles, tiles with a tail so far
       for (int turn = 0; take(turn); ++turn) {
         const int head = w.head, rows = w.rows, nt = rows > TM ? 2 : 1, row0 = w.row0, tiles = w.tiles, key0 = w.key0;
-        const int end = w.end;
+        const int end = w.end, first = w.first;
         bool bad = false;
         constexpr int CPR = D / 8, RPI = 32 / CPR;               // 16-byte chunks of a row, rows of a warp's copy
         constexpr int NI = (TK / RPI + kLoaders - 1) / kLoaders;  // copies of a tile by one warp
@@ -525,17 +527,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             const int4 pos = is_v ? maps.vpos : maps.kpos;
             const int R = min(a.page_size, TK), boxes = TK / R * (D / 64);
             const int row = lane / (D / 64) * R, half = lane % (D / 64);
+            // Whether any row sees a key of this lane's box.  (The first tile begins before a window does, perhaps on
+            // pages that are not the sequence's any more: they are not looked up, and the box is zeros.)
+            auto seen = [&](int key) { return lane < boxes && key < end && key + R > first; };
             // the table entry of this lane's box, read one tile ahead
             auto look_up = [&](int k0) {
               const int key = k0 + row;
-              return lane < boxes && key < end ? row_table[key / a.page_size] : -1;
+              return seen(key) ? row_table[key / a.page_size] : -1;
             };
             int ahead = look_up(key0), j = 0;
             for (; ok && j < tiles; ++j) {
               const int i = ring + 2 * j + lw, slot = i % NR, use = i / NR, k0 = key0 + j * TK;
               const int key = k0 + row, in_page = key % a.page_size;
               int page = a.num_pages;  // outside the map: reads as zeros
-              if (lane < boxes && key < end) {
+              if (seen(key)) {
                 if (ahead >= 0 && ahead < a.num_pages) page = ahead;
                 else bad = true;
               }
@@ -594,7 +599,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
                 const int q = hf * 32 + lane, r = (lw + kLoaders * (q / RPI)) * RPI + q % RPI;
                 const int key = key0 + (i >> 1) * TK + r;
                 off[0][hf] = off[1][hf] = -1;
-                if (r < TK && key < end) {
+                if (r < TK && key >= first && key < end) {
                   const int page = row_table[key / a.page_size], s = key % a.page_size;
                   if (page >= 0 && page < a.num_pages) {
                     off[0][hf] = (long long)page * a.kps.p + (long long)s * a.kps.s;

@@ -42,3 +42,27 @@ def test_the_longest_sequence_that_a_table_may_hold(dt, D, new, less) -> None:
     lists[1] -= room  # no keys at all, and fewer than none
     assert (ops.paged_attention(q, *pools, *lists, window=300) == 0).all()
     assert fault() == (2 if less else 0)
+
+
+@pytest.mark.parametrize("dt,D", [("bf16", 64), ("f16", 128), ("bf16", 72), ("f32", 64)])
+@pytest.mark.parametrize("page", [8, 16, 24, 100, 128, 384])
+@pytest.mark.parametrize("new,window", [([1, 2], 50), ([40, 300], 50), ([40, 300], 700), ([300], 1)])
+def test_pages_behind_the_window_are_not_looked_up(dt, D, page, new, window) -> None:
+    """Pages whose keys no token of the sequence sees may have been given back: no fault, and the same bits."""
+    lens = [1200 + n for n in new]
+    b = Batch(dt, 4, 2, D, page, new, lens)
+    want = b.check(window=window)
+    gone = [(n - k + 1 - window) // page for n, k in zip(lens, new)]  # pages before the first token's first key
+    assert all(n > 0 for n in gone)
+    used = set(b.block_table.flatten().tolist())
+    spare = next(p for p in range(b.key_pool.shape[0]) if p not in used)
+    assert torch.isnan(b.key_pool[spare].float()).all()
+    for other in (-1, b.key_pool.shape[0], spare):  # none, none, one that holds NaN
+        for row, n in enumerate(gone):
+            b.block_table[row, :n] = other
+        assert torch.equal(ops.paged_attention(b.q, *b.lists, window=window), want)
+        assert fault() == 0
+    row = len(new) - 1
+    b.block_table[row, gone[row]] = -1  # a page that is seen
+    ops.paged_attention(b.q, *b.lists, window=window)
+    assert fault() == 2
