@@ -754,11 +754,20 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_mma_kernel(const Paged
       }
     }
   }
-  // rows that do not all see the same keys, or fp32's parts, and a sum that is not finite: each row again on its own
+  // rows that do not all see the same keys, or fp32's parts, and a sum that is not finite: such a row on its own
   if ((DT == DT_F32 || every_lo > lo || every_hi < hi) && __syncthreads_or(odd)) {
     for (int r = warp; r < nrow; r += kWarps) {
+      bool spoiled = false;
+      for (int d = lane; d < DP; d += 32) {
+        float x = so[r * DP + d];
+        if (!CL)
+          for (int w = 1; w < kWarps; ++w) x += so[(w * RB + r) * DP + d];
+        spoiled = spoiled || !isfinite(x);
+      }
+      if (!__any_sync(0xffffffffu, spoiled)) continue;
       const int tok = p.seq.q0 + (row0 + r) / G, h = p.head * G + (row0 + r) % G;
       const int2 v = visible(a, p.seq.pos0 + (row0 + r) / G, p.seq.len);
+      if (DT != DT_F32 && !hidden_odd<DT, DP>(a, row_table, p.head, lo, hi, v)) continue;
       float x[DP / 32], M, l;
       const T* q_row = static_cast<const T*>(a.q) + (long long)tok * a.qs.t + (long long)h * a.qs.h;
       row_alone<DT, DP>(a, row_table, p.head, q_row, max(v.x, p.lo), min(v.y, p.hi), x, &M, &l);

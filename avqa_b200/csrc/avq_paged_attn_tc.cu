@@ -76,11 +76,11 @@ struct Plan {
   int* sum;          // key tiles of the items before
   int* split;        // [pairs] pieces
   int* slot;         // [pairs] first slot of partial sums, where there are several pieces
-  int* odd;          // [pairs] raised where a row's sums are not finite and keys that it does not see may be why
+  unsigned* odd;     // [pairs][8] a bit for each row whose sums are not finite where keys that it does not see may be why
 };
 
 __host__ __device__ inline long long plan_ints(long long B, long long items, long long Hkv) {
-  return 8 + (items * Hkv + kMaxSlots) * (long long)(sizeof(PieceWork) / 4) + (B + 1) + 4 * items + 3 * items * Hkv;
+  return 8 + (items * Hkv + kMaxSlots) * (long long)(sizeof(PieceWork) / 4) + (B + 1) + 4 * items + (2 + kItemRows / 32) * items * Hkv;
 }
 __host__ __device__ inline Plan plan_at(int* p, long long B, long long items, long long Hkv) {
   Plan q;
@@ -93,7 +93,7 @@ __host__ __device__ inline Plan plan_at(int* p, long long B, long long items, lo
   q.sum = q.tiles + items;
   q.split = q.sum + items;
   q.slot = q.split + items * Hkv;
-  q.odd = q.slot + items * Hkv;
+  q.odd = reinterpret_cast<unsigned*>(q.slot + items * Hkv);
   return q;
 }
 
@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PagedAttnArgs 
       }
       p.split[c] = n;
       p.slot[c] = slot;
-      p.odd[c] = 0;
+      for (int x = 0; x < kItemRows / 32; ++x) p.odd[(long long)c * (kItemRows / 32) + x] = 0;
     }
     pieces += total;
     slots += total_slots;
@@ -891,8 +891,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
             }
           }
         }
-        // (the joining kernel then takes the pair's rows one by one)
-        if (zero != 0.f && r < rows && (first > key0 || last < min(w.end, key0 + tiles * TK))) plan.odd[w.pair] = 1;
+        // (the joining kernel then looks at the row; scores that are not finite make NaN of all of it, which is right)
+        if (zero != 0.f && l == l && r < rows && (first > key0 || last < min(w.end, key0 + tiles * TK)))
+          atomicOr(&plan.odd[(long long)w.pair * (kItemRows / 32) + (r >> 5)], 1u << (r & 31));
         tc::tc_before_sync();
       }
       s_count += tiles;
@@ -905,11 +906,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
   if (tid == 0 && *abort) atomicOr(&g_fault_paged_tc, 1);
 }
 
-// Joins a pair's pieces: a block per (pair, 32 rows), in the order of the keys.
-constexpr int kJoinRows = 32;
+// Joins a pair's pieces: a block per (pair, 32 rows), in the order of the keys.  Rows that hidden values have spoiled
+// are formed again.
+constexpr int kJoinRows = 32;  // (a word of Plan::odd)
 
 template <int DT, int D>
-__global__ void __launch_bounds__(256) combine_tc_kernel(const PagedAttnArgs a, int max_items,
+__global__ void __launch_bounds__(256, 4) combine_tc_kernel(const PagedAttnArgs a, int max_items,
                                                          int* __restrict__ plan_ws,
                                                          const float* __restrict__ partials, int out_wide) {
   using T = typename Storage<DT>::T;
@@ -918,7 +920,7 @@ __global__ void __launch_bounds__(256) combine_tc_kernel(const PagedAttnArgs a, 
   const int items = plan.head[2], pair = blockIdx.x, G = a.H / a.Hkv;
   if (pair >= items * a.Hkv) return;
   const int np = plan.split[pair], head = pair / items, item = pair - head * items;
-  const bool odd = plan.odd[pair] != 0;
+  const unsigned odd = plan.odd[(long long)pair * (kItemRows / 32) + blockIdx.y];
   if (np <= 1 && !odd) return;
   bool bad = false;
   const SeqRange seq = load_seq(a.q_start, a.kv_len, plan.seq[item], a.N, (long long)a.W * a.page_size, &bad);
@@ -929,19 +931,30 @@ __global__ void __launch_bounds__(256) combine_tc_kernel(const PagedAttnArgs a, 
   __shared__ float weight[kMaxPieces][kJoinRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r0 = blockIdx.y * kJoinRows;
   if (r0 >= rows) return;
+  __shared__ unsigned s_alone;  // rows that are formed alone
   if (odd) {
+    if (threadIdx.x == 0) s_alone = 0;
+    __syncthreads();
+    const int* row_table = a.table + (long long)plan.seq[item] * a.table_stride;
+    const int2 keys = item_keys(a, seq, plan.part[item], G);
+    // (keys before the first one's page were not looked up)
+    const int lo = max(keys.x, window_start(a, seq.pos0 + row0 / G) / a.page_size * a.page_size);
     for (int r = r0 + warp; r < min(rows, r0 + kJoinRows); r += 8) {
+      if (!(odd >> (r - r0) & 1)) continue;
       const int tok = seq.q0 + (row0 + r) / G, h = head * G + (row0 + r) % G;
       const int2 v = visible(a, seq.pos0 + (row0 + r) / G, seq.len);
+      if (!hidden_odd<DT, D>(a, row_table, head, lo, keys.y, v)) continue;
       float x[D / 32], m, l;
       const T* q_row = static_cast<const T*>(a.q) + (long long)tok * a.qs.t + (long long)h * a.qs.h;
-      row_alone<DT, D>(a, a.table + (long long)plan.seq[item] * a.table_stride, head, q_row, v.x, v.y, x, &m, &l);
+      row_alone<DT, D>(a, row_table, head, q_row, v.x, v.y, x, &m, &l);
 #pragma unroll
       for (int i = 0; i < D / 32; ++i)
         static_cast<T*>(a.out)[(long long)tok * a.os.t + (long long)h * a.os.h + i * 32 + lane] =
             from_f<DT>(v.y > v.x ? x[i] / l : 0.f);
+      if (lane == 0) atomicOr(&s_alone, 1u << (r - r0));
     }
-    return;
+    __syncthreads();
+    if (np <= 1) return;
   }
 #pragma unroll
   for (int x = 0; x < kJoinRows / 8; ++x) {
@@ -965,7 +978,7 @@ __global__ void __launch_bounds__(256) combine_tc_kernel(const PagedAttnArgs a, 
   }
   __syncthreads();
   const int r = r0 + lane;
-  if (r >= rows) return;
+  if (r >= rows || (odd && s_alone >> lane & 1)) return;
   const int2 seen = visible(a, seq.pos0 + (row0 + r) / G, seq.len);
   constexpr int NC = D / 4 / 8;  // a thread's groups of four columns
   float4 x[NC];

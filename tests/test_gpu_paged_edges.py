@@ -66,3 +66,49 @@ def test_pages_behind_the_window_are_not_looked_up(dt, D, page, new, window) -> 
     b.block_table[row, gone[row]] = -1  # a page that is seen
     ops.paged_attention(b.q, *b.lists, window=window)
     assert fault() == 2
+
+
+@pytest.mark.parametrize("dt,D,page", [("bf16", 128, 16), ("f16", 64, 24), ("f16", 72, 16), ("bf16", 256, 16)])
+@pytest.mark.parametrize("new,length", [(3, 40), (60, 2000), (200, 200), (200, 6000)])
+def test_values_that_are_not_finite_leave_the_rest_its_bits(dt, D, page, new, length) -> None:
+    """A value that is not finite, and that every row sees, changes its own column; the rest keeps the bits that it has
+    without: no row is formed again another way.  A key or a query changes the rows that see it; the others stay within
+    the bounds of fp64 (the tensor-core kernel's rows of a warp take over a new maximum together, so that the bits of
+    a row hang on its neighbours' scores)."""
+    b = Batch(dt, 4, 2, D, page, [new, 1], [length, 30])
+    clean = b.check()
+    want, bound, _ = attention64(b.q, *b.lists)
+
+    def run():
+        got = ops.paged_attention(b.q, *b.lists)
+        return got, (got.view(torch.int16) == clean.view(torch.int16))
+
+    at = (length - new) // 2  # a token that every row of the first sequence sees
+    slot = int(b.block_table[0, at // page]), 1, at % page
+    for value in (float("nan"), float("inf")):  # a value, in one column of the second key head
+        kept = b.value_pool[slot].clone()
+        b.value_pool[slot][7] = value
+        got, same = run()
+        b.value_pool[slot] = kept
+        assert not torch.isfinite(got[:new, 2:, 7].float()).any()
+        same[:new, 2:, 7] = True
+        assert same.all()
+    at = length - new + new // 2  # a token that the later rows see
+    slot = int(b.block_table[0, at // page]), 1, at % page
+    kept = b.key_pool[slot].clone()
+    b.key_pool[slot][7] = float("nan")
+    got = run()[0]
+    b.key_pool[slot] = kept
+    assert torch.isnan(got[new // 2:new, 2:].float()).all()
+    seen = torch.zeros(b.N, 4, dtype=torch.bool, device="cuda")
+    seen[new // 2:new, 2:] = True
+    assert_within(got[~seen], want[~seen], bound[~seen], "a key")
+    kept = b.q[new // 2, 3].clone()
+    b.q[new // 2, 3, 5] = float("nan")
+    got = run()[0]
+    b.q[new // 2, 3] = kept
+    assert torch.isnan(got[new // 2, 3].float()).all()
+    seen.fill_(False)
+    seen[new // 2, 3] = True
+    assert_within(got[~seen], want[~seen], bound[~seen], "a query")
+    assert run()[1].all()
