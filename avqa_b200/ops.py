@@ -437,6 +437,41 @@ def _packed(t: torch.Tensor, name: str, heads: int, tokens: int, dim: int) -> ct
     return _lib.longs(st[0], st[1])
 
 
+@functools.lru_cache(maxsize=4096)
+def _rows_meet(delta: int, width: int, a: tuple, b: tuple) -> bool:
+    """Whether any row of ``b`` shares memory with a row of ``a``; each is (tokens, heads, bytes from
+    token to token, from head to head), with rows of ``width`` bytes, and b begins ``delta`` bytes
+    behind a."""
+    (Na, Ha, ta, ha), (Nb, Hb, tb, hb) = a, b
+    if (ta, ha) == (tb, hb):  # as rows of one grid
+        for dh in range(1 - Ha, Hb):
+            rest = -(delta + dh * ha)  # what dt tokens have to make up for
+            for dt in (rest // ta, rest // ta + 1) if ta else (0,):
+                if abs(rest - min(max(dt, 1 - Na), Nb - 1) * ta) < width:
+                    return True
+        return False
+    if Na * Ha + Nb * Hb > 1 << 22:
+        return True  # (grids of different strides, woven into each other: not looked into)
+    mine, theirs = (((torch.arange(N) * t)[:, None] + torch.arange(H) * h).flatten().sort()[0]
+                    for N, H, t, h in (a, b))
+    theirs = theirs + delta
+    at = torch.searchsorted(mine, theirs)
+    gap = torch.minimum((mine[at.clamp(max=len(mine) - 1)] - theirs).abs(), (mine[(at - 1).clamp(min=0)] - theirs).abs())
+    return bool((gap < width).any())
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two packed ``[tokens, heads, dim]`` operands of one dtype and dim share memory."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (Na, Ha, D), (Nb, Hb, _), n = a.shape, b.shape, a.element_size()
+    (ta, ha, _), (tb, hb, _) = a.stride(), b.stride()
+    delta = b.data_ptr() - a.data_ptr()
+    if delta >= ((Na - 1) * ta + (Ha - 1) * ha + D) * n or -delta >= ((Nb - 1) * tb + (Hb - 1) * hb + D) * n:
+        return False
+    return _rows_meet(delta, D * n, (Na, Ha, ta * n, ha * n), (Nb, Hb, tb * n, hb * n))
+
+
 def _packed_shape(t: torch.Tensor, name: str) -> torch.Size:
     if t.dim() != 3:
         raise ShapeError(f"{name} must be packed [tokens, heads, head_dim]", expected="[N, H, D]",
@@ -488,7 +523,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, key_pool: torch.Tensor, value
     the keys rotated on the way when ``rotary`` (a
     :class:`~avqa_b200.rotary.RotaryEmbedding`) is given; ``q [N, H, D]`` is
     rotated in the same launch and returned (in ``q_out`` if given, which may
-    be ``q``).
+    be ``q`` but must not overlap it, ``k`` or ``v`` otherwise).
 
     ``key_pool``/``value_pool`` ``[pages, Hkv, page_size, D]`` (any page, head
     and slot strides); ``block_table [B, W]``, ``kv_len [B]`` (with the new
@@ -513,9 +548,13 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, key_pool: torch.Tensor, value
         qs = _packed(q, "query", H, N, D)
         if q_out is None:
             q_out = torch.empty_like(q)
+            qos = _packed(q_out, "q_out", H, N, D)
         else:
             _same("q_out", q_out, at, dt)
-        qos = _packed(q_out, "q_out", H, N, D)
+            qos = _packed(q_out, "q_out", H, N, D)
+            itself = q_out.data_ptr() == q.data_ptr() and q_out.stride() == q.stride()
+            if (not itself and _overlap(q, q_out)) or _overlap(k, q_out) or _overlap(v, q_out):
+                raise BackendError("q_out must be q or share no memory with q, k and v")
         qp, qop = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise BackendError("q_out needs q")
@@ -567,7 +606,7 @@ def paged_attention(q: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.T
     ``h // (H // Hkv)``).  A token that sees no key gets zeros; rows behind
     ``q_start[B]`` are left as they are in ``out``.  ``max_q_len``: the most new
     tokens of a sequence, if known; it only steers the choice of kernels.
-    ``out`` must not overlap ``q``.
+    ``out`` must not overlap ``q``, also as another view of its memory.
     Probabilities are rounded to the dtype for the product with the values
     (bf16, fp16), all sums are fp32.  Serving only: no gradient is recorded."""
     lib = _lib.load()
@@ -584,9 +623,9 @@ def paged_attention(q: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.T
         out = q.new_empty((N, H, D))
     else:
         _same("out", out, at, dt)
-        if N and out.data_ptr() == q.data_ptr():
-            raise BackendError("out must not be the query's memory")
         os = _packed(out, "out", H, N, D)
+        if _overlap(q, out):
+            raise BackendError("out must not share memory with the query")
     if scale is None:
         scale = D ** -0.5 if D else 1.0
     code = _lib.dtype_code(dt)

@@ -289,7 +289,8 @@ int avq_rotary(int dtype, const void* q, const long long* q_strides, int Hq, con
  * operands [N, H, D] by {token, head}, unit stride along D.
  *
  * Writes k rotated (as avq_rotary; rotary_dim 0: unchanged) and v to their
- * slots, and with Hq > 0 also q rotated to q_out (which may be q).  positions:
+ * slots, and with Hq > 0 also q rotated to q_out (which may be q, but must not
+ * overlap q, k or v otherwise).  positions:
  * NULL for p on every axis, or device integers with strides {axis, token}.
  * Tokens behind q_start[B] are left alone.  A token whose position is negative
  * or beyond the table's row, or whose page is not in the pool, is not written;

@@ -5,7 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from avqa_b200 import ops
+from avqa_b200 import BackendError, RotaryEmbedding, ops
 from paged_reference import DTYPES, assert_within, attention64, half
 from test_gpu_paged import Batch, fault
 
@@ -112,3 +112,27 @@ def test_values_that_are_not_finite_leave_the_rest_its_bits(dt, D, page, new, le
     seen[new // 2, 3] = True
     assert_within(got[~seen], want[~seen], bound[~seen], "a query")
     assert run()[1].all()
+
+
+def test_outputs_in_the_memory_of_inputs_are_refused() -> None:
+    b = Batch("bf16", 4, 2, 64, 16, [3, 2], [20, 30])
+    want = ops.paged_attention(b.q, *b.lists)
+    room = torch.zeros(b.N * 2 + 1, 8, 64, device="cuda", dtype=b.dt)
+    q = room[:b.N, :4]
+    q.copy_(b.q)
+    for out in (q, room[1:b.N + 1, :4], room[:b.N, 3:7], room.view(-1, 64)[2:2 + 4 * b.N].view(b.N, 4, 64)):
+        with pytest.raises(BackendError):
+            ops.paged_attention(q, *b.lists, out=out)
+    out = room[:b.N, 4:]  # beside the query's heads, in the same rows
+    assert torch.equal(ops.paged_attention(q, *b.lists, out=out), want) and torch.equal(q, b.q)
+    rot = RotaryEmbedding(64)
+    k, v = room[b.N:2 * b.N, :2], room[b.N:2 * b.N, 2:4]
+    k.copy_(b.k)
+    v.copy_(b.v)
+    for out in (room[1:b.N + 1, :4], room[:b.N, 2:6], room[b.N:2 * b.N, 1:5], room[b.N + 1:2 * b.N + 1, 3:7]):
+        with pytest.raises(BackendError):
+            ops.paged_append(k, v, *b.lists, q=q, rotary=rot, q_out=out)
+    want = ops.paged_append(b.k, b.v, *b.lists, q=b.q, rotary=rot)
+    assert torch.equal(ops.paged_append(k, v, *b.lists, q=q, rotary=rot, q_out=room[:b.N, 4:]), want)
+    assert ops.paged_append(k, v, *b.lists, q=q, rotary=rot, q_out=q) is q
+    assert torch.equal(q, want) and torch.equal(k, b.k) and torch.equal(v, b.v)
