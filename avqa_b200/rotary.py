@@ -15,6 +15,7 @@ import ctypes
 from collections.abc import Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from avqa_b200 import ops
 from avqa_b200.exceptions import ConfigurationError, ShapeError
@@ -72,13 +73,15 @@ class RotaryEmbedding:
         batch entry and axis, with one axis ``[B, T]``, with several
         ``[axes, T]`` or ``[axes, B, T]``; without it token t is at
         ``offset + t``.  Returns the rotated tensor, or the pair with ``k``.
-        Differentiable in ``q`` and ``k``: the gradient is the rotation by the
-        negative angle.
+        Differentiable in ``q`` and ``k``, in reverse and forward mode and any
+        number of times: the gradient is the rotation by the negative angle.
+        (``torch.func`` transforms are refused by torch: the kernel has no
+        batching rule.)
         """
         if q.dim() != 4 or (k is not None and k.dim() != 4):
             raise ShapeError("query and key must be [B, H, T, head_dim]", expected=4,
                              actual=(tuple(q.shape), None if k is None else tuple(k.shape)))
-        if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        if _recorded(q) or (k is not None and _recorded(k)):
             out = _Rotate.apply(self, positions, offset, False, q, k)
             return out[0] if k is None else out
         q_out, k_out = ops.rotary(self, q, k, positions, offset)
@@ -89,6 +92,13 @@ class RotaryEmbedding:
                 f"sections={self.sections}, interleaved={self.interleaved})")
 
 
+def _recorded(x: torch.Tensor) -> bool:
+    """Whether a derivative through ``x`` is wanted, in reverse or forward mode."""
+    if x.requires_grad and torch.is_grad_enabled():
+        return True
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None
+
+
 class _Rotate(torch.autograd.Function):
     """The rotation and its transpose; both are the same kernel, so gradients of gradients work too."""
 
@@ -97,30 +107,41 @@ class _Rotate(torch.autograd.Function):
         ctx.args = (rotary, offset, reverse)
         if positions is not None:
             ctx.save_for_backward(positions)
+            ctx.save_for_forward(positions)
         ctx.set_materialize_grads(False)
+        if forward_ad._current_level >= 0:
+            ctx.shapes = [None if x is None else (x.shape, x.dtype, x.device) for x in (q, k)]
         return ops.rotary(rotary, q, k, positions, offset, reverse)
 
     @staticmethod
-    def backward(ctx, gq, gk):
-        rotary, offset, reverse = ctx.args
+    def _rotate(ctx, reverse, q, k):
+        """The rotation of ``q`` and ``k``, either of which may be ``None``."""
+        rotary, offset, _ = ctx.args
         saved = ctx.saved_tensors
         positions = saved[0] if saved else None
-        if not ctx.needs_input_grad[4]:
-            gq = None
-        if not ctx.needs_input_grad[5]:
-            gk = None
         # a gradient expanded along D (a sum's, say) has no unit stride there
-        have = [g if g.stride(-1) == 1 or g.shape[-1] == 1 else g.contiguous() for g in (gq, gk) if g is not None]
+        have = [x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous() for x in (q, k) if x is not None]
         if not have:
-            return None, None, None, None, None, None
+            return None, None
         second = have[1] if len(have) > 1 else None
-        if torch.is_grad_enabled():  # a gradient of this gradient is wanted
-            out = _Rotate.apply(rotary, positions, offset, not reverse, have[0], second)
+        if any(_recorded(x) for x in have):  # a derivative of this one is wanted
+            out = _Rotate.apply(rotary, positions, offset, reverse, have[0], second)
         else:
-            out = ops.rotary(rotary, have[0], second, positions, offset, not reverse)
-        if gq is None:
-            return None, None, None, None, None, out[0]
-        return None, None, None, None, out[0], out[1]
+            out = ops.rotary(rotary, have[0], second, positions, offset, reverse)
+        return (None, out[0]) if q is None else out
+
+    @staticmethod
+    def jvp(ctx, *tangents):
+        out = _Rotate._rotate(ctx, ctx.args[2], tangents[4], tangents[5])
+        # (an output whose input has no tangent still needs one)
+        return tuple(torch.zeros(like[0], dtype=like[1], device=like[2]) if t is None and like is not None else t
+                     for t, like in zip(out, ctx.shapes))
+
+    @staticmethod
+    def backward(ctx, gq, gk):
+        gq, gk = _Rotate._rotate(ctx, not ctx.args[2], gq if ctx.needs_input_grad[4] else None,
+                                 gk if ctx.needs_input_grad[5] else None)
+        return None, None, None, None, gq, gk
 
 
 __all__ = ["RotaryEmbedding"]
