@@ -318,6 +318,9 @@ class BlockKVCache(KVCache):
             raise ShapeError("the new tokens do not add up to the packed ones", expected=sum(new),
                              actual=key.shape[0])
         self._check(key, value)
+        if query.dim() != 3 or query.shape[0] != key.shape[0] or query.shape[2] != self.head_dim:
+            raise ShapeError("the queries must be the new tokens' own", expected=(key.shape[0], "Hq", self.head_dim),
+                             actual=tuple(query.shape))
         rotary = self.rotary if rotary is None else rotary
         with self._step(new) as batch:
             lists = (self.key_pool, self.value_pool, batch.block_table, batch.kv_len, batch.q_start)

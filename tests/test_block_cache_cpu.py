@@ -113,3 +113,14 @@ def test_what_changes_the_pages_drops_the_states_over_them(change) -> None:
     c.quant_states["a module's"] = object()
     change(c)
     assert c.quant_states == {}
+
+
+@pytest.mark.parametrize("shape", [(1, 4, 8), (3, 4, 8), (0, 4, 8), (2, 4, 16), (2, 8), (1, 2, 4, 8)])
+def test_queries_that_are_not_the_new_tokens_are_refused(shape) -> None:
+    """Without a rotation nothing else compared them with the step's tokens: missing rows were never written."""
+    c = _cache()
+    c.reserve([5])
+    x = torch.zeros(2, 2, 8)
+    with pytest.raises(ShapeError):
+        c.attend(torch.zeros(shape), x, x, [1, 1])
+    assert c.lengths == [5] and _whole(c)
