@@ -60,9 +60,7 @@ class RotaryEmbedding:
         self.head_dim, self.rotary_dim, self.base = head_dim, rotary_dim, float(base)
         self.sections, self.interleaved, self.frequencies = sections, bool(interleaved), frequencies
         self.num_axes = len(sections)
-        self.c_frequencies = (ctypes.c_double * pairs)(*frequencies)
-        axes = [a for a, n in enumerate(sections) for _ in range(n)]
-        self.c_axes = (ctypes.c_int * pairs)(*axes) if self.num_axes > 1 else None
+        self._c_arrays()
 
     def __call__(self, q: torch.Tensor, k: torch.Tensor | None = None, positions: torch.Tensor | None = None,
                  offset: int = 0):
@@ -86,6 +84,20 @@ class RotaryEmbedding:
             return out[0] if k is None else out
         q_out, k_out = ops.rotary(self, q, k, positions, offset)
         return q_out if k is None else (q_out, k_out)
+
+    def _c_arrays(self) -> None:
+        pairs = self.rotary_dim // 2
+        self.c_frequencies = (ctypes.c_double * pairs)(*self.frequencies)
+        axes = [a for a, n in enumerate(self.sections) for _ in range(n)]
+        self.c_axes = (ctypes.c_int * pairs)(*axes) if self.num_axes > 1 else None
+
+    def __getstate__(self) -> dict:
+        # the C arrays cannot be pickled, and a module that holds an embedding has to be
+        return {name: x for name, x in self.__dict__.items() if name not in ("c_frequencies", "c_axes")}
+
+    def __setstate__(self, state: dict) -> None:
+        self.__dict__.update(state)
+        self._c_arrays()
 
     def __repr__(self) -> str:
         return (f"RotaryEmbedding(head_dim={self.head_dim}, rotary_dim={self.rotary_dim}, base={self.base}, "
