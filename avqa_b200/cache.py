@@ -355,9 +355,11 @@ class BlockKVCache(KVCache):
     def append(self, key: torch.Tensor, value: torch.Tensor) -> None:
         """Append ``[B, H, T, D]``, T tokens to every sequence."""
         from avqa_b200 import ops
-        B, _, T, D = key.shape
-        k, v = (x.to(device=self.device, dtype=self.dtype).transpose(1, 2).reshape(B * T, -1, D) for x in (key, value))
-        self._check(k, v)
+        if key.dim() != 4 or key.shape != value.shape or (key.shape[1], key.shape[3]) != (self.num_heads, self.head_dim):
+            raise ShapeError(f"key/value shape mismatch: key={tuple(key.shape)}, value={tuple(value.shape)}",
+                             expected=("B", self.num_heads, "T", self.head_dim), actual=tuple(key.shape))
+        B, H, T, D = key.shape
+        k, v = (x.to(device=self.device, dtype=self.dtype).transpose(1, 2).reshape(B * T, H, D) for x in (key, value))
         with self._step([T] * B) as batch:
             ops.paged_append(k, v, self.key_pool, self.value_pool, batch.block_table, batch.kv_len, batch.q_start,
                              rotary=self.rotary)

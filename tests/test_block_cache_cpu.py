@@ -124,3 +124,19 @@ def test_queries_that_are_not_the_new_tokens_are_refused(shape) -> None:
     with pytest.raises(ShapeError):
         c.attend(torch.zeros(shape), x, x, [1, 1])
     assert c.lengths == [5] and _whole(c)
+
+
+def test_append_refuses_other_shapes_and_takes_no_tokens(monkeypatch) -> None:
+    c = _cache()
+    x = torch.zeros(2, 2, 3, 8)
+    for key, value in ((x, x[:, :, :2]), (x, x[:1]), (x[:, :1], x[:, :1]), (x[..., :4], x[..., :4]), (x[0], x[0]),
+                       (x.reshape(2, 1, 3, 16), x.reshape(2, 1, 3, 16))):
+        with pytest.raises(ShapeError):
+            c.append(key, value)
+        assert c.lengths == []
+    calls = []
+    monkeypatch.setattr(ops, "paged_append", lambda k, v, *a, **kw: calls.append((k.shape, v.shape)))
+    c.append(x[:, :, :0], x[:, :, :0])  # no token yet, of two sequences
+    assert c.lengths == [0, 0] and calls == [((0, 2, 8), (0, 2, 8))]
+    c.append(x, x)
+    assert c.lengths == [3, 3] and calls[1] == ((6, 2, 8), (6, 2, 8))
