@@ -284,10 +284,16 @@ def block_dense_path(m, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask:
     if positions is not None:
         if rotary is None and kv_cache.rotary is None:
             raise BackendError("positions need a rotary embedding")
-        if positions.dim() == 3 or (positions.dim() == 2 and (rotary or kv_cache.rotary).num_axes == 1):
-            positions = positions.expand(*positions.shape[:-2], B, T).flatten(-2)
+        axes, shape = (rotary or kv_cache.rotary).num_axes, tuple(positions.shape)
+        batched = len(shape) == 3 or (len(shape) == 2 and axes == 1)
+        if not (1 <= len(shape) <= 3 and shape[-1] == T and (not batched or shape[-2] in (1, B))
+                and (len(shape) < 2 or (len(shape) == 2 and axes == 1) or shape[0] == axes)):
+            raise ShapeError("positions do not fit the tokens", expected=f"[{T}] or [{axes} axes, {B}, {T}]",
+                             actual=shape)
+        if batched:
+            positions = positions.expand(*shape[:-2], B, T).flatten(-2)
         else:
-            positions = positions.repeat(*[1] * (positions.dim() - 1), B)
+            positions = positions.repeat(*[1] * (len(shape) - 1), B)
     qp, kp, vp = (x.transpose(1, 2).reshape(B * T, H, D) for x in (q, k, v))
     out = kv_cache.attend(qp, kp, vp, [T] * B, positions, causal=m.config.causal, rotary=rotary)
     return m.dropout(m.out_proj(out.view(B, T, H * D)))
