@@ -3,6 +3,7 @@
 #include <climits>
 #include <cmath>
 #include <cstdarg>
+#include <cstdint>
 #include <cstdio>
 #include <cstring>
 #include <map>
@@ -592,9 +593,14 @@ int avq_paged_attention(int dtype, const void* q, const long long* q_strides, in
   if (!q || !q_strides || !out || !out_strides || !key_pool_strides || !value_pool_strides || !kv_len || !q_start ||
       (num_pages && (!key_pool || !value_pool)) || (table_width && !block_table))
     return fail(AVQ_ERR_ARG, "avq_paged_attention: null pointer");
+  for (int i = 0; i < 3; ++i)
+    if (key_pool_strides[i] < 0 || value_pool_strides[i] < 0)
+      return fail(AVQ_ERR_ARG, "avq_paged_attention: negative pool strides");
   const size_t need = avq::paged_attn_workspace_bytes(dtype, B, N, H, Hkv, D, max_q_len);
   if (workspace_bytes < need || !workspace)
     return fail(AVQ_ERR_WORKSPACE, "avq_paged_attention: workspace %zu < %zu bytes", workspace_bytes, need);
+  if (reinterpret_cast<uintptr_t>(workspace) % 16)
+    return fail(AVQ_ERR_WORKSPACE, "avq_paged_attention: the workspace must lie on 16 bytes");
   avq::PagedAttnArgs a{};
   a.q = q;
   a.qs = st2(q_strides);

@@ -316,8 +316,9 @@ size_t avq_paged_attention_workspace_size(int dtype, int B, int N, int H, int Hk
  * sequence, or 0; it only steers the choice of kernels, a wrong one costs time
  * and never the result.  Keys on pages outside the pool count as zeros and raise
  * bit 1 of the device fault record.  D <= 256.  workspace:
- * avq_paged_attention_workspace_size(same sizes, same max_q_len) bytes, used
- * only during the call. */
+ * avq_paged_attention_workspace_size(same sizes, same max_q_len) bytes on a
+ * 16-byte boundary, used only during the call.  The pools' strides must not be
+ * negative. */
 int avq_paged_attention(int dtype, const void* q, const long long* q_strides, int H, const void* key_pool,
                         const long long* key_pool_strides, const void* value_pool,
                         const long long* value_pool_strides, int Hkv, int D, int num_pages, int page_size,

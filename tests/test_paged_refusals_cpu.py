@@ -1,6 +1,7 @@
 """More of what the page pool's operators refuse, without a GPU."""
 from __future__ import annotations
 
+import ctypes
 import random
 
 import pytest
@@ -58,3 +59,17 @@ def test_overlap_of_packed_operands_is_found() -> None:
     q, k, v = fused[:, :8], fused[:, 8:10], fused[:, 10:]
     assert not ops._overlap(q, k) and not ops._overlap(k, v) and ops._overlap(q, fused[:, 7:9])
     assert not ops._overlap(q[:0], q) and ops._overlap(q, q[3:])
+
+
+def test_attention_entry_refuses_a_shifted_workspace_and_negative_strides() -> None:
+    """Vector loads of the workspace, and offsets whose sign says that a page is missing."""
+    for shift in (1, 4, 8):
+        assert _attention(ws=16 + shift) == 4, _lib.last_error()
+    call = _lib.load().avq_paged_attention
+    two, three = ctypes.c_longlong * 2, ctypes.c_longlong * 3
+    for which in range(6):
+        strides = [8] * 6
+        strides[which] = -8
+        assert call(1, 16, two(8, 8), 4, 16, three(*strides[:3]), 16, three(*strides[3:]), 2, 8, 4, 16, 16, 2, 2, 16, 16,
+                    1, 1, 1, 0, 1.0, 0, 16, two(8, 8), 16, 1 << 40, None) == 1, _lib.last_error()
+        assert "strides" in _lib.last_error()
