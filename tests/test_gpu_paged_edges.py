@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from avqa_b200 import BackendError, RotaryEmbedding, ops
-from paged_reference import DTYPES, assert_within, attention64, half
+from paged_reference import DTYPES, assert_within, attention64, half, rotate64
 from test_gpu_paged import Batch, fault
 
 pytestmark = pytest.mark.gpu
@@ -136,3 +136,19 @@ def test_outputs_in_the_memory_of_inputs_are_refused() -> None:
     assert torch.equal(ops.paged_append(k, v, *b.lists, q=q, rotary=rot, q_out=room[:b.N, 4:]), want)
     assert ops.paged_append(k, v, *b.lists, q=q, rotary=rot, q_out=q) is q
     assert torch.equal(q, want) and torch.equal(k, b.k) and torch.equal(v, b.v)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("D", [80, 96, 112, 192])
+@pytest.mark.parametrize("new,lens,kw", [([1, 1], [300, 5], {}), ([30, 1], [200, 70], {}), ([90], [500], dict(window=40)),
+                                         ([20], [77], dict(causal=False))])
+def test_widths_between_the_padded_ones(dt, D, new, lens, kw) -> None:
+    b = Batch(dt, 6, 2, D, 16, new, lens, seed=D)
+    first = b.check(**kw)
+    assert torch.equal(ops.paged_attention(b.q, *b.lists, **kw), first)
+    rot = RotaryEmbedding(D, rotary_dim=D // 4 * 2)
+    pos = torch.cat([torch.arange(n - t, n) for t, n in zip(new, lens)]).cuda()
+    q = ops.paged_append(b.k, b.v, *b.lists, q=b.q, rotary=rot)
+    assert_within(q.transpose(0, 1), *rotate64(b.q.transpose(0, 1), pos[None], rot), "queries")
+    b.check("behind the append", q=q, **kw)
+    assert fault() == 0

@@ -7,7 +7,7 @@ import random
 import pytest
 import torch
 
-from avqa_b200 import _lib, ops
+from avqa_b200 import BackendError, _lib, ops
 from test_paged_cpu import _append, _attention
 
 MOST = 2 ** 31 - 1 - 65536  # tokens that a table's row may hold: the kernels step past the last key in 32 bits
@@ -73,3 +73,34 @@ def test_attention_entry_refuses_a_shifted_workspace_and_negative_strides() -> N
         assert call(1, 16, two(8, 8), 4, 16, three(*strides[:3]), 16, three(*strides[3:]), 2, 8, 4, 16, 16, 2, 2, 16, 16,
                     1, 1, 1, 0, 1.0, 0, 16, two(8, 8), 16, 1 << 40, None) == 1, _lib.last_error()
         assert "strides" in _lib.last_error()
+
+
+def test_a_call_on_another_device_makes_it_current(monkeypatch) -> None:
+    """A launch goes to the current device: a call for tensors of another one switches to it, and back."""
+    current = [0]
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *error):
+            current[0] = self.before
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 100 + index, raising=False)
+    calls = []
+
+    def entry(*args):
+        calls.append((current[0], args))
+        return 0
+
+    ops._call("entry", entry, 0, 5)
+    ops._call("entry", entry, 1, 6)
+    assert calls == [(0, (5, 100)), (1, (6, 101))] and current == [0]
+    with pytest.raises(BackendError):
+        ops._call("entry", lambda *a: 1, 1)
+    assert current == [0]
