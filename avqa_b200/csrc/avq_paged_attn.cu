@@ -48,6 +48,7 @@ constexpr int kMaxGroup = 16;   // rows of a group, at most
 // (32 sequences of up to 32768 keys, 8 heads of 128: 503 us at 2 per SM, 454 at 8, 455 at 16).  Short ones: a single
 // round, as a CTA's first loads and its merge are then most of its time (one sequence of 16384 keys, 8 heads of 128: 18
 // us at 2 per SM, 30 at 8; of 32768 keys 34 and 44).  The two meet between 2^19 keys (55 and 63 us) and 2^20 (104, 97).
+// Measured where two CTAs or more share an SM; where one does (wide rows, fp32), the single round becomes two.
 constexpr int kTargetCtas = 8 * kSms, kFewestCtas = 2 * kSms, kMinSpan = 128;
 constexpr long long kFewKeys = 1 << 19;
 // A cluster of eight CTAs for each (row group, key head), without a second kernel, where two CTAs to an SM hold them
@@ -322,8 +323,9 @@ template <int DT, int DP>
 constexpr int step_keys() { return DP * (int)sizeof(typename Storage<DT>::T) <= 128 ? 32 : 16; }
 template <int DT, int DP>
 constexpr int stage_elems() { return 2 * step_keys<DT, DP>() * (DP + Operand<DT>::kPad); }
-// Stages of a warp's ring: two, so that three CTAs or more (fp32: two) share an SM and one's first loads overlap the
-// others' streams (fp32 of 129 dimensions on: one stage, one CTA); three in a cluster, where fewer CTAs run.
+// Stages of a warp's ring: two, so that one CTA's first loads overlap another's streams: three CTAs share an SM at 16
+// bits up to 128 dimensions, two in fp32 up to 64.  Wider rows leave room for one (fp32 of 129 dimensions on: with one
+// stage).  Three stages in a cluster, where fewer CTAs run.
 template <int DT, int DP, bool CL>
 constexpr int ring_stages() {
   return DP * (int)sizeof(typename Storage<DT>::T) > 512 ? 1 : (CL && DT != DT_F32 ? 3 : 2);

@@ -1,6 +1,6 @@
 // Attention of chunks over a page pool on the tcgen05 tensor cores (bf16,
 // fp16; head_dim 64 and 128).  The operator is avq_paged_attn.cu's; this
-// kernel takes the sequences with more than kPagedFewRows rows.
+// kernel takes the sequences with more than kFewRows rows.
 //
 // The rows of one (sequence, key head) are its (token, head of the group)
 // pairs, token by token, so that a key tile serves the whole group and short
@@ -405,10 +405,9 @@ __device__ __forceinline__ float2 ex2_poly(float2 x) {
   return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(r.x) << 23)),
                      __int_as_float(__float_as_int(p.y) + (__float_as_int(r.y) << 23)));
 }
-// The pairs of eight that take the polynomial.  At head_dim 64 the softmax bounds the kernel and the exponential unit
-// the softmax: a quarter there (4 prompts of about 2048 tokens over 8192: 576 us with none, 559 a quarter, 590 three
-// eighths).  At head_dim 128 the tensor cores and the power they draw bound it, and the polynomial's instructions only
-// cost (256 queries over 131072 keys: 1012 us with none, 1015 a quarter, 1080 three eighths).
+// The pairs of eight that take the polynomial.  A quarter at head_dim 64, where a step has half the multiplications to
+// the same exponentials (4 prompts of about 2048 tokens over 8192: 576 us with none, 559 a quarter, 590 three eighths);
+// none at head_dim 128 (256 queries over 131072 keys: 1012 us with none, 1015 a quarter, 1080 three eighths).
 template <int D> constexpr uint32_t poly_pairs() { return D == 64 ? 0x12u : 0u; }
 
 template <int DT, int D, bool TMA>
@@ -519,8 +518,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_attn_tc_kernel(const __gr
         if constexpr (TMA) {
           // The first warp brings the keys, the second the values; lane x of it one box of a tile: 64 columns of the
           // rows of one page, or of the tile where the page is larger.  (The lanes' copies are issued one after the
-          // other, about 130 cycles each: with 16-token pages one warp for both took 4500 cycles a step, the tensor
-          // cores 3300.)
+          // other, about 130 cycles each: with 16-token pages one warp for both took 4500 cycles a step, the whole step
+          // 3300 with two.)
           if (lw < 2) {
             const bool is_v = lw == 1;
             const CUtensorMap* map = is_v ? &maps.v : &maps.k;

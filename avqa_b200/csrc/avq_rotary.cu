@@ -40,7 +40,7 @@ struct Div {
   __device__ int operator()(int n) const { return d == 1 ? n : (int)__umulhi((uint32_t)n, m); }
 };
 
-// 51 registers a thread: at D = 128 (bf16, 64 heads, 8192 tokens) 47.6 us, 5.6 TB/s; three blocks of 256 threads took
+// 48 registers a thread: at D = 128 (bf16, 64 heads, 8192 tokens) 47.6 us, 5.6 TB/s; three blocks of 256 threads took
 // 50.9, six of them, which spill, 63.0.
 constexpr int kMinBlocks = 10;
 

@@ -604,7 +604,8 @@ def paged_attention(q: torch.Tensor, key_pool: torch.Tensor, value_pool: torch.T
     and before, with ``window > 0`` the last ``window`` of these.  ``H`` may be
     a multiple of the pool's heads (query head h reads key head
     ``h // (H // Hkv)``).  A token that sees no key gets zeros; rows behind
-    ``q_start[B]`` are left as they are in ``out``.  ``max_q_len``: the most new
+    ``q_start[B]`` are left as they are in ``out`` (without ``out`` they hold
+    anything).  Pages whose keys no token sees, behind the window, are not looked up.  ``max_q_len``: the most new
     tokens of a sequence, if known; it only steers the choice of kernels.
     ``out`` must not overlap ``q``, also as another view of its memory.
     Probabilities are rounded to the dtype for the product with the values

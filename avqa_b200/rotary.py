@@ -32,7 +32,9 @@ class RotaryEmbedding:
     ``frequencies``  radians per position of each pair, instead of ``base``'s.
 
     It holds host values only: any device and stream may use it, and a call
-    can be captured into a CUDA graph.
+    can be captured into a CUDA graph.  (A backward pass captured into one needs,
+    as every one of torch's does, that no eager graph over the same leaves is
+    alive: their gradients are accumulated on the eager graph's stream.)
     """
 
     def __init__(self, head_dim: int, base: float = 10000.0, rotary_dim: int | None = None,
